@@ -446,6 +446,144 @@ int qwen_hip_op_sd_conv(float *Y, const float *X, const float *W, const float *b
 int qwen_hip_op_sd_conv_transpose(float *Y, const float *X, const float *W, const float *bias, int Tin, int Cin,
                                   int Cout, int kernel, int stride, int tile);
 
+/* ---- operators of paged, batched serving (no counterpart in the reference, whose caches are one
+ * contiguous block a stream) ----
+ * For callers that run many requests over one pool of cache pages and keep everything on the GPU: the step's
+ * bookkeeping, the cache's writer, the attention that reads it, whole prompts packed behind each other, and the
+ * rules on a batch's logits.  Every pointer in these descriptors is DEVICE memory of the device that `stream`
+ * belongs to; the descriptor itself is host memory, read during the call, so one made once can be used for every
+ * step.  Calls launch on `stream` (a hipStream_t; NULL = the null stream of the current device) and return
+ * without waiting: 0, or -1 with qwen_hip_last_error() set and nothing launched.  They allocate nothing and can
+ * be captured into a graph.  Lengths, tables and slots are read on the device: a replayed graph follows what
+ * they hold then. */
+enum { QWEN_HIP_DT_F32 = 0, QWEN_HIP_DT_BF16 = 1, QWEN_HIP_DT_F16 = 2 };
+
+/* One layer's cache in pages: position p of a request lies in page table[p / page_size] at place p % page_size
+ * (its slot: page * page_size + place); element (page, head, place, d) of k (of v) is
+ * k[page*page_stride + head*head_stride + place*slot_stride + d].  Any order of pages, heads and places is a choice
+ * of strides (in elements; [page][head][place][d] and [page][place][head][d] are the usual two).  dtype BF16 or
+ * F16; head_dim 64 or 128; k and v aligned to 16 bytes, strides multiples of 8 elements. */
+typedef struct {
+    void *k, *v;
+    long long page_stride, head_stride, slot_stride;
+    int dtype, n_pages, page_size, n_kv_heads, head_dim;
+} qwen_hip_kv_pages_t;
+
+/* The bookkeeping of one step.  For every request b < B (B <= 2048): kv_len[b] tokens are cached, in the pages
+ * table[b*table_stride + 0 .. ceil(kv_len[b] / page_size) - 1]; new_len[b] > 0 appends as many, 0 leaves the request
+ * as it is, < 0 ends it and gives its pages back.  free_pages[0 .. *n_free) is the free list (room for n_pages). */
+typedef struct {
+    const int *new_len;      /* [B] */
+    const int *kv_len;       /* [B] */
+    const int *n_free;       /* [1] */
+    int *table;              /* [B][table_stride]: pages taken are written, the rest stays */
+    int *free_pages;         /* [n_pages]: pages given back are written behind the first *n_free */
+    int *kv_len_out;         /* [B] kv_len + new_len, 0 for an ended request; may be kv_len */
+    int *n_free_out;         /* [1]; may be n_free */
+    int *cu_q;               /* [B + 1]: first row of each request's new tokens, and their number */
+    int *pos, *slot;         /* [max_tokens]: each new token's position and slot; -1 behind the last one */
+    int *status;             /* [1]: 0, or a sum of QWEN_HIP_PLAN_* */
+    long long table_stride;  /* entries between requests, >= table_cols */
+    int B, page_size, n_pages, table_cols, max_tokens;
+} qwen_hip_page_plan_t;
+/* reasons for which a step cannot be planned; then nothing is taken or given back: kv_len_out and n_free_out hold
+ * what kv_len and n_free hold, cu_q is all 0 and pos and slot all -1, so that the step's other calls do nothing */
+enum {
+    QWEN_HIP_PLAN_NO_PAGES = 1,     /* more pages needed than free (pages given back in this step count as free) */
+    QWEN_HIP_PLAN_TABLE_FULL = 2,   /* a request outgrows table_cols pages */
+    QWEN_HIP_PLAN_TOO_MANY = 4,     /* more than max_tokens new tokens */
+    QWEN_HIP_PLAN_INVALID = 8       /* a negative kv_len, a free count or page number out of range */
+};
+/* Pages given back go onto the free list's end in the order of requests and of their positions; pages are then
+ * taken from its end, for the requests in order.  The result depends on nothing else.  With separate kv_len_out
+ * and n_free_out a call can be repeated with the same result. */
+int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *plan, void *stream);
+
+/* New tokens' q, k, v rows into attention's inputs: per-head RMSNorm of q and k (x / sqrt(mean x^2 + eps) times
+ * q_norm / k_norm [head_dim] f32; NULL: none), RoPE of both on the halves of a head (tables f32 [rope_len][head_dim/2];
+ * NULL: none), q to q_out, k and v to the cache at slot[t], each rounded once to the nearest (the Talker's own
+ * cache truncates).  dtype: of q, k, v and q_out; F32 rows go with either cache type, BF16 and F16 rows with their
+ * own.  A token whose slot is outside the cache (the plan's -1), or whose pos is outside [0, rope_len) where there
+ * are tables, is skipped: nothing of it is written.  Slots of one call have to be distinct.  q may be NULL (k and v
+ * only); q_out may be q.  Pointers aligned to 16 bytes, strides (in elements, between tokens) multiples of 16 bytes. */
+typedef struct {
+    const void *q, *k, *v;
+    void *q_out;
+    long long q_stride, k_stride, v_stride, q_out_stride;
+    const float *q_norm, *k_norm;
+    const float *rope_cos, *rope_sin;
+    const int *pos, *slot;   /* [T]; pos may be NULL without tables */
+    int dtype, n_heads, T, rope_len;
+    float eps;
+} qwen_hip_page_append_t;
+int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_append_t *append, void *stream);
+
+/* Causal attention of new tokens over the cache that holds them and what came before: request b's rows are
+ * cu_q[b] .. cu_q[b+1] - 1 of q and out ([T] tokens, head h of a token at h*head_dim), row i of its n being position
+ * kv_len[b] - n + i (kv_len: with the new tokens).  A row sees positions up to its own, the last `window` of them
+ * where window > 0; query head h reads kv head h / (n_heads / n_kv_heads).  A row that sees nothing is 0; rows
+ * before cu_q[0] and behind cu_q[B] stay as they were.  A table entry outside [0, n_pages) holds no keys: its
+ * positions are not seen.  What lies in positions that a row does not see never reaches it, infinite or NaN
+ * included.  Scores, softmax and sums are f32; with F32 rows (over a BF16 cache) so are the products; with BF16 or
+ * F16 rows (over a cache of their own type) the probabilities are rounded to that type for the product with V.
+ * max_q and max_kv: the longest request's new tokens and kv_len as far as the host knows; they choose the launch
+ * shape and change no result beyond rounding.  scale > 0.  B <= 65535, n_heads / n_kv_heads <= 64.
+ * workspace: qwen_hip_op_page_attention_workspace() bytes (of the same descriptor), aligned to 16; its contents do
+ * not matter before or after; calls that may overlap need one each.  Alignment and strides as for append. */
+typedef struct {
+    const void *q;
+    void *out;
+    long long q_stride, out_stride;
+    const int *cu_q;         /* [B + 1] */
+    const int *kv_len;       /* [B] */
+    const int *table;        /* [B][table_stride] */
+    long long table_stride;
+    void *workspace;
+    long long workspace_bytes;
+    int dtype, n_heads, B, T, table_cols, max_q, max_kv, window;
+    float scale;
+} qwen_hip_page_attn_t;
+long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn);  /* -1: error */
+int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn, void *stream);
+
+/* The prefill's causal attention for several prompts at once, of different lengths, packed behind each other:
+ * sequence b is tokens cu[b] .. cu[b+1] - 1 of q, k, v and out.  q, k, v and out share one dtype (F32: f32 products,
+ * as qwen_hip_op_prefill_attention; BF16 / F16 as above); the rest as for the paged form. */
+typedef struct {
+    const void *q, *k, *v;
+    void *out;
+    long long q_stride, k_stride, v_stride, out_stride;
+    const int *cu;           /* [B + 1] */
+    int dtype, n_heads, n_kv_heads, head_dim, B, T, window;
+    float scale;
+} qwen_hip_packed_attn_t;
+int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *attn, void *stream);
+
+/* The rules on a batch's logits, before sampling.  Row b, token t, with n_all and n_out the times t stands in
+ * history b = hist[hist_off[b] .. hist_off[b+1]) and in its part behind the first n_prompt[b] entries (NULL: all):
+ *   n_all > 0:  x = x > 0 ? x / rep[b] : x * rep[b]     (rep_each: n_all times over, as qwen_hip_op_sample does)
+ *   n_out > 0:  x = x - n_out * frequency[b] - presence[b]
+ *   t listed in bias_tok[bias_off[b] .. bias_off[b+1]):  x += bias_val of its last entry
+ *   bit t % 32 of mask[b*mask_stride + t / 32] is 0:     x = -infinity
+ * in f32, rounded once to dtype (of logits and out).  rep, presence, frequency, bias_tok and mask may each be NULL:
+ * off.  Tokens outside [0, V) are passed over; offsets are clipped to hist_cap / bias_cap entries.  out may be
+ * logits (same stride).  A row whose mask allows nothing is all -infinity.  B <= 65535. */
+typedef struct {
+    const void *logits;
+    void *out;
+    long long logits_stride, out_stride;   /* elements between rows, >= V */
+    const int *hist, *hist_off;            /* [hist_cap], [B + 1]; NULL without rep, presence and frequency */
+    const int *n_prompt;                   /* [B] */
+    const float *rep, *presence, *frequency;   /* [B] */
+    const int *bias_tok;
+    const float *bias_val;
+    const int *bias_off;
+    const uint32_t *mask;
+    long long mask_stride;                 /* words between rows */
+    int dtype, B, V, hist_cap, bias_cap, rep_each;
+} qwen_hip_logit_rules_t;
+int qwen_hip_op_logit_rules(const qwen_hip_logit_rules_t *rules, void *stream);
+
 const char *qwen_hip_last_error(void);
 
 #ifdef __cplusplus

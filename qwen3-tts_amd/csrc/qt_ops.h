@@ -1,0 +1,132 @@
+// qt_ops.h — what the operators of paged, batched serving share: element types, rounding, the
+// division by a page size, and the host side of a call (the stream's device, argument checks).
+#pragma once
+#include <hip/hip_runtime.h>
+#include <stdint.h>
+
+#include "qt_device.h"
+#include "qwen_tts_hip.h"
+
+extern "C" void qt_seterr(const char *fmt, ...) __attribute__((format(printf, 1, 2)));   // qwen_hip_last_error's text
+
+// Element types, as template arguments.  Every load widens to f32, every store rounds once to the
+// nearest, ties to even (bf16 off by at most 2^-8 of the value, f16 by 2^-11).
+struct QtF32 { typedef float elem; };
+struct QtBf16 { typedef uint16_t elem; };
+struct QtF16 { typedef uint16_t elem; };
+
+template <typename T> __device__ __forceinline__ uint32_t qt_round2(float a, float b);
+template <> __device__ __forceinline__ uint32_t qt_round2<QtBf16>(float a, float b) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, __builtin_convertvector((f2{a, b}), b2));
+}
+template <> __device__ __forceinline__ uint32_t qt_round2<QtF16>(float a, float b) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_bit_cast(uint32_t, (h2{(_Float16)a, (_Float16)b}));
+}
+template <typename T> __device__ __forceinline__ float qt_lo(uint32_t u);
+template <typename T> __device__ __forceinline__ float qt_hi(uint32_t u);
+template <> __device__ __forceinline__ float qt_lo<QtBf16>(uint32_t u) { return __uint_as_float(u << 16); }
+template <> __device__ __forceinline__ float qt_hi<QtBf16>(uint32_t u) { return __uint_as_float(u & 0xFFFF0000u); }
+template <> __device__ __forceinline__ float qt_lo<QtF16>(uint32_t u) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(u & 0xFFFFu));
+}
+template <> __device__ __forceinline__ float qt_hi<QtF16>(uint32_t u) {
+    return (float)__builtin_bit_cast(_Float16, (uint16_t)(u >> 16));
+}
+
+// 8 consecutive elements; p needs `A` bytes of alignment
+typedef uint32_t qt_w4 __attribute__((ext_vector_type(4)));
+template <int A> __device__ __forceinline__ qt_w4 qt_load16(const void *p) {
+    qt_w4 a;
+    __builtin_memcpy(&a, __builtin_assume_aligned(p, A), 16);
+    return a;
+}
+template <int A> __device__ __forceinline__ void qt_store16(void *p, qt_w4 a) { __builtin_memcpy(__builtin_assume_aligned(p, A), &a, 16); }
+template <typename T, int A = 16> __device__ __forceinline__ void qt_load8(const void *p, float (&v)[8]) {
+    const uint8_t *b = (const uint8_t *)p;
+    if constexpr (sizeof(typename T::elem) == 4) {
+        const qt_w4 x = qt_load16<A>(b), y = qt_load16<A>(b + 16);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[i] = __uint_as_float(x[i]); v[4 + i] = __uint_as_float(y[i]); }
+    } else {
+        const qt_w4 x = qt_load16<A>(b);
+#pragma unroll
+        for (int i = 0; i < 4; i++) { v[2 * i] = qt_lo<T>(x[i]); v[2 * i + 1] = qt_hi<T>(x[i]); }
+    }
+}
+template <typename T, int A = 16> __device__ __forceinline__ void qt_store8(void *p, const float (&v)[8]) {
+    uint8_t *b = (uint8_t *)p;
+    qt_w4 x, y;
+    if constexpr (sizeof(typename T::elem) == 4) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) { x[i] = __float_as_uint(v[i]); y[i] = __float_as_uint(v[4 + i]); }
+        qt_store16<A>(b, x);
+        qt_store16<A>(b + 16, y);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) x[i] = qt_round2<T>(v[2 * i], v[2 * i + 1]);
+        qt_store16<A>(b, x);
+    }
+}
+template <typename T> __device__ __forceinline__ float qt_load1(const void *p) {
+    if constexpr (sizeof(typename T::elem) == 4) return *reinterpret_cast<const float *>(p);
+    else return qt_lo<T>(*reinterpret_cast<const uint16_t *>(p));
+}
+template <typename T> __device__ __forceinline__ void qt_store1(void *p, float v) {
+    if constexpr (sizeof(typename T::elem) == 4) *reinterpret_cast<float *>(p) = v;
+    else *reinterpret_cast<uint16_t *>(p) = (uint16_t)qt_round2<T>(v, 0.f);
+}
+
+// n / d for 0 <= n < 2^31 by one product: m = ceil(2^(31 + l) / d) with l = ceil(log2 d), so m d exceeds 2^(31 + l)
+// by less than d <= 2^l, and n times that excess stays under 2^(31 + l).
+struct QtDiv { uint32_t m, l; };
+static inline QtDiv qt_div_of(int d) {
+    uint32_t l = 0;
+    while ((1u << l) < (uint32_t)d) l++;
+    return {(uint32_t)(((1ull << (31 + l)) + (uint32_t)d - 1) / (uint32_t)d), l};
+}
+__device__ __forceinline__ int qt_quot(int n, QtDiv d) { return (int)(__umulhi(2u * (uint32_t)n, d.m) >> d.l); }
+
+// ---- host side ----
+
+// Makes the stream's device the current one while a call launches (kernels are looked up for the
+// current device), and the caller's current again afterwards.
+struct QtOnDevice {
+    int cur = -1, dev = -1;
+    hipError_t err = hipSuccess;
+    explicit QtOnDevice(hipStream_t st) {
+        if (!st) return;                                   // the null stream is the current device's
+        err = hipStreamGetDevice(st, &dev);
+        if (err == hipSuccess) err = hipGetDevice(&cur);
+        if (err == hipSuccess && cur != dev) err = hipSetDevice(dev);
+    }
+    ~QtOnDevice() {
+        if (cur >= 0 && dev >= 0 && cur != dev) (void)hipSetDevice(cur);
+    }
+    QtOnDevice(const QtOnDevice &) = delete;
+    QtOnDevice &operator=(const QtOnDevice &) = delete;
+};
+
+#define QT_REFUSE(cond, ...) do { if (cond) { qt_seterr(__VA_ARGS__); return -1; } } while (0)
+
+static inline int qt_dt_size(int dt) { return dt == QWEN_HIP_DT_F32 ? 4 : dt == QWEN_HIP_DT_BF16 || dt == QWEN_HIP_DT_F16 ? 2 : 0; }
+static inline bool qt_off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
+
+// the cache's descriptor; `who` names the call
+static inline int qt_check_pages(const char *who, const qwen_hip_kv_pages_t *kv) {
+    QT_REFUSE(!kv, "%s: null cache descriptor", who);
+    QT_REFUSE(!kv->k || !kv->v, "%s: null cache pointer", who);
+    QT_REFUSE(kv->dtype != QWEN_HIP_DT_BF16 && kv->dtype != QWEN_HIP_DT_F16, "%s: cache dtype %d (bf16 or f16)", who, kv->dtype);
+    QT_REFUSE(kv->head_dim != 64 && kv->head_dim != 128, "%s: head_dim %d (64 or 128)", who, kv->head_dim);
+    QT_REFUSE(kv->n_kv_heads < 1 || kv->n_kv_heads > 65535, "%s: n_kv_heads %d out of range (1..65535)", who, kv->n_kv_heads);
+    QT_REFUSE(kv->n_pages < 1 || kv->page_size < 1 || (long long)kv->n_pages * kv->page_size > 0x7FFFFFFFll,
+              "%s: %d pages of %d (both at least 1, 2^31 - 1 slots at most)", who, kv->n_pages, kv->page_size);
+    QT_REFUSE(qt_off16(kv->k) || qt_off16(kv->v), "%s: cache pointers have to be aligned to 16 bytes", who);
+    QT_REFUSE(kv->page_stride % 8 || kv->head_stride % 8 || kv->slot_stride % 8 || kv->page_stride < 0 || kv->head_stride < 0 ||
+                  kv->slot_stride < 0,
+              "%s: cache strides %lld, %lld, %lld (multiples of 8 elements, not negative)", who, kv->page_stride,
+              kv->head_stride, kv->slot_stride);
+    return 0;
+}

@@ -1,0 +1,588 @@
+// qt_pattn.hip — causal attention of several requests' new tokens: over paged caches
+// (qwen_hip_op_page_attention) and over whole packed prompts (qwen_hip_op_packed_attention).
+//
+// o_i = sum_j p_ij v_j / sum_j p_ij,  p_ij = 2^((s_ij - m_i) c),  s_ij = q_i . k_j,  c = scale log2(e), over the
+// positions j that row i sees, with the running maximum m_i and sum of one pass over the keys (all f32).
+//
+// Rows.  The new tokens of a request and the query heads of one kv head make its rows, row r = (token r / G, head
+// r % G): heads that read the same keys share them, a decode step's heads fill a tile as a prompt's tokens do, and the
+// causal edge crosses few key blocks.  A tile is 32 rows.
+//
+// Products.  Scores are made transposed, S^T = K Q^T by v_mfma_f32_32x32x16: lane l supplies key row l % 32 (A) and
+// query row l % 32 (B), each as 8 of the 16 dims (those of half h = l / 32), and ends with query row l % 32 and keys
+// 8 (i / 4) + 4 h + i % 4 in register i.  So a lane has one query row: the softmax needs one exchange with the other
+// half, scaling a row's sums is one factor a lane, and eight of its probabilities are, in place, the B operand
+// of O^T = V^T P^T over 16 keys (a sum over keys in the order of the registers: key 16 s + 8 (j / 4) + 4 h + j % 4 in
+// place (h, j)).  V's operand wants those 8 keys of one dim: a lane loads NT = HD / 32 neighbouring dims of each
+// key's row (the 32 lanes of a half a whole row) and transposes them in registers by byte permutes; dim NT m + t is row
+// m of product t.
+//
+// Types.  16-bit rows over a cache of their type: one product each; the probabilities are rounded to that type for
+// V's product (bf16: at most 2^-8 of each, f16: 2^-11, of either sign over the keys; the sum of a row keeps them
+// unrounded).  f32 rows over a bf16 cache: q and p as three bf16 planes whose sum is exact, three products.  All f32: both
+// operands as planes, six products (qt_planes.h).
+//
+// What a row does not see never reaches it: hidden scores become -infinity before the maximum.  Their probabilities
+// are 0, and 0 times an infinite or NaN v would still be NaN: where a tile ends with anything that is not
+// finite, its rows are done again key by key over what each of them sees (att_serial), which also serves f32 values
+// that have no planes (infinite, NaN, past bf16's range after rounding).
+#include "qt_ops.h"
+#include "qt_planes.h"
+
+typedef float qt_f32x16 __attribute__((ext_vector_type(16)));
+typedef _Float16 qt_f16x8 __attribute__((ext_vector_type(8)));
+
+#define ATT_MAX_KEYS (1 << 30)              // positions of a request: their arithmetic stays in 32 bits
+
+struct AttArgs {
+    const uint8_t *q, *k, *v;
+    uint8_t *out;
+    long long qs, os;                       // elements between tokens
+    long long ks_page, ks_head, ks_slot;    // paged: of k and v; packed: ks_slot, vs_slot between tokens, head HD apart
+    long long vs_slot;
+    const int *cu, *kv_len, *table;
+    long long ts;
+    int cols, n_pages, ps;
+    QtDiv div;
+    int B, T, nkv, G, window;
+    float c;                                // scale log2(e)
+    int tps;                                // > 0: launch slots a request, else slots by att_find
+    int splits, chunk;                      // key ranges a tile, 32-key blocks in each (the last takes the rest)
+    float *po, *pm;                         // splits > 1: sums [split][T nh][HD], and maximum, sum [split][T nh][2]
+};
+
+template <typename T> __device__ __forceinline__ qt_f32x16 att_mma(qt_u32x4 a, qt_u32x4 b, qt_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(qt_bf16x8, a), __builtin_bit_cast(qt_bf16x8, b), c, 0, 0, 0);
+}
+template <> __device__ __forceinline__ qt_f32x16 att_mma<QtF16>(qt_u32x4 a, qt_u32x4 b, qt_f32x16 c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(qt_f16x8, a), __builtin_bit_cast(qt_f16x8, b), c, 0, 0, 0);
+}
+// sum over planes, the smallest products first
+template <typename T, int NA, int NB>
+__device__ __forceinline__ qt_f32x16 att_planes(const qt_u32x4 (&a)[NA], const qt_u32x4 (&b)[NB], qt_f32x16 c) {
+#pragma unroll
+    for (int s = NA + NB - 2; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+            if (s - i >= 0 && s - i < NB && s <= 2) c = att_mma<T>(a[i], b[s - i], c);
+    return c;
+}
+
+__device__ __forceinline__ float att_other_half(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+// The request that a launch slot belongs to when a request begins at slot floor(first row / 32) + b: tiles
+// ceil(rows / 32) fit before the next one's, whatever the lengths, so floor(all rows / 32) + B slots are enough for
+// the host, which does not know them.  One load and ballot per 64 requests.
+// Offsets are the caller's: one out of range is brought into it, so that nothing is read or written past T.
+__device__ __forceinline__ int att_cu(const AttArgs &a, int b) { return min(max(a.cu[b], 0), a.T); }
+__device__ __forceinline__ int att_first(const AttArgs &a, int b) { return (int)((long long)att_cu(a, b) * a.G / 32) + b; }
+__device__ __forceinline__ int att_find(const AttArgs &a, int slot) {
+    const int lane = threadIdx.x & 63;
+    int b = -1;
+    for (int base = 0; base < a.B; base += 64) {
+        const int i = base + lane;
+        const bool before = i < a.B && att_first(a, i) <= slot;
+        const int n = __popcll(__ballot(before));
+        b += n;
+        if (n < 64) break;
+    }
+    return b;
+}
+
+// one tile's geometry, uniform over the workgroup
+struct AttTile {
+    int q0, rows, r0;           // first token of the request, its rows, the tile's first row
+    int shift, kmax;            // a token's position is shift + its place; keys at or past kmax do not exist
+    int lo, hi;                 // keys that some row of the tile may see
+};
+template <bool PAGED>
+__device__ __forceinline__ AttTile att_tile(const AttArgs &a, int b, int tile) {
+    AttTile t;
+    t.q0 = att_cu(a, b);
+    const int n = max(att_cu(a, b + 1) - t.q0, 0);
+    t.rows = n * a.G;
+    t.r0 = 32 * tile;
+    const int kv = PAGED ? min(max(a.kv_len[b], 0), ATT_MAX_KEYS) : n;
+    t.kmax = PAGED ? min(kv, a.cols * a.ps) : n;
+    t.shift = kv - n;
+    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 31, t.rows - 1) / a.G;
+    t.lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+    t.hi = min(t.kmax, last + 1);
+    return t;
+}
+
+// the page of a key, -1 for none
+__device__ __forceinline__ int att_page(const AttArgs &a, const int *table, const AttTile &t, int key) {
+    if (key >= t.kmax) return -1;
+    const int p = table[qt_quot(key, a.div)];
+    return (unsigned)p < (unsigned)a.n_pages ? p : -1;
+}
+__device__ __forceinline__ long long att_slot(const AttArgs &a, int page, int key) {
+    return page < 0 ? 0 : page * a.ks_page + (key - qt_quot(key, a.div) * a.ps) * a.ks_slot;
+}
+
+// Writes NT elements of a row's output, dim NT m.
+template <typename QT, int NT> __device__ __forceinline__ void att_put(uint8_t *p, const float (&v)[NT]) {
+    if constexpr (sizeof(typename QT::elem) == 4) {
+        typedef float fv __attribute__((ext_vector_type(NT)));
+        fv x;
+#pragma unroll
+        for (int t = 0; t < NT; t++) x[t] = v[t];
+        *reinterpret_cast<fv *>(p) = x;
+    } else {
+        typedef uint32_t uv __attribute__((ext_vector_type(NT / 2)));
+        uv x;
+#pragma unroll
+        for (int t = 0; t < NT / 2; t++) x[t] = qt_round2<QT>(v[2 * t], v[2 * t + 1]);
+        *reinterpret_cast<uv *>(p) = x;
+    }
+}
+
+// One row over keys [k0, k1), one after the other in f32.  A wave; lane: dims lane + 64 e.
+template <typename QT, typename KT, int HD, bool PAGED>
+__device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const int *table, int head, int r, int k0, int k1, bool part, int split) {
+    constexpr int EQ = sizeof(typename QT::elem), EK = sizeof(typename KT::elem), D = HD / 64;
+    const int lane = threadIdx.x & 63, tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
+    const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD) * EQ;
+    float q[D], o[D], m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int e = 0; e < D; e++) { q[e] = qt_load1<QT>(qp + (lane + 64 * e) * EQ); o[e] = 0.f; }
+    k0 = max(k0, a.window > 0 ? pos - a.window + 1 : 0);
+    k1 = min(k1, min(t.kmax, pos + 1));
+    for (int j = max(k0, 0); j < k1; j++) {
+        long long ko, vo;
+        if (PAGED) {
+            const int p = att_page(a, table, t, j);
+            if (p < 0) continue;
+            ko = vo = att_slot(a, p, j) + head * a.ks_head;
+        } else {
+            ko = (long long)(t.q0 + j) * a.ks_slot + head * HD;
+            vo = (long long)(t.q0 + j) * a.vs_slot + head * HD;
+        }
+        float s = 0.f;
+#pragma unroll
+        for (int e = 0; e < D; e++) s = fmaf(q[e], qt_load1<KT>(a.k + (ko + lane + 64 * e) * EK), s);
+        s = group_sum<64>(s);
+        const float mn = fmaxf(m, s), mr = mn == -INFINITY ? 0.f : mn;
+        const float f = qt_exp2((m - mr) * a.c), p = qt_exp2((s - mr) * a.c);
+        l = l * f + p;
+#pragma unroll
+        for (int e = 0; e < D; e++) o[e] = fmaf(p, qt_load1<KT>(a.v + (vo + lane + 64 * e) * EK), o[e] * f);
+        m = mn;
+    }
+    const size_t at = (size_t)(t.q0 + tok) * (a.nkv * a.G) + qh;
+    if (part) {
+        const size_t row = (size_t)split * a.T * (a.nkv * a.G) + at;
+#pragma unroll
+        for (int e = 0; e < D; e++) a.po[row * HD + lane + 64 * e] = o[e];
+        if (lane == 0) { a.pm[2 * row] = m; a.pm[2 * row + 1] = l; }
+    } else {
+        uint8_t *op = a.out + ((size_t)((t.q0 + tok) * a.os) + (size_t)qh * HD) * EQ;
+#pragma unroll
+        for (int e = 0; e < D; e++) qt_store1<QT>(op + (lane + 64 * e) * EQ, l == 0.f ? 0.f : o[e] / l);
+    }
+}
+
+// ---- few rows ------------------------------------------------------------------------------------
+// A workgroup takes one 32-row tile and one range of its keys; its four waves take the range's 32-key blocks in
+// turn, each with a softmax of its own, K and V going from memory into operand registers without LDS or barriers;
+// the waves' sums are merged through LDS at the end, and the ranges' by k_att_merge.
+#define ATT_WV 4
+template <typename QT, typename KT, int HD, bool PAGED>
+__global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))) void k_att_few(AttArgs a) {
+    constexpr bool QF = sizeof(typename QT::elem) == 4, KF = sizeof(typename KT::elem) == 4;
+    constexpr int EQ = sizeof(typename QT::elem), EK = sizeof(typename KT::elem);
+    constexpr int NT = HD / 32, NS = HD / 16, NQ = QF ? 3 : 1, NK = KF ? 3 : 1;
+    constexpr int OB = 32 * HD * 4;                     // one wave's sums
+    __shared__ __align__(16) uint8_t sm[OB * ATT_WV];   // QF: first the queries' planes [plane][32][HD] bf16
+    __shared__ float sst[2][ATT_WV][32];
+    __shared__ __align__(16) long long voff[PAGED ? ATT_WV : 1][32];
+    static_assert(3 * 32 * HD * 2 <= OB * ATT_WV, "the queries' planes and the sums share the LDS");
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
+    const int b = a.tps > 0 ? slot / a.tps : att_find(a, slot);
+    if (b < 0 || b >= a.B) return;
+    int tile = a.tps > 0 ? slot % a.tps : slot - att_first(a, b);
+    const int *table = PAGED ? a.table + b * a.ts : nullptr;
+    for (;; tile += a.tps) {
+    const AttTile t = att_tile<PAGED>(a, b, tile);
+    if (t.r0 >= t.rows) return;
+    const int r = min(t.r0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
+    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 31, t.rows - 1) / a.G;
+    // the queries' operands; step s: dims 16 s + 8 h ..
+    qt_u32x4 qf[NQ == 1 ? NS : 1];
+    if constexpr (QF) {
+        for (int u = tid; u < 32 * (HD / 8); u += 64 * ATT_WV) {
+            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1);
+            float v[8];
+            qt_u32x4 pl[3];
+            qt_load8<QT>(a.q + ((size_t)((t.q0 + rr / a.G) * a.qs) + (size_t)(head * a.G + rr % a.G) * HD + 8 * ch) * EQ, v);
+            qt_planes8(v, pl);
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                *reinterpret_cast<qt_u32x4 *>(sm + (p * 32 + row) * HD * 2 + 16 * (ch ^ (row & (HD / 8 - 1)))) = pl[p];
+        }
+        __syncthreads();
+    } else {
+        const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + 8 * h) * EQ;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + 16 * s * EQ);
+    }
+    // the range's 32-key blocks
+    const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
+    const int kb0 = min((long long)blk1, blk0 + (long long)split * a.chunk), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk);
+    float m = -INFINITY, l = 0.f;                       // l: of this half's keys
+    qt_f32x16 o[NT];
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+    const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD) + 8 * h) * EK;
+    const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + NT * lr) * EK;
+    qt_u32x4 kr[NS][KF ? 2 : 1];
+    uint32_t vr[2][8][NT * EK / 4];
+    int page = PAGED && kb0 + wave < kb1 ? att_page(a, table, t, 32 * (kb0 + wave) + lr) : 0;
+    for (int kb = kb0 + wave; kb < kb1; kb += ATT_WV) {
+        const int key = 32 * kb + lr;
+        uint32_t ok;                                    // keys of the block that exist
+        if constexpr (PAGED) {
+            const long long off = att_slot(a, page, key);
+            ok = (uint32_t)__ballot(page >= 0);
+            __builtin_amdgcn_wave_barrier();
+            if (h == 0) voff[wave][lr] = off;
+            __builtin_amdgcn_wave_barrier();
+            const uint8_t *kp = kbase + off * EK;
+#pragma unroll
+            for (int s = 0; s < NS; s++) kr[s][0] = *reinterpret_cast<const qt_u32x4 *>(kp + 16 * s * EK);
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const uint8_t *vp = vbase + voff[wave][16 * s + 8 * (j >> 2) + 4 * h + (j & 3)] * EK;
+                    __builtin_memcpy(vr[s][j], __builtin_assume_aligned(vp, NT * EK), NT * EK);
+                }
+            page = kb + ATT_WV < kb1 ? att_page(a, table, t, key + 32 * ATT_WV) : 0;
+        } else {
+            ok = key < t.kmax ? 1u : 0u;
+            ok = (uint32_t)__ballot(ok);
+            const uint8_t *kp = kbase + (long long)(t.q0 + min(key, t.kmax - 1)) * a.ks_slot * EK;
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int e = 0; e < (KF ? 2 : 1); e++) kr[s][e] = *reinterpret_cast<const qt_u32x4 *>(kp + 16 * s * EK + 16 * e);
+#pragma unroll
+            for (int s = 0; s < 2; s++)
+#pragma unroll
+                for (int j = 0; j < 8; j++) {
+                    const int vk = min(32 * kb + 16 * s + 8 * (j >> 2) + 4 * h + (j & 3), t.kmax - 1);
+                    const uint8_t *vp = vbase + (long long)(t.q0 + vk) * a.vs_slot * EK;
+                    __builtin_memcpy(vr[s][j], __builtin_assume_aligned(vp, NT * EK), NT * EK);
+                }
+        }
+        qt_f32x16 sc;
+#pragma unroll
+        for (int i = 0; i < 16; i++) sc[i] = 0.f;
+#pragma unroll
+        for (int s = 0; s < NS; s++) {
+            qt_u32x4 ka[NK], qa[NQ];
+            if constexpr (KF) {
+                float v[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = __uint_as_float(kr[s][e >> 2][e & 3]);
+                qt_planes8(v, ka);
+            } else {
+                ka[0] = kr[s][0];
+            }
+#pragma unroll
+            for (int p = 0; p < NQ; p++)
+                if constexpr (QF) qa[p] = qt_lds16(sm + (p * 32 + lr) * HD * 2 + 16 * ((2 * s + h) ^ (lr & (HD / 8 - 1))));
+                else qa[p] = qf[s];
+            sc = att_planes<KT, NK, NQ>(ka, qa, sc);
+        }
+        // hidden keys; a block that every row sees whole needs no look
+        if (!(ok == 0xFFFFFFFFu && 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window))) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                const int j = 8 * (i >> 2) + 4 * h + (i & 3), k = 32 * kb + j;
+                const bool see = k <= pos && (a.window <= 0 || k > pos - a.window) && (ok >> j & 1u);
+                sc[i] = see ? sc[i] : -INFINITY;
+            }
+        }
+        float bm = m;
+#pragma unroll
+        for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[i]);
+        bm = fmaxf(bm, att_other_half(bm));
+        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c;
+        const float f = qt_exp2((m - mr) * a.c);
+        m = bm;
+        float p[16], sum = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            p[i] = qt_exp2(fmaf(sc[i], a.c, -mc));
+            sum += p[i];
+        }
+        l = l * f + sum;
+#pragma unroll
+        for (int d = 0; d < NT; d++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) o[d][i] *= f;
+#pragma unroll
+        for (int s = 0; s < 2; s++) {
+            qt_u32x4 pb[NQ];
+            if constexpr (QF) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = p[8 * s + j];
+                qt_planes8(v, pb);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) pb[0][j] = qt_round2<QT>(p[8 * s + 2 * j], p[8 * s + 2 * j + 1]);
+            }
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                qt_u32x4 va[NK];
+                if constexpr (KF) {
+                    float v[8];
+#pragma unroll
+                    for (int j = 0; j < 8; j++) v[j] = __uint_as_float(vr[s][j][d]);
+                    qt_planes8(v, va);
+                } else {
+#pragma unroll
+                    for (int j = 0; j < 4; j++)
+                        va[0][j] = __builtin_amdgcn_perm(vr[s][2 * j + 1][d >> 1], vr[s][2 * j][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
+                }
+                o[d] = att_planes<KT, NK, NQ>(va, pb, o[d]);
+            }
+        }
+    }
+    l += att_other_half(l);
+    if (h == 0) { sst[0][wave][lr] = m; sst[1][wave][lr] = l; }
+    __syncthreads();                                    // also: the queries' planes are read
+    {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ATT_WV; w++) M = fmaxf(M, sst[0][w][lr]);
+        const float f = M == -INFINITY ? 0.f : qt_exp2((m - M) * a.c);
+        float *os = reinterpret_cast<float *>(sm + wave * OB) + lr * HD;
+#pragma unroll
+        for (int i = 0; i < 16; i++) {
+            const int mm = 8 * (i >> 2) + 4 * h + (i & 3);
+#pragma unroll
+            for (int d = 0; d < NT; d++) os[NT * (mm ^ lr) + d] = o[d][i] * f;
+        }
+    }
+    __syncthreads();
+    bool bad = false;
+    for (int u = tid; u < 32 * 32; u += 64 * ATT_WV) {
+        const int row = u >> 5, mm = u & 31, rr = t.r0 + row;
+        float M = -INFINITY, L = 0.f, v[NT];
+#pragma unroll
+        for (int w = 0; w < ATT_WV; w++) M = fmaxf(M, sst[0][w][row]);
+#pragma unroll
+        for (int d = 0; d < NT; d++) v[d] = 0.f;
+        if (M != -INFINITY)
+#pragma unroll
+            for (int w = 0; w < ATT_WV; w++) L += sst[1][w][row] * qt_exp2((sst[0][w][row] - M) * a.c);
+#pragma unroll
+        for (int w = 0; w < ATT_WV; w++)
+#pragma unroll
+            for (int d = 0; d < NT; d++) v[d] += (reinterpret_cast<const float *>(sm + w * OB) + row * HD)[NT * (mm ^ row) + d];
+        float chk = L;
+#pragma unroll
+        for (int d = 0; d < NT; d++) chk = fmaf(v[d], 0.f, chk);
+        if (rr >= t.rows) continue;
+        bad |= !(chk - chk == 0.f);
+        const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G, at = tk * (a.nkv * a.G) + hd;
+        if (a.splits > 1) {
+            const size_t prow = (size_t)split * a.T * (a.nkv * a.G) + at;
+            att_put<QtF32, NT>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NT * mm), v);
+            if (mm == 0) { a.pm[2 * prow] = M; a.pm[2 * prow + 1] = L; }
+        } else {
+            const float inv = L > 0.f ? 1.0f / L : 0.f;
+#pragma unroll
+            for (int d = 0; d < NT; d++) v[d] *= inv;
+            att_put<QT, NT>(a.out + (tk * a.os + hd * HD + NT * mm) * EQ, v);
+        }
+    }
+    if (__syncthreads_or(bad))
+        for (int row = wave; row < 32 && t.r0 + row < t.rows; row += ATT_WV)
+            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, a.splits > 1, split);
+    if (a.tps <= 0) return;
+    __syncthreads();                                    // the next tile's planes take the LDS
+    }
+}
+
+// A row's ranges under their common maximum: a wave a row, 4 rows a workgroup.  splits <= 64.
+template <typename QT, int HD>
+__global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
+    constexpr int D = HD / 64, EQ = sizeof(typename QT::elem);
+    const int nh = a.nkv * a.G, lane = threadIdx.x & 63;
+    const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long long)a.T * nh;
+    if (at >= rows) return;
+    const int tok = (int)(at / nh), hd = (int)(at % nh);
+    if (tok < att_cu(a, 0) || tok >= att_cu(a, a.B)) return;      // rows of no request stay
+    float m = -INFINITY, l = 0.f;
+    if (lane < a.splits) {
+        m = a.pm[2 * (lane * rows + at)];
+        l = a.pm[2 * (lane * rows + at) + 1];
+    }
+    const float M = group_max<64>(m), f = M == -INFINITY ? 0.f : qt_exp2((m - M) * a.c);
+    const float L = group_sum<64>(l * f);
+    float o[D];
+#pragma unroll
+    for (int e = 0; e < D; e++) o[e] = 0.f;
+    for (int s = 0; s < a.splits; s++) {
+        const float fs = lane_bcast(f, s);
+#pragma unroll
+        for (int e = 0; e < D; e++) o[e] = fmaf(fs, a.po[(s * rows + at) * HD + D * lane + e], o[e]);
+    }
+    const float inv = L == 0.f ? 0.f : 1.0f / L;
+#pragma unroll
+    for (int e = 0; e < D; e++) qt_store1<QT>(a.out + ((size_t)tok * a.os + (size_t)hd * HD + D * lane + e) * EQ, o[e] * inv);
+}
+
+// ---- host side -------------------------------------------------------------------------------------
+
+// launch slots: by request (max_q as far as known) or by rows, whichever is fewer
+static void att_slots(AttArgs &a, int max_q, long long &slots) {
+    const long long by_rows = (long long)a.T * a.G / 32 + a.B;
+    const long long tps = ((long long)max_q * a.G + 31) / 32, by_req = tps * a.B;
+    a.tps = max_q > 0 && by_req <= by_rows ? (int)tps : 0;
+    slots = a.tps > 0 ? by_req : by_rows;
+}
+
+// Key ranges a tile: enough workgroups for two a CU, ranges of 256 keys (two blocks a wave) at least.
+static void att_ranges(AttArgs &a, long long slots, int max_kv) {
+    const long long wgs = slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
+    long long n = (1024 + wgs - 1) / wgs;
+    if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
+    if (n > 64) n = 64;
+    if (n < 1) n = 1;
+    a.splits = (int)n;
+    a.chunk = (int)((blocks + n - 1) / n);
+    if (a.chunk < 1) a.chunk = 1;
+}
+
+static int check_rows(const char *who, int dtype, int n_heads, int nkv, int hd, int B, int T, int window, float scale) {
+    QT_REFUSE(!qt_dt_size(dtype), "%s: dtype %d (f32, bf16 or f16)", who, dtype);
+    QT_REFUSE(hd != 64 && hd != 128, "%s: head_dim %d (64 or 128)", who, hd);
+    QT_REFUSE(nkv < 1 || nkv > 65535 || n_heads < nkv || n_heads % nkv || n_heads / nkv > 64,
+              "%s: %d query heads over %d kv heads (a multiple, 64 a kv head at most)", who, n_heads, nkv);
+    QT_REFUSE(B < 0 || B > 65535, "%s: B %d out of range (0..65535)", who, B);
+    QT_REFUSE(T < 0 || (long long)T * n_heads > 0x3FFFFFFFll, "%s: %d tokens of %d heads (2^30 - 1 rows at most)", who, T, n_heads);
+    QT_REFUSE(window < 0, "%s: window %d is negative", who, window);
+    QT_REFUSE(!(scale > 0.f) || scale > 1e30f, "%s: scale has to be positive and finite", who);
+    return 0;
+}
+
+static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, AttArgs &a, long long &slots) {
+    if (qt_check_pages("page_attention", kv)) return -1;
+    QT_REFUSE(!p, "page_attention: null descriptor");
+    if (check_rows("page_attention", p->dtype, p->n_heads, kv->n_kv_heads, kv->head_dim, p->B, p->T, p->window, p->scale)) return -1;
+    QT_REFUSE(p->dtype == QWEN_HIP_DT_F32 ? kv->dtype != QWEN_HIP_DT_BF16 : p->dtype != kv->dtype,
+              "page_attention: rows of dtype %d over a cache of dtype %d (f32 over bf16, else the cache's own)", p->dtype, kv->dtype);
+    QT_REFUSE(p->max_q < 0 || p->max_kv < 0, "page_attention: max_q %d, max_kv %d", p->max_q, p->max_kv);
+    QT_REFUSE(p->table_cols < 1 || (long long)p->table_cols * kv->page_size > ATT_MAX_KEYS || p->table_stride < p->table_cols,
+              "page_attention: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
+    a = AttArgs{};
+    a.B = p->B; a.T = p->T; a.nkv = kv->n_kv_heads; a.G = p->n_heads / kv->n_kv_heads;
+    att_slots(a, p->max_q < p->T ? p->max_q : p->T, slots);
+    att_ranges(a, slots > 0 ? slots : 1, p->max_kv);
+    return 0;
+}
+
+extern "C" long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p) {
+    AttArgs a;
+    long long slots;
+    if (paged_args(kv, p, a, slots)) return -1;
+    return a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
+}
+
+template <typename QT, typename KT, int HD, bool PAGED>
+static hipError_t att_launch(const AttArgs &a, long long slots, hipStream_t st) {
+    hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), dim3((unsigned)(slots * a.nkv), a.splits), dim3(64 * ATT_WV), 0, st, a);
+    hipError_t e = hipGetLastError();
+    if (e == hipSuccess && a.splits > 1) {
+        const long long rows = (long long)a.T * a.nkv * a.G;
+        hipLaunchKernelGGL((k_att_merge<QT, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
+        e = hipGetLastError();
+    }
+    return e;
+}
+
+extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, void *stream) {
+    AttArgs a;
+    long long slots;
+    if (paged_args(kv, p, a, slots)) return -1;
+    if (p->B == 0 || p->T == 0) return 0;
+    QT_REFUSE(!p->q || !p->out || !p->cu_q || !p->kv_len || !p->table, "page_attention: null pointer");
+    const int A = 16 / qt_dt_size(p->dtype);
+    QT_REFUSE(qt_off16(p->q) || qt_off16(p->out) || qt_off16(p->workspace), "page_attention: pointers have to be aligned to 16 bytes");
+    QT_REFUSE(p->q_stride % A || p->q_stride < 0 || p->out_stride % A || p->out_stride < (long long)p->n_heads * kv->head_dim,
+              "page_attention: strides %lld, %lld (multiples of 16 bytes, out's at least a token's)", p->q_stride, p->out_stride);
+    const long long need = a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
+    QT_REFUSE(need > 0 && (!p->workspace || p->workspace_bytes < need), "page_attention: a workspace of %lld bytes is needed, %lld given",
+              need, p->workspace ? p->workspace_bytes : 0ll);
+    QT_REFUSE(slots * a.nkv > 0x7FFFFFFFll, "page_attention: too many tiles for one launch");
+    hipStream_t st = (hipStream_t)stream;
+    QtOnDevice on(st);
+    QT_REFUSE(on.err != hipSuccess, "page_attention: the stream's device: %s", hipGetErrorString(on.err));
+    a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)kv->k; a.v = (const uint8_t *)kv->v; a.out = (uint8_t *)p->out;
+    a.qs = p->q_stride; a.os = p->out_stride;
+    a.ks_page = kv->page_stride; a.ks_head = kv->head_stride; a.ks_slot = a.vs_slot = kv->slot_stride;
+    a.cu = p->cu_q; a.kv_len = p->kv_len; a.table = p->table; a.ts = p->table_stride;
+    a.cols = p->table_cols; a.n_pages = kv->n_pages; a.ps = kv->page_size; a.div = qt_div_of(kv->page_size);
+    a.window = p->window <= ATT_MAX_KEYS ? p->window : 0;
+    a.c = p->scale * QT_LOG2E;
+    a.po = (float *)p->workspace;
+    a.pm = a.po + (size_t)a.splits * a.T * p->n_heads * kv->head_dim;
+    hipError_t e;
+    if (p->dtype == QWEN_HIP_DT_F32)
+        e = kv->head_dim == 128 ? att_launch<QtF32, QtBf16, 128, true>(a, slots, st) : att_launch<QtF32, QtBf16, 64, true>(a, slots, st);
+    else if (p->dtype == QWEN_HIP_DT_BF16)
+        e = kv->head_dim == 128 ? att_launch<QtBf16, QtBf16, 128, true>(a, slots, st) : att_launch<QtBf16, QtBf16, 64, true>(a, slots, st);
+    else
+        e = kv->head_dim == 128 ? att_launch<QtF16, QtF16, 128, true>(a, slots, st) : att_launch<QtF16, QtF16, 64, true>(a, slots, st);
+    QT_REFUSE(e != hipSuccess, "page_attention: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, void *stream) {
+    QT_REFUSE(!p, "packed_attention: null descriptor");
+    if (check_rows("packed_attention", p->dtype, p->n_heads, p->n_kv_heads, p->head_dim, p->B, p->T, p->window, p->scale)) return -1;
+    if (p->B == 0 || p->T == 0) return 0;
+    QT_REFUSE(!p->q || !p->k || !p->v || !p->out || !p->cu, "packed_attention: null pointer");
+    const int A = 16 / qt_dt_size(p->dtype);
+    QT_REFUSE(qt_off16(p->q) || qt_off16(p->k) || qt_off16(p->v) || qt_off16(p->out), "packed_attention: pointers have to be aligned to 16 bytes");
+    QT_REFUSE(p->q_stride % A || p->k_stride % A || p->v_stride % A || p->out_stride % A || p->q_stride < 0 || p->k_stride < 0 ||
+                  p->v_stride < 0 || p->out_stride < (long long)p->n_heads * p->head_dim,
+              "packed_attention: strides %lld, %lld, %lld, %lld (multiples of 16 bytes, out's at least a token's)", p->q_stride,
+              p->k_stride, p->v_stride, p->out_stride);
+    AttArgs a = {};
+    a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
+    long long slots;
+    att_slots(a, 0, slots);
+    QT_REFUSE(slots * a.nkv > 0x7FFFFFFFll, "packed_attention: too many tiles for one launch");
+    a.splits = 1;
+    a.chunk = 1;
+    a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)p->k; a.v = (const uint8_t *)p->v; a.out = (uint8_t *)p->out;
+    a.qs = p->q_stride; a.os = p->out_stride; a.ks_slot = p->k_stride; a.vs_slot = p->v_stride;
+    a.cu = p->cu;
+    a.window = p->window <= ATT_MAX_KEYS ? p->window : 0;
+    a.c = p->scale * QT_LOG2E;
+    hipStream_t st = (hipStream_t)stream;
+    QtOnDevice on(st);
+    QT_REFUSE(on.err != hipSuccess, "packed_attention: the stream's device: %s", hipGetErrorString(on.err));
+    hipError_t e;
+    if (p->dtype == QWEN_HIP_DT_F32)
+        e = p->head_dim == 128 ? att_launch<QtF32, QtF32, 128, false>(a, slots, st) : att_launch<QtF32, QtF32, 64, false>(a, slots, st);
+    else if (p->dtype == QWEN_HIP_DT_BF16)
+        e = p->head_dim == 128 ? att_launch<QtBf16, QtBf16, 128, false>(a, slots, st) : att_launch<QtBf16, QtBf16, 64, false>(a, slots, st);
+    else
+        e = p->head_dim == 128 ? att_launch<QtF16, QtF16, 128, false>(a, slots, st) : att_launch<QtF16, QtF16, 64, false>(a, slots, st);
+    QT_REFUSE(e != hipSuccess, "packed_attention: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}

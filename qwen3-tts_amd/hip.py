@@ -15,6 +15,9 @@ LIB_PATH = os.path.join(PKG, "libqwen_tts_hip.so")
 
 BF16, INT8, Q4_0 = 0, 1, 2
 PREC = {"bf16": BF16, "int8": INT8, "int4": Q4_0, "q4_0": Q4_0}
+# element types of the paged, batched operators (QWEN_HIP_DT_*)
+DT = {"f32": 0, "bf16": 1, "f16": 2}
+PLAN_NO_PAGES, PLAN_TABLE_FULL, PLAN_TOO_MANY, PLAN_INVALID = 1, 2, 4, 8
 
 # every symbol the header declares (checked by the CPU test suite)
 EXPORTS = [
@@ -42,6 +45,8 @@ EXPORTS = [
     "qwen_hip_sd_latent", "qwen_hip_sd_stream", "qwen_hip_sd_free", "qwen_hip_op_sd_conv",
     "qwen_hip_op_sd_conv_transpose", "qwen_hip_sd_stream_new", "qwen_hip_sd_stream_decode",
     "qwen_hip_sd_stream_reset", "qwen_hip_sd_stream_free",
+    "qwen_hip_op_page_plan", "qwen_hip_op_page_append", "qwen_hip_op_page_attention_workspace",
+    "qwen_hip_op_page_attention", "qwen_hip_op_packed_attention", "qwen_hip_op_logit_rules",
 ]
 
 SD_GET_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.c_char_p, C.c_longlong)
@@ -76,6 +81,50 @@ class CpDesc(C.Structure):
 class SampleParams(C.Structure):
     _fields_ = [("temperature", C.c_float), ("top_k", C.c_int), ("top_p", C.c_float), ("rep_penalty", C.c_float),
                 ("greedy_warmup", C.c_int), ("text_len", C.c_int)]
+
+
+# The descriptors of the paged, batched operators: addresses are device memory (a torch tensor's data_ptr()).
+
+class KvPages(C.Structure):
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_longlong), ("head_stride", C.c_longlong),
+                ("slot_stride", C.c_longlong), ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+
+
+class PagePlan(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("new_len", "kv_len", "n_free", "table", "free_pages", "kv_len_out", "n_free_out",
+                                          "cu_q", "pos", "slot", "status")] + \
+               [("table_stride", C.c_longlong)] + \
+               [(n, C.c_int) for n in ("B", "page_size", "n_pages", "table_cols", "max_tokens")]
+
+
+class PageAppend(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "q_out")] + \
+               [(n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "q_out_stride")] + \
+               [(n, C.c_void_p) for n in ("q_norm", "k_norm", "rope_cos", "rope_sin", "pos", "slot")] + \
+               [(n, C.c_int) for n in ("dtype", "n_heads", "T", "rope_len")] + [("eps", C.c_float)]
+
+
+class PageAttn(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("out", C.c_void_p), ("q_stride", C.c_longlong), ("out_stride", C.c_longlong),
+                ("cu_q", C.c_void_p), ("kv_len", C.c_void_p), ("table", C.c_void_p), ("table_stride", C.c_longlong),
+                ("workspace", C.c_void_p), ("workspace_bytes", C.c_longlong)] + \
+               [(n, C.c_int) for n in ("dtype", "n_heads", "B", "T", "table_cols", "max_q", "max_kv", "window")] + \
+               [("scale", C.c_float)]
+
+
+class PackedAttn(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("q", "k", "v", "out")] + \
+               [(n, C.c_longlong) for n in ("q_stride", "k_stride", "v_stride", "out_stride")] + [("cu", C.c_void_p)] + \
+               [(n, C.c_int) for n in ("dtype", "n_heads", "n_kv_heads", "head_dim", "B", "T", "window")] + \
+               [("scale", C.c_float)]
+
+
+class LogitRules(C.Structure):
+    _fields_ = [("logits", C.c_void_p), ("out", C.c_void_p), ("logits_stride", C.c_longlong), ("out_stride", C.c_longlong)] + \
+               [(n, C.c_void_p) for n in ("hist", "hist_off", "n_prompt", "rep", "presence", "frequency", "bias_tok", "bias_val",
+                                          "bias_off", "mask")] + \
+               [("mask_stride", C.c_longlong)] + [(n, C.c_int) for n in ("dtype", "B", "V", "hist_cap", "bias_cap", "rep_each")]
 
 
 def _p(a):
@@ -188,6 +237,16 @@ def lib():
         L.qwen_hip_sd_stream_decode.argtypes = [vp, vp, i, vp, i]; L.qwen_hip_sd_stream_decode.restype = i
         L.qwen_hip_sd_stream_reset.argtypes = [vp]; L.qwen_hip_sd_stream_reset.restype = i
         L.qwen_hip_sd_stream_free.argtypes = [vp]
+        L.qwen_hip_op_page_plan.argtypes = [C.POINTER(PagePlan), vp]; L.qwen_hip_op_page_plan.restype = i
+        L.qwen_hip_op_page_append.argtypes = [C.POINTER(KvPages), C.POINTER(PageAppend), vp]
+        L.qwen_hip_op_page_append.restype = i
+        L.qwen_hip_op_page_attention_workspace.argtypes = [C.POINTER(KvPages), C.POINTER(PageAttn)]
+        L.qwen_hip_op_page_attention_workspace.restype = C.c_longlong
+        L.qwen_hip_op_page_attention.argtypes = [C.POINTER(KvPages), C.POINTER(PageAttn), vp]
+        L.qwen_hip_op_page_attention.restype = i
+        L.qwen_hip_op_packed_attention.argtypes = [C.POINTER(PackedAttn), vp]
+        L.qwen_hip_op_packed_attention.restype = i
+        L.qwen_hip_op_logit_rules.argtypes = [C.POINTER(LogitRules), vp]; L.qwen_hip_op_logit_rules.restype = i
         _lib = L
     return _lib
 
