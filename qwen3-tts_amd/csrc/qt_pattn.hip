@@ -28,6 +28,7 @@
 // that have no planes (infinite, NaN, past bf16's range after rounding).
 #include "qt_ops.h"
 #include "qt_planes.h"
+#include <type_traits>
 
 typedef float qt_f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 qt_f16x8 __attribute__((ext_vector_type(8)));
@@ -73,18 +74,20 @@ __device__ __forceinline__ float att_other_half(float v) {
     return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-// The request that a launch slot belongs to when a request begins at slot floor(first row / 32) + b: tiles
-// ceil(rows / 32) fit before the next one's, whatever the lengths, so floor(all rows / 32) + B slots are enough for
-// the host, which does not know them.  One load and ballot per 64 requests.
+// The request that a launch slot belongs to when a request begins at slot floor(first row / TR) + b, TR rows a tile:
+// its ceil(rows / TR) tiles fit before the next one's, whatever the lengths, so floor(all rows / TR) + B slots are
+// enough for the host, which does not know them.  One load and ballot per 64 requests.
 // Offsets are the caller's: one out of range is brought into it, so that nothing is read or written past T.
 __device__ __forceinline__ int att_cu(const AttArgs &a, int b) { return min(max(a.cu[b], 0), a.T); }
-__device__ __forceinline__ int att_first(const AttArgs &a, int b) { return (int)((long long)att_cu(a, b) * a.G / 32) + b; }
-__device__ __forceinline__ int att_find(const AttArgs &a, int slot) {
+template <int TR> __device__ __forceinline__ int att_first(const AttArgs &a, int b) {
+    return (int)((long long)att_cu(a, b) * a.G / TR) + b;
+}
+template <int TR> __device__ __forceinline__ int att_find(const AttArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
     int b = -1;
     for (int base = 0; base < a.B; base += 64) {
         const int i = base + lane;
-        const bool before = i < a.B && att_first(a, i) <= slot;
+        const bool before = i < a.B && att_first<TR>(a, i) <= slot;
         const int n = __popcll(__ballot(before));
         b += n;
         if (n < 64) break;
@@ -98,17 +101,17 @@ struct AttTile {
     int shift, kmax;            // a token's position is shift + its place; keys at or past kmax do not exist
     int lo, hi;                 // keys that some row of the tile may see
 };
-template <bool PAGED>
+template <int TR, bool PAGED>
 __device__ __forceinline__ AttTile att_tile(const AttArgs &a, int b, int tile) {
     AttTile t;
     t.q0 = att_cu(a, b);
     const int n = max(att_cu(a, b + 1) - t.q0, 0);
     t.rows = n * a.G;
-    t.r0 = 32 * tile;
+    t.r0 = TR * tile;
     const int kv = PAGED ? min(max(a.kv_len[b], 0), ATT_MAX_KEYS) : n;
     t.kmax = PAGED ? min(kv, a.cols * a.ps) : n;
     t.shift = kv - n;
-    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 31, t.rows - 1) / a.G;
+    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + TR - 1, t.rows - 1) / a.G;
     t.lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
     t.hi = min(t.kmax, last + 1);
     return t;
@@ -122,6 +125,14 @@ __device__ __forceinline__ int att_page(const AttArgs &a, const int *table, cons
 }
 __device__ __forceinline__ long long att_slot(const AttArgs &a, int page, int key) {
     return page < 0 ? 0 : page * a.ks_page + (key - qt_quot(key, a.div) * a.ps) * a.ks_slot;
+}
+
+// A key that does not exist takes the place of one in its block that does (`ok`, not 0 in any block that is worked on unless
+// its pages are bad): places that nobody has written may hold NaN, which would send the tile to att_serial.
+__device__ __forceinline__ long long att_instead(long long off, bool mine, unsigned long long ok) {
+    const int from = ok ? __ffsll((unsigned long long)ok) - 1 : 0;
+    const int lo = __builtin_amdgcn_readlane((int)off, from), hi = __builtin_amdgcn_readlane((int)(off >> 32), from);
+    return mine ? off : (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
 }
 
 // Writes NT elements of a row's output, dim NT m.
@@ -186,6 +197,9 @@ __device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const in
     }
 }
 
+// Waits for the wave's stores: what it writes next to the same places comes after them.
+__device__ __forceinline__ void att_stored() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
 // ---- few rows ------------------------------------------------------------------------------------
 // A workgroup takes one 32-row tile and one range of its keys; its four waves take the range's 32-key blocks in
 // turn, each with a softmax of its own, K and V going from memory into operand registers without LDS or barriers;
@@ -203,12 +217,12 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     static_assert(3 * 32 * HD * 2 <= OB * ATT_WV, "the queries' planes and the sums share the LDS");
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
-    const int b = a.tps > 0 ? slot / a.tps : att_find(a, slot);
+    const int b = a.tps > 0 ? slot / a.tps : att_find<32>(a, slot);
     if (b < 0 || b >= a.B) return;
-    int tile = a.tps > 0 ? slot % a.tps : slot - att_first(a, b);
+    int tile = a.tps > 0 ? slot % a.tps : slot - att_first<32>(a, b);
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
     for (;; tile += a.tps) {
-    const AttTile t = att_tile<PAGED>(a, b, tile);
+    const AttTile t = att_tile<32, PAGED>(a, b, tile);
     if (t.r0 >= t.rows) return;
     const int r = min(t.r0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
     const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 31, t.rows - 1) / a.G;
@@ -249,8 +263,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         const int key = 32 * kb + lr;
         uint32_t ok;                                    // keys of the block that exist
         if constexpr (PAGED) {
-            const long long off = att_slot(a, page, key);
             ok = (uint32_t)__ballot(page >= 0);
+            const long long off = att_instead(att_slot(a, page, key), page >= 0, ok);
             __builtin_amdgcn_wave_barrier();
             if (h == 0) voff[wave][lr] = off;
             __builtin_amdgcn_wave_barrier();
@@ -415,6 +429,210 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     }
 }
 
+// ---- many rows -----------------------------------------------------------------------------------
+// A workgroup takes 128 rows, 32 a wave, and goes through its keys 64 at a time: K and V of a block are copied from
+// memory straight into LDS (no registers), two blocks deep, one barrier a block, and every wave reads both
+// operands from there.  16-bit types only.
+//   K, row k: 16-byte chunk c at place c ^ swk(k): the 16 lanes of a phase of a wave's read (16 rows, one chunk)
+//   fall on 16 different groups of banks.  V: chunk c at place c ^ swv(k): a transposing read takes 4 rows by 64 bytes
+//   a half-wave, which fall on different banks.
+template <int HD> __device__ __forceinline__ int att_swk(int row) { return HD == 128 ? row & 15 : (row >> 1) & 7; }
+template <int HD> __device__ __forceinline__ int att_swv(int row) { return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
+
+// 16 bytes a lane from memory to LDS at dst + 16 lane (dst uniform), as assembly: the compiler, which would take
+// every later LDS read for a reader of these bytes, does not wait for them; att_wait does.
+__device__ __forceinline__ void att_copy16(const uint8_t *src, void *dst) {
+    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst);
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+}
+__device__ __forceinline__ void att_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+template <typename T, int HD, bool PAGED>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_att_tile(AttArgs a) {
+    constexpr int NT = HD / 32, NS = HD / 16, RB = 2 * HD, CPR = RB / 16, RPC = 64 / CPR, NC = 64 / RPC / 4;
+    __shared__ __align__(16) uint8_t sk[2 * 64 * RB], sv[2 * 64 * RB];
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
+    const int head = blockIdx.x % a.nkv, slot = gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv, split = blockIdx.y;   // long tiles first
+    const int b = a.tps > 0 ? slot / a.tps : att_find<128>(a, slot);
+    if (b < 0 || b >= a.B) return;
+    int tile = a.tps > 0 ? slot % a.tps : slot - att_first<128>(a, b);
+    const int *table = PAGED ? a.table + b * a.ts : nullptr;
+    // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4
+    int ka[NS], va[NT];
+#pragma unroll
+    for (int s = 0; s < NS; s++) ka[s] = lr * RB + 16 * ((2 * s + h) ^ att_swk<HD>(lr));
+    {
+        const int i = lane & 15, row = 4 * h + (i >> 2);
+#pragma unroll
+        for (int d = 0; d < NT; d++)
+            va[d] = row * RB + 16 * ((4 * d + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ att_swv<HD>(row)) + 8 * (i & 1);
+    }
+    for (;; tile += a.tps) {
+    const AttTile t = att_tile<128, PAGED>(a, b, tile);
+    if (t.r0 >= t.rows) return;
+    const int w0 = t.r0 + 32 * wave, r = min(w0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
+    // the wave's first and last position; last < first: no rows
+    const int first = t.shift + min(w0, t.rows - 1) / a.G, last = w0 < t.rows ? t.shift + min(w0 + 31, t.rows - 1) / a.G : -1;
+    qt_u32x4 qf[NS];
+    {
+        const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + 8 * h) * 2;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + 32 * s);
+    }
+    // the range's 64-key blocks; chunk is in blocks of 32, even
+    const int blk0 = t.lo / 64, blk1 = t.hi > t.lo ? (t.hi + 63) / 64 : blk0;
+    const int kb0 = min((long long)blk1, blk0 + (long long)split * (a.chunk / 2)), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk / 2);
+    float m = -INFINITY, l = 0.f;                       // l: of this half's keys
+    qt_f32x16 o[NT];
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) o[d][i] = 0.f;
+    const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD)) * 2;
+    const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD)) * 2;
+    const int crow = wave * NC * RPC + lane / CPR, cc = lane % CPR;      // this lane's row and place in the first copy
+    int page = -1;                                                       // of key 64 kb + lane, the block to copy next
+    unsigned long long ok = 0, okn = 0;                                  // keys of a block that exist: this one's, the next one's
+    const auto copy = [&](int kb, int buf) {
+        if constexpr (PAGED) {
+            okn = __ballot(page >= 0);
+            const long long off = 2 * att_instead(att_slot(a, page, 64 * kb + lane), page >= 0, okn);
+            const int lo = (int)off, hi = (int)(off >> 32);
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int row = crow + i * RPC;
+                const long long at = ((long long)__shfl(hi, row) << 32) | (unsigned)__shfl(lo, row);
+                att_copy16(kbase + at + 16 * (cc ^ att_swk<HD>(row)), sk + (buf * 64 + (wave * NC + i) * RPC) * RB);
+                att_copy16(vbase + at + 16 * (cc ^ att_swv<HD>(row)), sv + (buf * 64 + (wave * NC + i) * RPC) * RB);
+            }
+        } else {
+            okn = __ballot(64 * kb + lane < t.kmax);
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int row = crow + i * RPC;
+                const long long key = t.q0 + min(64 * kb + row, t.kmax - 1);
+                att_copy16(kbase + key * a.ks_slot * 2 + 16 * (cc ^ att_swk<HD>(row)), sk + (buf * 64 + (wave * NC + i) * RPC) * RB);
+                att_copy16(vbase + key * a.vs_slot * 2 + 16 * (cc ^ att_swv<HD>(row)), sv + (buf * 64 + (wave * NC + i) * RPC) * RB);
+            }
+        }
+    };
+    const auto step = [&](int kb, auto bufc) {
+        constexpr int BUF = decltype(bufc)::value;
+        // this block's copies are in (the wave's own by the wait, the others' by the barrier, which they pass after
+        // theirs), and every wave has left the other buffer
+        att_wait();
+        __syncthreads();
+        ok = okn;
+        if (kb + 1 < kb1) {
+            copy(kb + 1, BUF ^ 1);
+            if (PAGED && kb + 2 < kb1) page = att_page(a, table, t, 64 * (kb + 2) + lane);
+        }
+        if (64 * kb > last || (a.window > 0 && 64 * kb + 63 <= first - a.window)) return;   // nothing for this wave
+        qt_f32x16 sc[2];
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++) {
+#pragma unroll
+            for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+                sc[kt] = att_mma<T>(qt_lds16(sk + BUF * 64 * RB + 32 * kt * RB + ka[s]), qf[s], sc[kt]);
+        }
+        if (!(ok == ~0ull && 64 * kb + 63 <= first && (a.window <= 0 || 64 * kb > last - a.window))) {
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) {
+                    const int j = 32 * kt + 8 * (i >> 2) + 4 * h + (i & 3), k = 64 * kb + j;
+                    const bool see = k <= pos && (a.window <= 0 || k > pos - a.window) && (ok >> j & 1ull);
+                    sc[kt][i] = see ? sc[kt][i] : -INFINITY;
+                }
+        }
+        float bm = m;
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[kt][i]);
+        bm = fmaxf(bm, att_other_half(bm));
+        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c;
+        if (__ballot(bm > m)) {                                          // a row's maximum rose: its sums shrink
+            const float f = qt_exp2((m - mr) * a.c);
+            l *= f;
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+#pragma unroll
+                for (int i = 0; i < 16; i++) o[d][i] *= f;
+        }
+        m = bm;
+        float sum[2] = {0.f, 0.f};
+#pragma unroll
+        for (int kt = 0; kt < 2; kt++)
+#pragma unroll
+            for (int i = 0; i < 16; i++) {
+                sc[kt][i] = qt_exp2(fmaf(sc[kt][i], a.c, -mc));
+                sum[kt] += sc[kt][i];
+            }
+        l += sum[0] + sum[1];
+#pragma unroll
+        for (int s = 0; s < 4; s++) {
+            qt_u32x4 pb;
+#pragma unroll
+            for (int j = 0; j < 4; j++) pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
+#pragma unroll
+            for (int d = 0; d < NT; d++) {
+                const uint16_t *vp = reinterpret_cast<const uint16_t *>(sv + BUF * 64 * RB + 16 * s * RB + va[d]);
+                o[d] = att_mma<T>(qt_lds_tr8x2(vp, vp + 8 * HD), pb, o[d]);
+            }
+        }
+    };
+    if (kb0 < kb1) {
+        if (PAGED) page = att_page(a, table, t, 64 * kb0 + lane);
+        copy(kb0, 0);
+        if (PAGED && kb0 + 1 < kb1) page = att_page(a, table, t, 64 * (kb0 + 1) + lane);
+    }
+    for (int kb = kb0; kb < kb1; kb += 2) {
+        step(kb, std::integral_constant<int, 0>{});
+        if (kb + 1 < kb1) step(kb + 1, std::integral_constant<int, 1>{});
+    }
+    // the rows' results; o[d][i] is dim 32 d + 8 (i / 4) + 4 h + i % 4
+    l += att_other_half(l);
+    float chk = l;
+#pragma unroll
+    for (int d = 0; d < NT; d++)
+#pragma unroll
+        for (int i = 0; i < 16; i++) chk = fmaf(o[d][i], 0.f, chk);
+    const bool live = w0 + lr < t.rows;
+    const size_t tk = t.q0 + tok;
+    if (live) {
+        if (a.splits > 1) {
+            const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + qh;
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<float4 *>(a.po + prow * HD + 32 * d + 8 * i + 4 * h) =
+                        make_float4(o[d][4 * i], o[d][4 * i + 1], o[d][4 * i + 2], o[d][4 * i + 3]);
+            if (h == 0) { a.pm[2 * prow] = m; a.pm[2 * prow + 1] = l; }
+        } else {
+            const float inv = l > 0.f ? 1.0f / l : 0.f;
+            uint8_t *op = a.out + (tk * a.os + (size_t)qh * HD + 4 * h) * 2;
+#pragma unroll
+            for (int d = 0; d < NT; d++)
+#pragma unroll
+                for (int i = 0; i < 4; i++)
+                    *reinterpret_cast<uint2 *>(op + 2 * (32 * d + 8 * i)) =
+                        make_uint2(qt_round2<T>(o[d][4 * i] * inv, o[d][4 * i + 1] * inv), qt_round2<T>(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv));
+        }
+    }
+    if (__ballot(live && !(chk - chk == 0.f))) {
+        att_stored();
+        for (int row = w0; row < min(w0 + 32, t.rows); row++)
+            att_serial<T, T, HD, PAGED>(a, t, table, head, row, 64 * kb0, 64 * kb1, a.splits > 1, split);
+    }
+    if (a.tps <= 0) return;
+    __syncthreads();                                    // the next tile's copies take the LDS
+    }
+}
+
 // A row's ranges under their common maximum: a wave a row, 4 rows a workgroup.  splits <= 64.
 template <typename QT, int HD>
 __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
@@ -446,24 +664,27 @@ __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
 
 // ---- host side -------------------------------------------------------------------------------------
 
-// launch slots: by request (max_q as far as known) or by rows, whichever is fewer
-static void att_slots(AttArgs &a, int max_q, long long &slots) {
-    const long long by_rows = (long long)a.T * a.G / 32 + a.B;
-    const long long tps = ((long long)max_q * a.G + 31) / 32, by_req = tps * a.B;
+// The kernel, its launch slots and key ranges.  Launch slots: by request (max_q as far as known) or by rows, whichever is
+// fewer.  Key ranges: enough workgroups to fill the CUs, 256 keys each at least.
+struct AttPlan { bool tile; long long slots; };
+static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_split) {
+    AttPlan p;
+    // 16-bit rows, 64 a request on average: many rows
+    p.tile = dtype != QWEN_HIP_DT_F32 && (long long)a.T * a.G >= 64ll * a.B;
+    const int tr = p.tile ? 128 : 32;
+    const long long by_rows = (long long)a.T * a.G / tr + a.B;
+    const long long tps = ((long long)max_q * a.G + tr - 1) / tr, by_req = tps * a.B;
     a.tps = max_q > 0 && by_req <= by_rows ? (int)tps : 0;
-    slots = a.tps > 0 ? by_req : by_rows;
-}
-
-// Key ranges a tile: enough workgroups for two a CU, ranges of 256 keys (two blocks a wave) at least.
-static void att_ranges(AttArgs &a, long long slots, int max_kv) {
-    const long long wgs = slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
-    long long n = (1024 + wgs - 1) / wgs;
+    p.slots = a.tps > 0 ? by_req : by_rows;
+    const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
+    long long n = wgs > 0 ? ((p.tile ? 512 : 1024) + wgs - 1) / wgs : 1;
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
-    if (n < 1) n = 1;
+    if (n < 1 || !may_split) n = 1;
     a.splits = (int)n;
-    a.chunk = (int)((blocks + n - 1) / n);
-    if (a.chunk < 1) a.chunk = 1;
+    a.chunk = (int)((blocks + n - 1) / n + 1) & ~1;
+    if (a.chunk < 2) a.chunk = 2;
+    return p;
 }
 
 static int check_rows(const char *who, int dtype, int n_heads, int nkv, int hd, int B, int T, int window, float scale) {
@@ -478,7 +699,7 @@ static int check_rows(const char *who, int dtype, int n_heads, int nkv, int hd, 
     return 0;
 }
 
-static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, AttArgs &a, long long &slots) {
+static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, AttArgs &a, AttPlan &plan) {
     if (qt_check_pages("page_attention", kv)) return -1;
     QT_REFUSE(!p, "page_attention: null descriptor");
     if (check_rows("page_attention", p->dtype, p->n_heads, kv->n_kv_heads, kv->head_dim, p->B, p->T, p->window, p->scale)) return -1;
@@ -489,21 +710,26 @@ static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t 
               "page_attention: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
     a = AttArgs{};
     a.B = p->B; a.T = p->T; a.nkv = kv->n_kv_heads; a.G = p->n_heads / kv->n_kv_heads;
-    att_slots(a, p->max_q < p->T ? p->max_q : p->T, slots);
-    att_ranges(a, slots > 0 ? slots : 1, p->max_kv);
+    plan = att_plan(a, p->dtype, p->max_q < p->T ? p->max_q : p->T, p->max_kv, true);
     return 0;
 }
 
 extern "C" long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p) {
     AttArgs a;
-    long long slots;
-    if (paged_args(kv, p, a, slots)) return -1;
+    AttPlan plan;
+    if (paged_args(kv, p, a, plan)) return -1;
     return a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
 }
 
 template <typename QT, typename KT, int HD, bool PAGED>
-static hipError_t att_launch(const AttArgs &a, long long slots, hipStream_t st) {
-    hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), dim3((unsigned)(slots * a.nkv), a.splits), dim3(64 * ATT_WV), 0, st, a);
+static hipError_t att_launch(const AttArgs &a, const AttPlan &plan, hipStream_t st) {
+    const dim3 grid((unsigned)(plan.slots * a.nkv), a.splits);
+    if constexpr (sizeof(typename QT::elem) == 2) {
+        if (plan.tile) hipLaunchKernelGGL((k_att_tile<QT, HD, PAGED>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
+    } else {
+        hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
+    }
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.splits > 1) {
         const long long rows = (long long)a.T * a.nkv * a.G;
@@ -515,8 +741,8 @@ static hipError_t att_launch(const AttArgs &a, long long slots, hipStream_t st) 
 
 extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, void *stream) {
     AttArgs a;
-    long long slots;
-    if (paged_args(kv, p, a, slots)) return -1;
+    AttPlan plan;
+    if (paged_args(kv, p, a, plan)) return -1;
     if (p->B == 0 || p->T == 0) return 0;
     QT_REFUSE(!p->q || !p->out || !p->cu_q || !p->kv_len || !p->table, "page_attention: null pointer");
     const int A = 16 / qt_dt_size(p->dtype);
@@ -526,7 +752,7 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     const long long need = a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
     QT_REFUSE(need > 0 && (!p->workspace || p->workspace_bytes < need), "page_attention: a workspace of %lld bytes is needed, %lld given",
               need, p->workspace ? p->workspace_bytes : 0ll);
-    QT_REFUSE(slots * a.nkv > 0x7FFFFFFFll, "page_attention: too many tiles for one launch");
+    QT_REFUSE(plan.slots * a.nkv > 0x7FFFFFFFll, "page_attention: too many tiles for one launch");
     hipStream_t st = (hipStream_t)stream;
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_attention: the stream's device: %s", hipGetErrorString(on.err));
@@ -541,11 +767,11 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     a.pm = a.po + (size_t)a.splits * a.T * p->n_heads * kv->head_dim;
     hipError_t e;
     if (p->dtype == QWEN_HIP_DT_F32)
-        e = kv->head_dim == 128 ? att_launch<QtF32, QtBf16, 128, true>(a, slots, st) : att_launch<QtF32, QtBf16, 64, true>(a, slots, st);
+        e = kv->head_dim == 128 ? att_launch<QtF32, QtBf16, 128, true>(a, plan, st) : att_launch<QtF32, QtBf16, 64, true>(a, plan, st);
     else if (p->dtype == QWEN_HIP_DT_BF16)
-        e = kv->head_dim == 128 ? att_launch<QtBf16, QtBf16, 128, true>(a, slots, st) : att_launch<QtBf16, QtBf16, 64, true>(a, slots, st);
+        e = kv->head_dim == 128 ? att_launch<QtBf16, QtBf16, 128, true>(a, plan, st) : att_launch<QtBf16, QtBf16, 64, true>(a, plan, st);
     else
-        e = kv->head_dim == 128 ? att_launch<QtF16, QtF16, 128, true>(a, slots, st) : att_launch<QtF16, QtF16, 64, true>(a, slots, st);
+        e = kv->head_dim == 128 ? att_launch<QtF16, QtF16, 128, true>(a, plan, st) : att_launch<QtF16, QtF16, 64, true>(a, plan, st);
     QT_REFUSE(e != hipSuccess, "page_attention: launch failed: %s", hipGetErrorString(e));
     return 0;
 }
@@ -563,11 +789,8 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
               p->k_stride, p->v_stride, p->out_stride);
     AttArgs a = {};
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
-    long long slots;
-    att_slots(a, 0, slots);
-    QT_REFUSE(slots * a.nkv > 0x7FFFFFFFll, "packed_attention: too many tiles for one launch");
-    a.splits = 1;
-    a.chunk = 1;
+    const AttPlan plan = att_plan(a, p->dtype, 0, 0, false);
+    QT_REFUSE(plan.slots * a.nkv > 0x7FFFFFFFll, "packed_attention: too many tiles for one launch");
     a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)p->k; a.v = (const uint8_t *)p->v; a.out = (uint8_t *)p->out;
     a.qs = p->q_stride; a.os = p->out_stride; a.ks_slot = p->k_stride; a.vs_slot = p->v_stride;
     a.cu = p->cu;
@@ -578,11 +801,11 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
     QT_REFUSE(on.err != hipSuccess, "packed_attention: the stream's device: %s", hipGetErrorString(on.err));
     hipError_t e;
     if (p->dtype == QWEN_HIP_DT_F32)
-        e = p->head_dim == 128 ? att_launch<QtF32, QtF32, 128, false>(a, slots, st) : att_launch<QtF32, QtF32, 64, false>(a, slots, st);
+        e = p->head_dim == 128 ? att_launch<QtF32, QtF32, 128, false>(a, plan, st) : att_launch<QtF32, QtF32, 64, false>(a, plan, st);
     else if (p->dtype == QWEN_HIP_DT_BF16)
-        e = p->head_dim == 128 ? att_launch<QtBf16, QtBf16, 128, false>(a, slots, st) : att_launch<QtBf16, QtBf16, 64, false>(a, slots, st);
+        e = p->head_dim == 128 ? att_launch<QtBf16, QtBf16, 128, false>(a, plan, st) : att_launch<QtBf16, QtBf16, 64, false>(a, plan, st);
     else
-        e = p->head_dim == 128 ? att_launch<QtF16, QtF16, 128, false>(a, slots, st) : att_launch<QtF16, QtF16, 64, false>(a, slots, st);
+        e = p->head_dim == 128 ? att_launch<QtF16, QtF16, 128, false>(a, plan, st) : att_launch<QtF16, QtF16, 64, false>(a, plan, st);
     QT_REFUSE(e != hipSuccess, "packed_attention: launch failed: %s", hipGetErrorString(e));
     return 0;
 }

@@ -457,6 +457,17 @@ def test_page_attention_chunks(t, kv, nh, nkv, hd, page, layout, window):
 
 
 @pytest.mark.parametrize("t,kv", KINDS)
+@pytest.mark.parametrize("nh,nkv,hd,page,layout,window", [(16, 8, 128, 16, "head", 0), (16, 16, 64, 24, "slot", 72), (8, 4, 64, 64, "head", 5),
+                                                          (6, 2, 128, 3, "slot", 300)])
+def test_page_attention_long_chunks(t, kv, nh, nkv, hd, page, layout, window):
+    """Chunks of many rows: whole tiles, the first and last rows of tiles, keys that end inside a block."""
+    print(f"[case] paged long chunks {t} {nh}/{nkv}x{hd} page={page} {layout} window={window}", flush=True)
+    reqs = [(0, 257), (63, 128), (300, 64), (1, 0), (0, 191), (128, 129)]
+    Paged(reqs, nh, nkv, hd, t, kv, page, layout, seed=14, window=window).check()
+    Paged(reqs, nh, nkv, hd, t, kv, page, layout, seed=14, window=window, max_q=20, max_kv=6000).check()
+
+
+@pytest.mark.parametrize("t,kv", KINDS)
 def test_page_attention_many_requests_and_padding(t, kv):
     """More requests than a ballot looks at, empty ones among them, and rows behind the last one."""
     reqs = [((b * 37) % 90, (b * 5) % 4 * (b % 3)) for b in range(150)]
@@ -487,10 +498,11 @@ def test_rows_that_see_nothing_are_zero(t, kv):
 
 @pytest.mark.parametrize("t,kv", KINDS)
 @pytest.mark.parametrize("value", [math.nan, math.inf, -math.inf])
-def test_hidden_values_never_reach_a_row(t, kv, value):
+@pytest.mark.parametrize("nh,nkv,hd", [(4, 2, 64), (16, 2, 128)])
+def test_hidden_values_never_reach_a_row(t, kv, value, nh, nkv, hd):
     """Keys and values that only later rows see hold NaN or infinities: the earlier rows do not change."""
     reqs = [(40, 50), (2000, 6)]
-    p = Paged(reqs, 4, 2, 64, t, kv, 16, "head", seed=9)
+    p = Paged(reqs, nh, nkv, hd, t, kv, 16, "head", seed=9)
     exact, mag = p.want()
     for b, bad in ((0, 70), (1, 2003)):
         pg = int(p.table[b, bad // 16])
@@ -578,7 +590,8 @@ def packed_want(rows, lens, nh, nkv, hd, window):
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("nh,nkv,hd,lens,window", [
     (16, 8, 128, [1], 0), (16, 8, 128, [45, 1, 128, 0, 33], 0), (16, 16, 64, [200, 31, 32, 64, 65], 72), (12, 2, 64, [301, 17], 0),
-    (7, 1, 128, [100, 0, 0, 50], 30), (32, 4, 128, [513], 0), (4, 2, 64, [3] * 130 + [0] * 20 + [40], 0), (16, 8, 128, [600, 90], 1000)])
+    (7, 1, 128, [100, 0, 0, 50], 30), (32, 4, 128, [513], 0), (4, 2, 64, [3] * 130 + [0] * 20 + [40], 0), (16, 8, 128, [600, 90], 1000),
+    (16, 8, 128, [129, 63, 64, 65, 0, 1, 256], 0), (6, 2, 64, [43, 171, 300], 65)])
 def test_packed_attention(t, nh, nkv, hd, lens, window):
     print(f"[case] packed {t} {nh}/{nkv}x{hd} {lens[:6]} window={window}", flush=True)
     g = torch.Generator().manual_seed(len(lens) + hd)
