@@ -95,6 +95,56 @@ template <int TR> __device__ __forceinline__ int att_find(const AttArgs &a, int 
     return b;
 }
 
+// The tile of 128 rows that comes at `slot` when all requests' tiles are in the order of their keys, longest first: few
+// workgroups are left over at the end, and the long ones share a CU with short ones.  Tile i of a request weighs s + i, s
+// the keys before its new tokens in tiles' measure; how many tiles weigh w or more is a sum over the requests (four a lane), and
+// a search by halves finds the weight that holds the slot: under half a us for 64 requests and 8192 keys.  False: no tile.
+#define ATT_SORT_B 256
+template <bool PAGED> __device__ __forceinline__ bool att_longest(const AttArgs &a, int slot, int &b, int &tile) {
+    const int lane = threadIdx.x & 63;
+    int n[4], s[4], top = 0;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const int i = 64 * r + lane;
+        n[r] = s[r] = 0;
+        if (i < a.B) {
+            const int q0 = att_cu(a, i), len = max(att_cu(a, i + 1) - q0, 0);
+            n[r] = (len * a.G + 127) / 128;
+            if (PAGED) s[r] = (int)((long long)max(min(a.kv_len[i], ATT_MAX_KEYS) - len, 0) * a.G / 128);
+            top = max(top, s[r] + n[r]);
+        }
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+    const auto heavier = [&](int w) {                   // tiles of weight w or more
+        int c = 0;
+#pragma unroll
+        for (int r = 0; r < 4; r++) c += n[r] - min(max(w - s[r], 0), n[r]);
+        return group_sum_i<64>(c);
+    };
+    if (heavier(0) <= slot) return false;
+    int lo = 0, hi = top, over = 0;                     // heavier(lo) > slot >= heavier(hi) = over
+    while (hi - lo > 1) {
+        const int mid = lo + (hi - lo) / 2, c = heavier(mid);
+        if (c > slot) lo = mid; else { hi = mid; over = c; }
+    }
+    int k = slot - over;                                // the k-th request with a tile of this weight
+    b = -1;
+#pragma unroll
+    for (int r = 0; r < 4; r++) {
+        const unsigned long long has = __ballot(s[r] <= lo && lo < s[r] + n[r]);
+        const int c = __popcll(has);
+        if (b < 0 && k < c) {
+            const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
+            const int at = __ffsll((unsigned long long)__ballot((has >> lane & 1) && before == k)) - 1;
+            b = 64 * r + at;
+            tile = lo - __builtin_amdgcn_readlane(s[r], at);
+        }
+        k -= c;
+    }
+    return b >= 0;
+}
+
 // one tile's geometry, uniform over the workgroup
 struct AttTile {
     int q0, rows, r0;           // first token of the request, its rows, the tile's first row
@@ -318,11 +368,12 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         }
         // hidden keys; a block that every row sees whole needs no look
         if (!(ok == 0xFFFFFFFFu && 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window))) {
+            const int d = pos - 32 * kb - 4 * h, w = a.window > 0 ? d - a.window : -1000;
+            const uint32_t mine = ok >> (4 * h);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
-                const int j = 8 * (i >> 2) + 4 * h + (i & 3), k = 32 * kb + j;
-                const bool see = k <= pos && (a.window <= 0 || k > pos - a.window) && (ok >> j & 1u);
-                sc[i] = see ? sc[i] : -INFINITY;
+                const int j = 8 * (i >> 2) + (i & 3);
+                sc[i] = j <= d && j > w && (mine >> j & 1u) ? sc[i] : -INFINITY;
             }
         }
         float bm = m;
@@ -412,7 +463,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G, at = tk * (a.nkv * a.G) + hd;
         if (a.splits > 1) {
             const size_t prow = (size_t)split * a.T * (a.nkv * a.G) + at;
-            att_put<QtF32, NT>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NT * mm), v);
+            if (kb0 < kb1) att_put<QtF32, NT>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NT * mm), v);
             if (mm == 0) { a.pm[2 * prow] = M; a.pm[2 * prow + 1] = L; }
         } else {
             const float inv = L > 0.f ? 1.0f / L : 0.f;
@@ -440,22 +491,35 @@ template <int HD> __device__ __forceinline__ int att_swk(int row) { return HD ==
 template <int HD> __device__ __forceinline__ int att_swv(int row) { return HD == 128 ? 4 * (row & 3) : 4 * ((row >> 1) & 1); }
 
 // 16 bytes a lane from memory to LDS at dst + 16 lane (dst uniform), as assembly: the compiler, which would take
-// every later LDS read for a reader of these bytes, does not wait for them; att_wait does.
+// every later LDS read for a reader of these bytes, does not wait for them; att_wait does.  The second form reads at
+// base + off, base uniform.
+__device__ __forceinline__ unsigned att_lds(void *dst) {
+    return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst);
+}
 __device__ __forceinline__ void att_copy16(const uint8_t *src, void *dst) {
-    const unsigned lds = __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst);
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(lds) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(att_lds(dst)) : "memory", "m0");
+}
+__device__ __forceinline__ void att_copy16(const uint8_t *base, unsigned off, void *dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(att_lds(dst)) : "memory", "m0");
 }
 __device__ __forceinline__ void att_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 template <typename T, int HD, bool PAGED>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_att_tile(AttArgs a) {
     constexpr int NT = HD / 32, NS = HD / 16, RB = 2 * HD, CPR = RB / 16, RPC = 64 / CPR, NC = 64 / RPC / 4;
-    __shared__ __align__(16) uint8_t sk[2 * 64 * RB], sv[2 * 64 * RB];
+    __shared__ __align__(16) uint8_t sk[2 * 64 * RB], sv[3 * 64 * RB];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
-    const int head = blockIdx.x % a.nkv, slot = gridDim.x / a.nkv - 1 - blockIdx.x / a.nkv, split = blockIdx.y;   // long tiles first
-    const int b = a.tps > 0 ? slot / a.tps : att_find<128>(a, slot);
-    if (b < 0 || b >= a.B) return;
-    int tile = a.tps > 0 ? slot % a.tps : slot - att_first<128>(a, b);
+    const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
+    int b, tile;
+    if (a.B <= ATT_SORT_B) {
+        if (!att_longest<PAGED>(a, slot, b, tile)) return;
+    } else {
+        b = att_find<128>(a, slot);
+        if (b < 0) return;
+        tile = slot - att_first<128>(a, b);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    tile = __builtin_amdgcn_readfirstlane(tile);
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
     // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4
     int ka[NS], va[NT];
@@ -467,12 +531,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int d = 0; d < NT; d++)
             va[d] = row * RB + 16 * ((4 * d + 2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ att_swv<HD>(row)) + 8 * (i & 1);
     }
-    for (;; tile += a.tps) {
+    // where this lane's copies read: row crow + i RPC of a block, and the chunk that belongs at its place
+    const int crow = wave * NC * RPC + lane / CPR, cc = lane % CPR;
     const AttTile t = att_tile<128, PAGED>(a, b, tile);
     if (t.r0 >= t.rows) return;
     const int w0 = t.r0 + 32 * wave, r = min(w0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
-    // the wave's first and last position; last < first: no rows
-    const int first = t.shift + min(w0, t.rows - 1) / a.G, last = w0 < t.rows ? t.shift + min(w0 + 31, t.rows - 1) / a.G : -1;
+    // the wave's first and last position
+    const int first = t.shift + min(w0, t.rows - 1) / a.G, last = t.shift + min(w0 + 31, t.rows - 1) / a.G;
     qt_u32x4 qf[NS];
     {
         const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + 8 * h) * 2;
@@ -482,87 +547,100 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     // the range's 64-key blocks; chunk is in blocks of 32, even
     const int blk0 = t.lo / 64, blk1 = t.hi > t.lo ? (t.hi + 63) / 64 : blk0;
     const int kb0 = min((long long)blk1, blk0 + (long long)split * (a.chunk / 2)), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk / 2);
-    float m = -INFINITY, l = 0.f;                       // l: of this half's keys
+    float m = -INFINITY, l = 0.f;                       // m: the maximum so far, or up to 2^8 under it; l: of this half's keys
     qt_f32x16 o[NT];
 #pragma unroll
     for (int d = 0; d < NT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-    const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD)) * 2;
-    const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD)) * 2;
-    const int crow = wave * NC * RPC + lane / CPR, cc = lane % CPR;      // this lane's row and place in the first copy
-    int page = -1;                                                       // of key 64 kb + lane, the block to copy next
-    unsigned long long ok = 0, okn = 0;                                  // keys of a block that exist: this one's, the next one's
-    const auto copy = [&](int kb, int buf) {
+    const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD) + (PAGED ? 0 : t.q0 * a.ks_slot)) * 2;
+    const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + (PAGED ? 0 : t.q0 * a.vs_slot)) * 2;
+    int page = -1;                                                       // PAGED: of key 64 kb + lane, block kb the next to copy
+    unsigned long long okv = ~0ull, okk = ~0ull, okn = ~0ull;            // keys that exist: of the block of V, of K, of the next K
+    // block kb to a K and a V buffer
+    const auto copy = [&](int kb, uint8_t *kdst, uint8_t *vdst) {
+        long long off = 0;
+        int place = cc;
         if constexpr (PAGED) {
+            asm volatile("" : "+v"(place));              // addresses are formed here: held over the loop they cost 20 registers
             okn = __ballot(page >= 0);
-            const long long off = 2 * att_instead(att_slot(a, page, 64 * kb + lane), page >= 0, okn);
-            const int lo = (int)off, hi = (int)(off >> 32);
+            off = 2 * att_instead(att_slot(a, page, 64 * kb + lane), page >= 0, okn);
+        }
 #pragma unroll
-            for (int i = 0; i < NC; i++) {
-                const int row = crow + i * RPC;
-                const long long at = ((long long)__shfl(hi, row) << 32) | (unsigned)__shfl(lo, row);
-                att_copy16(kbase + at + 16 * (cc ^ att_swk<HD>(row)), sk + (buf * 64 + (wave * NC + i) * RPC) * RB);
-                att_copy16(vbase + at + 16 * (cc ^ att_swv<HD>(row)), sv + (buf * 64 + (wave * NC + i) * RPC) * RB);
-            }
-        } else {
-            okn = __ballot(64 * kb + lane < t.kmax);
-#pragma unroll
-            for (int i = 0; i < NC; i++) {
-                const int row = crow + i * RPC;
-                const long long key = t.q0 + min(64 * kb + row, t.kmax - 1);
-                att_copy16(kbase + key * a.ks_slot * 2 + 16 * (cc ^ att_swk<HD>(row)), sk + (buf * 64 + (wave * NC + i) * RPC) * RB);
-                att_copy16(vbase + key * a.vs_slot * 2 + 16 * (cc ^ att_swv<HD>(row)), sv + (buf * 64 + (wave * NC + i) * RPC) * RB);
+        for (int i = 0; i < NC; i++) {
+            const int row = crow + i * RPC, ck = 16 * (place ^ att_swk<HD>(row)), cv = 16 * (place ^ att_swv<HD>(row));
+            const int to = (wave * NC + i) * RPC * RB;
+            if constexpr (PAGED) {
+                const long long at = ((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row);
+                att_copy16(kbase + at + ck, kdst + to);
+                att_copy16(vbase + at + cv, vdst + to);
+            } else {
+                const int real = min(row, t.kmax - 1 - 64 * kb);         // rows past the sequence: its last one again
+                att_copy16(kbase + 64ll * kb * a.ks_slot * 2, (unsigned)(real * (int)a.ks_slot * 2 + ck), kdst + to);
+                att_copy16(vbase + 64ll * kb * a.vs_slot * 2, (unsigned)(real * (int)a.vs_slot * 2 + cv), vdst + to);
             }
         }
+        if (PAGED) page = kb + 1 < kb1 ? att_page(a, table, t, 64 * (kb + 1) + lane) : -1;
     };
-    const auto step = [&](int kb, auto bufc) {
-        constexpr int BUF = decltype(bufc)::value;
-        // this block's copies are in (the wave's own by the wait, the others' by the barrier, which they pass after
-        // theirs), and every wave has left the other buffer
-        att_wait();
-        __syncthreads();
-        ok = okn;
-        if (kb + 1 < kb1) {
-            copy(kb + 1, BUF ^ 1);
-            if (PAGED && kb + 2 < kb1) page = att_page(a, table, t, 64 * (kb + 2) + lane);
-        }
-        if (64 * kb > last || (a.window > 0 && 64 * kb + 63 <= first - a.window)) return;   // nothing for this wave
-        qt_f32x16 sc[2];
+    const auto scores = [&](qt_f32x16 (&sc)[2], const uint8_t *kbuf) {
 #pragma unroll
-        for (int kt = 0; kt < 2; kt++) {
+        for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
 #pragma unroll
-            for (int s = 0; s < NS; s++)
-                sc[kt] = att_mma<T>(qt_lds16(sk + BUF * 64 * RB + 32 * kt * RB + ka[s]), qf[s], sc[kt]);
-        }
-        if (!(ok == ~0ull && 64 * kb + 63 <= first && (a.window <= 0 || 64 * kb > last - a.window))) {
+        for (int s = 0; s < NS; s++)
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) sc[kt] = att_mma<T>(qt_lds16(kbuf + 32 * kt * RB + ka[s]), qf[s], sc[kt]);
+    };
+    // block kb: its scores are in sc, K of block kb + 1 is in the other K buffer than kb's was, V in buffer vb
+    int vb = 0;
+    const auto step = [&](int kb, qt_f32x16 (&sc)[2], qt_f32x16 (&sn)[2], auto bufc) {
+        constexpr int BUF = decltype(bufc)::value;
+        // K of the next block is in, V of this one since the last step (the wave's own copies by the wait, the others' by
+        // the barrier, which they pass after theirs), and every wave has left the buffers that block kb + 2 takes
+        att_wait();
+        __syncthreads();
+        okv = okk;
+        okk = okn;
+        const uint8_t *vbuf = sv + vb * 64 * RB;
+        vb = vb == 2 ? 0 : vb + 1;
+        if (kb + 2 < kb1) copy(kb + 2, sk + BUF * 64 * RB, sv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
+        if (64 * kb + 63 > first || (a.window > 0 && 64 * kb <= last - a.window)) {
+            const int d = pos - 64 * kb - 4 * h, w = a.window > 0 ? d - a.window : -1000;
 #pragma unroll
             for (int kt = 0; kt < 2; kt++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
-                    const int j = 32 * kt + 8 * (i >> 2) + 4 * h + (i & 3), k = 64 * kb + j;
-                    const bool see = k <= pos && (a.window <= 0 || k > pos - a.window) && (ok >> j & 1ull);
-                    sc[kt][i] = see ? sc[kt][i] : -INFINITY;
+                    const int j = 32 * kt + 8 * (i >> 2) + (i & 3);
+                    sc[kt][i] = j <= d && j > w ? sc[kt][i] : -INFINITY;
                 }
         }
-        float bm = m;
+        if (PAGED && okv != ~0ull) {                                     // the end of the keys, or a bad page
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) {
+                const uint32_t w = (uint32_t)(okv >> (32 * kt)) >> (4 * h);
+#pragma unroll
+                for (int i = 0; i < 16; i++) sc[kt][i] = w >> (8 * (i >> 2) + (i & 3)) & 1u ? sc[kt][i] : -INFINITY;
+            }
+        }
+        float bm = sc[0][0];
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[kt][i]);
         bm = fmaxf(bm, att_other_half(bm));
-        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c;
-        if (__ballot(bm > m)) {                                          // a row's maximum rose: its sums shrink
-            const float f = qt_exp2((m - mr) * a.c);
+        // probabilities up to 2^8 are as good as up to 1: the sums shrink only when a row's maximum has risen by more
+        if (__ballot((bm - m) * a.c > 8.0f || (m == -INFINITY && bm > m))) {
+            const float mn = fmaxf(m, bm), f = mn == -INFINITY ? 0.f : qt_exp2((m - mn) * a.c);
+            m = mn;
             l *= f;
 #pragma unroll
             for (int d = 0; d < NT; d++)
 #pragma unroll
                 for (int i = 0; i < 16; i++) o[d][i] *= f;
         }
-        m = bm;
+        const float mc = m == -INFINITY ? 0.f : m * a.c;
+        if (kb + 1 < kb1) scores(sn, sk + (BUF ^ 1) * 64 * RB);
         float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
@@ -579,19 +657,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             for (int j = 0; j < 4; j++) pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
 #pragma unroll
             for (int d = 0; d < NT; d++) {
-                const uint16_t *vp = reinterpret_cast<const uint16_t *>(sv + BUF * 64 * RB + 16 * s * RB + va[d]);
+                const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + va[d]);
                 o[d] = att_mma<T>(qt_lds_tr8x2(vp, vp + 8 * HD), pb, o[d]);
             }
         }
     };
     if (kb0 < kb1) {
         if (PAGED) page = att_page(a, table, t, 64 * kb0 + lane);
-        copy(kb0, 0);
-        if (PAGED && kb0 + 1 < kb1) page = att_page(a, table, t, 64 * (kb0 + 1) + lane);
-    }
-    for (int kb = kb0; kb < kb1; kb += 2) {
-        step(kb, std::integral_constant<int, 0>{});
-        if (kb + 1 < kb1) step(kb + 1, std::integral_constant<int, 1>{});
+        copy(kb0, sk, sv);
+        okk = okn;
+        if (kb0 + 1 < kb1) copy(kb0 + 1, sk + 64 * RB, sv + 64 * RB);
+        att_wait();
+        __syncthreads();
+        qt_f32x16 s0[2], s1[2];
+        scores(s0, sk);
+        for (int kb = kb0; kb < kb1; kb += 2) {
+            step(kb, s0, s1, std::integral_constant<int, 0>{});
+            if (kb + 1 < kb1) step(kb + 1, s1, s0, std::integral_constant<int, 1>{});
+        }
     }
     // the rows' results; o[d][i] is dim 32 d + 8 (i / 4) + 4 h + i % 4
     l += att_other_half(l);
@@ -605,6 +688,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     if (live) {
         if (a.splits > 1) {
             const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + qh;
+            if (kb0 < kb1)
 #pragma unroll
             for (int d = 0; d < NT; d++)
 #pragma unroll
@@ -628,12 +712,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int row = w0; row < min(w0 + 32, t.rows); row++)
             att_serial<T, T, HD, PAGED>(a, t, table, head, row, 64 * kb0, 64 * kb1, a.splits > 1, split);
     }
-    if (a.tps <= 0) return;
-    __syncthreads();                                    // the next tile's copies take the LDS
-    }
 }
 
-// A row's ranges under their common maximum: a wave a row, 4 rows a workgroup.  splits <= 64.
+// A row's ranges under their common maximum: a wave a row, 4 rows a workgroup.  splits <= 64.  A range without keys (its
+// sum 0) has written no sums.
 template <typename QT, int HD>
 __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
     constexpr int D = HD / 64, EQ = sizeof(typename QT::elem);
@@ -647,12 +729,14 @@ __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
         m = a.pm[2 * (lane * rows + at)];
         l = a.pm[2 * (lane * rows + at) + 1];
     }
-    const float M = group_max<64>(m), f = M == -INFINITY ? 0.f : qt_exp2((m - M) * a.c);
+    const float M = group_max<64>(m), f = l == 0.f ? 0.f : qt_exp2((m - M) * a.c);
+    const unsigned long long some = __ballot(l != 0.f);
     const float L = group_sum<64>(l * f);
     float o[D];
 #pragma unroll
     for (int e = 0; e < D; e++) o[e] = 0.f;
     for (int s = 0; s < a.splits; s++) {
+        if (!(some >> s & 1)) continue;
         const float fs = lane_bcast(f, s);
 #pragma unroll
         for (int e = 0; e < D; e++) o[e] = fmaf(fs, a.po[(s * rows + at) * HD + D * lane + e], o[e]);
@@ -674,7 +758,7 @@ static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_s
     const int tr = p.tile ? 128 : 32;
     const long long by_rows = (long long)a.T * a.G / tr + a.B;
     const long long tps = ((long long)max_q * a.G + tr - 1) / tr, by_req = tps * a.B;
-    a.tps = max_q > 0 && by_req <= by_rows ? (int)tps : 0;
+    a.tps = !p.tile && max_q > 0 && by_req <= by_rows ? (int)tps : 0;
     p.slots = a.tps > 0 ? by_req : by_rows;
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
     long long n = wgs > 0 ? ((p.tile ? 512 : 1024) + wgs - 1) / wgs : 1;
