@@ -1,15 +1,16 @@
 // qt_logits.hip — the rules on a batch's logits before sampling (qwen_hip_op_logit_rules): repetition,
 // presence and frequency penalties, token biases, an allowed-token bit mask.
 //
-// A workgroup takes RULES_CH neighbouring tokens of one row.  It counts the row's history entries that fall on them in
-// LDS (integer atomics: the order does not matter), finds each token's last bias entry there the same way (the
-// largest index wins), then streams its logits once.  So a row's history is read once a workgroup, from the L2,
-// and no counts of V tokens a row are held in global memory, cleared or read back.
+// A workgroup takes RULES_CH neighbouring tokens of one row, 16 a thread, loaded at once.  Few of them are in the row's history or
+// its biases: those are marked in LDS, then counted there (integer atomics: the order does not matter; of a token's
+// bias entries the largest index wins), and a thread goes through the marked ones of its own before it stores.  So a row's
+// history is read once a workgroup, from the L2, and no counts of V tokens a row are held in memory, cleared or read back.
 // Bound by the logits' bytes for a large vocabulary, by the latency of offsets, history and logits for a small one.
 #include "qt_ops.h"
 
 #define RULES_T 256
 #define RULES_CH 4096
+#define RULES_HELD 16          // history entries a thread keeps between marking and counting
 
 struct RulesArgs {
     const uint8_t *x;
@@ -24,76 +25,117 @@ struct RulesArgs {
     int V, hcap, bcap, each;
 };
 
-// BIAS: with bias lists.  Rows may begin anywhere that their elements can: 16-byte accesses at 2- or 4-byte
-// alignment are one instruction on this GPU.
-template <typename T, bool BIAS>
+// BIAS: with bias lists.  EACH: the penalty once for every entry.  Rows may begin anywhere that their elements can: 16-byte
+// accesses at 2- or 4-byte alignment are one instruction on this GPU.
+template <typename T, bool BIAS, bool EACH>
 __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
-    constexpr int E = sizeof(typename T::elem);
-    __shared__ __align__(16) unsigned seen[RULES_CH], said[RULES_CH];
-    __shared__ __align__(16) int last[BIAS ? RULES_CH : 4];
+    constexpr int E = sizeof(typename T::elem), NV = RULES_CH / RULES_T / 8;
+    __shared__ unsigned bits[RULES_CH / 32], seen[RULES_CH / 32], said[RULES_CH], times[EACH ? RULES_CH : 1];
+    __shared__ int last[BIAS ? RULES_CH : 1];
+    __shared__ float value[BIAS ? RULES_T : 1];         // of the first bias entries
     const int tid = threadIdx.x, b = blockIdx.y, v0 = blockIdx.x * RULES_CH, n = min(RULES_CH, a.V - v0);
     const bool counts = a.rep || a.pres || a.freq;
-    if (counts || BIAS) {
-        for (int i = tid; i < RULES_CH; i += RULES_T) {
-            seen[i] = 0; said[i] = 0;
-            if (BIAS) last[i] = -1;
-        }
-        __syncthreads();
-        if (counts) {
-            const int h0 = max(a.hoff[b], 0), h1 = min(a.hoff[b + 1], a.hcap);
-            const long long h2 = a.npr ? (long long)h0 + max(a.npr[b], 0) : h0;
-            for (int i = h0 + tid; i < h1; i += RULES_T) {
-                const unsigned t = (unsigned)a.hist[i] - (unsigned)v0;
-                if (t >= (unsigned)n) continue;
-                atomicAdd(&seen[t], 1u);
-                if (i >= h2) atomicAdd(&said[t], 1u);
-            }
-        }
-        if (BIAS) {
-            const int e0 = max(a.boff[b], 0), e1 = min(a.boff[b + 1], a.bcap);
-            for (int i = e0 + tid; i < e1; i += RULES_T) {
-                const unsigned t = (unsigned)a.btok[i] - (unsigned)v0;
-                if (t < (unsigned)n) atomicMax(&last[t], i);
-            }
-        }
-        __syncthreads();
-    }
-    const float rep = a.rep ? a.rep[b] : 1.f, pres = a.pres ? a.pres[b] : 0.f, freq = a.freq ? a.freq[b] : 0.f;
-    const uint8_t *xr = a.x + (size_t)b * a.xs * E;
-    uint8_t *yr = a.out + (size_t)b * a.os * E;
-    const uint32_t *mr = a.mask ? a.mask + (size_t)b * a.ms : nullptr;
-    const auto rules = [&](float x, int i, uint32_t allowed) {
-        if (counts) {
-            const unsigned c = seen[i], o = said[i];
-            if (c && a.rep) {
-                // once, or once for every entry until nothing changes any more
-                float was;
-                unsigned k = a.each ? c : 1u;
-                do { was = x; x = x > 0.f ? x / rep : x * rep; } while (--k && x != was);
-            }
-            if (o) {
-                if (a.freq) x -= (float)o * freq;
-                if (a.pres) x -= pres;
-            }
-        }
-        if (BIAS) {
-            const int e = last[i];
-            if (e >= 0) x += a.bval[e];
-        }
-        return allowed & 1u ? x : -INFINITY;
-    };
-    for (int i = 8 * tid; i < n; i += 8 * RULES_T) {
-        const int t = v0 + i;
-        const uint32_t bits = mr ? mr[t >> 5] >> (t & 31) : 0xFFu;
-        if (i + 8 <= n) {
-            float x[8];
-            qt_load8<T, E>(xr + (size_t)t * E, x);
+    const uint8_t *xr = a.x + ((size_t)b * a.xs + v0) * E;
+    uint8_t *yr = a.out + ((size_t)b * a.os + v0) * E;
+    const uint32_t *mr = a.mask ? a.mask + (size_t)b * a.ms + v0 / 32 : nullptr;
+    // a thread's tokens: 8 at 8 tid + 8 RULES_T v
+    float x[NV][8];
+    uint32_t allow[NV];
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = rules(x[e], i + e, bits >> e);
-            qt_store8<T, E>(yr + (size_t)t * E, x);
+    for (int v = 0; v < NV; v++) {
+        const int i = 8 * (tid + RULES_T * v);
+        allow[v] = mr && i < n ? mr[i >> 5] >> (i & 31) : 0xFFu;
+        if (i + 8 <= n) qt_load8<T, E>(xr + (size_t)i * E, x[v]);
+    }
+    const int h0 = counts ? max(a.hoff[b], 0) : 0, h1 = counts ? min(a.hoff[b + 1], a.hcap) : 0;
+    const int e0 = BIAS ? max(a.boff[b], 0) : 0, e1 = BIAS ? min(a.boff[b + 1], a.bcap) : 0;
+    const float rep = a.rep ? a.rep[b] : 1.f, pres = a.pres ? a.pres[b] : 0.f, freq = a.freq ? a.freq[b] : 0.f;
+    const long long h2 = h0 + (long long)(counts && a.npr ? max(a.npr[b], 0) : 0);
+    unsigned held[RULES_HELD];
+#pragma unroll
+    for (int k = 0; k < RULES_HELD; k++) {
+        const int i = h0 + tid + k * RULES_T;
+        held[k] = i < h1 ? (unsigned)a.hist[i] - (unsigned)v0 : ~0u;
+    }
+    unsigned held_bias = ~0u;
+    if (BIAS && e0 + tid < e1) {
+        held_bias = (unsigned)a.btok[e0 + tid] - (unsigned)v0;
+        value[tid] = a.bval[e0 + tid];
+    }
+    if (tid < RULES_CH / 32) bits[tid] = seen[tid] = 0;
+    __syncthreads();
+    const auto mark = [&](unsigned t, bool hist) {
+        if (t >= (unsigned)n) return;
+        said[t] = 0;                                    // the same from every thread
+        if (EACH) times[t] = 0;
+        if (BIAS) last[t] = -1;
+        const unsigned bit = 1u << (t & 31);
+        if (hist) atomicOr(&seen[t >> 5], bit);
+        else atomicOr(&bits[t >> 5], bit);
+    };
+    const auto count = [&](unsigned t, int i) {
+        if (t >= (unsigned)n) return;
+        if (EACH) atomicAdd(&times[t], 1u);
+        if (i >= h2) atomicAdd(&said[t], 1u);
+    };
+#pragma unroll
+    for (int k = 0; k < RULES_HELD; k++) mark(held[k], true);
+    for (int i = h0 + tid + RULES_HELD * RULES_T; i < h1; i += RULES_T) mark((unsigned)a.hist[i] - (unsigned)v0, true);
+    if (BIAS) {
+        mark(held_bias, false);
+        for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) mark((unsigned)a.btok[i] - (unsigned)v0, false);
+    }
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < RULES_HELD; k++) count(held[k], h0 + tid + k * RULES_T);
+    for (int i = h0 + tid + RULES_HELD * RULES_T; i < h1; i += RULES_T) count((unsigned)a.hist[i] - (unsigned)v0, i);
+    if (BIAS) {
+        if (held_bias < (unsigned)n) atomicMax(&last[held_bias], tid);
+        for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) {
+            const unsigned t = (unsigned)a.btok[i] - (unsigned)v0;
+            if (t < (unsigned)n) atomicMax(&last[t], i - e0);
+        }
+    }
+    __syncthreads();
+    const auto rules = [&](float y, int t) {
+        if (a.rep && (seen[t >> 5] >> (t & 31) & 1u)) {
+            unsigned k = EACH ? times[t] : 1u;
+            float was;
+            do { was = y; y = y > 0.f ? y / rep : y * rep; } while (--k && y != was);   // until nothing changes any more
+        }
+        if (const unsigned o = said[t]) {
+            if (a.freq) y -= (float)o * freq;
+            if (a.pres) y -= pres;
+        }
+        if (BIAS)
+            if (const int e = last[t]; e >= 0) y += e < RULES_T ? value[e] : a.bval[e0 + e];
+        return y;
+    };
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int i = 8 * (tid + RULES_T * v);
+        if (i >= n) continue;
+        unsigned todo = (seen[i >> 5] | bits[i >> 5]) >> (i & 31) & allow[v] & 0xFFu;
+        if (i + 8 <= n) {
+            while (todo) {
+                const int e = __builtin_ctz(todo);
+                todo &= todo - 1;
+                float y = x[v][0];
+#pragma unroll
+                for (int k = 1; k < 8; k++) y = k == e ? x[v][k] : y;
+                y = rules(y, i + e);
+#pragma unroll
+                for (int k = 0; k < 8; k++) x[v][k] = k == e ? y : x[v][k];
+            }
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[v][e] = allow[v] >> e & 1u ? x[v][e] : -INFINITY;
+            qt_store8<T, E>(yr + (size_t)i * E, x[v]);
         } else {
-            for (int e = 0; i + e < n; e++)
-                qt_store1<T>(yr + (size_t)(t + e) * E, rules(qt_load1<T>(xr + (size_t)(t + e) * E), i + e, bits >> e));
+            for (int e = 0; i + e < n; e++) {
+                float y = qt_load1<T>(xr + (size_t)(i + e) * E);
+                if (todo >> e & 1u) y = rules(y, i + e);
+                qt_store1<T>(yr + (size_t)(i + e) * E, allow[v] >> e & 1u ? y : -INFINITY);
+            }
         }
     }
 }
@@ -121,8 +163,10 @@ extern "C" int qwen_hip_op_logit_rules(const qwen_hip_logit_rules_t *p, void *st
                          p->mask, p->V, p->hist_cap, p->bias_cap, p->rep_each};
     const dim3 grid((p->V + RULES_CH - 1) / RULES_CH, p->B);
 #define RULES(T) do { \
-        if (p->bias_tok) hipLaunchKernelGGL((k_logit_rules<T, true>), grid, dim3(RULES_T), 0, st, a); \
-        else hipLaunchKernelGGL((k_logit_rules<T, false>), grid, dim3(RULES_T), 0, st, a); } while (0)
+        if (p->bias_tok && p->rep_each) hipLaunchKernelGGL((k_logit_rules<T, true, true>), grid, dim3(RULES_T), 0, st, a); \
+        else if (p->bias_tok) hipLaunchKernelGGL((k_logit_rules<T, true, false>), grid, dim3(RULES_T), 0, st, a); \
+        else if (p->rep_each) hipLaunchKernelGGL((k_logit_rules<T, false, true>), grid, dim3(RULES_T), 0, st, a); \
+        else hipLaunchKernelGGL((k_logit_rules<T, false, false>), grid, dim3(RULES_T), 0, st, a); } while (0)
     if (p->dtype == QWEN_HIP_DT_F32) RULES(QtF32);
     else if (p->dtype == QWEN_HIP_DT_BF16) RULES(QtBf16);
     else RULES(QtF16);

@@ -472,6 +472,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
             att_put<QT, NT>(a.out + (tk * a.os + hd * HD + NT * mm) * EQ, v);
         }
     }
+    att_stored();
     if (__syncthreads_or(bad))
         for (int row = wave; row < 32 && t.r0 + row < t.rows; row += ATT_WV)
             att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, a.splits > 1, split);
