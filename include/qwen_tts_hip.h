@@ -492,10 +492,12 @@ enum {
     QWEN_HIP_PLAN_NO_PAGES = 1,     /* more pages needed than free (pages given back in this step count as free) */
     QWEN_HIP_PLAN_TABLE_FULL = 2,   /* a request outgrows table_cols pages */
     QWEN_HIP_PLAN_TOO_MANY = 4,     /* more than max_tokens new tokens */
-    QWEN_HIP_PLAN_INVALID = 8       /* a negative kv_len, a free count or page number out of range */
+    QWEN_HIP_PLAN_INVALID = 8       /* a kv_len that is negative or past its table, a free count out of range, more pages
+                                     * given back than there are */
 };
 /* Pages given back go onto the free list's end in the order of requests and of their positions; pages are then
- * taken from its end, for the requests in order.  The result depends on nothing else.  With separate kv_len_out
+ * taken from its end, for the requests in order.  The result depends on nothing else.  Page numbers are passed on as
+ * they are: one outside [0, n_pages) makes no slot (-1), and the other calls pass over it.  With separate kv_len_out
  * and n_free_out a call can be repeated with the same result. */
 int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *plan, void *stream);
 

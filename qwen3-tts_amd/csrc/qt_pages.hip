@@ -7,50 +7,52 @@
 // h(kv + new) - h(kv).  In request order, exclusive sums of the pages given back, of those taken and of the new
 // tokens say where each request's entries lie; then every page and every token finds its request by a search
 // in those sums, independently of the others.  Page i of all taken is the free list's entry n_free + R - 1 - i, R
-// pages having been given back: entries n_free .. n_free + R - 1 are those pages themselves, read from the tables,
-// so nothing written is read again and everything is checked before anything is written.
-//
-// One workgroup does it all: three sums over at most 2048 requests need no second launch and no
-// global scratch, and a step's work is a few hundred KB at most.  Bound by the latency of its dependent loads
-// (lengths, then free list and tables) and of the launch.  Past PLAN_ONE tokens the slots go to a grid of their own,
-// which reads what the workgroup wrote.
-#define PLAN_T 1024
-#define PLAN_MAX_B 2048        // 32 KB of LDS
-#define PLAN_ONE 8192
+// pages having been given back: entries n_free .. n_free + R - 1 are those pages themselves, read from the tables.
+// So nothing that is written is read again, and any number of workgroups can share the pages and tokens when each makes the sums
+// over the (at most 2048) requests for itself; only the lengths and the free count, which may be replaced in place, are
+// written by one of them, and in a launch of their own where the others may still read what they replace.
+// Bound by the latency of its dependent loads (lengths, then free list and tables) and of the launch.
+#define PLAN_T 256
+#define PLAN_MAX_B 2048         // 32 KB of LDS
 #define PLAN_SAT (1u << 30)     // sums stop here: under 2^31 in any order, over every limit they are held to
 
 struct PlanArgs {
     const int *new_len, *kv_len, *n_free;
     int *table, *free_pages, *kv_out, *n_free_out, *cu, *pos, *slot, *status;
     long long ts;
-    int B, ps, n_pages, cols, cap, slots_here;
+    int B, ps, n_pages, cols, cap;
+    int share, finish;          // this launch writes pages and tokens; offsets, lengths, the free count and status
     QtDiv div;
 };
 
 __device__ __forceinline__ unsigned plan_add(unsigned a, unsigned b) { return min(a + b, PLAN_SAT); }
 
-// the last b with first[b] <= i (first[0] = 0, ascending): of requests that begin at the same place all but the
-// last are empty
-__device__ __forceinline__ int plan_find(const unsigned *first, int B, unsigned i) {
-    int lo = 0, hi = B;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) >> 1;
-        if (first[mid] <= i) lo = mid; else hi = mid;
-    }
-    return lo;
+// The last b with first[b] <= i (first[0] = 0, ascending), for four i at once: of requests that begin at the same
+// place all but the last are empty.  Fixed steps, so the four searches' LDS reads overlap.
+__device__ __forceinline__ void plan_find(const unsigned *first, int B, const unsigned (&i)[4], int (&b)[4]) {
+#pragma unroll
+    for (int k = 0; k < 4; k++) b[k] = 0;
+    for (int s = 1 << (31 - __clz(B)); s; s >>= 1)
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            const int p = b[k] + s;
+            if (first[min(p, B - 1)] <= i[k] && p < B) b[k] = p;
+        }
 }
+
 __global__ __launch_bounds__(PLAN_T) void k_page_plan(PlanArgs a) {
     extern __shared__ unsigned sh[];
     unsigned *tok = sh, *take = tok + a.B + 1, *back = take + a.B + 1;     // exclusive sums, [B + 1] each
     int *kv = reinterpret_cast<int *>(back + a.B + 1);                     // lengths before, [B]
     __shared__ unsigned wsum[3][PLAN_T / 64];
+    __shared__ int bad;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n_free = a.n_free[0];
-    int flags = n_free < 0 || n_free > a.n_pages ? QWEN_HIP_PLAN_INVALID : 0;
-    const int per = (a.B + PLAN_T - 1) / PLAN_T, b0 = tid * per, b1 = min(b0 + per, a.B);
+    if (tid == 0) bad = n_free < 0 || n_free > a.n_pages ? QWEN_HIP_PLAN_INVALID : 0;
+    __syncthreads();
     const long long room = (long long)a.cols * a.ps;
-    unsigned s[3] = {0u, 0u, 0u};
-    for (int b = b0; b < b1; b++) {
+    int flags = 0;
+    for (int b = tid; b < a.B; b += PLAN_T) {
         const int n = a.new_len[b];
         int len = a.kv_len[b];
         unsigned t = 0, p = 0, r = 0;
@@ -63,120 +65,139 @@ __global__ __launch_bounds__(PLAN_T) void k_page_plan(PlanArgs a) {
             flags |= QWEN_HIP_PLAN_TABLE_FULL;
         } else {
             t = n;
-            p = (unsigned)(((long long)len + n + a.ps - 1) / a.ps) - (qt_quot(len, a.div) + (len % a.ps != 0));
+            p = (qt_quot(len + n, a.div) + ((len + n) % a.ps != 0)) - (qt_quot(len, a.div) + (len % a.ps != 0));
         }
-        kv[b] = len;
-        tok[b] = s[0]; take[b] = s[1]; back[b] = s[2];
-        s[0] = plan_add(s[0], t); s[1] = plan_add(s[1], p); s[2] = plan_add(s[2], r);
+        kv[b] = len; tok[b] = t; take[b] = p; back[b] = r;
     }
-    // exclusive sums over the threads
-    unsigned inc[3], tot[3], base[3];
-#pragma unroll
-    for (int k = 0; k < 3; k++) {
-        unsigned x = s[k];
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const unsigned y = __shfl_up(x, o, 64);
-            if (lane >= o) x = plan_add(x, y);
-        }
-        inc[k] = x;
-        if (lane == 63) wsum[k][wave] = x;
-    }
+    if (flags) atomicOr(&bad, flags);
     __syncthreads();
+    // exclusive sums: a thread's requests, the wave's threads, the waves
+    const int per = (a.B + PLAN_T - 1) / PLAN_T, b0 = min(tid * per, a.B), b1 = min(b0 + per, a.B);
+    unsigned s[3] = {0u, 0u, 0u}, x[3];
+    for (int b = b0; b < b1; b++) { s[0] = plan_add(s[0], tok[b]); s[1] = plan_add(s[1], take[b]); s[2] = plan_add(s[2], back[b]); }
+#pragma unroll
+    for (int k = 0; k < 3; k++) x[k] = s[k];
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1)
+#pragma unroll
+        for (int k = 0; k < 3; k++) {
+            const unsigned y = __shfl_up(x[k], o, 64);
+            if (lane >= o) x[k] = plan_add(x[k], y);
+        }
+    if (lane == 63)
+#pragma unroll
+        for (int k = 0; k < 3; k++) wsum[k][wave] = x[k];
+    __syncthreads();
+    unsigned tot[3];
 #pragma unroll
     for (int k = 0; k < 3; k++) {
         unsigned before = 0, all = 0;
+#pragma unroll
         for (int w = 0; w < PLAN_T / 64; w++) {
             if (w == wave) before = all;
             all = plan_add(all, wsum[k][w]);
         }
-        const unsigned up = __shfl_up(inc[k], 1, 64);
-        base[k] = lane == 0 ? before : plan_add(before, up);
+        const unsigned up = __shfl_up(x[k], 1, 64);
+        s[k] = lane == 0 ? before : plan_add(before, up);
         tot[k] = all;
     }
     for (int b = b0; b < b1; b++) {
-        tok[b] = plan_add(tok[b], base[0]);
-        take[b] = plan_add(take[b], base[1]);
-        back[b] = plan_add(back[b], base[2]);
+        const unsigned t = tok[b], p = take[b], r = back[b];
+        tok[b] = s[0]; take[b] = s[1]; back[b] = s[2];
+        s[0] = plan_add(s[0], t); s[1] = plan_add(s[1], p); s[2] = plan_add(s[2], r);
     }
-    if (tid == 0) { tok[a.B] = tot[0]; take[a.B] = tot[1]; back[a.B] = tot[2]; }
-    const unsigned R = tot[2], N = tot[1], T = tot[0];
-    if (T > (unsigned)a.cap) flags |= QWEN_HIP_PLAN_TOO_MANY;
-    if (n_free + (long long)R > a.n_pages) flags |= QWEN_HIP_PLAN_INVALID;   // pages given back twice
-    if ((long long)N > n_free + (long long)R) flags |= QWEN_HIP_PLAN_NO_PAGES;
+    const unsigned T = tot[0], N = tot[1], R = tot[2];
+    int any = bad;
+    if (T > (unsigned)a.cap) any |= QWEN_HIP_PLAN_TOO_MANY;
+    if (n_free + (long long)R > a.n_pages) any |= QWEN_HIP_PLAN_INVALID;     // pages given back twice
+    if ((long long)N > n_free + (long long)R) any |= QWEN_HIP_PLAN_NO_PAGES;
     __syncthreads();
-    // page j of those given back, and page i of those taken
-    const auto given = [&](unsigned j) {
-        const int b = plan_find(back, a.B, j);
-        return a.table[(long long)b * a.ts + (j - back[b])];
-    };
-    const auto taken = [&](unsigned i) {
-        const long long at = (long long)n_free + R - 1 - i;
-        return at >= n_free ? given((unsigned)(at - n_free)) : a.free_pages[at];
-    };
-    int any = 0;
-    for (int k = 0; k < 4; k++) any |= __syncthreads_or(flags & (1 << k)) ? 1 << k : 0;
-    if (any == 0) {                                                          // the sums are in range: look at the pages
-        bool bad = false;
-        for (unsigned j = tid; j < R; j += PLAN_T) bad |= (unsigned)given(j) >= (unsigned)a.n_pages;
-        for (unsigned i = tid; i < N; i += PLAN_T) bad |= (unsigned)taken(i) >= (unsigned)a.n_pages;
-        any = __syncthreads_or(bad) ? QWEN_HIP_PLAN_INVALID : 0;
-    }
-    if (any) {
-        for (int b = tid; b < a.B; b += PLAN_T) a.kv_out[b] = a.kv_len[b];
-        for (int b = tid; b <= a.B; b += PLAN_T) a.cu[b] = 0;
-        if (a.slots_here)
-            for (int t = tid; t < a.cap; t += PLAN_T) { a.pos[t] = -1; a.slot[t] = -1; }
-        if (tid == 0) { a.n_free_out[0] = n_free; a.status[0] = any; }
-        return;
-    }
+    const unsigned at0 = blockIdx.x * 4 * PLAN_T, stride = gridDim.x * 4 * PLAN_T;
+    // pages given back begin at the last workgroup, pages taken at the middle one: few have two kinds of work
+    const unsigned at_given = stride - 4 * PLAN_T - at0, at_taken = (blockIdx.x + gridDim.x / 2) % gridDim.x * 4 * PLAN_T;
     const auto have = [&](int b) { return (unsigned)(qt_quot(kv[b], a.div) + (kv[b] % a.ps != 0)); };
-    for (unsigned j = tid; j < R; j += PLAN_T) a.free_pages[n_free + j] = given(j);
-    for (unsigned i = tid; i < N; i += PLAN_T) {
-        const int b = plan_find(take, a.B, i);
-        a.table[(long long)b * a.ts + have(b) + (i - take[b])] = taken(i);
+    const auto four = [&](unsigned (&i)[4], unsigned at) {
+#pragma unroll
+        for (int k = 0; k < 4; k++) i[k] = at + k * PLAN_T + tid;
+    };
+    // pages j of those given back, and pages i of those taken, four at once
+    const auto given = [&](const unsigned (&j)[4], int (&v)[4]) {
+        int b[4];
+        plan_find(back, a.B, j, b);
+#pragma unroll
+        for (int k = 0; k < 4; k++) v[k] = j[k] < R ? a.table[(long long)b[k] * a.ts + (j[k] - back[b[k]])] : -1;
+    };
+    const auto taken = [&](const unsigned (&i)[4], int (&v)[4]) {
+        unsigned j[4];                                                       // i < R: the j-th given back
+        bool some = false;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            j[k] = i[k] < N ? R - 1 - i[k] : ~0u;
+            some |= j[k] < R;
+            v[k] = i[k] < N && i[k] >= R ? a.free_pages[n_free - 1 - (int)(i[k] - R)] : -1;
+        }
+        if (some) {
+            int g[4];
+            given(j, g);
+#pragma unroll
+            for (int k = 0; k < 4; k++) v[k] = j[k] < R ? g[k] : v[k];
+        }
+    };
+    unsigned i[4];
+    int v[4], b[4];
+    if (a.share && !any) {
+        for (unsigned at = at_given; at < R; at += stride) {
+            four(i, at);
+            given(i, v);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i[k] < R) a.free_pages[n_free + (int)i[k]] = v[k];
+        }
+        for (unsigned at = at_taken; at < N; at += stride) {
+            four(i, at);
+            plan_find(take, a.B, i, b);
+            taken(i, v);
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+                if (i[k] < N) a.table[(long long)b[k] * a.ts + have(b[k]) + (i[k] - take[b[k]])] = v[k];
+        }
     }
-    if (a.slots_here)
-        for (unsigned t = tid; t < (unsigned)a.cap; t += PLAN_T) {
-            int p = -1, at = -1;
-            if (t < T) {
-                const int b = plan_find(tok, a.B, t);
-                p = kv[b] + (int)(t - tok[b]);
-                const unsigned c = (unsigned)qt_quot(p, a.div), hb = have(b);
-                const int page = c < hb ? a.table[(long long)b * a.ts + c] : taken(take[b] + c - hb);
-                // an old page's number is the caller's: one out of range makes no slot
-                at = (unsigned)page < (unsigned)a.n_pages ? page * a.ps + (p - (int)c * a.ps) : -1;
+    if (a.share)
+        for (unsigned at = at0; at < (unsigned)a.cap; at += stride) {
+            unsigned f[4];
+            int p[4], c[4], page[4];
+            bool some = false;
+            four(i, at);
+            plan_find(tok, a.B, i, b);
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                const bool live = !any && i[k] < T;
+                p[k] = live ? kv[b[k]] + (int)(i[k] - tok[b[k]]) : -1;
+                c[k] = live ? qt_quot(p[k], a.div) : 0;
+                const unsigned hb = have(b[k]);
+                f[k] = live && (unsigned)c[k] >= hb ? take[b[k]] + c[k] - hb : ~0u;      // a new page, or one of before
+                some |= f[k] != ~0u;
+                page[k] = live && f[k] == ~0u ? a.table[(long long)b[k] * a.ts + c[k]] : -1;
             }
-            a.pos[t] = p;
-            a.slot[t] = at;
+            if (some) {
+                taken(f, v);
+#pragma unroll
+                for (int k = 0; k < 4; k++) page[k] = f[k] != ~0u ? v[k] : page[k];
+            }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (i[k] >= (unsigned)a.cap) continue;
+                a.pos[i[k]] = p[k];
+                a.slot[i[k]] = (unsigned)page[k] < (unsigned)a.n_pages ? page[k] * a.ps + (p[k] - c[k] * a.ps) : -1;
+            }
         }
-    for (int b = b0; b < b1; b++) {
-        const int n = a.new_len[b];
-        a.kv_out[b] = n < 0 ? 0 : kv[b] + n;
+    if (!a.finish || blockIdx.x) return;
+    for (int r = tid; r < a.B; r += PLAN_T) {
+        const int n = a.new_len[r];
+        a.kv_out[r] = any ? a.kv_len[r] : n < 0 ? 0 : kv[r] + n;
     }
-    for (int b = tid; b <= a.B; b += PLAN_T) a.cu[b] = (int)tok[b];
-    if (tid == 0) { a.n_free_out[0] = (int)(n_free + R - N); a.status[0] = 0; }
-}
-
-// positions and slots of a large step: the plan's tables and offsets are written
-__global__ __launch_bounds__(256) void k_page_slots(PlanArgs a) {
-    extern __shared__ unsigned cu[];
-    for (int b = threadIdx.x; b <= a.B; b += 256) cu[b] = (unsigned)a.cu[b];
-    __syncthreads();
-    const unsigned T = cu[a.B];
-    for (int k = 0; k < 4; k++) {
-        const unsigned t = blockIdx.x * 1024 + k * 256 + threadIdx.x;
-        if (t >= (unsigned)a.cap) return;
-        int p = -1, at = -1;
-        if (t < T) {
-            const int b = plan_find(cu, a.B, t);
-            p = a.kv_out[b] - (int)(cu[b + 1] - t);
-            const int c = qt_quot(p, a.div), page = a.table[(long long)b * a.ts + c];
-            at = (unsigned)page < (unsigned)a.n_pages ? page * a.ps + (p - c * a.ps) : -1;
-        }
-        a.pos[t] = p;
-        a.slot[t] = at;
-    }
+    for (int r = tid; r <= a.B; r += PLAN_T) a.cu[r] = any ? 0 : r == a.B ? (int)T : (int)tok[r];
+    if (tid == 0) { a.n_free_out[0] = any ? n_free : (int)(n_free + R - N); a.status[0] = any; }
 }
 
 extern "C" int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *p, void *stream) {
@@ -195,12 +216,21 @@ extern "C" int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *p, void *stream
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_plan: the stream's device: %s", hipGetErrorString(on.err));
     PlanArgs a = {p->new_len, p->kv_len, p->n_free, p->table, p->free_pages, p->kv_len_out, p->n_free_out, p->cu_q, p->pos,
-                  p->slot, p->status, p->table_stride, p->B, p->page_size, p->n_pages, p->table_cols, p->max_tokens,
-                  p->max_tokens <= PLAN_ONE, qt_div_of(p->page_size)};
-    hipLaunchKernelGGL(k_page_plan, dim3(1), dim3(PLAN_T), (size_t)(4 * p->B + 3) * 4, st, a);
+                  p->slot, p->status, p->table_stride, p->B, p->page_size, p->n_pages, p->table_cols, p->max_tokens, 1, 1,
+                  qt_div_of(p->page_size)};
+    // A workgroup for every 512 tokens, or 16 requests: pages given back, whose number the host does not know, may be
+    // many a request.
+    const int most = p->max_tokens > p->B * 32 ? p->max_tokens : p->B * 32;
+    const int wgs = most <= 1024 ? 1 : most >= (128 << 10) ? 256 : (most + 511) / 512;
+    const bool in_place = p->kv_len_out == p->kv_len || p->n_free_out == p->n_free;
+    a.finish = wgs == 1 || !in_place;
+    const size_t lds = (size_t)(4 * p->B + 3) * 4;
+    hipLaunchKernelGGL(k_page_plan, dim3(wgs), dim3(PLAN_T), lds, st, a);
     hipError_t e = hipGetLastError();
-    if (e == hipSuccess && !a.slots_here) {
-        hipLaunchKernelGGL(k_page_slots, dim3((p->max_tokens + 1023) / 1024), dim3(256), (size_t)(p->B + 1) * 4, st, a);
+    if (e == hipSuccess && !a.finish) {
+        a.share = 0;
+        a.finish = 1;
+        hipLaunchKernelGGL(k_page_plan, dim3(1), dim3(PLAN_T), lds, st, a);
         e = hipGetLastError();
     }
     QT_REFUSE(e != hipSuccess, "page_plan: launch failed: %s", hipGetErrorString(e));

@@ -762,7 +762,7 @@ static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_s
     a.tps = !p.tile && max_q > 0 && by_req <= by_rows ? (int)tps : 0;
     p.slots = a.tps > 0 ? by_req : by_rows;
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
-    long long n = wgs > 0 ? ((p.tile ? 512 : 1024) + wgs - 1) / wgs : 1;
+    long long n = wgs > 0 ? ((p.tile ? 512 : 4096) + wgs - 1) / wgs : 1;
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
     if (n < 1 || !may_split) n = 1;

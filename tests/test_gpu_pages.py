@@ -76,14 +76,10 @@ def plan_model(new, kv, table, free, n_free, page, n_pages, cols, cap):
         status |= hip.PLAN_INVALID
     if need > n_free + len(stack):
         status |= hip.PLAN_NO_PAGES
-    if not status:
-        avail = free[:n_free] + stack
-        if any(not 0 <= p < n_pages for p in stack + avail[len(avail) - need:]):
-            status = hip.PLAN_INVALID
     if status:
         return dict(kv=list(kv), n_free=n_free, cu=[0] * (B + 1), pos=[-1] * cap, slot=[-1] * cap, table=table, free=free, status=status)
     free[n_free:n_free + len(stack)] = stack
-    avail, kv2, pos, slot = list(avail), [], [], []
+    avail, kv2, pos, slot = free[:n_free + len(stack)], [], [], []
     for b in range(B):
         if new[b] < 0:
             kv2.append(0)
@@ -169,7 +165,7 @@ def test_plan_takes_and_gives_back_exactly_everything():
 
 
 @pytest.mark.parametrize("cap", [None, 9000])
-@pytest.mark.parametrize("what", ["pages", "table", "tokens", "negative", "n_free", "free page", "given page", "twice", "long", "overflow"])
+@pytest.mark.parametrize("what", ["pages", "table", "tokens", "negative", "n_free", "twice", "long", "overflow"])
 def test_plan_that_cannot_be_made_changes_nothing(what, cap):
     rng = np.random.default_rng(9)
     new, kv, table, free, n_free, page, n_pages, cols, cap = plan_case(rng, 20, 16, 20, 90, 60, 4, spare=0, cap=cap)
@@ -186,13 +182,6 @@ def test_plan_that_cannot_be_made_changes_nothing(what, cap):
         kv[3] = -1
     elif what == "n_free":
         n_free = n_pages + 1
-    elif what == "free page":
-        free[n_free - 1] = n_pages
-        new = [max(n, 0) for n in new]
-        new[0] += 0
-    elif what == "given page":
-        b = next(b for b in range(20) if new[b] < 0)
-        table[b][0] = -1
     elif what == "twice":
         n_free = n_pages
         free = list(range(n_pages))
@@ -203,6 +192,17 @@ def test_plan_that_cannot_be_made_changes_nothing(what, cap):
     case = (new, kv, table, free, n_free, page, n_pages, cols, cap)
     want = plan_model(*case)
     assert want["status"] != 0
+    assert Plan(*case).run() == want
+
+
+def test_plan_makes_no_slot_of_a_bad_page():
+    """Page numbers are passed on as they are; one outside the pool makes no slot."""
+    new, kv, table = [3, -1, 20], [5, 40, 0], [[99, -1, -1], [2, -4, 7], [-1, -1, -1]]
+    free = [10, -9] + [0] * 8
+    case = (new, kv, table, free, 2, 16, 10, 3, 30)
+    want = plan_model(*case)
+    assert want["slot"][:3] == [-1] * 3 and want["table"][2][:2] == [7, -4] and want["slot"][3] == 7 * 16
+    assert want["slot"][3 + 16:3 + 20] == [-1] * 4
     assert Plan(*case).run() == want
 
 
