@@ -188,11 +188,7 @@ __device__ __forceinline__ long long att_instead(long long off, bool mine, unsig
 // Writes NT elements of a row's output, dim NT m.
 template <typename QT, int NT> __device__ __forceinline__ void att_put(uint8_t *p, const float (&v)[NT]) {
     if constexpr (sizeof(typename QT::elem) == 4) {
-        typedef float fv __attribute__((ext_vector_type(NT)));
-        fv x;
-#pragma unroll
-        for (int t = 0; t < NT; t++) x[t] = v[t];
-        *reinterpret_cast<fv *>(p) = x;
+        __builtin_memcpy(__builtin_assume_aligned(p, NT * 4 < 16 ? NT * 4 : 16), v, NT * 4);
     } else {
         typedef uint32_t uv __attribute__((ext_vector_type(NT / 2)));
         uv x;
@@ -273,7 +269,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
     for (;; tile += a.tps) {
     const AttTile t = att_tile<32, PAGED>(a, b, tile);
-    if (t.r0 >= t.rows) return;
+    if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
     const int r = min(t.r0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
     const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 31, t.rows - 1) / a.G;
     // the queries' operands; step s: dims 16 s + 8 h ..
@@ -481,6 +477,254 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     }
 }
 
+// ---- rows of one tile of 16 ------------------------------------------------------------------------
+// The same with v_mfma_f32_16x16x32 for the rows of single tokens, and for calls whose 32-row tiles leave CUs without
+// work: half the registers, so 12 waves a CU have their loads in flight.  Lane l supplies key row l % 16 of two
+// 16-key tiles and query row l % 16, each as the 8 dims of group g = l / 16 of 32, and ends with query row l % 16 and keys
+// 16 t + 4 g + i; the 8 probabilities of a lane are the operand of V's product in place, V's rows are loaded 8 keys by
+// HD / 16 dims a lane, and dim (HD / 16) m + u is row m of product u.
+template <typename T> __device__ __forceinline__ qt_f32x4 att_mma16(qt_u32x4 a, qt_u32x4 b, qt_f32x4 c) { return qt_mfma_bf16(a, b, c); }
+template <> __device__ __forceinline__ qt_f32x4 att_mma16<QtF16>(qt_u32x4 a, qt_u32x4 b, qt_f32x4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qt_f16x8, a), __builtin_bit_cast(qt_f16x8, b), c, 0, 0, 0);
+}
+template <typename T, int NA, int NB>
+__device__ __forceinline__ qt_f32x4 att_planes16(const qt_u32x4 (&a)[NA], const qt_u32x4 (&b)[NB], qt_f32x4 c) {
+#pragma unroll
+    for (int s = NA + NB - 2; s >= 0; s--)
+#pragma unroll
+        for (int i = 0; i < NA; i++)
+            if (s - i >= 0 && s - i < NB && s <= 2) c = att_mma16<T>(a[i], b[s - i], c);
+    return c;
+}
+// over the four groups of a query row's lanes
+__device__ __forceinline__ float att_max4(float v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float t = fmaxf(__uint_as_float(p[0]), __uint_as_float(p[1]));
+    const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+    return fmaxf(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+__device__ __forceinline__ float att_sum4(float v) {
+    const auto p = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    const float t = __uint_as_float(p[0]) + __uint_as_float(p[1]);
+    const auto q = __builtin_amdgcn_permlane32_swap(__float_as_uint(t), __float_as_uint(t), false, false);
+    return __uint_as_float(q[0]) + __uint_as_float(q[1]);
+}
+
+template <typename QT, typename KT, int HD, bool PAGED>
+__global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(sizeof(typename KT::elem) == 4 ? 2 : 3))) void k_att_one(AttArgs a) {
+    constexpr bool QF = sizeof(typename QT::elem) == 4, KF = sizeof(typename KT::elem) == 4;
+    constexpr int EQ = sizeof(typename QT::elem), EK = sizeof(typename KT::elem);
+    constexpr int NU = HD / 16, NS = HD / 32, NQ = QF ? 3 : 1, NK = KF ? 3 : 1;
+    constexpr int OB = 16 * HD * 4;                     // one wave's sums
+    __shared__ __align__(16) uint8_t sm[OB * ATT_WV];   // QF: first the queries' planes [plane][16][HD] bf16
+    __shared__ float sst[2][ATT_WV][16];
+    __shared__ __align__(16) long long voff[PAGED ? ATT_WV : 1][32];
+    static_assert(3 * 16 * HD * 2 <= OB * ATT_WV, "the queries' planes and the sums share the LDS");
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
+    const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
+    const int b = a.tps > 0 ? slot / a.tps : att_find<16>(a, slot);
+    if (b < 0 || b >= a.B) return;
+    int tile = a.tps > 0 ? slot % a.tps : slot - att_first<16>(a, b);
+    const int *table = PAGED ? a.table + b * a.ts : nullptr;
+    for (;; tile += a.tps) {
+    const AttTile t = att_tile<16, PAGED>(a, b, tile);
+    if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
+    const int r = min(t.r0 + li, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
+    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 15, t.rows - 1) / a.G;
+    // the queries' operands; step s: dims 32 s + 8 g ..
+    qt_u32x4 qf[QF ? 1 : NS];
+    if constexpr (QF) {
+        for (int u = tid; u < 16 * (HD / 8); u += 64 * ATT_WV) {
+            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1);
+            float v[8];
+            qt_u32x4 pl[3];
+            qt_load8<QT>(a.q + ((size_t)((t.q0 + rr / a.G) * a.qs) + (size_t)(head * a.G + rr % a.G) * HD + 8 * ch) * EQ, v);
+            qt_planes8(v, pl);
+#pragma unroll
+            for (int p = 0; p < 3; p++)
+                *reinterpret_cast<qt_u32x4 *>(sm + (p * 16 + row) * HD * 2 + 16 * (ch ^ (row & (HD / 8 - 1)))) = pl[p];
+        }
+        __syncthreads();
+    } else {
+        const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + 8 * g) * EQ;
+#pragma unroll
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + 32 * s * EQ);
+    }
+    // the range's 32-key blocks
+    const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
+    const int kb0 = min((long long)blk1, blk0 + (long long)split * a.chunk), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk);
+    float m = -INFINITY, l = 0.f;                       // l: of this group's keys
+    const qt_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+    qt_f32x4 o[NU];
+#pragma unroll
+    for (int u = 0; u < NU; u++) o[u] = zero;
+    const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD) + 8 * g) * EK;
+    const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + NU * li) * EK;
+    int page = PAGED && kb0 + wave < kb1 ? att_page(a, table, t, 32 * (kb0 + wave) + (lane & 31)) : 0;
+    for (int kb = kb0 + wave; kb < kb1; kb += ATT_WV) {
+        const int key = 32 * kb + (lane & 31);
+        qt_u32x4 kr[2][NS][KF ? 2 : 1];
+        uint32_t vr[8][NU * EK / 4];
+        uint32_t ok;                                    // keys of the block that exist
+        long long koff[2];
+        if constexpr (PAGED) {
+            ok = (uint32_t)__ballot(page >= 0);
+            const long long off = att_instead(att_slot(a, page, key), page >= 0, ok);
+            __builtin_amdgcn_wave_barrier();
+            if (lane < 32) voff[wave][lane] = off;
+            __builtin_amdgcn_wave_barrier();
+#pragma unroll
+            for (int u = 0; u < 2; u++) koff[u] = voff[wave][16 * u + li];
+            page = kb + ATT_WV < kb1 ? att_page(a, table, t, key + 32 * ATT_WV) : 0;
+        } else {
+            ok = (uint32_t)__ballot(key < t.kmax);
+#pragma unroll
+            for (int u = 0; u < 2; u++) koff[u] = (long long)(t.q0 + min(32 * kb + 16 * u + li, t.kmax - 1)) * a.ks_slot;
+        }
+#pragma unroll
+        for (int u = 0; u < 2; u++)
+#pragma unroll
+            for (int s = 0; s < NS; s++)
+#pragma unroll
+                for (int e = 0; e < (KF ? 2 : 1); e++)
+                    kr[u][s][e] = *reinterpret_cast<const qt_u32x4 *>(kbase + (koff[u] + 32 * s) * EK + 16 * e);
+        const auto values = [&] {
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int vk = 16 * (j >> 2) + 4 * g + (j & 3);
+                const long long vo = PAGED ? voff[wave][vk] : (long long)(t.q0 + min(32 * kb + vk, t.kmax - 1)) * a.vs_slot;
+                __builtin_memcpy(vr[j], __builtin_assume_aligned(vbase + vo * EK, NU * EK < 16 ? NU * EK : 16), NU * EK);
+            }
+        };
+        if constexpr (!KF) values();
+        qt_f32x4 sc[2];
+#pragma unroll
+        for (int u = 0; u < 2; u++) {
+            sc[u] = zero;
+#pragma unroll
+            for (int s = 0; s < NS; s++) {
+                qt_u32x4 ka[NK], qa[NQ];
+                if constexpr (KF) {
+                    float v[8];
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = __uint_as_float(kr[u][s][e >> 2][e & 3]);
+                    qt_planes8(v, ka);
+                } else {
+                    ka[0] = kr[u][s][0];
+                }
+#pragma unroll
+                for (int p = 0; p < NQ; p++)
+                    if constexpr (QF) qa[p] = qt_lds16(sm + (p * 16 + li) * HD * 2 + 16 * ((4 * s + g) ^ (li & (HD / 8 - 1))));
+                    else qa[p] = qf[s];
+                sc[u] = att_planes16<KT, NK, NQ>(ka, qa, sc[u]);
+            }
+        }
+        if constexpr (KF) {                             // f32 keys leave no room for the values earlier
+            __builtin_amdgcn_sched_barrier(0);
+            values();
+        }
+        if (!(ok == 0xFFFFFFFFu && 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window))) {
+            const int d = pos - 32 * kb - 4 * g, w = a.window > 0 ? d - a.window : -1000;
+            const uint32_t mine = ok >> (4 * g);
+#pragma unroll
+            for (int u = 0; u < 2; u++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int j = 16 * u + i;
+                    sc[u][i] = j <= d && j > w && (mine >> j & 1u) ? sc[u][i] : -INFINITY;
+                }
+        }
+        float bm = fmaxf(fmaxf(fmaxf(sc[0][0], sc[0][1]), fmaxf(sc[0][2], sc[0][3])), fmaxf(fmaxf(sc[1][0], sc[1][1]), fmaxf(sc[1][2], sc[1][3])));
+        bm = fmaxf(m, att_max4(bm));
+        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c, f = qt_exp2((m - mr) * a.c);
+        m = bm;
+        float p[8], sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            p[j] = qt_exp2(fmaf(sc[j >> 2][j & 3], a.c, -mc));
+            sum += p[j];
+        }
+        l = l * f + sum;
+        qt_u32x4 pb[NQ];
+        if constexpr (QF) {
+            qt_planes8(p, pb);
+        } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) pb[0][j] = qt_round2<QT>(p[2 * j], p[2 * j + 1]);
+        }
+#pragma unroll
+        for (int u = 0; u < NU; u++) {
+            qt_u32x4 va[NK];
+            if constexpr (KF) {
+                float v[8];
+#pragma unroll
+                for (int j = 0; j < 8; j++) v[j] = __uint_as_float(vr[j][u]);
+                qt_planes8(v, va);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    va[0][j] = __builtin_amdgcn_perm(vr[2 * j + 1][u >> 1], vr[2 * j][u >> 1], u & 1 ? 0x07060302u : 0x05040100u);
+            }
+            o[u] = att_planes16<KT, NK, NQ>(va, pb, o[u] * f);
+        }
+    }
+    l = att_sum4(l);
+    if (g == 0) { sst[0][wave][li] = m; sst[1][wave][li] = l; }
+    __syncthreads();                                    // also: the queries' planes are read
+    {
+        float M = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < ATT_WV; w++) M = fmaxf(M, sst[0][w][li]);
+        const float f = M == -INFINITY ? 0.f : qt_exp2((m - M) * a.c);
+        float *os = reinterpret_cast<float *>(sm + wave * OB) + li * HD;
+#pragma unroll
+        for (int i = 0; i < 4; i++)
+#pragma unroll
+            for (int u = 0; u < NU; u++) os[NU * ((4 * g + i) ^ li) + u] = o[u][i] * f;
+    }
+    __syncthreads();
+    bool bad = false;
+    {
+        const int row = tid >> 4, mm = tid & 15, rr = t.r0 + row;
+        float M = -INFINITY, L = 0.f, v[NU];
+#pragma unroll
+        for (int w = 0; w < ATT_WV; w++) M = fmaxf(M, sst[0][w][row]);
+#pragma unroll
+        for (int u = 0; u < NU; u++) v[u] = 0.f;
+        if (M != -INFINITY)
+#pragma unroll
+            for (int w = 0; w < ATT_WV; w++) L += sst[1][w][row] * qt_exp2((sst[0][w][row] - M) * a.c);
+#pragma unroll
+        for (int w = 0; w < ATT_WV; w++)
+#pragma unroll
+            for (int u = 0; u < NU; u++) v[u] += (reinterpret_cast<const float *>(sm + w * OB) + row * HD)[NU * (mm ^ row) + u];
+        float chk = L;
+#pragma unroll
+        for (int u = 0; u < NU; u++) chk = fmaf(v[u], 0.f, chk);
+        if (rr < t.rows) {
+            bad = !(chk - chk == 0.f);
+            const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G;
+            if (a.splits > 1) {
+                const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + hd;
+                if (kb0 < kb1) att_put<QtF32, NU>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NU * mm), v);
+                if (mm == 0) { a.pm[2 * prow] = M; a.pm[2 * prow + 1] = L; }
+            } else {
+                const float inv = L > 0.f ? 1.0f / L : 0.f;
+#pragma unroll
+                for (int u = 0; u < NU; u++) v[u] *= inv;
+                att_put<QT, NU>(a.out + (tk * a.os + hd * HD + NU * mm) * EQ, v);
+            }
+        }
+    }
+    att_stored();
+    if (__syncthreads_or(bad))
+        for (int row = wave; row < 16 && t.r0 + row < t.rows; row += ATT_WV)
+            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, a.splits > 1, split);
+    if (a.tps <= 0) return;
+    __syncthreads();                                    // the next tile's planes take the LDS
+    }
+}
+
 // ---- many rows -----------------------------------------------------------------------------------
 // A workgroup takes 128 rows, 32 a wave, and goes through its keys 64 at a time: K and V of a block are copied from
 // memory straight into LDS (no registers), two blocks deep, one barrier a block, and every wave reads both
@@ -535,7 +779,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     // where this lane's copies read: row crow + i RPC of a block, and the chunk that belongs at its place
     const int crow = wave * NC * RPC + lane / CPR, cc = lane % CPR;
     const AttTile t = att_tile<128, PAGED>(a, b, tile);
-    if (t.r0 >= t.rows) return;
+    if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
     const int w0 = t.r0 + 32 * wave, r = min(w0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
     // the wave's first and last position
     const int first = t.shift + min(w0, t.rows - 1) / a.G, last = t.shift + min(w0 + 31, t.rows - 1) / a.G;
@@ -751,18 +995,31 @@ __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
 
 // The kernel, its launch slots and key ranges.  Launch slots: by request (max_q as far as known) or by rows, whichever is
 // fewer.  Key ranges: enough workgroups to fill the CUs, 256 keys each at least.
-struct AttPlan { bool tile; long long slots; };
+enum AttKind { ATT_ONE, ATT_FEW, ATT_TILE };
+struct AttPlan { AttKind kind; long long slots; };
 static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_split) {
     AttPlan p;
+    const long long rows = (long long)a.T * a.G;
+    const auto slots = [&](int tr) {
+        const long long by_rows = rows / tr + a.B, tps = ((long long)max_q * a.G + tr - 1) / tr, by_req = tps * a.B;
+        a.tps = max_q > 0 && by_req <= by_rows ? (int)tps : 0;
+        return a.tps > 0 ? by_req : by_rows;
+    };
     // 16-bit rows, 64 a request on average: many rows
-    p.tile = dtype != QWEN_HIP_DT_F32 && (long long)a.T * a.G >= 64ll * a.B;
-    const int tr = p.tile ? 128 : 32;
-    const long long by_rows = (long long)a.T * a.G / tr + a.B;
-    const long long tps = ((long long)max_q * a.G + tr - 1) / tr, by_req = tps * a.B;
-    a.tps = !p.tile && max_q > 0 && by_req <= by_rows ? (int)tps : 0;
-    p.slots = a.tps > 0 ? by_req : by_rows;
+    if (dtype != QWEN_HIP_DT_F32 && rows >= 64ll * a.B) {
+        p.kind = ATT_TILE;
+        p.slots = rows / 128 + a.B;
+        a.tps = 0;
+    } else {
+        p.kind = ATT_FEW;
+        p.slots = slots(32);
+        if ((max_q > 0 && (long long)max_q * a.G <= 16) || p.slots * a.nkv < 256) {
+            p.kind = ATT_ONE;
+            p.slots = slots(16);
+        }
+    }
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
-    long long n = wgs > 0 ? ((p.tile ? 512 : 4096) + wgs - 1) / wgs : 1;
+    long long n = wgs > 0 ? ((p.kind == ATT_TILE ? 512 : 4096) + wgs - 1) / wgs : 1;
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
     if (n < 1 || !may_split) n = 1;
@@ -809,12 +1066,9 @@ extern "C" long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_page
 template <typename QT, typename KT, int HD, bool PAGED>
 static hipError_t att_launch(const AttArgs &a, const AttPlan &plan, hipStream_t st) {
     const dim3 grid((unsigned)(plan.slots * a.nkv), a.splits);
-    if constexpr (sizeof(typename QT::elem) == 2) {
-        if (plan.tile) hipLaunchKernelGGL((k_att_tile<QT, HD, PAGED>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
-    } else {
-        hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
-    }
+    if (plan.kind == ATT_ONE) hipLaunchKernelGGL((k_att_one<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
+    else if (plan.kind == ATT_FEW) hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
+    else if constexpr (sizeof(typename QT::elem) == 2) hipLaunchKernelGGL((k_att_tile<QT, HD, PAGED>), grid, dim3(256), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.splits > 1) {
         const long long rows = (long long)a.T * a.nkv * a.G;

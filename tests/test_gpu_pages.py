@@ -623,13 +623,15 @@ def test_packed_hidden_values_never_reach_a_row(t):
     assert bool(out[100:].isnan().all()) and not bool(out[57:90].isfinite().any())
 
 
-def test_packed_offsets_out_of_range_stay_inside():
-    """Offsets past T or backwards touch nothing outside the tensors."""
-    rows = torch.randn(20, 8 * 64, device=DEV).to(torch.bfloat16)
-    out = torch.full((24, 256), 7.0, dtype=torch.bfloat16, device=DEV)
-    for cu in ([0, 8, 500], [0, 15, 10], [-4, 6, 20], [2 ** 31 - 1, -2 ** 31, 7]):
-        ok(packed(rows, [0, 0], 4, 2, 64, "bf16", out, cu=i32(cu)))
-    assert bool((out[20:] == 7).all())
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("T,nh", [(20, 4), (400, 4), (2000, 16)])
+def test_packed_offsets_out_of_range_stay_inside(t, T, nh):
+    """Offsets past T or backwards write nothing outside the tensors (16-row, 32-row and 128-row tiles)."""
+    rows = torch.randn(T, 8 * nh // 4 * 64, device=DEV).to(TYPES[t])
+    out = torch.full((T + 24, nh * 64), 7.0, dtype=TYPES[t], device=DEV)
+    for cu in ([0, T // 2, 25 * T], [0, T - 5, T // 2], [-4, 6, T], [2 ** 31 - 1, -2 ** 31, 7], [T, 0, T], [T - 1, 3, T - 1]):
+        ok(packed(rows, [0, 0], nh, nh // 2, 64, t, out[12:], cu=i32(cu)))
+    assert bool((out[:12] == 7).all()) and bool((out[12 + T:] == 7).all())
 
 
 def test_packed_matches_the_prefill_attention():
