@@ -294,6 +294,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     // the range's 32-key blocks
     const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
     const int kb0 = min((long long)blk1, blk0 + (long long)split * a.chunk), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk);
+    const bool part = a.splits > 1 && blk1 - blk0 > a.chunk;             // else the first range has it all
+    if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
     float m = -INFINITY, l = 0.f;                       // l: of this half's keys
     qt_f32x16 o[NT];
 #pragma unroll
@@ -457,12 +459,13 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         if (rr >= t.rows) continue;
         bad |= !(chk - chk == 0.f);
         const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G, at = tk * (a.nkv * a.G) + hd;
-        if (a.splits > 1) {
+        if (part) {
             const size_t prow = (size_t)split * a.T * (a.nkv * a.G) + at;
             if (kb0 < kb1) att_put<QtF32, NT>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NT * mm), v);
             if (mm == 0) { a.pm[2 * prow] = M; a.pm[2 * prow + 1] = L; }
         } else {
             const float inv = L > 0.f ? 1.0f / L : 0.f;
+            if (a.splits > 1 && mm == 0) a.pm[2 * at + 1] = -1.0f;
 #pragma unroll
             for (int d = 0; d < NT; d++) v[d] *= inv;
             att_put<QT, NT>(a.out + (tk * a.os + hd * HD + NT * mm) * EQ, v);
@@ -471,7 +474,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     att_stored();
     if (__syncthreads_or(bad))
         for (int row = wave; row < 32 && t.r0 + row < t.rows; row += ATT_WV)
-            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, a.splits > 1, split);
+            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, part, split);
     if (a.tps <= 0) return;
     __syncthreads();                                    // the next tile's planes take the LDS
     }
@@ -559,6 +562,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     // the range's 32-key blocks
     const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
     const int kb0 = min((long long)blk1, blk0 + (long long)split * a.chunk), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk);
+    const bool part = a.splits > 1 && blk1 - blk0 > a.chunk;             // else the first range has it all
+    if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
     float m = -INFINITY, l = 0.f;                       // l: of this group's keys
     const qt_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     qt_f32x4 o[NU];
@@ -715,12 +720,13 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         if (rr < t.rows) {
             bad = !(chk - chk == 0.f);
             const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G;
-            if (a.splits > 1) {
+            if (part) {
                 const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + hd;
                 if (kb0 < kb1) att_put<QtF32, NU>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NU * mm), v);
                 if (mm == 0) { a.pm[2 * prow] = M; a.pm[2 * prow + 1] = L; }
             } else {
                 const float inv = L > 0.f ? 1.0f / L : 0.f;
+                if (a.splits > 1 && mm == 0) a.pm[2 * (tk * (a.nkv * a.G) + hd) + 1] = -1.0f;
 #pragma unroll
                 for (int u = 0; u < NU; u++) v[u] *= inv;
                 att_put<QT, NU>(a.out + (tk * a.os + hd * HD + NU * mm) * EQ, v);
@@ -730,7 +736,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     att_stored();
     if (__syncthreads_or(bad))
         for (int row = wave; row < 16 && t.r0 + row < t.rows; row += ATT_WV)
-            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, a.splits > 1, split);
+            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, part, split);
     if (a.tps <= 0) return;
     __syncthreads();                                    // the next tile's planes take the LDS
     }
@@ -803,6 +809,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     // the range's 64-key blocks; chunk is in blocks of 32, even
     const int blk0 = t.lo / 64, blk1 = t.hi > t.lo ? (t.hi + 63) / 64 : blk0;
     const int kb0 = min((long long)blk1, blk0 + (long long)split * (a.chunk / 2)), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk / 2);
+    const bool part = a.splits > 1 && blk1 - blk0 > a.chunk / 2;         // else the first range has it all
+    if (split > 0 && !part) return;
     float m = -INFINITY, l = 0.f;                       // m: the maximum so far, or up to 2^8 under it; l: of this half's keys
     qt_f32x16 o[NT];
 #pragma unroll
@@ -942,7 +950,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const bool live = w0 + lr < t.rows;
     const size_t tk = t.q0 + tok;
     if (live) {
-        if (a.splits > 1) {
+        if (part) {
             const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + qh;
             if (kb0 < kb1)
 #pragma unroll
@@ -954,6 +962,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             if (h == 0) { a.pm[2 * prow] = m; a.pm[2 * prow + 1] = l; }
         } else {
             const float inv = l > 0.f ? 1.0f / l : 0.f;
+            if (a.splits > 1 && h == 0) a.pm[2 * (tk * (a.nkv * a.G) + qh) + 1] = -1.0f;
             uint8_t *op = a.out + (tk * a.os + (size_t)qh * HD + 4 * h) * 2;
 #pragma unroll
             for (int d = 0; d < NT; d++)
@@ -966,7 +975,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     if (__ballot(live && !(chk - chk == 0.f))) {
         att_stored();
         for (int row = w0; row < min(w0 + 32, t.rows); row++)
-            att_serial<T, T, HD, PAGED>(a, t, table, head, row, 64 * kb0, 64 * kb1, a.splits > 1, split);
+            att_serial<T, T, HD, PAGED>(a, t, table, head, row, 64 * kb0, 64 * kb1, part, split);
     }
 }
 
@@ -979,23 +988,32 @@ __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
     const long long at = (long long)blockIdx.x * 4 + (threadIdx.x >> 6), rows = (long long)a.T * nh;
     if (at >= rows) return;
     const int tok = (int)(at / nh), hd = (int)(at % nh);
-    if (tok < att_cu(a, 0) || tok >= att_cu(a, a.B)) return;      // rows of no request stay
     float m = -INFINITY, l = 0.f;
     if (lane < a.splits) {
         m = a.pm[2 * (lane * rows + at)];
         l = a.pm[2 * (lane * rows + at) + 1];
     }
+    if (tok < att_cu(a, 0) || tok >= att_cu(a, a.B)) return;      // rows of no request stay
+    if (lane_bcast(l, 0) < 0.f) return;                           // the first range had all its keys and wrote it
     const float M = group_max<64>(m), f = l == 0.f ? 0.f : qt_exp2((m - M) * a.c);
-    const unsigned long long some = __ballot(l != 0.f);
     const float L = group_sum<64>(l * f);
     float o[D];
 #pragma unroll
     for (int e = 0; e < D; e++) o[e] = 0.f;
-    for (int s = 0; s < a.splits; s++) {
-        if (!(some >> s & 1)) continue;
-        const float fs = lane_bcast(f, s);
+    for (unsigned long long some = __ballot(l != 0.f); some;) {   // four ranges' loads at a time
+        float v[4][D], fs[4];
 #pragma unroll
-        for (int e = 0; e < D; e++) o[e] = fmaf(fs, a.po[(s * rows + at) * HD + D * lane + e], o[e]);
+        for (int k = 0; k < 4; k++) {
+            const int s = some ? __ffsll(some) - 1 : 0;
+            fs[k] = some ? lane_bcast(f, s) : 0.f;
+#pragma unroll
+            for (int e = 0; e < D; e++) v[k][e] = some ? a.po[(s * rows + at) * HD + D * lane + e] : 0.f;
+            some &= some - 1;
+        }
+#pragma unroll
+        for (int k = 0; k < 4; k++)
+#pragma unroll
+            for (int e = 0; e < D; e++) o[e] = fmaf(fs[k], v[k][e], o[e]);
     }
     const float inv = L == 0.f ? 0.f : 1.0f / L;
 #pragma unroll

@@ -440,6 +440,9 @@ def test_page_attention_single_tokens(t, kv, nh, nkv, hd):
     reqs = [(0, 1), (1, 1), (30, 1), (31, 1), (32, 1), (15, 1), (700, 1), (255, 1), (256, 1), (333, 1)]
     Paged(reqs, nh, nkv, hd, t, kv, 16, "head", seed=1).check()
     Paged(reqs[:3], nh, nkv, hd, t, kv, 5, "slot", seed=2, window=17).check()
+    # as if the longest held 10^5 keys: many ranges, streamed; of 256 keys, and the last range takes what is left
+    Paged(reqs, nh, nkv, hd, t, kv, 16, "slot", seed=2, max_kv=100000).check()
+    Paged(reqs, nh, nkv, hd, t, kv, 16, "slot", seed=2, max_kv=512).check()
 
 
 @pytest.mark.parametrize("t,kv", KINDS)
