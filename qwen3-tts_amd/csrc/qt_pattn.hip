@@ -29,6 +29,7 @@
 #include "qt_ops.h"
 #include "qt_planes.h"
 #include <type_traits>
+#include <stdlib.h>
 
 typedef float qt_f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 qt_f16x8 __attribute__((ext_vector_type(8)));
@@ -44,11 +45,12 @@ struct AttArgs {
     const int *cu, *kv_len, *table;
     long long ts;
     int cols, n_pages, ps;
+    int near;                               // paged: every element of k (of v) within 2^32 bytes of its first
     QtDiv div;
     int B, T, nkv, G, window;
     float c;                                // scale log2(e)
     int tps;                                // > 0: launch slots a request, else slots by att_find
-    int splits, chunk;                      // key ranges a tile, 32-key blocks in each (the last takes the rest)
+    int splits, chunk;                      // key ranges a tile at most, 32-key blocks in each (att_ranges)
     float *po, *pm;                         // splits > 1: sums [split][T nh][HD], and maximum, sum [split][T nh][2]
 };
 
@@ -95,52 +97,58 @@ template <int TR> __device__ __forceinline__ int att_find(const AttArgs &a, int 
     return b;
 }
 
-// The tile of 128 rows that comes at `slot` when all requests' tiles are in the order of their keys, longest first: few
-// workgroups are left over at the end, and the long ones share a CU with short ones.  Tile i of a request weighs s + i, s
-// the keys before its new tokens in tiles' measure; how many tiles weigh w or more is a sum over the requests (four a lane), and
-// a search by halves finds the weight that holds the slot: under half a us for 64 requests and 8192 keys.  False: no tile.
+// The tile of 128 rows that comes at `slot` when the requests are in the order of their keys, longest first (in 64s), and
+// each one's tiles from its last to its first: little work is left for the end, and tiles that read the same keys run at
+// the same time and find them in the L2.  How many tiles belong to requests of w keys or more is a sum over the requests (four
+// a lane); a search by halves finds the w that holds the slot, a running sum the request among its equals: about half
+// a us.  False: no tile.
 #define ATT_SORT_B 256
 template <bool PAGED> __device__ __forceinline__ bool att_longest(const AttArgs &a, int slot, int &b, int &tile) {
     const int lane = threadIdx.x & 63;
-    int n[4], s[4], top = 0;
+    int n[4], w[4], top = 0;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
         const int i = 64 * r + lane;
-        n[r] = s[r] = 0;
+        n[r] = w[r] = 0;
         if (i < a.B) {
-            const int q0 = att_cu(a, i), len = max(att_cu(a, i + 1) - q0, 0);
+            const int len = max(att_cu(a, i + 1) - att_cu(a, i), 0);
             n[r] = (len * a.G + 127) / 128;
-            if (PAGED) s[r] = (int)((long long)max(min(a.kv_len[i], ATT_MAX_KEYS) - len, 0) * a.G / 128);
-            top = max(top, s[r] + n[r]);
+            w[r] = (PAGED ? min(max(a.kv_len[i], 0), ATT_MAX_KEYS) : len) >> 6;
+            top = max(top, w[r]);
         }
     }
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
-    const auto heavier = [&](int w) {                   // tiles of weight w or more
+    const auto longer = [&](int x) {                    // tiles of requests of x or more
         int c = 0;
 #pragma unroll
-        for (int r = 0; r < 4; r++) c += n[r] - min(max(w - s[r], 0), n[r]);
+        for (int r = 0; r < 4; r++) c += w[r] >= x ? n[r] : 0;
         return group_sum_i<64>(c);
     };
-    if (heavier(0) <= slot) return false;
-    int lo = 0, hi = top, over = 0;                     // heavier(lo) > slot >= heavier(hi) = over
+    if (longer(0) <= slot) return false;
+    int lo = 0, hi = top + 1, over = 0;                 // longer(lo) > slot >= longer(hi) = over
     while (hi - lo > 1) {
-        const int mid = lo + (hi - lo) / 2, c = heavier(mid);
+        const int mid = lo + (hi - lo) / 2, c = longer(mid);
         if (c > slot) lo = mid; else { hi = mid; over = c; }
     }
-    int k = slot - over;                                // the k-th request with a tile of this weight
+    int k = slot - over;                                // the k-th tile of the requests of lo
     b = -1;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        const unsigned long long has = __ballot(s[r] <= lo && lo < s[r] + n[r]);
-        const int c = __popcll(has);
-        if (b < 0 && k < c) {
-            const int before = __builtin_amdgcn_mbcnt_hi((unsigned)(has >> 32), __builtin_amdgcn_mbcnt_lo((unsigned)has, 0));
-            const int at = __ffsll((unsigned long long)__ballot((has >> lane & 1) && before == k)) - 1;
-            b = 64 * r + at;
-            tile = lo - __builtin_amdgcn_readlane(s[r], at);
+        const int mine = w[r] == lo ? n[r] : 0;
+        int upto = mine;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += y;
         }
-        k -= c;
+        const unsigned long long past = __ballot(upto > k);
+        if (b < 0 && past) {
+            const int at = __ffsll((unsigned long long)past) - 1;
+            b = 64 * r + at;
+            tile = __builtin_amdgcn_readlane(upto, at) - 1 - k;
+        }
+        k -= __builtin_amdgcn_readlane(upto, 63);
     }
     return b >= 0;
 }
@@ -167,21 +175,29 @@ __device__ __forceinline__ AttTile att_tile(const AttArgs &a, int b, int tile) {
     return t;
 }
 
-// the page of a key, -1 for none
-__device__ __forceinline__ int att_page(const AttArgs &a, const int *table, const AttTile &t, int key) {
-    if (key >= t.kmax) return -1;
-    const int p = table[qt_quot(key, a.div)];
-    return (unsigned)p < (unsigned)a.n_pages ? p : -1;
+// The ranges that a tile's blocks of keys make, equal ones: of `chunk` blocks at most where the host's bound on the
+// keys holds, longer ones in as many ranges as there are where it does not.
+__device__ __forceinline__ int att_ranges(const AttArgs &a, int blocks, int chunk) {
+    return max(min((blocks + chunk - 1) / chunk, a.splits), 1);
 }
+
+// The table's entry for a key, -1 past the keys.  It is looked at (att_has) only where it is used: that waits for the
+// load, and with it for every load before it.
+__device__ __forceinline__ int att_page(const AttArgs &a, const int *table, const AttTile &t, int key) {
+    int p = -1;
+    if (key < t.kmax) p = table[qt_quot(key, a.div)];
+    return p;
+}
+__device__ __forceinline__ bool att_has(const AttArgs &a, int page) { return (unsigned)page < (unsigned)a.n_pages; }
 __device__ __forceinline__ long long att_slot(const AttArgs &a, int page, int key) {
-    return page < 0 ? 0 : page * a.ks_page + (key - qt_quot(key, a.div) * a.ps) * a.ks_slot;
+    return page * a.ks_page + (key - qt_quot(key, a.div) * a.ps) * a.ks_slot;
 }
 
 // A key that does not exist takes the place of one in its block that does (`ok`, not 0 in any block that is worked on unless
 // its pages are bad): places that nobody has written may hold NaN, which would send the tile to att_serial.
 __device__ __forceinline__ long long att_instead(long long off, bool mine, unsigned long long ok) {
     const int from = ok ? __ffsll((unsigned long long)ok) - 1 : 0;
-    const int lo = __builtin_amdgcn_readlane((int)off, from), hi = __builtin_amdgcn_readlane((int)(off >> 32), from);
+    const int lo = ok ? __builtin_amdgcn_readlane((int)off, from) : 0, hi = ok ? __builtin_amdgcn_readlane((int)(off >> 32), from) : 0;
     return mine ? off : (long long)(((unsigned long long)(unsigned)hi << 32) | (unsigned)lo);
 }
 
@@ -213,7 +229,7 @@ __device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const in
         long long ko, vo;
         if (PAGED) {
             const int p = att_page(a, table, t, j);
-            if (p < 0) continue;
+            if (!att_has(a, p)) continue;
             ko = vo = att_slot(a, p, j) + head * a.ks_head;
         } else {
             ko = (long long)(t.q0 + j) * a.ks_slot + head * HD;
@@ -293,9 +309,10 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     }
     // the range's 32-key blocks
     const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
-    const int kb0 = min((long long)blk1, blk0 + (long long)split * a.chunk), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk);
-    const bool part = a.splits > 1 && blk1 - blk0 > a.chunk;             // else the first range has it all
+    const int n = att_ranges(a, blk1 - blk0, a.chunk), size = (blk1 - blk0 + n - 1) / n;
+    const bool part = n > 1;                            // else the first range has it all
     if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
+    const int kb0 = min(blk1, blk0 + split * size), kb1 = min(blk1, kb0 + size);
     float m = -INFINITY, l = 0.f;                       // l: of this half's keys
     qt_f32x16 o[NT];
 #pragma unroll
@@ -311,8 +328,9 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         const int key = 32 * kb + lr;
         uint32_t ok;                                    // keys of the block that exist
         if constexpr (PAGED) {
-            ok = (uint32_t)__ballot(page >= 0);
-            const long long off = att_instead(att_slot(a, page, key), page >= 0, ok);
+            const bool has = att_has(a, page);
+            ok = (uint32_t)__ballot(has);
+            const long long off = att_instead(att_slot(a, page, key), has, ok);
             __builtin_amdgcn_wave_barrier();
             if (h == 0) voff[wave][lr] = off;
             __builtin_amdgcn_wave_barrier();
@@ -561,9 +579,10 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     }
     // the range's 32-key blocks
     const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
-    const int kb0 = min((long long)blk1, blk0 + (long long)split * a.chunk), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk);
-    const bool part = a.splits > 1 && blk1 - blk0 > a.chunk;             // else the first range has it all
+    const int n = att_ranges(a, blk1 - blk0, a.chunk), size = (blk1 - blk0 + n - 1) / n;
+    const bool part = n > 1;                            // else the first range has it all
     if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
+    const int kb0 = min(blk1, blk0 + split * size), kb1 = min(blk1, kb0 + size);
     float m = -INFINITY, l = 0.f;                       // l: of this group's keys
     const qt_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     qt_f32x4 o[NU];
@@ -579,8 +598,9 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         uint32_t ok;                                    // keys of the block that exist
         long long koff[2];
         if constexpr (PAGED) {
-            ok = (uint32_t)__ballot(page >= 0);
-            const long long off = att_instead(att_slot(a, page, key), page >= 0, ok);
+            const bool has = att_has(a, page);
+            ok = (uint32_t)__ballot(has);
+            const long long off = att_instead(att_slot(a, page, key), has, ok);
             __builtin_amdgcn_wave_barrier();
             if (lane < 32) voff[wave][lane] = off;
             __builtin_amdgcn_wave_barrier();
@@ -808,9 +828,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     }
     // the range's 64-key blocks; chunk is in blocks of 32, even
     const int blk0 = t.lo / 64, blk1 = t.hi > t.lo ? (t.hi + 63) / 64 : blk0;
-    const int kb0 = min((long long)blk1, blk0 + (long long)split * (a.chunk / 2)), kb1 = split == a.splits - 1 ? blk1 : min(blk1, kb0 + a.chunk / 2);
-    const bool part = a.splits > 1 && blk1 - blk0 > a.chunk / 2;         // else the first range has it all
+    const int n = att_ranges(a, blk1 - blk0, a.chunk / 2), size = (blk1 - blk0 + n - 1) / n;
+    const bool part = n > 1;                            // else the first range has it all
     if (split > 0 && !part) return;
+    const int kb0 = min(blk1, blk0 + split * size), kb1 = min(blk1, kb0 + size);
     float m = -INFINITY, l = 0.f;                       // m: the maximum so far, or up to 2^8 under it; l: of this half's keys
     qt_f32x16 o[NT];
 #pragma unroll
@@ -823,28 +844,44 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     unsigned long long okv = ~0ull, okk = ~0ull, okn = ~0ull;            // keys that exist: of the block of V, of K, of the next K
     // block kb to a K and a V buffer
     const auto copy = [&](int kb, uint8_t *kdst, uint8_t *vdst) {
-        long long off = 0;
-        int place = cc;
         if constexpr (PAGED) {
-            asm volatile("" : "+v"(place));              // addresses are formed here: held over the loop they cost 20 registers
-            okn = __ballot(page >= 0);
-            off = 2 * att_instead(att_slot(a, page, 64 * kb + lane), page >= 0, okn);
-        }
+            const bool has = att_has(a, page);
+            okn = __ballot(has);
+            const int key = 64 * kb + lane, from = okn ? __ffsll(okn) - 1 : 0;
+            if (a.near) {
+                const int c = qt_quot(key, a.div);
+                unsigned off = 2u * ((unsigned)page * (unsigned)a.ks_page + (unsigned)(key - c * a.ps) * (unsigned)a.ks_slot);
+                const unsigned other = okn ? (unsigned)__builtin_amdgcn_readlane((int)off, from) : 0u;
+                off = has ? off : other;
 #pragma unroll
-        for (int i = 0; i < NC; i++) {
-            const int row = crow + i * RPC, ck = 16 * (place ^ att_swk<HD>(row)), cv = 16 * (place ^ att_swv<HD>(row));
-            const int to = (wave * NC + i) * RPC * RB;
-            if constexpr (PAGED) {
-                const long long at = ((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row);
-                att_copy16(kbase + at + ck, kdst + to);
-                att_copy16(vbase + at + cv, vdst + to);
+                for (int i = 0; i < NC; i++) {
+                    const int row = crow + i * RPC, to = (wave * NC + i) * RPC * RB;
+                    const unsigned at = (unsigned)__shfl((int)off, row);
+                    att_copy16(kbase, at + 16 * (cc ^ att_swk<HD>(row)), kdst + to);
+                    att_copy16(vbase, at + 16 * (cc ^ att_swv<HD>(row)), vdst + to);
+                }
             } else {
+                int place = cc;
+                asm volatile("" : "+v"(place));          // addresses are formed here: held over the loop they cost 20 registers
+                const long long off = 2 * att_instead(att_slot(a, page, key), has, okn);
+#pragma unroll
+                for (int i = 0; i < NC; i++) {
+                    const int row = crow + i * RPC, to = (wave * NC + i) * RPC * RB;
+                    const long long at = ((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row);
+                    att_copy16(kbase + at + 16 * (place ^ att_swk<HD>(row)), kdst + to);
+                    att_copy16(vbase + at + 16 * (place ^ att_swv<HD>(row)), vdst + to);
+                }
+            }
+            page = kb + 1 < kb1 ? att_page(a, table, t, 64 * (kb + 1) + lane) : -1;
+        } else {
+#pragma unroll
+            for (int i = 0; i < NC; i++) {
+                const int row = crow + i * RPC, to = (wave * NC + i) * RPC * RB;
                 const int real = min(row, t.kmax - 1 - 64 * kb);         // rows past the sequence: its last one again
-                att_copy16(kbase + 64ll * kb * a.ks_slot * 2, (unsigned)(real * (int)a.ks_slot * 2 + ck), kdst + to);
-                att_copy16(vbase + 64ll * kb * a.vs_slot * 2, (unsigned)(real * (int)a.vs_slot * 2 + cv), vdst + to);
+                att_copy16(kbase + 64ll * kb * a.ks_slot * 2, (unsigned)(real * (int)a.ks_slot * 2 + 16 * (cc ^ att_swk<HD>(row))), kdst + to);
+                att_copy16(vbase + 64ll * kb * a.vs_slot * 2, (unsigned)(real * (int)a.vs_slot * 2 + 16 * (cc ^ att_swv<HD>(row))), vdst + to);
             }
         }
-        if (PAGED) page = kb + 1 < kb1 ? att_page(a, table, t, 64 * (kb + 1) + lane) : -1;
     };
     const auto scores = [&](qt_f32x16 (&sc)[2], const uint8_t *kbuf) {
 #pragma unroll
@@ -1053,6 +1090,7 @@ static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_s
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
     if (n < 1 || !may_split) n = 1;
+    if (may_split && getenv("QT_SPLIT")) n = atoi(getenv("QT_SPLIT"));
     a.splits = (int)n;
     a.chunk = (int)((blocks + n - 1) / n + 1) & ~1;
     if (a.chunk < 2) a.chunk = 2;
@@ -1135,6 +1173,7 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     a.cu = p->cu_q; a.kv_len = p->kv_len; a.table = p->table; a.ts = p->table_stride;
     a.cols = p->table_cols; a.n_pages = kv->n_pages; a.ps = kv->page_size; a.div = qt_div_of(kv->page_size);
     a.window = p->window <= ATT_MAX_KEYS ? p->window : 0;
+    a.near = (kv->n_pages - 1.0) * kv->page_stride + (kv->n_kv_heads - 1.0) * kv->head_stride + (kv->page_size - 1.0) * kv->slot_stride < 2147000000.0;
     a.c = p->scale * QT_LOG2E;
     a.po = (float *)p->workspace;
     a.pm = a.po + (size_t)a.splits * a.T * p->n_heads * kv->head_dim;
@@ -1157,8 +1196,8 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
     const int A = 16 / qt_dt_size(p->dtype);
     QT_REFUSE(qt_off16(p->q) || qt_off16(p->k) || qt_off16(p->v) || qt_off16(p->out), "packed_attention: pointers have to be aligned to 16 bytes");
     QT_REFUSE(p->q_stride % A || p->k_stride % A || p->v_stride % A || p->out_stride % A || p->q_stride < 0 || p->k_stride < 0 ||
-                  p->v_stride < 0 || p->out_stride < (long long)p->n_heads * p->head_dim,
-              "packed_attention: strides %lld, %lld, %lld, %lld (multiples of 16 bytes, out's at least a token's)", p->q_stride,
+                  p->v_stride < 0 || p->out_stride < (long long)p->n_heads * p->head_dim || p->k_stride >= 1 << 24 || p->v_stride >= 1 << 24,
+              "packed_attention: strides %lld, %lld, %lld, %lld (multiples of 16 bytes, out's at least a token's, k's and v's under 2^24)", p->q_stride,
               p->k_stride, p->v_stride, p->out_stride);
     AttArgs a = {};
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
