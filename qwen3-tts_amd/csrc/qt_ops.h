@@ -89,6 +89,28 @@ static inline QtDiv qt_div_of(int d) {
 }
 __device__ __forceinline__ int qt_quot(int n, QtDiv d) { return (int)(__umulhi(2u * (uint32_t)n, d.m) >> d.l); }
 
+// Over a wave's 64 lanes by DPP: the largest of non-negative v, in every lane; the running sum up to each lane.
+template <int CTRL, int ROWS> __device__ __forceinline__ int qt_dpp0(int v) {        // 0 from lanes that there are not
+    return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xf, false);
+}
+__device__ __forceinline__ int wave_scan_i(int v) {
+    v += qt_dpp0<0x111, 0xf>(v);                         // lanes 1, 2, 4, 8 before, in rows of 16
+    v += qt_dpp0<0x112, 0xf>(v);
+    v += qt_dpp0<0x114, 0xf>(v);
+    v += qt_dpp0<0x118, 0xf>(v);
+    v += qt_dpp0<DPP_BCAST15, 0xa>(v);
+    return v + qt_dpp0<DPP_BCAST31, 0xc>(v);
+}
+__device__ __forceinline__ int wave_max_i(int v) {
+    v = max(v, qt_dpp0<0x111, 0xf>(v));
+    v = max(v, qt_dpp0<0x112, 0xf>(v));
+    v = max(v, qt_dpp0<0x114, 0xf>(v));
+    v = max(v, qt_dpp0<0x118, 0xf>(v));
+    v = max(v, qt_dpp0<DPP_BCAST15, 0xa>(v));
+    v = max(v, qt_dpp0<DPP_BCAST31, 0xc>(v));
+    return __builtin_amdgcn_readlane(v, 63);
+}
+
 // ---- host side ----
 
 // Makes the stream's device the current one while a call launches (kernels are looked up for the

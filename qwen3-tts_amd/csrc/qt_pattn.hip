@@ -29,7 +29,6 @@
 #include "qt_ops.h"
 #include "qt_planes.h"
 #include <type_traits>
-#include <stdlib.h>
 
 typedef float qt_f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 qt_f16x8 __attribute__((ext_vector_type(8)));
@@ -46,7 +45,7 @@ struct AttArgs {
     long long ts;
     int cols, n_pages, ps;
     int near;                               // paged: every element of k (of v) within 2^32 bytes of its first
-    QtDiv div;
+    QtDiv div, gdiv;                        // by page_size, by G
     int B, T, nkv, G, window;
     float c;                                // scale log2(e)
     int tps;                                // > 0: launch slots a request, else slots by att_find
@@ -97,28 +96,52 @@ template <int TR> __device__ __forceinline__ int att_find(const AttArgs &a, int 
     return b;
 }
 
+// one tile's geometry, uniform over the workgroup
+struct AttTile {
+    int q0, rows, r0;           // first token of the request, its rows, the tile's first row
+    int shift, kmax;            // a token's position is shift + its place; keys at or past kmax do not exist
+    int lo, hi;                 // keys that some row of the tile may see
+};
+// one request's tokens and keys
+struct AttReq { int q0, n, kv; };
+template <bool PAGED> __device__ __forceinline__ AttReq att_req(const AttArgs &a, int b) {
+    const int q0 = att_cu(a, b), n = max(att_cu(a, b + 1) - q0, 0);
+    return {q0, n, PAGED ? min(max(a.kv_len[b], 0), ATT_MAX_KEYS) : n};
+}
+template <int TR, bool PAGED>
+__device__ __forceinline__ AttTile att_tile(const AttArgs &a, AttReq q, int tile) {
+    AttTile t;
+    t.q0 = q.q0;
+    const int n = q.n, kv = q.kv;
+    t.rows = n * a.G;
+    t.r0 = TR * tile;
+    t.kmax = PAGED ? min(kv, a.cols * a.ps) : n;
+    t.shift = kv - n;
+    const int first = t.shift + qt_quot(t.r0, a.gdiv), last = t.shift + qt_quot(min(t.r0 + TR - 1, t.rows - 1), a.gdiv);
+    t.lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
+    t.hi = min(t.kmax, last + 1);
+    return t;
+}
+
 // The tile of 128 rows that comes at `slot` when the requests are in the order of their keys, longest first (in 64s), and
 // each one's tiles from its last to its first: little work is left for the end, and tiles that read the same keys run at
 // the same time and find them in the L2.  How many tiles belong to requests of w keys or more is a sum over the requests (four
 // a lane); a search by halves finds the w that holds the slot, a running sum the request among its equals: about half
 // a us.  False: no tile.
 #define ATT_SORT_B 256
-template <bool PAGED> __device__ __forceinline__ bool att_longest(const AttArgs &a, int slot, int &b, int &tile) {
+template <bool PAGED> __device__ __forceinline__ bool att_longest(const AttArgs &a, int slot, int &b, int &tile, AttReq &req) {
     const int lane = threadIdx.x & 63;
+    AttReq q[4];
     int n[4], w[4], top = 0;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        const int i = 64 * r + lane;
-        n[r] = w[r] = 0;
-        if (i < a.B) {
-            const int len = max(att_cu(a, i + 1) - att_cu(a, i), 0);
-            n[r] = (len * a.G + 127) / 128;
-            w[r] = (PAGED ? min(max(a.kv_len[i], 0), ATT_MAX_KEYS) : len) >> 6;
-            top = max(top, w[r]);
-        }
+        q[r] = {0, 0, 0};
+        if (64 * r < a.B && 64 * r + lane < a.B) q[r] = att_req<PAGED>(a, 64 * r + lane);
+        n[r] = (q[r].n * a.G + 127) / 128;
+        w[r] = q[r].kv >> 6;
+        top = max(top, w[r]);
     }
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) top = max(top, __shfl_xor(top, o, 64));
+    top = wave_max_i(top);
     const auto longer = [&](int x) {                    // tiles of requests of x or more
         int c = 0;
 #pragma unroll
@@ -135,44 +158,18 @@ template <bool PAGED> __device__ __forceinline__ bool att_longest(const AttArgs 
     b = -1;
 #pragma unroll
     for (int r = 0; r < 4; r++) {
-        const int mine = w[r] == lo ? n[r] : 0;
-        int upto = mine;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(upto, o, 64);
-            if (lane >= o) upto += y;
-        }
+        if (b >= 0 || 64 * r >= a.B) break;
+        const int upto = wave_scan_i(w[r] == lo ? n[r] : 0);
         const unsigned long long past = __ballot(upto > k);
-        if (b < 0 && past) {
+        if (past) {
             const int at = __ffsll((unsigned long long)past) - 1;
             b = 64 * r + at;
             tile = __builtin_amdgcn_readlane(upto, at) - 1 - k;
+            req = {__builtin_amdgcn_readlane(q[r].q0, at), __builtin_amdgcn_readlane(q[r].n, at), __builtin_amdgcn_readlane(q[r].kv, at)};
         }
         k -= __builtin_amdgcn_readlane(upto, 63);
     }
     return b >= 0;
-}
-
-// one tile's geometry, uniform over the workgroup
-struct AttTile {
-    int q0, rows, r0;           // first token of the request, its rows, the tile's first row
-    int shift, kmax;            // a token's position is shift + its place; keys at or past kmax do not exist
-    int lo, hi;                 // keys that some row of the tile may see
-};
-template <int TR, bool PAGED>
-__device__ __forceinline__ AttTile att_tile(const AttArgs &a, int b, int tile) {
-    AttTile t;
-    t.q0 = att_cu(a, b);
-    const int n = max(att_cu(a, b + 1) - t.q0, 0);
-    t.rows = n * a.G;
-    t.r0 = TR * tile;
-    const int kv = PAGED ? min(max(a.kv_len[b], 0), ATT_MAX_KEYS) : n;
-    t.kmax = PAGED ? min(kv, a.cols * a.ps) : n;
-    t.shift = kv - n;
-    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + TR - 1, t.rows - 1) / a.G;
-    t.lo = a.window > 0 ? max(first - a.window + 1, 0) : 0;
-    t.hi = min(t.kmax, last + 1);
-    return t;
 }
 
 // The ranges that a tile's blocks of keys make, equal ones: of `chunk` blocks at most where the host's bound on the
@@ -218,7 +215,7 @@ template <typename QT, int NT> __device__ __forceinline__ void att_put(uint8_t *
 template <typename QT, typename KT, int HD, bool PAGED>
 __device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const int *table, int head, int r, int k0, int k1, bool part, int split) {
     constexpr int EQ = sizeof(typename QT::elem), EK = sizeof(typename KT::elem), D = HD / 64;
-    const int lane = threadIdx.x & 63, tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
+    const int lane = threadIdx.x & 63, tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
     const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD) * EQ;
     float q[D], o[D], m = -INFINITY, l = 0.f;
 #pragma unroll
@@ -283,19 +280,20 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     if (b < 0 || b >= a.B) return;
     int tile = a.tps > 0 ? slot % a.tps : slot - att_first<32>(a, b);
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
+    const AttReq req = att_req<PAGED>(a, b);
     for (;; tile += a.tps) {
-    const AttTile t = att_tile<32, PAGED>(a, b, tile);
+    const AttTile t = att_tile<32, PAGED>(a, req, tile);
     if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
-    const int r = min(t.r0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
-    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 31, t.rows - 1) / a.G;
+    const int r = min(t.r0 + lr, t.rows - 1), tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
+    const int first = t.shift + qt_quot(t.r0, a.gdiv), last = t.shift + qt_quot(min(t.r0 + 31, t.rows - 1), a.gdiv);
     // the queries' operands; step s: dims 16 s + 8 h ..
     qt_u32x4 qf[NQ == 1 ? NS : 1];
     if constexpr (QF) {
         for (int u = tid; u < 32 * (HD / 8); u += 64 * ATT_WV) {
-            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1);
+            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1), tk = qt_quot(rr, a.gdiv);
             float v[8];
             qt_u32x4 pl[3];
-            qt_load8<QT>(a.q + ((size_t)((t.q0 + rr / a.G) * a.qs) + (size_t)(head * a.G + rr % a.G) * HD + 8 * ch) * EQ, v);
+            qt_load8<QT>(a.q + ((size_t)((t.q0 + tk) * a.qs) + (size_t)(head * a.G + rr - tk * a.G) * HD + 8 * ch) * EQ, v);
             qt_planes8(v, pl);
 #pragma unroll
             for (int p = 0; p < 3; p++)
@@ -476,7 +474,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         for (int d = 0; d < NT; d++) chk = fmaf(v[d], 0.f, chk);
         if (rr >= t.rows) continue;
         bad |= !(chk - chk == 0.f);
-        const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G, at = tk * (a.nkv * a.G) + hd;
+        const int rt = qt_quot(rr, a.gdiv);
+        const size_t tk = t.q0 + rt, hd = head * a.G + rr - rt * a.G, at = tk * (a.nkv * a.G) + hd;
         if (part) {
             const size_t prow = (size_t)split * a.T * (a.nkv * a.G) + at;
             if (kb0 < kb1) att_put<QtF32, NT>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NT * mm), v);
@@ -553,19 +552,20 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     if (b < 0 || b >= a.B) return;
     int tile = a.tps > 0 ? slot % a.tps : slot - att_first<16>(a, b);
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
+    const AttReq req = att_req<PAGED>(a, b);
     for (;; tile += a.tps) {
-    const AttTile t = att_tile<16, PAGED>(a, b, tile);
+    const AttTile t = att_tile<16, PAGED>(a, req, tile);
     if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
-    const int r = min(t.r0 + li, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
-    const int first = t.shift + t.r0 / a.G, last = t.shift + min(t.r0 + 15, t.rows - 1) / a.G;
+    const int r = min(t.r0 + li, t.rows - 1), tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
+    const int first = t.shift + qt_quot(t.r0, a.gdiv), last = t.shift + qt_quot(min(t.r0 + 15, t.rows - 1), a.gdiv);
     // the queries' operands; step s: dims 32 s + 8 g ..
     qt_u32x4 qf[QF ? 1 : NS];
     if constexpr (QF) {
         for (int u = tid; u < 16 * (HD / 8); u += 64 * ATT_WV) {
-            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1);
+            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1), tk = qt_quot(rr, a.gdiv);
             float v[8];
             qt_u32x4 pl[3];
-            qt_load8<QT>(a.q + ((size_t)((t.q0 + rr / a.G) * a.qs) + (size_t)(head * a.G + rr % a.G) * HD + 8 * ch) * EQ, v);
+            qt_load8<QT>(a.q + ((size_t)((t.q0 + tk) * a.qs) + (size_t)(head * a.G + rr - tk * a.G) * HD + 8 * ch) * EQ, v);
             qt_planes8(v, pl);
 #pragma unroll
             for (int p = 0; p < 3; p++)
@@ -739,7 +739,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         for (int u = 0; u < NU; u++) chk = fmaf(v[u], 0.f, chk);
         if (rr < t.rows) {
             bad = !(chk - chk == 0.f);
-            const size_t tk = t.q0 + rr / a.G, hd = head * a.G + rr % a.G;
+            const int rt = qt_quot(rr, a.gdiv);
+        const size_t tk = t.q0 + rt, hd = head * a.G + rr - rt * a.G;
             if (part) {
                 const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + hd;
                 if (kb0 < kb1) att_put<QtF32, NU>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NU * mm), v);
@@ -775,14 +776,12 @@ template <int HD> __device__ __forceinline__ int att_swv(int row) { return HD ==
 // 16 bytes a lane from memory to LDS at dst + 16 lane (dst uniform), as assembly: the compiler, which would take
 // every later LDS read for a reader of these bytes, does not wait for them; att_wait does.  The second form reads at
 // base + off, base uniform.
-__device__ __forceinline__ unsigned att_lds(void *dst) {
-    return __builtin_amdgcn_readfirstlane((unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst);
+__device__ __forceinline__ unsigned att_lds(void *dst) { return (unsigned)(uintptr_t)(__attribute__((address_space(3))) void *)dst; }
+__device__ __forceinline__ void att_copy16(const uint8_t *src, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
-__device__ __forceinline__ void att_copy16(const uint8_t *src, void *dst) {
-    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(src), "s"(att_lds(dst)) : "memory", "m0");
-}
-__device__ __forceinline__ void att_copy16(const uint8_t *base, unsigned off, void *dst) {
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(att_lds(dst)) : "memory", "m0");
+__device__ __forceinline__ void att_copy16(const uint8_t *base, unsigned off, unsigned dst) {
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(__builtin_amdgcn_readfirstlane(dst)) : "memory", "m0");
 }
 __device__ __forceinline__ void att_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
@@ -793,15 +792,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
     int b, tile;
+    AttReq req;
     if (a.B <= ATT_SORT_B) {
-        if (!att_longest<PAGED>(a, slot, b, tile)) return;
+        if (!att_longest<PAGED>(a, slot, b, tile, req)) return;
     } else {
         b = att_find<128>(a, slot);
         if (b < 0) return;
         tile = slot - att_first<128>(a, b);
+        req = att_req<PAGED>(a, b);
     }
     b = __builtin_amdgcn_readfirstlane(b);
     tile = __builtin_amdgcn_readfirstlane(tile);
+    req = {__builtin_amdgcn_readfirstlane(req.q0), __builtin_amdgcn_readfirstlane(req.n), __builtin_amdgcn_readfirstlane(req.kv)};
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
     // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4
     int ka[NS], va[NT];
@@ -815,11 +817,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     }
     // where this lane's copies read: row crow + i RPC of a block, and the chunk that belongs at its place
     const int crow = wave * NC * RPC + lane / CPR, cc = lane % CPR;
-    const AttTile t = att_tile<128, PAGED>(a, b, tile);
+    const AttTile t = att_tile<128, PAGED>(a, req, tile);
     if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
-    const int w0 = t.r0 + 32 * wave, r = min(w0 + lr, t.rows - 1), tok = r / a.G, qh = head * a.G + r % a.G, pos = t.shift + tok;
+    const int w0 = t.r0 + 32 * wave, r = min(w0 + lr, t.rows - 1), tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
     // the wave's first and last position
-    const int first = t.shift + min(w0, t.rows - 1) / a.G, last = t.shift + min(w0 + 31, t.rows - 1) / a.G;
+    const int first = t.shift + qt_quot(min(w0, t.rows - 1), a.gdiv), last = t.shift + qt_quot(min(w0 + 31, t.rows - 1), a.gdiv);
     qt_u32x4 qf[NS];
     {
         const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + 8 * h) * 2;
@@ -843,7 +845,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     int page = -1;                                                       // PAGED: of key 64 kb + lane, block kb the next to copy
     unsigned long long okv = ~0ull, okk = ~0ull, okn = ~0ull;            // keys that exist: of the block of V, of K, of the next K
     // block kb to a K and a V buffer
-    const auto copy = [&](int kb, uint8_t *kdst, uint8_t *vdst) {
+    const unsigned lk = att_lds(sk), lv = att_lds(sv);
+    const auto copy = [&](int kb, unsigned kdst, unsigned vdst) {
         if constexpr (PAGED) {
             const bool has = att_has(a, page);
             okn = __ballot(has);
@@ -905,7 +908,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         okk = okn;
         const uint8_t *vbuf = sv + vb * 64 * RB;
         vb = vb == 2 ? 0 : vb + 1;
-        if (kb + 2 < kb1) copy(kb + 2, sk + BUF * 64 * RB, sv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
+        if (kb + 2 < kb1) copy(kb + 2, lk + BUF * 64 * RB, lv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
         if (64 * kb + 63 > first || (a.window > 0 && 64 * kb <= last - a.window)) {
             const int d = pos - 64 * kb - 4 * h, w = a.window > 0 ? d - a.window : -1000;
 #pragma unroll
@@ -965,9 +968,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     };
     if (kb0 < kb1) {
         if (PAGED) page = att_page(a, table, t, 64 * kb0 + lane);
-        copy(kb0, sk, sv);
+        copy(kb0, lk, lv);
         okk = okn;
-        if (kb0 + 1 < kb1) copy(kb0 + 1, sk + 64 * RB, sv + 64 * RB);
+        if (kb0 + 1 < kb1) copy(kb0 + 1, lk + 64 * RB, lv + 64 * RB);
         att_wait();
         __syncthreads();
         qt_f32x16 s0[2], s1[2];
@@ -1065,6 +1068,7 @@ enum AttKind { ATT_ONE, ATT_FEW, ATT_TILE };
 struct AttPlan { AttKind kind; long long slots; bool stream; };
 static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_split) {
     AttPlan p;
+    a.gdiv = qt_div_of(a.G);
     const long long rows = (long long)a.T * a.G;
     const auto slots = [&](int tr) {
         const long long by_rows = rows / tr + a.B, tps = ((long long)max_q * a.G + tr - 1) / tr, by_req = tps * a.B;
@@ -1090,7 +1094,6 @@ static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_s
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
     if (n < 1 || !may_split) n = 1;
-    if (may_split && getenv("QT_SPLIT")) n = atoi(getenv("QT_SPLIT"));
     a.splits = (int)n;
     a.chunk = (int)((blocks + n - 1) / n + 1) & ~1;
     if (a.chunk < 2) a.chunk = 2;
