@@ -568,7 +568,8 @@ int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *attn, void *strea
  *   t listed in bias_tok[bias_off[b] .. bias_off[b+1]):  x += bias_val of its last entry
  *   bit t % 32 of mask[b*mask_stride + t / 32] is 0:     x = -infinity
  * in f32, rounded once to dtype (of logits and out).  rep, presence, frequency, bias_tok and mask may each be NULL:
- * off.  Tokens outside [0, V) are passed over; offsets are clipped to hist_cap / bias_cap entries.  out may be
+ * off.  Tokens outside [0, V) are passed over; offsets are clipped to hist_cap / bias_cap entries, a row's biases to
+ * its first 65534, and n_out counts up to 65535.  out may be
  * logits (same stride).  A row whose mask allows nothing is all -infinity.  B <= 65535. */
 typedef struct {
     const void *logits;

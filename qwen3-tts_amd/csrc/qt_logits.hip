@@ -5,7 +5,9 @@
 // its biases: those are marked in LDS, then counted there (integer atomics: the order does not matter; of a token's
 // bias entries the largest index wins), and a thread goes through the marked ones of its own before it stores.  So a row's
 // history is read once a workgroup, from the L2, and no counts of V tokens a row are held in memory, cleared or read back.
-// Bound by the logits' bytes for a large vocabulary, by the latency of offsets, history and logits for a small one.
+// A token has one word, its count in the lower 16 bits and its last bias entry in the upper, so that eight workgroups fit a CU.
+// Bound by the logits' bytes for a large vocabulary (and the chain of offsets, history, marks and counts before the first
+// store), by that latency alone for a small one.
 #include "qt_ops.h"
 
 #define RULES_T 256
@@ -30,53 +32,61 @@ struct RulesArgs {
 template <typename T, bool BIAS, bool EACH>
 __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
     constexpr int E = sizeof(typename T::elem), NV = RULES_CH / RULES_T / 8;
-    __shared__ unsigned bits[RULES_CH / 32], seen[RULES_CH / 32], said[RULES_CH], times[EACH ? RULES_CH : 1];
-    __shared__ int last[BIAS ? RULES_CH : 1];
+    __shared__ unsigned bits[RULES_CH / 32], seen[RULES_CH / 32], word[RULES_CH], times[EACH ? RULES_CH : 1];
     __shared__ float value[BIAS ? RULES_T : 1];         // of the first bias entries
     const int tid = threadIdx.x, b = blockIdx.y, v0 = blockIdx.x * RULES_CH, n = min(RULES_CH, a.V - v0);
     const bool counts = a.rep || a.pres || a.freq;
     const uint8_t *xr = a.x + ((size_t)b * a.xs + v0) * E;
     uint8_t *yr = a.out + ((size_t)b * a.os + v0) * E;
     const uint32_t *mr = a.mask ? a.mask + (size_t)b * a.ms + v0 / 32 : nullptr;
-    // a thread's tokens: 8 at 8 tid + 8 RULES_T v
-    float x[NV][8];
-    uint32_t allow[NV];
-#pragma unroll
-    for (int v = 0; v < NV; v++) {
-        const int i = 8 * (tid + RULES_T * v);
-        allow[v] = mr && i < n ? mr[i >> 5] >> (i & 31) : 0xFFu;
-        if (i + 8 <= n) qt_load8<T, E>(xr + (size_t)i * E, x[v]);
-    }
     const int h0 = counts ? max(a.hoff[b], 0) : 0, h1 = counts ? min(a.hoff[b + 1], a.hcap) : 0;
-    const int e0 = BIAS ? max(a.boff[b], 0) : 0, e1 = BIAS ? min(a.boff[b + 1], a.bcap) : 0;
+    const int e0 = BIAS ? max(a.boff[b], 0) : 0, e1 = BIAS ? (int)min((long long)min(a.boff[b + 1], a.bcap), e0 + 65534ll) : 0;
     const float rep = a.rep ? a.rep[b] : 1.f, pres = a.pres ? a.pres[b] : 0.f, freq = a.freq ? a.freq[b] : 0.f;
     const long long h2 = h0 + (long long)(counts && a.npr ? max(a.npr[b], 0) : 0);
-    unsigned held[RULES_HELD];
+    const bool full = (long long)h1 - h0 > 65535;       // counts may reach the word's lower half
+    unsigned held[RULES_HELD], held_bias = ~0u;
 #pragma unroll
     for (int k = 0; k < RULES_HELD; k++) {
         const int i = h0 + tid + k * RULES_T;
         held[k] = i < h1 ? (unsigned)a.hist[i] - (unsigned)v0 : ~0u;
     }
-    unsigned held_bias = ~0u;
     if (BIAS && e0 + tid < e1) {
         held_bias = (unsigned)a.btok[e0 + tid] - (unsigned)v0;
         value[tid] = a.bval[e0 + tid];
+    }
+    // a thread's tokens: 8 at 8 tid + 8 RULES_T v, as they are in memory; after the lists, whose marks need not wait for them
+    qt_w4 raw[NV][E / 2];
+    uint32_t allow[NV];
+#pragma unroll
+    for (int v = 0; v < NV; v++) {
+        const int i = 8 * (tid + RULES_T * v);
+        allow[v] = mr && i < n ? mr[i >> 5] >> (i & 31) : 0xFFu;
+        if (i + 8 <= n)
+#pragma unroll
+            for (int e = 0; e < E / 2; e++) raw[v][e] = qt_load16<E>(xr + (size_t)i * E + 16 * e);
     }
     if (tid < RULES_CH / 32) bits[tid] = seen[tid] = 0;
     __syncthreads();
     const auto mark = [&](unsigned t, bool hist) {
         if (t >= (unsigned)n) return;
-        said[t] = 0;                                    // the same from every thread
+        word[t] = 0;                                    // the same from every thread
         if (EACH) times[t] = 0;
-        if (BIAS) last[t] = -1;
-        const unsigned bit = 1u << (t & 31);
-        if (hist) atomicOr(&seen[t >> 5], bit);
-        else atomicOr(&bits[t >> 5], bit);
+        atomicOr(hist ? &seen[t >> 5] : &bits[t >> 5], 1u << (t & 31));
     };
     const auto count = [&](unsigned t, int i) {
         if (t >= (unsigned)n) return;
         if (EACH) atomicAdd(&times[t], 1u);
-        if (i >= h2) atomicAdd(&said[t], 1u);
+        if (i < h2) return;
+        if (!full) {
+            atomicAdd(&word[t], 1u);
+        } else {                                        // up to 65535
+            unsigned was = word[t], now;
+            while ((was & 0xFFFFu) != 0xFFFFu && (now = atomicCAS(&word[t], was, was + 1u)) != was) was = now;
+        }
+    };
+    // entry e of the biases, before any count: the largest word is the last entry's
+    const auto bias = [&](unsigned t, int e) {
+        if (t < (unsigned)n) atomicMax(&word[t], ((unsigned)e + 1u) << 16);
     };
 #pragma unroll
     for (int k = 0; k < RULES_HELD; k++) mark(held[k], true);
@@ -84,18 +94,14 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
     if (BIAS) {
         mark(held_bias, false);
         for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) mark((unsigned)a.btok[i] - (unsigned)v0, false);
+        __syncthreads();
+        bias(held_bias, tid);
+        for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) bias((unsigned)a.btok[i] - (unsigned)v0, i - e0);
     }
     __syncthreads();
 #pragma unroll
     for (int k = 0; k < RULES_HELD; k++) count(held[k], h0 + tid + k * RULES_T);
     for (int i = h0 + tid + RULES_HELD * RULES_T; i < h1; i += RULES_T) count((unsigned)a.hist[i] - (unsigned)v0, i);
-    if (BIAS) {
-        if (held_bias < (unsigned)n) atomicMax(&last[held_bias], tid);
-        for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) {
-            const unsigned t = (unsigned)a.btok[i] - (unsigned)v0;
-            if (t < (unsigned)n) atomicMax(&last[t], i - e0);
-        }
-    }
     __syncthreads();
     const auto rules = [&](float y, int t) {
         if (a.rep && (seen[t >> 5] >> (t & 31) & 1u)) {
@@ -103,12 +109,12 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
             float was;
             do { was = y; y = y > 0.f ? y / rep : y * rep; } while (--k && y != was);   // until nothing changes any more
         }
-        if (const unsigned o = said[t]) {
+        const unsigned w = word[t], o = w & 0xFFFFu, e = w >> 16;
+        if (o) {
             if (a.freq) y -= (float)o * freq;
             if (a.pres) y -= pres;
         }
-        if (BIAS)
-            if (const int e = last[t]; e >= 0) y += e < RULES_T ? value[e] : a.bval[e0 + e];
+        if (BIAS && e) y += e <= RULES_T ? value[e - 1] : a.bval[e0 + (int)e - 1];
         return y;
     };
 #pragma unroll
@@ -117,19 +123,21 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
         if (i >= n) continue;
         unsigned todo = (seen[i >> 5] | bits[i >> 5]) >> (i & 31) & allow[v] & 0xFFu;
         if (i + 8 <= n) {
+            float x[8];
+            qt_widen8<T>(raw[v], x);
             while (todo) {
                 const int e = __builtin_ctz(todo);
                 todo &= todo - 1;
-                float y = x[v][0];
+                float y = x[0];
 #pragma unroll
-                for (int k = 1; k < 8; k++) y = k == e ? x[v][k] : y;
+                for (int k = 1; k < 8; k++) y = k == e ? x[k] : y;
                 y = rules(y, i + e);
 #pragma unroll
-                for (int k = 0; k < 8; k++) x[v][k] = k == e ? y : x[v][k];
+                for (int k = 0; k < 8; k++) x[k] = k == e ? y : x[k];
             }
 #pragma unroll
-            for (int e = 0; e < 8; e++) x[v][e] = allow[v] >> e & 1u ? x[v][e] : -INFINITY;
-            qt_store8<T, E>(yr + (size_t)i * E, x[v]);
+            for (int e = 0; e < 8; e++) x[e] = allow[v] >> e & 1u ? x[e] : -INFINITY;
+            qt_store8<T, E>(yr + (size_t)i * E, x);
         } else {
             for (int e = 0; i + e < n; e++) {
                 float y = qt_load1<T>(xr + (size_t)(i + e) * E);

@@ -44,17 +44,20 @@ template <int A> __device__ __forceinline__ qt_w4 qt_load16(const void *p) {
     return a;
 }
 template <int A> __device__ __forceinline__ void qt_store16(void *p, qt_w4 a) { __builtin_memcpy(__builtin_assume_aligned(p, A), &a, 16); }
-template <typename T, int A = 16> __device__ __forceinline__ void qt_load8(const void *p, float (&v)[8]) {
-    const uint8_t *b = (const uint8_t *)p;
-    if constexpr (sizeof(typename T::elem) == 4) {
-        const qt_w4 x = qt_load16<A>(b), y = qt_load16<A>(b + 16);
+template <typename T, int N> __device__ __forceinline__ void qt_widen8(const qt_w4 (&w)[N], float (&v)[8]) {
+    if constexpr (N == 2) {
 #pragma unroll
-        for (int i = 0; i < 4; i++) { v[i] = __uint_as_float(x[i]); v[4 + i] = __uint_as_float(y[i]); }
+        for (int i = 0; i < 8; i++) v[i] = __uint_as_float(w[i >> 2][i & 3]);
     } else {
-        const qt_w4 x = qt_load16<A>(b);
 #pragma unroll
-        for (int i = 0; i < 4; i++) { v[2 * i] = qt_lo<T>(x[i]); v[2 * i + 1] = qt_hi<T>(x[i]); }
+        for (int i = 0; i < 4; i++) { v[2 * i] = qt_lo<T>(w[0][i]); v[2 * i + 1] = qt_hi<T>(w[0][i]); }
     }
+}
+template <typename T, int A = 16> __device__ __forceinline__ void qt_load8(const void *p, float (&v)[8]) {
+    qt_w4 w[sizeof(typename T::elem) / 2];
+#pragma unroll
+    for (unsigned e = 0; e < sizeof(typename T::elem) / 2; e++) w[e] = qt_load16<A>((const uint8_t *)p + 16 * e);
+    qt_widen8<T>(w, v);
 }
 template <typename T, int A = 16> __device__ __forceinline__ void qt_store8(void *p, const float (&v)[8]) {
     uint8_t *b = (uint8_t *)p;
