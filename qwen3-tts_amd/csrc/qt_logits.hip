@@ -1,18 +1,16 @@
 // qt_logits.hip — the rules on a batch's logits before sampling (qwen_hip_op_logit_rules): repetition,
 // presence and frequency penalties, token biases, an allowed-token bit mask.
 //
-// A workgroup takes RULES_CH neighbouring tokens of one row, 16 a thread, loaded at once.  Few of them are in the row's history or
+// A workgroup of RULES_T threads takes 16 RULES_T neighbouring tokens of one row, loaded at once.  Few of them are in the row's history or
 // its biases: those are marked in LDS, then counted there (integer atomics: the order does not matter; of a token's
 // bias entries the largest index wins), and a thread goes through the marked ones of its own before it stores.  So a row's
 // history is read once a workgroup, from the L2, and no counts of V tokens a row are held in memory, cleared or read back.
-// A token has one word, its count in the lower 16 bits and its last bias entry in the upper, so that eight workgroups fit a CU.
+// A token has one word, its count in the lower 16 bits and its last bias entry in the upper, so that all threads of a CU have one
+// in LDS.
 // Bound by the logits' bytes for a large vocabulary (and the chain of offsets, history, marks and counts before the first
 // store), by that latency alone for a small one.
 #include "qt_ops.h"
 
-#define RULES_T 256
-#define RULES_CH 4096
-#define RULES_HELD 16          // history entries a thread keeps between marking and counting
 
 struct RulesArgs {
     const uint8_t *x;
@@ -29,9 +27,10 @@ struct RulesArgs {
 
 // BIAS: with bias lists.  EACH: the penalty once for every entry.  Rows may begin anywhere that their elements can: 16-byte
 // accesses at 2- or 4-byte alignment are one instruction on this GPU.
-template <typename T, bool BIAS, bool EACH>
+template <typename T, bool BIAS, bool EACH, int RULES_T>
 __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
-    constexpr int E = sizeof(typename T::elem), NV = RULES_CH / RULES_T / 8;
+    constexpr int E = sizeof(typename T::elem), NV = 2, RULES_CH = 8 * NV * RULES_T;
+    constexpr int RULES_HELD = 4096 / RULES_T;          // history entries a thread keeps between marking and counting
     __shared__ unsigned bits[RULES_CH / 32], seen[RULES_CH / 32], word[RULES_CH], times[EACH ? RULES_CH : 1];
     __shared__ float value[BIAS ? RULES_T : 1];         // of the first bias entries
     const int tid = threadIdx.x, b = blockIdx.y, v0 = blockIdx.x * RULES_CH, n = min(RULES_CH, a.V - v0);
@@ -169,16 +168,24 @@ extern "C" int qwen_hip_op_logit_rules(const qwen_hip_logit_rules_t *p, void *st
     const RulesArgs a = {(const uint8_t *)p->logits, (uint8_t *)p->out, p->logits_stride, p->out_stride, p->mask_stride, p->hist,
                          p->hist_off, p->n_prompt, p->rep, p->presence, p->frequency, p->bias_tok, p->bias_val, p->bias_off,
                          p->mask, p->V, p->hist_cap, p->bias_cap, p->rep_each};
-    const dim3 grid((p->V + RULES_CH - 1) / RULES_CH, p->B);
+    // A row's history is read by each of its workgroups, so large vocabularies take large ones (64 rows of 128003 with histories
+    // of up to 4000: 11.5 us with 1024 threads, 12.4 with 512, 18.9 with 256); up to two small ones take those (6 rows
+    // of 2048: 5.8 us against 6.4).
+    const int threads = p->V > 8192 ? 1024 : 256;
+    const dim3 grid((p->V + 16 * threads - 1) / (16 * threads), p->B);
+#define RULES3(T, BIAS, EACH) do { \
+        if (threads == 1024) hipLaunchKernelGGL((k_logit_rules<T, BIAS, EACH, 1024>), grid, dim3(1024), 0, st, a); \
+        else hipLaunchKernelGGL((k_logit_rules<T, BIAS, EACH, 256>), grid, dim3(256), 0, st, a); } while (0)
 #define RULES(T) do { \
-        if (p->bias_tok && p->rep_each) hipLaunchKernelGGL((k_logit_rules<T, true, true>), grid, dim3(RULES_T), 0, st, a); \
-        else if (p->bias_tok) hipLaunchKernelGGL((k_logit_rules<T, true, false>), grid, dim3(RULES_T), 0, st, a); \
-        else if (p->rep_each) hipLaunchKernelGGL((k_logit_rules<T, false, true>), grid, dim3(RULES_T), 0, st, a); \
-        else hipLaunchKernelGGL((k_logit_rules<T, false, false>), grid, dim3(RULES_T), 0, st, a); } while (0)
+        if (p->bias_tok && p->rep_each) RULES3(T, true, true); \
+        else if (p->bias_tok) RULES3(T, true, false); \
+        else if (p->rep_each) RULES3(T, false, true); \
+        else RULES3(T, false, false); } while (0)
     if (p->dtype == QWEN_HIP_DT_F32) RULES(QtF32);
     else if (p->dtype == QWEN_HIP_DT_BF16) RULES(QtBf16);
     else RULES(QtF16);
 #undef RULES
+#undef RULES3
     const hipError_t e = hipGetLastError();
     QT_REFUSE(e != hipSuccess, "logit_rules: launch failed: %s", hipGetErrorString(e));
     return 0;

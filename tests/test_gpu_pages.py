@@ -682,7 +682,7 @@ def rules64(x, hist, npr, rep, pres, freq, bias, mask, each):
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("V,on,each", [(1, "rpfbm", 0), (7, "rpfbm", 0), (1000, "rpfbm", 1), (4099, "rpfbm", 0), (4099, "m", 0), (513, "b", 0),
-                                       (513, "f", 0), (513, "p", 0), (513, "r", 1), (100, "", 0), (8192, "rm", 0)])
+                                       (513, "f", 0), (513, "p", 0), (513, "r", 1), (100, "", 0), (8192, "rm", 0), (8193, "rpfbm", 0), (16385, "rpfb", 1)])
 def test_logit_rules(t, V, on, each):
     print(f"[case] rules {t} V={V} {on} each={each}", flush=True)
     rng = np.random.default_rng(V + len(on))
@@ -736,6 +736,33 @@ def test_logit_rules(t, V, on, each):
         assert bool(((g - want).abs() <= tol)[~inf].all()), (b, float((g - want).abs()[~inf].max()))
     call(dev["x"], V + pad)                                     # in place: the same bits
     assert torch.equal(dev["x"][:, :V].cpu(), got[:B, :V])
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_logit_rules_of_long_lists(t):
+    """A history past 65535 entries, one token in it more often than a count goes, and more biases than one a thread."""
+    V, n = 9001, 70000
+    rng = np.random.default_rng(8)
+    h = np.concatenate([np.full(66000, 7), rng.integers(0, V, n - 66000)])
+    rng.shuffle(h)
+    x = torch.from_numpy(rng.standard_normal(V)).to(TYPES[t])
+    btok, bval = rng.integers(0, V, 5000), rng.standard_normal(5000).astype(np.float32)
+    dev = [x.to(DEV), i32(h.tolist()), i32([0, n]), torch.tensor([1.2], device=DEV), torch.tensor([0.001], device=DEV), i32(btok.tolist()),
+           torch.from_numpy(bval).to(DEV), i32([0, 5000]), torch.empty(V, dtype=TYPES[t], device=DEV)]
+    d = hip.LogitRules(dtype=hip.DT[t], B=1, V=V, logits=dp(dev[0]), out=dp(dev[8]), logits_stride=V, out_stride=V, hist=dp(dev[1]),
+                       hist_off=dp(dev[2]), hist_cap=n, rep=dp(dev[3]), frequency=dp(dev[4]), bias_tok=dp(dev[5]), bias_val=dp(dev[6]),
+                       bias_off=dp(dev[7]), bias_cap=5000)
+    ok(hip.lib().qwen_hip_op_logit_rules(C.byref(d), stream()))
+    torch.cuda.synchronize()
+    c = np.minimum(np.bincount(h, minlength=V), 65535)
+    rep, freq = float(np.float32(1.2)), float(np.float32(0.001))
+    w = x.double().numpy()
+    w = np.where(c > 0, np.where(w > 0, w / rep, w * rep), w) - c * freq
+    last = np.zeros(V)
+    last[btok] = bval                                           # the last entry of a token counts
+    w = torch.from_numpy(w + last)
+    tol = 4 * 2.0 ** -24 * (w.abs() + torch.from_numpy(c * freq) + 8) + (0 if t == "f32" else 2.0 ** -8 * w.abs() * 1.01)
+    assert bool(((dev[8].double().cpu() - w).abs() <= tol).all())
 
 
 def test_rules_then_argmax_is_the_sampler_of_one_stream():
