@@ -6,16 +6,16 @@
 //
 // Rows.  The new tokens of a request and the query heads of one kv head make its rows, row r = (token r / G, head
 // r % G): heads that read the same keys share them, a decode step's heads fill a tile as a prompt's tokens do, and the
-// causal edge crosses few key blocks.  A tile is 32 rows.
+// causal edge crosses few key blocks.
 //
 // Products.  Scores are made transposed, S^T = K Q^T by v_mfma_f32_32x32x16: lane l supplies key row l % 32 (A) and
 // query row l % 32 (B), each as 8 of the 16 dims (those of half h = l / 32), and ends with query row l % 32 and keys
 // 8 (i / 4) + 4 h + i % 4 in register i.  So a lane has one query row: the softmax needs one exchange with the other
 // half, scaling a row's sums is one factor a lane, and eight of its probabilities are, in place, the B operand
 // of O^T = V^T P^T over 16 keys (a sum over keys in the order of the registers: key 16 s + 8 (j / 4) + 4 h + j % 4 in
-// place (h, j)).  V's operand wants those 8 keys of one dim: a lane loads NT = HD / 32 neighbouring dims of each
-// key's row (the 32 lanes of a half a whole row) and transposes them in registers by byte permutes; dim NT m + t is row
-// m of product t.
+// place (h, j)).  V's operand wants those 8 keys of one dim: read transposed from LDS where K and V are there (k_att_tile),
+// else a lane loads NT = HD / 32 neighbouring dims of each key's row (the 32 lanes of a half a whole row) and transposes
+// them in registers; dim NT m + t is row m of product t.
 //
 // Types.  16-bit rows over a cache of their type: one product each; the probabilities are rounded to that type for
 // V's product (bf16: at most 2^-8 of each, f16: 2^-11, of either sign over the keys; the sum of a row keeps them
@@ -259,149 +259,93 @@ __device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const in
 // Waits for the wave's stores: what it writes next to the same places comes after them.
 __device__ __forceinline__ void att_stored() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// ---- few rows ------------------------------------------------------------------------------------
-// A workgroup takes one 32-row tile and one range of its keys; its four waves take the range's 32-key blocks in
-// turn, each with a softmax of its own, K and V going from memory into operand registers without LDS or barriers;
-// the waves' sums are merged through LDS at the end, and the ranges' by k_att_merge.
 #define ATT_WV 4
-template <typename QT, typename KT, int HD, bool PAGED>
-__global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))) void k_att_few(AttArgs a) {
-    constexpr bool QF = sizeof(typename QT::elem) == 4, KF = sizeof(typename KT::elem) == 4;
-    constexpr int EQ = sizeof(typename QT::elem), EK = sizeof(typename KT::elem);
-    constexpr int NT = HD / 32, NS = HD / 16, NQ = QF ? 3 : 1, NK = KF ? 3 : 1;
+
+// ---- f32 prompts ---------------------------------------------------------------------------------
+// A workgroup takes 32 rows; its four waves take the 32-key blocks in turn, each with a softmax of its own, K and V
+// going from memory into operand registers without LDS or barriers and split there; the waves' sums are merged through
+// LDS at the end.  V is loaded when K is used up: both at once spill.  Bound by the splitting (VALU) next to the
+// products: two prompts of 4000 positions 922 us, 142 TFLOP/s of f32 products (a library's f32 matrix product of 8192^3:
+// 153); with V loaded ahead of the scores 1105, in 16-row tiles (k_att_one) 1377.
+template <int HD>
+__global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))) void k_att_f32(AttArgs a) {
+    constexpr int NT = HD / 32, NS = HD / 16;
     constexpr int OB = 32 * HD * 4;                     // one wave's sums
-    __shared__ __align__(16) uint8_t sm[OB * ATT_WV];   // QF: first the queries' planes [plane][32][HD] bf16
+    __shared__ __align__(16) uint8_t sm[OB * ATT_WV];   // first the queries' planes [plane][32][HD] bf16
     __shared__ float sst[2][ATT_WV][32];
-    __shared__ __align__(16) long long voff[PAGED ? ATT_WV : 1][32];
     static_assert(3 * 32 * HD * 2 <= OB * ATT_WV, "the queries' planes and the sums share the LDS");
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
-    const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
-    const int b = a.tps > 0 ? slot / a.tps : att_find<32>(a, slot);
-    if (b < 0 || b >= a.B) return;
-    int tile = a.tps > 0 ? slot % a.tps : slot - att_first<32>(a, b);
-    const int *table = PAGED ? a.table + b * a.ts : nullptr;
-    const AttReq req = att_req<PAGED>(a, b);
-    for (;; tile += a.tps) {
-    const AttTile t = att_tile<32, PAGED>(a, req, tile);
-    if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
-    const int r = min(t.r0 + lr, t.rows - 1), tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
-    const int first = t.shift + qt_quot(t.r0, a.gdiv), last = t.shift + qt_quot(min(t.r0 + 31, t.rows - 1), a.gdiv);
-    // the queries' operands; step s: dims 16 s + 8 h ..
-    qt_u32x4 qf[NQ == 1 ? NS : 1];
-    if constexpr (QF) {
-        for (int u = tid; u < 32 * (HD / 8); u += 64 * ATT_WV) {
-            const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1), tk = qt_quot(rr, a.gdiv);
-            float v[8];
-            qt_u32x4 pl[3];
-            qt_load8<QT>(a.q + ((size_t)((t.q0 + tk) * a.qs) + (size_t)(head * a.G + rr - tk * a.G) * HD + 8 * ch) * EQ, v);
-            qt_planes8(v, pl);
+    const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv;
+    const int b = att_find<32>(a, slot);
+    if (b < 0) return;
+    const int tile = slot - att_first<32>(a, b);
+    const AttTile t = att_tile<32, false>(a, att_req<false>(a, b), tile);
+    if (tile < 0 || t.r0 >= t.rows) return;             // (offsets that fall give tiles before the first)
+    const int r = min(t.r0 + lr, t.rows - 1), pos = qt_quot(r, a.gdiv);
+    const int first = qt_quot(t.r0, a.gdiv), last = qt_quot(min(t.r0 + 31, t.rows - 1), a.gdiv);
+    for (int u = tid; u < 32 * (HD / 8); u += 64 * ATT_WV) {
+        const int row = u / (HD / 8), ch = u % (HD / 8), rr = min(t.r0 + row, t.rows - 1), tk = qt_quot(rr, a.gdiv);
+        float v[8];
+        qt_u32x4 pl[3];
+        qt_load8<QtF32>(a.q + ((size_t)((t.q0 + tk) * a.qs) + (size_t)(head * a.G + rr - tk * a.G) * HD + 8 * ch) * 4, v);
+        qt_planes8(v, pl);
 #pragma unroll
-            for (int p = 0; p < 3; p++)
-                *reinterpret_cast<qt_u32x4 *>(sm + (p * 32 + row) * HD * 2 + 16 * (ch ^ (row & (HD / 8 - 1)))) = pl[p];
-        }
-        __syncthreads();
-    } else {
-        const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + 8 * h) * EQ;
-#pragma unroll
-        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + 16 * s * EQ);
+        for (int p = 0; p < 3; p++)
+            *reinterpret_cast<qt_u32x4 *>(sm + (p * 32 + row) * HD * 2 + 16 * (ch ^ (row & (HD / 8 - 1)))) = pl[p];
     }
-    // the range's 32-key blocks
-    const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
-    const int n = att_ranges(a, blk1 - blk0, a.chunk), size = (blk1 - blk0 + n - 1) / n;
-    const bool part = n > 1;                            // else the first range has it all
-    if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
-    const int kb0 = min(blk1, blk0 + split * size), kb1 = min(blk1, kb0 + size);
+    __syncthreads();
+    const int kb0 = t.lo / 32, kb1 = t.hi > t.lo ? (t.hi + 31) / 32 : kb0;
     float m = -INFINITY, l = 0.f;                       // l: of this half's keys
     qt_f32x16 o[NT];
 #pragma unroll
     for (int d = 0; d < NT; d++)
 #pragma unroll
         for (int i = 0; i < 16; i++) o[d][i] = 0.f;
-    const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD) + 8 * h) * EK;
-    const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + NT * lr) * EK;
-    qt_u32x4 kr[NS][KF ? 2 : 1];
-    uint32_t vr[2][8][NT * EK / 4];
-    int page = PAGED && kb0 + wave < kb1 ? att_page(a, table, t, 32 * (kb0 + wave) + lr) : 0;
+    const uint8_t *kbase = a.k + (head * HD + 8 * h) * 4, *vbase = a.v + (head * HD + NT * lr) * 4;
     for (int kb = kb0 + wave; kb < kb1; kb += ATT_WV) {
-        const int key = 32 * kb + lr;
-        uint32_t ok;                                    // keys of the block that exist
-        if constexpr (PAGED) {
-            const bool has = att_has(a, page);
-            ok = (uint32_t)__ballot(has);
-            const long long off = att_instead(att_slot(a, page, key), has, ok);
-            __builtin_amdgcn_wave_barrier();
-            if (h == 0) voff[wave][lr] = off;
-            __builtin_amdgcn_wave_barrier();
-            const uint8_t *kp = kbase + off * EK;
+        float kr[NS][8], vr[2][8][NT];
+        const uint8_t *kp = kbase + (long long)(t.q0 + min(32 * kb + lr, t.kmax - 1)) * a.ks_slot * 4;
 #pragma unroll
-            for (int s = 0; s < NS; s++) kr[s][0] = *reinterpret_cast<const qt_u32x4 *>(kp + 16 * s * EK);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const uint8_t *vp = vbase + voff[wave][16 * s + 8 * (j >> 2) + 4 * h + (j & 3)] * EK;
-                    __builtin_memcpy(vr[s][j], __builtin_assume_aligned(vp, NT * EK), NT * EK);
-                }
-            page = kb + ATT_WV < kb1 ? att_page(a, table, t, key + 32 * ATT_WV) : 0;
-        } else {
-            ok = key < t.kmax ? 1u : 0u;
-            ok = (uint32_t)__ballot(ok);
-            const uint8_t *kp = kbase + (long long)(t.q0 + min(key, t.kmax - 1)) * a.ks_slot * EK;
-#pragma unroll
-            for (int s = 0; s < NS; s++)
-#pragma unroll
-                for (int e = 0; e < (KF ? 2 : 1); e++) kr[s][e] = *reinterpret_cast<const qt_u32x4 *>(kp + 16 * s * EK + 16 * e);
-#pragma unroll
-            for (int s = 0; s < 2; s++)
-#pragma unroll
-                for (int j = 0; j < 8; j++) {
-                    const int vk = min(32 * kb + 16 * s + 8 * (j >> 2) + 4 * h + (j & 3), t.kmax - 1);
-                    const uint8_t *vp = vbase + (long long)(t.q0 + vk) * a.vs_slot * EK;
-                    __builtin_memcpy(vr[s][j], __builtin_assume_aligned(vp, NT * EK), NT * EK);
-                }
-        }
+        for (int s = 0; s < NS; s++) qt_load8<QtF32>(kp + 64 * s, kr[s]);
         qt_f32x16 sc;
 #pragma unroll
         for (int i = 0; i < 16; i++) sc[i] = 0.f;
 #pragma unroll
         for (int s = 0; s < NS; s++) {
-            qt_u32x4 ka[NK], qa[NQ];
-            if constexpr (KF) {
-                float v[8];
+            qt_u32x4 ka[3], qa[3];
+            qt_planes8(kr[s], ka);
 #pragma unroll
-                for (int e = 0; e < 8; e++) v[e] = __uint_as_float(kr[s][e >> 2][e & 3]);
-                qt_planes8(v, ka);
-            } else {
-                ka[0] = kr[s][0];
-            }
-#pragma unroll
-            for (int p = 0; p < NQ; p++)
-                if constexpr (QF) qa[p] = qt_lds16(sm + (p * 32 + lr) * HD * 2 + 16 * ((2 * s + h) ^ (lr & (HD / 8 - 1))));
-                else qa[p] = qf[s];
-            sc = att_planes<KT, NK, NQ>(ka, qa, sc);
+            for (int p = 0; p < 3; p++) qa[p] = qt_lds16(sm + (p * 32 + lr) * HD * 2 + 16 * ((2 * s + h) ^ (lr & (HD / 8 - 1))));
+            sc = att_planes<QtBf16, 3, 3>(ka, qa, sc);
         }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int s = 0; s < 2; s++)
+#pragma unroll
+            for (int j = 0; j < 8; j++) {
+                const int vk = min(32 * kb + 16 * s + 8 * (j >> 2) + 4 * h + (j & 3), t.kmax - 1);
+                __builtin_memcpy(vr[s][j], __builtin_assume_aligned(vbase + (long long)(t.q0 + vk) * a.vs_slot * 4, NT * 4), NT * 4);
+            }
         // hidden keys; a block that every row sees whole needs no look
-        if (!(ok == 0xFFFFFFFFu && 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window))) {
+        if (32 * kb + 31 > first || (a.window > 0 && 32 * kb <= last - a.window)) {
             const int d = pos - 32 * kb - 4 * h, w = a.window > 0 ? d - a.window : -1000;
-            const uint32_t mine = ok >> (4 * h);
 #pragma unroll
             for (int i = 0; i < 16; i++) {
                 const int j = 8 * (i >> 2) + (i & 3);
-                sc[i] = j <= d && j > w && (mine >> j & 1u) ? sc[i] : -INFINITY;
+                sc[i] = j <= d && j > w ? sc[i] : -INFINITY;
             }
         }
         float bm = m;
 #pragma unroll
         for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[i]);
         bm = fmaxf(bm, att_other_half(bm));
-        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c;
-        const float f = qt_exp2((m - mr) * a.c);
+        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c, f = qt_exp2((m - mr) * a.c);
         m = bm;
-        float p[16], sum = 0.f;
+        float p[2][8], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            p[i] = qt_exp2(fmaf(sc[i], a.c, -mc));
-            sum += p[i];
+            p[i >> 3][i & 7] = qt_exp2(fmaf(sc[i], a.c, -mc));
+            sum += p[i >> 3][i & 7];
         }
         l = l * f + sum;
 #pragma unroll
@@ -410,30 +354,16 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
             for (int i = 0; i < 16; i++) o[d][i] *= f;
 #pragma unroll
         for (int s = 0; s < 2; s++) {
-            qt_u32x4 pb[NQ];
-            if constexpr (QF) {
-                float v[8];
-#pragma unroll
-                for (int j = 0; j < 8; j++) v[j] = p[8 * s + j];
-                qt_planes8(v, pb);
-            } else {
-#pragma unroll
-                for (int j = 0; j < 4; j++) pb[0][j] = qt_round2<QT>(p[8 * s + 2 * j], p[8 * s + 2 * j + 1]);
-            }
+            qt_u32x4 pb[3];
+            qt_planes8(p[s], pb);
 #pragma unroll
             for (int d = 0; d < NT; d++) {
-                qt_u32x4 va[NK];
-                if constexpr (KF) {
-                    float v[8];
+                float v[8];
+                qt_u32x4 va[3];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) v[j] = __uint_as_float(vr[s][j][d]);
-                    qt_planes8(v, va);
-                } else {
-#pragma unroll
-                    for (int j = 0; j < 4; j++)
-                        va[0][j] = __builtin_amdgcn_perm(vr[s][2 * j + 1][d >> 1], vr[s][2 * j][d >> 1], d & 1 ? 0x07060302u : 0x05040100u);
-                }
-                o[d] = att_planes<KT, NK, NQ>(va, pb, o[d]);
+                for (int j = 0; j < 8; j++) v[j] = vr[s][j][d];
+                qt_planes8(v, va);
+                o[d] = att_planes<QtBf16, 3, 3>(va, pb, o[d]);
             }
         }
     }
@@ -475,26 +405,15 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
         if (rr >= t.rows) continue;
         bad |= !(chk - chk == 0.f);
         const int rt = qt_quot(rr, a.gdiv);
-        const size_t tk = t.q0 + rt, hd = head * a.G + rr - rt * a.G, at = tk * (a.nkv * a.G) + hd;
-        if (part) {
-            const size_t prow = (size_t)split * a.T * (a.nkv * a.G) + at;
-            if (kb0 < kb1) att_put<QtF32, NT>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NT * mm), v);
-            if (mm == 0) { a.pm[2 * prow] = M; a.pm[2 * prow + 1] = L; }
-        } else {
-            const float inv = L > 0.f ? 1.0f / L : 0.f;
-            if (a.splits > 1 && mm == 0) a.pm[2 * at + 1] = -1.0f;
+        const float inv = L > 0.f ? 1.0f / L : 0.f;
 #pragma unroll
-            for (int d = 0; d < NT; d++) v[d] *= inv;
-            att_put<QT, NT>(a.out + (tk * a.os + hd * HD + NT * mm) * EQ, v);
-        }
+        for (int d = 0; d < NT; d++) v[d] *= inv;
+        att_put<QtF32, NT>(a.out + ((size_t)((t.q0 + rt) * a.os) + (size_t)(head * a.G + rr - rt * a.G) * HD + NT * mm) * 4, v);
     }
     att_stored();
     if (__syncthreads_or(bad))
         for (int row = wave; row < 32 && t.r0 + row < t.rows; row += ATT_WV)
-            att_serial<QT, KT, HD, PAGED>(a, t, table, head, t.r0 + row, 32 * kb0, 32 * kb1, part, split);
-    if (a.tps <= 0) return;
-    __syncthreads();                                    // the next tile's planes take the LDS
-    }
+            att_serial<QtF32, QtF32, HD, false>(a, t, nullptr, head, t.r0 + row, 32 * kb0, 32 * kb1, false, 0);
 }
 
 // ---- rows of one tile of 16 ------------------------------------------------------------------------
@@ -1064,39 +983,44 @@ __global__ __launch_bounds__(256) void k_att_merge(AttArgs a) {
 
 // The kernel, its launch slots and key ranges.  Launch slots: by request (max_q as far as known) or by rows, whichever is
 // fewer.  Key ranges: enough workgroups to fill the CUs, 256 keys each at least.
-enum AttKind { ATT_ONE, ATT_FEW, ATT_TILE };
+enum AttKind { ATT_ONE, ATT_F32, ATT_TILE };
 struct AttPlan { AttKind kind; long long slots; bool stream; };
-static AttPlan att_plan(AttArgs &a, int dtype, int max_q, int max_kv, bool may_split) {
-    AttPlan p;
+static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv) {
+    AttPlan p = {ATT_ONE, 0, false};
     a.gdiv = qt_div_of(a.G);
+    a.tps = 0;
     const long long rows = (long long)a.T * a.G;
-    const auto slots = [&](int tr) {
-        const long long by_rows = rows / tr + a.B, tps = ((long long)max_q * a.G + tr - 1) / tr, by_req = tps * a.B;
-        a.tps = max_q > 0 && by_req <= by_rows ? (int)tps : 0;
-        return a.tps > 0 ? by_req : by_rows;
-    };
-    // 16-bit rows, 64 a request on average: many rows
-    if (dtype != QWEN_HIP_DT_F32 && rows >= 64ll * a.B) {
+    if (dtype == QWEN_HIP_DT_F32) {
+        // 32-row tiles for prompts while they give every CU work (one of 512 positions 23.7 us against 25.4 in 16-row tiles,
+        // 16 of 64 16.6 against 20.4; three of 21 to 128 11.9 against 8.9)
+        if (!paged && (rows / 32 + a.B) * a.nkv >= 256) p.kind = ATT_F32;
+    } else if (rows >= 32ll * a.B && (paged || (rows / 128 + a.B) * a.nkv >= 96)) {
+        // 128-row tiles from 32 rows a request on (64 requests of 32 tokens 42 us against 79 in 16-row tiles, 8 of 16 over
+        // 3000 keys 27.3 against 27.8, 32 of 4 70 against 60); prompts, whose keys are not split, while there are tiles
+        // enough (8 of 100 to 300 13.1 us against 20.3; one of 512 15.9 against 13.0, three of 21 to 128 9.2 against 8.4)
         p.kind = ATT_TILE;
-        p.slots = rows / 128 + a.B;
-        a.tps = 0;
-    } else {
-        p.kind = ATT_FEW;
-        p.slots = slots(32);
-        if ((max_q > 0 && (long long)max_q * a.G <= 16) || p.slots * a.nkv < 256) {
-            p.kind = ATT_ONE;
-            p.slots = slots(16);
-        }
     }
-    p.stream = false;
+    if (p.kind == ATT_ONE) {
+        const long long by_rows = rows / 16 + a.B, tps = ((long long)max_q * a.G + 15) / 16, by_req = tps * a.B;
+        if (max_q > 0 && by_req <= by_rows) a.tps = (int)tps;
+        p.slots = a.tps > 0 ? by_req : by_rows;
+    } else {
+        p.slots = rows / (p.kind == ATT_TILE ? 128 : 32) + a.B;
+    }
+    // Single tokens want many ranges (64 streams of up to 8000 keys: 2 of them 217 us, 8 199, 16 200), since a workgroup
+    // only reads; a tile's sums are large, and two workgroups a CU are enough (chunks over up to 7000 keys: 2 ranges
+    // 171 us, 1 226, 3 190, 4 205).
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
-    long long n = wgs > 0 ? ((p.kind == ATT_TILE ? 512 : 4096) + wgs - 1) / wgs : 1;
+    long long n = wgs > 0 && paged ? ((p.kind == ATT_TILE ? 512 : 4096) + wgs - 1) / wgs : 1;
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
-    if (n < 1 || !may_split) n = 1;
+    if (n < 1) n = 1;
     a.splits = (int)n;
     a.chunk = (int)((blocks + n - 1) / n + 1) & ~1;
     if (a.chunk < 2) a.chunk = 2;
+    // One tile a request: K and V are read once.  Past the 256 MB that the last-level cache holds they are not kept
+    // there (64 streams of up to 8000 keys 210 -> 200 us; 4 of 1500, whose 14 MB stay, 12.5 -> 13.8).
+    p.stream = a.tps == 1;
     return p;
 }
 
@@ -1123,10 +1047,8 @@ static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t 
               "page_attention: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
     a = AttArgs{};
     a.B = p->B; a.T = p->T; a.nkv = kv->n_kv_heads; a.G = p->n_heads / kv->n_kv_heads;
-    plan = att_plan(a, p->dtype, p->max_q < p->T ? p->max_q : p->T, p->max_kv, true);
-    // One tile a request: K and V are read once.  Past the 256 MB that the last-level cache holds they are not kept
-    // there (64 streams of up to 8000 keys 210 -> 200 us; 4 of 1500, whose 14 MB stay, 12.5 -> 13.8).
-    plan.stream = a.tps == 1 && 4ll * p->B * p->max_kv * kv->n_kv_heads * kv->head_dim > 256ll << 20;
+    plan = att_plan(a, p->dtype, true, p->max_q < p->T ? p->max_q : p->T, p->max_kv);
+    plan.stream = plan.stream && 4ll * p->B * p->max_kv * kv->n_kv_heads * kv->head_dim > 256ll << 20;
     return 0;
 }
 
@@ -1142,8 +1064,8 @@ static hipError_t att_launch(const AttArgs &a, const AttPlan &plan, hipStream_t 
     const dim3 grid((unsigned)(plan.slots * a.nkv), a.splits);
     if (plan.kind == ATT_ONE && PAGED && plan.stream) hipLaunchKernelGGL((k_att_one<QT, KT, HD, PAGED, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
     else if (plan.kind == ATT_ONE) hipLaunchKernelGGL((k_att_one<QT, KT, HD, PAGED, false>), grid, dim3(64 * ATT_WV), 0, st, a);
-    else if (plan.kind == ATT_FEW) hipLaunchKernelGGL((k_att_few<QT, KT, HD, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
     else if constexpr (sizeof(typename QT::elem) == 2) hipLaunchKernelGGL((k_att_tile<QT, HD, PAGED>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((k_att_f32<HD>), grid, dim3(64 * ATT_WV), 0, st, a);
     hipError_t e = hipGetLastError();
     if (e == hipSuccess && a.splits > 1) {
         const long long rows = (long long)a.T * a.nkv * a.G;
@@ -1204,7 +1126,7 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
               p->k_stride, p->v_stride, p->out_stride);
     AttArgs a = {};
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
-    const AttPlan plan = att_plan(a, p->dtype, 0, 0, false);
+    const AttPlan plan = att_plan(a, p->dtype, false, 0, 0);
     QT_REFUSE(plan.slots * a.nkv > 0x7FFFFFFFll, "packed_attention: too many tiles for one launch");
     a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)p->k; a.v = (const uint8_t *)p->v; a.out = (uint8_t *)p->out;
     a.qs = p->q_stride; a.os = p->out_stride; a.ks_slot = p->k_stride; a.vs_slot = p->v_stride;
