@@ -529,7 +529,8 @@ int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_a
  * included.  Scores, softmax and sums are f32; with F32 rows (over a BF16 cache) so are the products; with BF16 or
  * F16 rows (over a cache of their own type) the probabilities are rounded to that type for the product with V.
  * max_q and max_kv: the longest request's new tokens and kv_len as far as the host knows; they choose the launch
- * shape and change no result beyond rounding.  scale > 0.  B <= 65535, n_heads / n_kv_heads <= 64.
+ * shape and change no result beyond rounding.  scale > 0.  B <= 65535, n_heads / n_kv_heads <= 64, T * n_heads < 2^26.
+ * out must not overlap q or the cache.
  * workspace: qwen_hip_op_page_attention_workspace() bytes (of the same descriptor), aligned to 16; its contents do
  * not matter before or after; calls that may overlap need one each.  Alignment and strides as for append. */
 typedef struct {

@@ -153,5 +153,9 @@ static inline int qt_check_pages(const char *who, const qwen_hip_kv_pages_t *kv)
                   kv->slot_stride < 0,
               "%s: cache strides %lld, %lld, %lld (multiples of 8 elements, not negative)", who, kv->page_stride,
               kv->head_stride, kv->slot_stride);
+    QT_REFUSE((kv->n_pages > 1 && kv->page_stride < kv->head_dim) || (kv->n_kv_heads > 1 && kv->head_stride < kv->head_dim) ||
+                  (kv->page_size > 1 && kv->slot_stride < kv->head_dim),
+              "%s: cache strides %lld, %lld, %lld under head_dim %d: rows would overlap", who, kv->page_stride, kv->head_stride,
+              kv->slot_stride, kv->head_dim);
     return 0;
 }

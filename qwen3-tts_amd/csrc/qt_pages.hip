@@ -308,7 +308,7 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
     const int E = qt_dt_size(p->dtype);
     QT_REFUSE(!E || (p->dtype != QWEN_HIP_DT_F32 && p->dtype != kv->dtype),
               "page_append: rows of dtype %d into a cache of dtype %d (f32, or the cache's own)", p->dtype, kv->dtype);
-    QT_REFUSE(p->T < 0 || p->T > (1 << 28), "page_append: T %d out of range (0..2^28)", p->T);
+    QT_REFUSE(p->T < 0 || p->T >= 1 << 24, "page_append: T %d out of range (0..2^24 - 1)", p->T);
     if (p->T == 0) return 0;
     QT_REFUSE(!p->k || !p->v || !p->slot || (p->q && !p->q_out), "page_append: null pointer");
     QT_REFUSE(!p->rope_cos != !p->rope_sin || (p->rope_cos && (!p->pos || p->rope_len < 1)),

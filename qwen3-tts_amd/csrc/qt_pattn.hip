@@ -77,7 +77,7 @@ __device__ __forceinline__ float att_other_half(float v) {
 
 // The request that a launch slot belongs to when a request begins at slot floor(first row / TR) + b, TR rows a tile:
 // its ceil(rows / TR) tiles fit before the next one's, whatever the lengths, so floor(all rows / TR) + B slots are
-// enough for the host, which does not know them.  One load and ballot per 64 requests.
+// enough for the host, which does not know them.
 // Offsets are the caller's: one out of range is brought into it, so that nothing is read or written past T.
 __device__ __forceinline__ int att_cu(const AttArgs &a, int b) { return min(max(a.cu[b], 0), a.T); }
 template <int TR> __device__ __forceinline__ int att_first(const AttArgs &a, int b) {
@@ -85,13 +85,13 @@ template <int TR> __device__ __forceinline__ int att_first(const AttArgs &a, int
 }
 template <int TR> __device__ __forceinline__ int att_find(const AttArgs &a, int slot) {
     const int lane = threadIdx.x & 63;
-    int b = -1;
-    for (int base = 0; base < a.B; base += 64) {
-        const int i = base + lane;
-        const bool before = i < a.B && att_first<TR>(a, i) <= slot;
-        const int n = __popcll(__ballot(before));
-        b += n;
-        if (n < 64) break;
+    int b = 0;
+    for (int n = a.B; n > 1;) {                         // 64 requests' first slots at a time, one of every `step`
+        const int step = (n + 63) / 64;
+        const bool before = lane * step < n && att_first<TR>(a, b + lane * step) <= slot;
+        const int c = max((int)__popcll(__ballot(before)) - 1, 0);
+        b += c * step;
+        n = min(step, n - c * step);
     }
     return b;
 }
@@ -277,7 +277,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv;
     const int b = att_find<32>(a, slot);
-    if (b < 0) return;
     const int tile = slot - att_first<32>(a, b);
     const AttTile t = att_tile<32, false>(a, att_req<false>(a, b), tile);
     if (tile < 0 || t.r0 >= t.rows) return;             // (offsets that fall give tiles before the first)
@@ -339,12 +338,13 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
 #pragma unroll
         for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[i]);
         bm = fmaxf(bm, att_other_half(bm));
-        const float mr = bm == -INFINITY ? 0.f : bm, mc = mr * a.c, f = qt_exp2((m - mr) * a.c);
+        const float mr = bm == -INFINITY ? 0.f : bm, f = qt_exp2((m - mr) * a.c);
         m = bm;
         float p[2][8], sum = 0.f;
 #pragma unroll
         for (int i = 0; i < 16; i++) {
-            p[i >> 3][i & 7] = qt_exp2(fmaf(sc[i], a.c, -mc));
+            // the difference first: the rounding of a large m c would not cancel between blocks
+            p[i >> 3][i & 7] = qt_exp2((sc[i] - mr) * a.c);
             sum += p[i >> 3][i & 7];
         }
         l = l * f + sum;
@@ -468,7 +468,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, li = lane & 15, g = lane >> 4;
     const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
     const int b = a.tps > 0 ? slot / a.tps : att_find<16>(a, slot);
-    if (b < 0 || b >= a.B) return;
     int tile = a.tps > 0 ? slot % a.tps : slot - att_first<16>(a, b);
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
     const AttReq req = att_req<PAGED>(a, b);
@@ -596,7 +595,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         float p[8], sum = 0.f;
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            p[j] = qt_exp2(fmaf(sc[j >> 2][j & 3], a.c, -mc));
+            // f32: the difference first, since the rounding of a large m c would not cancel between blocks
+            p[j] = QF ? qt_exp2((sc[j >> 2][j & 3] - mr) * a.c) : qt_exp2(fmaf(sc[j >> 2][j & 3], a.c, -mc));
             sum += p[j];
         }
         l = l * f + sum;
@@ -716,7 +716,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         if (!att_longest<PAGED>(a, slot, b, tile, req)) return;
     } else {
         b = att_find<128>(a, slot);
-        if (b < 0) return;
         tile = slot - att_first<128>(a, b);
         req = att_req<PAGED>(a, b);
     }
@@ -1030,7 +1029,7 @@ static int check_rows(const char *who, int dtype, int n_heads, int nkv, int hd, 
     QT_REFUSE(nkv < 1 || nkv > 65535 || n_heads < nkv || n_heads % nkv || n_heads / nkv > 64,
               "%s: %d query heads over %d kv heads (a multiple, 64 a kv head at most)", who, n_heads, nkv);
     QT_REFUSE(B < 0 || B > 65535, "%s: B %d out of range (0..65535)", who, B);
-    QT_REFUSE(T < 0 || (long long)T * n_heads > 0x3FFFFFFFll, "%s: %d tokens of %d heads (2^30 - 1 rows at most)", who, T, n_heads);
+    QT_REFUSE(T < 0 || (long long)T * n_heads > 0x3FFFFFFll, "%s: %d tokens of %d heads (2^26 - 1 rows at most)", who, T, n_heads);
     QT_REFUSE(window < 0, "%s: window %d is negative", who, window);
     QT_REFUSE(!(scale > 0.f) || scale > 1e30f, "%s: scale has to be positive and finite", who);
     return 0;
@@ -1081,6 +1080,7 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     if (paged_args(kv, p, a, plan)) return -1;
     if (p->B == 0 || p->T == 0) return 0;
     QT_REFUSE(!p->q || !p->out || !p->cu_q || !p->kv_len || !p->table, "page_attention: null pointer");
+    QT_REFUSE(p->out == p->q, "page_attention: out must not be q");
     const int A = 16 / qt_dt_size(p->dtype);
     QT_REFUSE(qt_off16(p->q) || qt_off16(p->out) || qt_off16(p->workspace), "page_attention: pointers have to be aligned to 16 bytes");
     QT_REFUSE(p->q_stride % A || p->q_stride < 0 || p->out_stride % A || p->out_stride < (long long)p->n_heads * kv->head_dim,
@@ -1088,7 +1088,7 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     const long long need = a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
     QT_REFUSE(need > 0 && (!p->workspace || p->workspace_bytes < need), "page_attention: a workspace of %lld bytes is needed, %lld given",
               need, p->workspace ? p->workspace_bytes : 0ll);
-    QT_REFUSE(plan.slots * a.nkv > 0x7FFFFFFFll, "page_attention: too many tiles for one launch");
+    QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "page_attention: too many tiles for one launch");
     hipStream_t st = (hipStream_t)stream;
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_attention: the stream's device: %s", hipGetErrorString(on.err));
@@ -1118,6 +1118,7 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
     if (check_rows("packed_attention", p->dtype, p->n_heads, p->n_kv_heads, p->head_dim, p->B, p->T, p->window, p->scale)) return -1;
     if (p->B == 0 || p->T == 0) return 0;
     QT_REFUSE(!p->q || !p->k || !p->v || !p->out || !p->cu, "packed_attention: null pointer");
+    QT_REFUSE(p->out == p->q || p->out == p->k || p->out == p->v, "packed_attention: out must not be q, k or v");
     const int A = 16 / qt_dt_size(p->dtype);
     QT_REFUSE(qt_off16(p->q) || qt_off16(p->k) || qt_off16(p->v) || qt_off16(p->out), "packed_attention: pointers have to be aligned to 16 bytes");
     QT_REFUSE(p->q_stride % A || p->k_stride % A || p->v_stride % A || p->out_stride % A || p->q_stride < 0 || p->k_stride < 0 ||
@@ -1127,7 +1128,7 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
     AttArgs a = {};
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
     const AttPlan plan = att_plan(a, p->dtype, false, 0, 0);
-    QT_REFUSE(plan.slots * a.nkv > 0x7FFFFFFFll, "packed_attention: too many tiles for one launch");
+    QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "packed_attention: too many tiles for one launch");
     a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)p->k; a.v = (const uint8_t *)p->v; a.out = (uint8_t *)p->out;
     a.qs = p->q_stride; a.os = p->out_stride; a.ks_slot = p->k_stride; a.vs_slot = p->v_stride;
     a.cu = p->cu;

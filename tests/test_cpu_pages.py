@@ -80,7 +80,8 @@ def test_null_descriptors_are_refused():
 
 BAD_PAGES = [(dict(k=None), "null"), (dict(dtype=0), "dtype"), (dict(dtype=3), "dtype"), (dict(head_dim=96), "head_dim"),
              (dict(n_kv_heads=0), "n_kv_heads"), (dict(n_pages=0), "pages"), (dict(page_size=-1), "pages"),
-             (dict(k=P + 8), "aligned"), (dict(slot_stride=124), "strides"), (dict(page_stride=-8), "strides")]
+             (dict(k=P + 8), "aligned"), (dict(slot_stride=124), "strides"), (dict(page_stride=-8), "strides"),
+             (dict(slot_stride=0), "overlap"), (dict(head_stride=64), "overlap"), (dict(page_stride=0), "overlap")]
 
 
 def append(**kw):
@@ -91,7 +92,7 @@ def append(**kw):
 
 @pytest.mark.parametrize("kw,word", [
     (dict(dtype=2), "dtype"), (dict(dtype=7), "dtype"), (dict(k=None), "null"), (dict(slot=None), "null"), (dict(q_out=None), "null"),
-    (dict(rope_sin=None), "RoPE"), (dict(pos=None), "RoPE"), (dict(rope_len=0), "RoPE"), (dict(T=-1), "T -1"),
+    (dict(rope_sin=None), "RoPE"), (dict(pos=None), "RoPE"), (dict(rope_len=0), "RoPE"), (dict(T=-1), "T -1"), (dict(T=1 << 24), "T 16777216"),
     (dict(n_heads=0), "n_heads"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(v=P + 4), "aligned"),
     (dict(k_stride=4098), "strides"), (dict(q_out_stride=1024), "strides"), (dict(q_stride=-4), "strides")])
 def test_append_refuses(kw, word):
@@ -106,7 +107,7 @@ def test_bad_cache_descriptors_are_refused(kw, word):
 
 
 def attn(**kw):
-    d = dict(q=P, out=P, q_stride=2048, out_stride=2048, cu_q=P, kv_len=P, table=P, table_stride=8, table_cols=8, workspace=P,
+    d = dict(q=P, out=2 * P, q_stride=2048, out_stride=2048, cu_q=P, kv_len=P, table=P, table_stride=8, table_cols=8, workspace=P,
              workspace_bytes=1 << 40, dtype=1, n_heads=16, B=4, T=4, max_q=1, max_kv=128, window=0, scale=0.1)
     return hip.PageAttn(**{**d, **kw})
 
@@ -115,7 +116,8 @@ BAD_ROWS = [(dict(dtype=9), "dtype"), (dict(n_heads=12), "heads"), (dict(n_heads
             (dict(B=-1), "B -1"), (dict(B=65536), "B 65536"), (dict(T=-1), "tokens"), (dict(T=1 << 28), "tokens"),
             (dict(window=-1), "window"), (dict(scale=0.0), "scale"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
             (dict(scale=float("inf")), "scale"), (dict(q=None), "null"), (dict(out=None), "null"), (dict(q=P + 8), "aligned"),
-            (dict(q_stride=2050), "strides"), (dict(out_stride=1024), "strides")]
+            (dict(q_stride=2050), "strides"), (dict(out_stride=1024), "strides"),
+            (dict(out=P), "must not"), (dict(T=1 << 22), "rows")]
 
 
 @pytest.mark.parametrize("kw,word", BAD_ROWS + [
@@ -125,6 +127,11 @@ BAD_ROWS = [(dict(dtype=9), "dtype"), (dict(n_heads=12), "heads"), (dict(n_heads
     (dict(max_kv=1 << 16, workspace=P + 4), "aligned")])
 def test_page_attention_refuses(kw, word):
     refused(hip.lib().qwen_hip_op_page_attention(C.byref(pages()), C.byref(attn(**kw)), None), word)
+
+
+def test_more_tiles_than_a_launch_takes_are_refused():
+    refused(hip.lib().qwen_hip_op_page_attention(C.byref(pages(n_kv_heads=65535, page_size=1)),
+                                                 C.byref(attn(n_heads=65535, B=65535, T=1, out_stride=65535 * 128)), None), "tiles")
 
 
 def test_f32_rows_need_a_bf16_cache():
@@ -143,7 +150,7 @@ def test_workspace_follows_the_descriptor():
 @pytest.mark.parametrize("kw,word", BAD_ROWS + [(dict(k=None), "null"), (dict(cu=None), "null"), (dict(v=P + 2), "aligned"),
                                                 (dict(k_stride=1028), "strides"), (dict(v_stride=-8), "strides"), (dict(head_dim=80), "head_dim")])
 def test_packed_attention_refuses(kw, word):
-    d = dict(q=P, k=P, v=P, out=P, q_stride=4096, k_stride=4096, v_stride=4096, out_stride=2048, cu=P, dtype=1, n_heads=16, n_kv_heads=8,
+    d = dict(q=P, k=P, v=P, out=2 * P, q_stride=4096, k_stride=4096, v_stride=4096, out_stride=2048, cu=P, dtype=1, n_heads=16, n_kv_heads=8,
              head_dim=128, B=4, T=4, window=0, scale=0.1)
     refused(hip.lib().qwen_hip_op_packed_attention(C.byref(hip.PackedAttn(**{**d, **kw})), None), word)
 

@@ -535,6 +535,23 @@ def test_bad_pages_hold_no_keys():
         close_attention(got[i:i + 1], exact, mag, "bf16", 103, float(v.abs().max()))
 
 
+def test_f32_keeps_the_differences_of_large_scores():
+    """Scores near 1000 that differ by little, over many blocks of keys: the softmax is one of differences, so only the
+    scores' own rounding counts, 64 terms of an f32 sum around 1000 (2^-24 1000 a term at most, 8 of them by chance)."""
+    p = Paged([(900, 1), (0, 40)], 2, 1, 64, "f32", "bf16", 16, "head", seed=19)
+    k0 = torch.full((64,), 4.0)
+    p.q[:] = 30.0
+    p.qd[:, :128] = 30.0
+    for b, (k, v) in enumerate(p.kv):
+        k[:] = (k0 + 0.02 * torch.randn(k.shape, generator=torch.Generator().manual_seed(b))).to(torch.bfloat16)
+        n, pg = k.shape[0], p.table[b].cpu()
+        for i in range(n):
+            p.kc[int(pg[i // 16]), :, i % 16] = k[i].to(DEV)
+    got, (exact, _) = p.run().double().cpu(), p.want()
+    off = float((got - exact).norm() / exact.norm())
+    assert off < 8 * 1000 * 2.0 ** -24, off
+
+
 def test_large_scores_do_not_overflow():
     """Scores of thousands: the softmax is one of differences."""
     for t, kv in KINDS:
@@ -569,6 +586,48 @@ def test_cache_past_32_bits():
     p.pages.k, p.pages.v, p.pages.page_stride = dp(k), dp(v), k.stride(0)
     assert int(p.table.max()) * k.stride(0) * 2 > 1 << 32
     p.check()
+
+
+@pytest.mark.parametrize("t,kv", KINDS)
+def test_chunk_over_a_cache_past_32_bits(t, kv):
+    """The same for chunks of many rows."""
+    p = Paged([(70, 120), (0, 90)], 4, 1, 128, t, kv, 16, "head", seed=15)
+    total = 7 << 30
+    far = total // 2 // p.pages.n_pages // 128 * 128
+    k, v = (torch.zeros(total // 2, dtype=TYPES[kv], device=DEV).as_strided((p.pages.n_pages, 1, 16, 128), (far, 2048, 128, 1)) for _ in range(2))
+    k.copy_(p.kc)
+    v.copy_(p.vc)
+    p.pages.k, p.pages.v, p.pages.page_stride = dp(k), dp(v), far
+    assert int(p.table.max()) * far * 2 > 1 << 32
+    p.check()
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+def test_many_long_requests(t):
+    """More requests than the order by length looks at (256), of many rows each."""
+    lens = [(b * 13) % 40 + 20 * (b % 2) for b in range(300)]
+    T, g = sum(lens), torch.Generator().manual_seed(16)
+    rows = torch.randn(T, 6 * 64, generator=g).to(TYPES[t])
+    out = torch.full((T, 256), 7.0, dtype=TYPES[t], device=DEV)
+    ok(packed(rows.to(DEV), lens, 4, 1, 64, t, out))
+    exact, mag = packed_want(rows, lens, 4, 1, 64, 0)
+    close_attention(out.cpu().view(T, 4, 64), exact, mag, t, 60, float(rows.abs().max()))
+    Paged([(b % 7, n) for b, n in enumerate(lens)], 4, 1, 64, t, "bf16", 8, "slot", seed=17).check()
+
+
+def test_most_requests():
+    """65535 requests, most of them empty, in every launch that finds them by their rows."""
+    B, g = 65535, torch.Generator().manual_seed(18)
+    lens = [0] * B
+    for b, n in ((0, 3), (1, 40), (63, 1), (64, 2), (1023, 33), (1024, 5), (40000, 70), (65534, 17)):
+        lens[b] = n
+    T = sum(lens)
+    for t, nh in (("f32", 2), ("bf16", 2)):
+        rows = torch.randn(T, (nh + 2) * 64, generator=g).to(TYPES[t])
+        out = torch.full((T, nh * 64), 7.0, dtype=TYPES[t], device=DEV)
+        ok(packed(rows.to(DEV), lens, nh, 1, 64, t, out))
+        exact, mag = packed_want(rows, [n for n in lens if n], nh, 1, 64, 0)
+        close_attention(out.cpu().view(T, nh, 64), exact, mag, t, 70, float(rows.abs().max()))
 
 
 def packed(rows, lens, nh, nkv, hd, t, out, window=0, cu=None, T=None):
