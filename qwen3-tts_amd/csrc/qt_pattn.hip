@@ -18,8 +18,8 @@
 // them in registers; dim NT m + t is row m of product t.
 //
 // Types.  16-bit rows over a cache of their type: one product each; the probabilities are rounded to that type for
-// V's product (bf16: at most 2^-8 of each, f16: 2^-11, of either sign over the keys; the sum of a row keeps them
-// unrounded).  f32 rows over a bf16 cache: q and p as three bf16 planes whose sum is exact, three products.  All f32: both
+// V's product (bf16: at most 2^-8 of each, f16: 2^-11, of either sign over the keys), and a row's sum is that of the
+// rounded ones, so a key that outweighs the rest gives its value whatever its probability rounds to.  f32 rows over a bf16 cache: q and p as three bf16 planes whose sum is exact, three products.  All f32: both
 // operands as planes, six products (qt_planes.h).
 //
 // What a row does not see never reaches it: hidden scores become -infinity before the maximum.  Their probabilities
@@ -58,6 +58,15 @@ template <typename T> __device__ __forceinline__ qt_f32x16 att_mma(qt_u32x4 a, q
 }
 template <> __device__ __forceinline__ qt_f32x16 att_mma<QtF16>(qt_u32x4 a, qt_u32x4 b, qt_f32x16 c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(qt_f16x8, a), __builtin_bit_cast(qt_f16x8, b), c, 0, 0, 0);
+}
+// c + both halves of p, in f32
+template <typename T> __device__ __forceinline__ float att_add2(uint32_t p, float c) {
+    typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(b2, p), __builtin_bit_cast(b2, 0x3F803F80u), c, false);
+}
+template <> __device__ __forceinline__ float att_add2<QtF16>(uint32_t p, float c) {
+    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, p), __builtin_bit_cast(h2, 0x3C003C00u), c, false);
 }
 // sum over planes, the smallest products first
 template <typename T, int NA, int NB>
@@ -597,16 +606,19 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         for (int j = 0; j < 8; j++) {
             // f32: the difference first, since the rounding of a large m c would not cancel between blocks
             p[j] = QF ? qt_exp2((sc[j >> 2][j & 3] - mr) * a.c) : qt_exp2(fmaf(sc[j >> 2][j & 3], a.c, -mc));
-            sum += p[j];
+            if (QF) sum += p[j];
         }
-        l = l * f + sum;
         qt_u32x4 pb[NQ];
         if constexpr (QF) {
             qt_planes8(p, pb);
         } else {
 #pragma unroll
-            for (int j = 0; j < 4; j++) pb[0][j] = qt_round2<QT>(p[2 * j], p[2 * j + 1]);
+            for (int j = 0; j < 4; j++) {
+                pb[0][j] = qt_round2<QT>(p[2 * j], p[2 * j + 1]);
+                sum = att_add2<QT>(pb[0][j], sum);
+            }
         }
+        l = l * f + sum;
 #pragma unroll
         for (int u = 0; u < NU; u++) {
             qt_u32x4 va[NK];
@@ -863,20 +875,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         }
         const float mc = m == -INFINITY ? 0.f : m * a.c;
         if (kb + 1 < kb1) scores(sn, sk + (BUF ^ 1) * 64 * RB);
-        float sum[2] = {0.f, 0.f};
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                sc[kt][i] = qt_exp2(fmaf(sc[kt][i], a.c, -mc));
-                sum[kt] += sc[kt][i];
-            }
-        l += sum[0] + sum[1];
+            for (int i = 0; i < 16; i++) sc[kt][i] = qt_exp2(fmaf(sc[kt][i], a.c, -mc));
 #pragma unroll
         for (int s = 0; s < 4; s++) {
             qt_u32x4 pb;
+            float sum = 0.f;
 #pragma unroll
-            for (int j = 0; j < 4; j++) pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
+            for (int j = 0; j < 4; j++) {
+                pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
+                sum = att_add2<T>(pb[j], sum);
+            }
+            l += sum;
 #pragma unroll
             for (int d = 0; d < NT; d++) {
                 const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + va[d]);

@@ -4,9 +4,11 @@ Tolerances.  A rounding to a type is off by at most half a step, eps / 2 of the 
   append     f32 arithmetic: the sum of squares 12 roundings (a lane's 8 terms, 4 exchanges), each counting half in the
              root, then division, root, two products and the rotation's three: under 16 roundings of 2^-24 on |y1| + |y2|
              (the rotation's two terms); then one rounding to the stored type.
-  attention  16-bit: every probability rounded once, so sum p |v| / sum p times eps / 2 (f16: and 2^-25 absolutely
-             a key below its normal range, n 2^-25 max|v| / sum p <= n 2^-25 max|v|, since the largest p is 1); the output's
-             own rounding; and the f32 part below.
+  attention  16-bit: every probability rounded once, p' = p (1 + d) with |d| <= eps / 2, in the sum over v and in the sum of
+             the row.  sum p' v is off by at most eps / 2 sum p |v|, sum p' by at most eps / 2 of itself, so their quotient o
+             by eps / 2 (sum p |v| / sum p + |o|), to first order in eps (1 % covers the second); the output's own
+             rounding is another eps / 2 |o|.  f16: a p below its normal range is off by 2^-25 absolutely, n 2^-25 max|v| over
+             the row's sum, which is 1 at least, and as much of o through the sum.  And the f32 part below.
              f32 part, in the 2-norm over all outputs: each score is a sum of head_dim exact plane products in at most
              6 head_dim / 16 f32 additions of partial sums that stay near its standard size: with scores up to about 8
              (in units of their softmax) sqrt(48) 2^-24 8 = 3.3e-6, and the sums over keys add the same order of 2^-24
@@ -361,7 +363,7 @@ def close_attention(got, exact, mag, t, n_max, vmax):
         assert off <= 8e-6, off
         assert bool(((got - exact).abs() <= 5e-5 * vmax).all())
         return
-    tol = eps / 2 * 1.01 * (exact.abs() + mag) + 5e-5 * vmax + (n_max * 2.0 ** -25 * vmax + 2.0 ** -25 if t == "f16" else 0.0)
+    tol = eps / 2 * 1.01 * (2 * exact.abs() + mag) + 5e-5 * vmax + (2 * n_max * 2.0 ** -25 * vmax + 2.0 ** -25 if t == "f16" else 0.0)
     bad = ((got - exact).abs() / tol).max()
     assert bool(bad <= 1), float(bad)
 
