@@ -11,7 +11,9 @@
 // So nothing that is written is read again, and any number of workgroups can share the pages and tokens when each makes the sums
 // over the (at most 2048) requests for itself; only the lengths and the free count, which may be replaced in place, are
 // written by one of them, and in a launch of their own where the others may still read what they replace.
-// Bound by the latency of its dependent loads (lengths, then free list and tables) and of the launch.
+// Bound by the latency of its dependent loads (lengths, then free list and tables) and of the launch: 8 requests of one
+// token 6 us a pass, 512 requests, 37 of them ended, 47 680 tokens 8.9 (one workgroup for all pages, a second launch for
+// the slots: 30).
 #define PLAN_T 256
 #define PLAN_MAX_B 2048         // 32 KB of LDS
 #define PLAN_SAT (1u << 30)     // sums stop here: under 2^31 in any order, over every limit they are held to
@@ -241,7 +243,8 @@ extern "C" int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *p, void *stream
 // y = x / sqrt(mean x^2 + eps) g, then (y1, y2) -> (y1 c - y2 s, y2 c + y1 s) on a head's halves, all in f32,
 // rounded once.  A head's row is HD / 8 lanes of 8 elements (16-byte loads); its sum of squares and its rotation's
 // other half are lane exchanges.  A workgroup takes one token: its lanes' angles and gains are loaded once
-// and serve every head.  Bound by the rows' bytes for prompts, by the latency of slot, angles and rows for a step.
+// and serve every head.  Bound by the rows' bytes for prompts (8190 tokens bf16, 16 query and 8 kv heads of 128: 33 us, 4.2 TB/s,
+// the copy rate being 4.9), by the launch and the latency of slot, angles and rows for a step (32 tokens f32: 6.4 us).
 struct AppendArgs {
     const uint8_t *q, *k, *v;
     uint8_t *qo, *kc, *vc;
