@@ -24,7 +24,7 @@
 //
 // What a row does not see never reaches it: hidden scores become -infinity before the maximum.  Their probabilities
 // are 0, and 0 times an infinite or NaN v would still be NaN: where a tile ends with anything that is not
-// finite, its rows are done again key by key over what each of them sees (att_serial), which also serves f32 values
+// finite, its rows are done again one by one over what each of them sees (att_serial), which also serves f32 values
 // that have no planes (infinite, NaN, past bf16's range after rounding).
 #include "qt_ops.h"
 #include "qt_planes.h"
@@ -220,36 +220,54 @@ template <typename QT, int NT> __device__ __forceinline__ void att_put(uint8_t *
     }
 }
 
-// One row over keys [k0, k1), one after the other in f32.  A wave; lane: dims lane + 64 e.
+// One row over keys [k0, k1) in f32 without the matrix core; only what the row sees is read into its sums.  A wave: 64 keys
+// at a time, a lane a key for the scores, dims lane + 64 e for the sums.  It ends where the row is NaN whatever follows.
 template <typename QT, typename KT, int HD, bool PAGED>
 __device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const int *table, int head, int r, int k0, int k1, bool part, int split) {
     constexpr int EQ = sizeof(typename QT::elem), EK = sizeof(typename KT::elem), D = HD / 64;
     const int lane = threadIdx.x & 63, tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
     const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD) * EQ;
-    float q[D], o[D], m = -INFINITY, l = 0.f;
+    float o[D], m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int e = 0; e < D; e++) { q[e] = qt_load1<QT>(qp + (lane + 64 * e) * EQ); o[e] = 0.f; }
-    k0 = max(k0, a.window > 0 ? pos - a.window + 1 : 0);
+    for (int e = 0; e < D; e++) o[e] = 0.f;
+    k0 = max(max(k0, a.window > 0 ? pos - a.window + 1 : 0), 0);
     k1 = min(k1, min(t.kmax, pos + 1));
-    for (int j = max(k0, 0); j < k1; j++) {
-        long long ko, vo;
+    for (int j0 = k0; j0 < k1 && l == l; j0 += 64) {
+        const int j = j0 + lane;
+        bool see = j < k1;
+        long long ko = 0, vo = 0;
         if (PAGED) {
-            const int p = att_page(a, table, t, j);
-            if (!att_has(a, p)) continue;
-            ko = vo = att_slot(a, p, j) + head * a.ks_head;
-        } else {
+            const int p = see ? att_page(a, table, t, j) : -1;
+            see = att_has(a, p);
+            if (see) ko = vo = att_slot(a, p, j) + head * a.ks_head;
+        } else if (see) {
             ko = (long long)(t.q0 + j) * a.ks_slot + head * HD;
             vo = (long long)(t.q0 + j) * a.vs_slot + head * HD;
         }
-        float s = 0.f;
+        float s = -INFINITY;
+        if (see) {
+            s = 0.f;
+            for (int d = 0; d < HD; d += 8) {
+                float q[8], k[8];
+                qt_load8<QT>(qp + d * EQ, q);
+                qt_load8<KT>(a.k + (ko + d) * EK, k);
 #pragma unroll
-        for (int e = 0; e < D; e++) s = fmaf(q[e], qt_load1<KT>(a.k + (ko + lane + 64 * e) * EK), s);
-        s = group_sum<64>(s);
-        const float mn = fmaxf(m, s), mr = mn == -INFINITY ? 0.f : mn;
-        const float f = qt_exp2((m - mr) * a.c), p = qt_exp2((s - mr) * a.c);
-        l = l * f + p;
+                for (int e = 0; e < 8; e++) s = fmaf(q[e], k[e], s);
+            }
+        }
+        const float mn = fmaxf(m, group_max<64>(s)), mr = mn == -INFINITY ? 0.f : mn, f = qt_exp2((m - mr) * a.c);
+        const float p = see ? qt_exp2((s - mr) * a.c) : 0.f;
+        l = l * f + group_sum<64>(p);
 #pragma unroll
-        for (int e = 0; e < D; e++) o[e] = fmaf(p, qt_load1<KT>(a.v + (vo + lane + 64 * e) * EK), o[e] * f);
+        for (int e = 0; e < D; e++) o[e] *= f;
+        const int lo = (int)vo, hi = (int)(vo >> 32);
+        for (unsigned long long some = __ballot(see); some; some &= some - 1) {
+            const int i = __ffsll(some) - 1;
+            const float pi = lane_bcast(p, i);
+            const long long v = ((long long)__builtin_amdgcn_readlane(hi, i) << 32) | (unsigned)__builtin_amdgcn_readlane(lo, i);
+#pragma unroll
+            for (int e = 0; e < D; e++) o[e] = fmaf(pi, qt_load1<KT>(a.v + (v + lane + 64 * e) * EK), o[e]);
+        }
         m = mn;
     }
     const size_t at = (size_t)(t.q0 + tok) * (a.nkv * a.G) + qh;

@@ -489,6 +489,47 @@ def test_page_attention_one_long_request(t, kv):
 
 
 @pytest.mark.parametrize("t,kv", KINDS)
+@pytest.mark.parametrize("reqs", [[(40, 1), (600, 1), (33, 1)], [(40, 50), (200, 90)]])
+def test_rows_before_the_first_request_stay(t, kv, reqs):
+    p = Paged(reqs, 4, 2, 64, t, kv, 16, "head", seed=22, T=sum(n for _, n in reqs))
+    exact, mag = p.want()
+    lead = 5                                                    # the same rows five tokens later
+    q, out = p.qd, p.out
+    p.qd, p.out = torch.cat((torch.full((lead, q.shape[1]), math.nan, dtype=q.dtype, device=DEV), q)), torch.full((q.shape[0] + lead, out.shape[1]), 7.0, dtype=out.dtype, device=DEV)
+    p.cud.copy_(i32([c + lead for c in p.cu]))
+    p.d.q, p.d.out, p.d.T = dp(p.qd), dp(p.out), q.shape[0] + lead
+    n = hip.lib().qwen_hip_op_page_attention_workspace(C.byref(p.pages), C.byref(p.d))
+    ws = torch.full((n + 1,), 255, dtype=torch.uint8, device=DEV)
+    p.d.workspace, p.d.workspace_bytes = dp(ws), n
+    ok(hip.lib().qwen_hip_op_page_attention(C.byref(p.pages), C.byref(p.d), stream()))
+    torch.cuda.synchronize()
+    assert bool((p.out[:lead] == 7).all())
+    close_attention(p.out[lead:, :256].reshape(-1, 4, 64), exact, mag, t, 700, 6.0)
+
+
+@pytest.mark.parametrize("t,kv", KINDS)
+def test_two_calls_at_once(t, kv):
+    """Two streams, a workspace each, the same cache."""
+    ps = [Paged([(900, 1), (50, 1), (300, 1)], 4, 2, 64, t, kv, 16, "head", seed=23) for _ in range(2)]
+    ps[1].d.q = dp(ps[0].qd)
+    ps[1].pages, ps[1].d.table = ps[0].pages, dp(ps[0].table)
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    ws = []
+    for p in ps:
+        n = hip.lib().qwen_hip_op_page_attention_workspace(C.byref(p.pages), C.byref(p.d))
+        ws.append(torch.full((n + 1,), 255, dtype=torch.uint8, device=DEV))
+        p.d.workspace, p.d.workspace_bytes = dp(ws[-1]), n
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for p, st in zip(ps, streams):
+            ok(hip.lib().qwen_hip_op_page_attention(C.byref(p.pages), C.byref(p.d), st.cuda_stream))
+    torch.cuda.synchronize()
+    exact, mag = ps[0].want()
+    assert torch.equal(ps[0].out[:3], ps[1].out[:3])
+    close_attention(ps[0].out[:, :256].reshape(3, 4, 64), exact, mag, t, 901, 6.0)
+
+
+@pytest.mark.parametrize("t,kv", KINDS)
 def test_rows_that_see_nothing_are_zero(t, kv):
     """Fewer keys than new tokens (the first rows lie before position 0), no keys, a negative length, no pages."""
     p = Paged([(0, 40), (0, 3), (0, 5), (9, 4)], 4, 2, 64, t, kv, 16, "head", seed=8)
@@ -669,6 +710,45 @@ def test_packed_attention(t, nh, nkv, hd, lens, window):
     w = rows[:T, :(nh + 2 * nkv) * hd]
     exact, mag = packed_want(w, lens, nh, nkv, hd, window)
     close_attention(out[:T, :nh * hd].view(T, nh, hd), exact, mag, t, max(lens), float(w.abs().max()))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("where", ["v", "k", "q", "all"])
+def test_values_that_are_not_finite(t, where):
+    """An infinity in one value of one early token, or in everything: each row and dim as the formula has it, and a long
+    prompt of such rows ends soon (each of them passes its keys 64 at a time, and no further once it is NaN)."""
+    g = torch.Generator().manual_seed(20)
+    n, nh, nkv, hd = 1500, 4, 2, 64
+    rows = torch.randn(n, 8 * 64, generator=g).to(TYPES[t])
+    clean = rows.clone()
+    if where == "v":
+        rows[3, 6 * 64 + 5] = math.inf                          # dim 5 of kv head 0
+    elif where == "k":
+        rows[3, 4 * 64:5 * 64] = math.nan                       # kv head 0
+    elif where == "q":
+        rows[700, 64:128] = math.inf                            # head 1 of one token
+    else:
+        rows[:] = math.nan
+    out = torch.empty(n, 256, dtype=TYPES[t], device=DEV)
+    ok(packed(rows.to(DEV), [n], nh, nkv, hd, t, out))
+    out = out.cpu().view(n, nh, hd)
+    exact, mag = packed_want(clean, [n], nh, nkv, hd, 0)
+    bad = torch.zeros(n, nh, hd, dtype=torch.bool)
+    if where == "v":
+        bad[3:, :2, 5] = True
+        # the infinite value times a probability: infinite, or NaN where that is 0 in f32
+        assert bool((out[bad].isinf() & (out[bad] > 0) | out[bad].isnan()).all())
+    elif where == "k":
+        bad[3:, :2] = True
+        assert bool(out[bad].isnan().all())
+    elif where == "q":
+        bad[700, 1] = True
+        assert not bool(out[bad].isfinite().any())
+    else:
+        assert bool(out.isnan().all())
+        return
+    vmax = float(clean.abs().max())
+    close_attention(torch.where(bad, exact.to(out.dtype), out), exact, mag, t, n, vmax)
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
