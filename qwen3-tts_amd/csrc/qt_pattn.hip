@@ -507,6 +507,14 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
     const int r = min(t.r0 + li, t.rows - 1), tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
     const int first = t.shift + qt_quot(t.r0, a.gdiv), last = t.shift + qt_quot(min(t.r0 + 15, t.rows - 1), a.gdiv);
+    // the range's 32-key blocks
+    const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
+    const int n = att_ranges(a, blk1 - blk0, a.chunk), size = (blk1 - blk0 + n - 1) / n;
+    const bool part = n > 1;                            // else the first range has it all
+    if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
+    const int kb0 = min(blk1, blk0 + split * size), kb1 = min(blk1, kb0 + size);
+    // (looked up here, so that the entry and the queries come in together)
+    int page = PAGED && kb0 + wave < kb1 ? att_page(a, table, t, 32 * (kb0 + wave) + (lane & 31)) : 0;
     // the queries' operands; step s: dims 32 s + 8 g ..
     qt_u32x4 qf[QF ? 1 : NS];
     if constexpr (QF) {
@@ -526,12 +534,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + 32 * s * EQ);
     }
-    // the range's 32-key blocks
-    const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
-    const int n = att_ranges(a, blk1 - blk0, a.chunk), size = (blk1 - blk0 + n - 1) / n;
-    const bool part = n > 1;                            // else the first range has it all
-    if (split > 0 && !part) { if (a.tps <= 0) return; continue; }
-    const int kb0 = min(blk1, blk0 + split * size), kb1 = min(blk1, kb0 + size);
     float m = -INFINITY, l = 0.f;                       // l: of this group's keys
     const qt_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
     qt_f32x4 o[NU];
@@ -539,7 +541,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     for (int u = 0; u < NU; u++) o[u] = zero;
     const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD) + 8 * g) * EK;
     const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + NU * li) * EK;
-    int page = PAGED && kb0 + wave < kb1 ? att_page(a, table, t, 32 * (kb0 + wave) + (lane & 31)) : 0;
     for (int kb = kb0 + wave; kb < kb1; kb += ATT_WV) {
         const int key = 32 * kb + (lane & 31);
         qt_u32x4 kr[2][NS][KF ? 2 : 1];
