@@ -523,9 +523,9 @@ int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_a
 /* Causal attention of new tokens over the cache that holds them and what came before: request b's rows are
  * cu_q[b] .. cu_q[b+1] - 1 of q and out ([T] tokens, head h of a token at h*head_dim), row i of its n being position
  * kv_len[b] - n + i (kv_len: with the new tokens).  A row sees positions up to its own, the last `window` of them
- * where window > 0; query head h reads kv head h / (n_heads / n_kv_heads).  A row that sees nothing is 0; rows
- * before cu_q[0] and behind cu_q[B] stay as they were.  A table entry outside [0, n_pages) holds no keys: its
- * positions are not seen.  What lies in positions that a row does not see never reaches it, infinite or NaN
+ * where window > 0; query head h reads kv head h / (n_heads / n_kv_heads).  A row that sees nothing, or
+ * only scores of -infinity, is 0; rows before cu_q[0] and behind cu_q[B] stay as they were.  A table entry outside
+ * [0, n_pages) holds no keys: its positions are not seen.  What lies in positions that a row does not see never reaches it, infinite or NaN
  * included.  Scores, softmax and sums are f32; with F32 rows (over a BF16 cache) so are the products; with BF16 or
  * F16 rows (over a cache of their own type) the probabilities are rounded to that type for the product with V.
  * max_q and max_kv: the longest request's new tokens and kv_len as far as the host knows; they choose the launch

@@ -292,7 +292,7 @@ __device__ __forceinline__ void att_stored() { asm volatile("s_waitcnt vmcnt(0)"
 // A workgroup takes 32 rows; its four waves take the 32-key blocks in turn, each with a softmax of its own, K and V
 // going from memory into operand registers without LDS or barriers and split there; the waves' sums are merged through
 // LDS at the end.  V is loaded when K is used up: both at once spill.  Bound by the splitting (VALU) next to the
-// products: two prompts of 4000 positions 922 us, 142 TFLOP/s of f32 products (a library's f32 matrix product of 8192^3:
+// products: two prompts of 4000 positions 911 us, 144 TFLOP/s of f32 products (a library's f32 matrix product of 8192^3:
 // 153); with V loaded ahead of the scores 1105, in 16-row tiles (k_att_one) 1377.
 template <int HD>
 __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))) void k_att_f32(AttArgs a) {
@@ -450,9 +450,9 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))
 // 16 t + 4 g + i; the 8 probabilities of a lane are the operand of V's product in place, V's rows are loaded 8 keys by
 // HD / 16 dims a lane, and dim (HD / 16) m + u is row m of product u.  The four waves take the blocks of 32 keys in
 // turn, each with a softmax of its own and no barrier, and are merged through LDS; the ranges of keys by k_att_merge.
-// Bound by the cache's bytes for many streams: 64 of 1000 to 8000 keys bf16 196 us, 6.0 TB/s of reads (32-row tiles 217); by
-// the chain of dependent loads (lengths, table, keys) for few: 4 streams f32 11.8 us with the merge (15.6), three prompts
-// of 21 to 128 f32 8.2 (15.9).
+// Bound by the cache's bytes for many streams: 64 of 1000 to 8000 keys bf16 197 us, 6.0 TB/s of reads (32-row tiles 217); by
+// the chain of dependent loads (lengths, table, keys) for few: 4 streams f32 11.5 us with the merge (15.6), three prompts
+// of 21 to 128 f32 8.1 (15.9).
 template <typename T> __device__ __forceinline__ qt_f32x4 att_mma16(qt_u32x4 a, qt_u32x4 b, qt_f32x4 c) { return qt_mfma_bf16(a, b, c); }
 template <> __device__ __forceinline__ qt_f32x4 att_mma16<QtF16>(qt_u32x4 a, qt_u32x4 b, qt_f32x4 c) {
     return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(qt_f16x8, a), __builtin_bit_cast(qt_f16x8, b), c, 0, 0, 0);
@@ -694,7 +694,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         if (rr < t.rows) {
             bad = !(chk - chk == 0.f);
             const int rt = qt_quot(rr, a.gdiv);
-        const size_t tk = t.q0 + rt, hd = head * a.G + rr - rt * a.G;
+            const size_t tk = t.q0 + rt, hd = head * a.G + rr - rt * a.G;
             if (part) {
                 const size_t prow = ((size_t)split * a.T + tk) * (a.nkv * a.G) + hd;
                 if (kb0 < kb1) att_put<QtF32, NU>(reinterpret_cast<uint8_t *>(a.po + prow * HD + NU * mm), v);
@@ -722,8 +722,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
 // memory straight into LDS (no registers), two blocks deep, one barrier a block, and every wave reads both
 // operands from there.  16-bit types only.  Block kb + 1's scores do not wait for block kb's softmax: K is a block ahead of
 // V.  Bound by the matrix core's and the vector unit's shares together (53 and 54 % of the cycles of two prompts of 5003 and
-// 8191 f16: 428 us, 881 TFLOP/s at the 1.7 GHz that the load leaves; LDS 27 %, no bank conflicts; 32-row tiles
-// straight from memory 1031 us), by the first loads of each workgroup for short prompts (16 of 40 to 1500 bf16: 86 us, 211).
+// 8191 f16: 411 to 428 us, 881 TFLOP/s and more at the 1.7 GHz that the load leaves; LDS 27 %, no bank conflicts; 32-row tiles
+// straight from memory 1031 us), by the first loads of each workgroup for short prompts (16 of 40 to 1500 bf16: 84 us, 211).
 //   K, row k: 16-byte chunk c at place c ^ swk(k): the 16 lanes of a phase of a wave's read (16 rows, one chunk)
 //   fall on 16 different groups of banks.  V: chunk c at place c ^ swv(k): a transposing read takes 4 rows by 64 bytes
 //   a half-wave, which fall on different banks.

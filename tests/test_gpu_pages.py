@@ -752,6 +752,28 @@ def test_values_that_are_not_finite(t, where):
 
 
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("lens", [[90], [40, 75, 33], [600, 700, 690, 512, 800, 640, 720, 555]])
+def test_scores_of_minus_infinity(t, lens):
+    """The first 30 keys of each prompt score -infinity against every row: they count for nothing, and a row that has
+    no others is 0."""
+    g = torch.Generator().manual_seed(23)
+    T, nh, nkv, hd = sum(lens), 8, 4, 64
+    rows = torch.randn(T, (nh + 2 * nkv) * hd, generator=g).to(TYPES[t])
+    rows[:, 0:nh * hd:hd] = rows[:, 0:nh * hd:hd].abs() + 0.25
+    only = torch.zeros(T, dtype=torch.bool)
+    for a in cu_of(lens)[:-1]:
+        rows[a:a + 30, nh * hd:(nh + nkv) * hd:hd] = -math.inf
+        only[a:a + 30] = True
+    out = torch.empty(T, nh * hd, dtype=TYPES[t], device=DEV)
+    ok(packed(rows.to(DEV), lens, nh, nkv, hd, t, out))
+    out = out.cpu().view(T, nh, hd)
+    exact, mag = packed_want(rows, lens, nh, nkv, hd, 0)
+    assert bool(exact[only].isnan().all()) and bool(exact[~only].isfinite().all())
+    assert bool((out[only] == 0).all())
+    close_attention(out[~only], exact[~only], mag[~only], t, max(lens), float(rows[:, (nh + nkv) * hd:].abs().max()))
+
+
+@pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 def test_packed_hidden_values_never_reach_a_row(t):
     g = torch.Generator().manual_seed(2)
     lens, nh, nkv, hd = [90, 40], 4, 2, 64
