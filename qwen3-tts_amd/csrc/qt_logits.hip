@@ -26,6 +26,14 @@ struct RulesArgs {
     int V, hcap, bcap, each;
 };
 
+// Row b's part of a list of `cap` entries.  Offsets are the caller's: one out of range is brought into it, and entries are
+// counted from the part's begin, unsigned, so that no sum of an index and a step passes 2^32.
+struct ListPart { int at; unsigned n; };
+__device__ __forceinline__ ListPart list_part(const int *off, int b, int cap) {
+    const int at = min(max(off[b], 0), cap), end = min(max(off[b + 1], at), cap);
+    return {at, (unsigned)(end - at)};
+}
+
 // BIAS: with bias lists.  EACH: the penalty once for every entry.  Rows may begin anywhere that their elements can: 16-byte
 // accesses at 2- or 4-byte alignment are one instruction on this GPU.
 template <typename T, bool BIAS, bool EACH, int RULES_T>
@@ -39,20 +47,23 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
     const uint8_t *xr = a.x + ((size_t)b * a.xs + v0) * E;
     uint8_t *yr = a.out + ((size_t)b * a.os + v0) * E;
     const uint32_t *mr = a.mask ? a.mask + (size_t)b * a.ms + v0 / 32 : nullptr;
-    const int h0 = counts ? max(a.hoff[b], 0) : 0, h1 = counts ? min(a.hoff[b + 1], a.hcap) : 0;
-    const int e0 = BIAS ? max(a.boff[b], 0) : 0, e1 = BIAS ? (int)min((long long)min(a.boff[b + 1], a.bcap), e0 + 65534ll) : 0;
+    const ListPart h = counts ? list_part(a.hoff, b, a.hcap) : ListPart{0, 0u};
+    const ListPart e = BIAS ? list_part(a.boff, b, a.bcap) : ListPart{0, 0u};
+    const int *hist = a.hist + h.at, *btok = a.btok + e.at;
+    const float *bval = a.bval + e.at;
+    const unsigned hn = h.n, en = min(e.n, 65534u);
     const float rep = a.rep ? a.rep[b] : 1.f, pres = a.pres ? a.pres[b] : 0.f, freq = a.freq ? a.freq[b] : 0.f;
-    const long long h2 = h0 + (long long)(counts && a.npr ? max(a.npr[b], 0) : 0);
-    const bool full = (long long)h1 - h0 > 65535;       // counts may reach the word's lower half
+    const unsigned prompt = counts && a.npr ? max(a.npr[b], 0) : 0;
+    const bool full = hn > 65535;                       // counts may reach the word's lower half
     unsigned held[RULES_HELD], held_bias = ~0u;
 #pragma unroll
     for (int k = 0; k < RULES_HELD; k++) {
-        const int i = h0 + tid + k * RULES_T;
-        held[k] = i < h1 ? (unsigned)a.hist[i] - (unsigned)v0 : ~0u;
+        const unsigned i = tid + k * RULES_T;
+        held[k] = i < hn ? (unsigned)hist[i] - (unsigned)v0 : ~0u;
     }
-    if (BIAS && e0 + tid < e1) {
-        held_bias = (unsigned)a.btok[e0 + tid] - (unsigned)v0;
-        value[tid] = a.bval[e0 + tid];
+    if (BIAS && (unsigned)tid < en) {
+        held_bias = (unsigned)btok[tid] - (unsigned)v0;
+        value[tid] = bval[tid];
     }
     // a thread's tokens: 8 at 8 tid + 8 RULES_T v, as they are in memory; after the lists, whose marks need not wait for them
     qt_w4 raw[NV][E / 2];
@@ -73,10 +84,10 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
         if (EACH) times[t] = 0;
         atomicOr(hist ? &seen[t >> 5] : &bits[t >> 5], 1u << (t & 31));
     };
-    const auto count = [&](unsigned t, int i) {
+    const auto count = [&](unsigned t, unsigned i) {
         if (t >= (unsigned)n) return;
         if (EACH) atomicAdd(&times[t], 1u);
-        if (i < h2) return;
+        if (i < prompt) return;
         if (!full) {
             atomicAdd(&word[t], 1u);
         } else {                                        // up to 65535
@@ -84,24 +95,24 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
             while ((was & 0xFFFFu) != 0xFFFFu && (now = atomicCAS(&word[t], was, was + 1u)) != was) was = now;
         }
     };
-    // entry e of the biases, before any count: the largest word is the last entry's
-    const auto bias = [&](unsigned t, int e) {
-        if (t < (unsigned)n) atomicMax(&word[t], ((unsigned)e + 1u) << 16);
+    // entry i of the biases, before any count: the largest word is the last entry's
+    const auto bias = [&](unsigned t, unsigned i) {
+        if (t < (unsigned)n) atomicMax(&word[t], (i + 1u) << 16);
     };
 #pragma unroll
     for (int k = 0; k < RULES_HELD; k++) mark(held[k], true);
-    for (int i = h0 + tid + RULES_HELD * RULES_T; i < h1; i += RULES_T) mark((unsigned)a.hist[i] - (unsigned)v0, true);
+    for (unsigned i = tid + RULES_HELD * RULES_T; i < hn; i += RULES_T) mark((unsigned)hist[i] - (unsigned)v0, true);
     if (BIAS) {
         mark(held_bias, false);
-        for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) mark((unsigned)a.btok[i] - (unsigned)v0, false);
+        for (unsigned i = tid + RULES_T; i < en; i += RULES_T) mark((unsigned)btok[i] - (unsigned)v0, false);
         __syncthreads();
         bias(held_bias, tid);
-        for (int i = e0 + tid + RULES_T; i < e1; i += RULES_T) bias((unsigned)a.btok[i] - (unsigned)v0, i - e0);
+        for (unsigned i = tid + RULES_T; i < en; i += RULES_T) bias((unsigned)btok[i] - (unsigned)v0, i);
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < RULES_HELD; k++) count(held[k], h0 + tid + k * RULES_T);
-    for (int i = h0 + tid + RULES_HELD * RULES_T; i < h1; i += RULES_T) count((unsigned)a.hist[i] - (unsigned)v0, i);
+    for (int k = 0; k < RULES_HELD; k++) count(held[k], tid + k * RULES_T);
+    for (unsigned i = tid + RULES_HELD * RULES_T; i < hn; i += RULES_T) count((unsigned)hist[i] - (unsigned)v0, i);
     __syncthreads();
     const auto rules = [&](float y, int t) {
         if (a.rep && (seen[t >> 5] >> (t & 31) & 1u)) {
@@ -109,12 +120,12 @@ __global__ __launch_bounds__(RULES_T) void k_logit_rules(RulesArgs a) {
             float was;
             do { was = y; y = y > 0.f ? y / rep : y * rep; } while (--k && y != was);   // until nothing changes any more
         }
-        const unsigned w = word[t], o = w & 0xFFFFu, e = w >> 16;
+        const unsigned w = word[t], o = w & 0xFFFFu, last = w >> 16;
         if (o) {
             if (a.freq) y -= (float)o * freq;
             if (a.pres) y -= pres;
         }
-        if (BIAS && e) y += e <= RULES_T ? value[e - 1] : a.bval[e0 + (int)e - 1];
+        if (BIAS && last) y += last <= RULES_T ? value[last - 1] : bval[last - 1];
         return y;
     };
 #pragma unroll

@@ -928,6 +928,40 @@ def test_logit_rules_of_long_lists(t):
     assert bool(((dev[8].double().cpu() - w).abs() <= tol).all())
 
 
+@pytest.mark.parametrize("V", [300, 9000])
+@pytest.mark.parametrize("each", [0, 1])
+def test_logit_rules_offsets_out_of_range_stay_inside(V, each):
+    """Offsets past the lists, negative, falling and at both ends of their type are brought into the lists; what lies next to
+    a list, tokens that would change every row, is not read.  A cap of 2^31 - 1 over sane offsets changes nothing."""
+    rng = np.random.default_rng(V + each)
+    cap, far = 50, 2 ** 31 - 1
+    tok, btok = rng.integers(0, V - 3, cap), rng.integers(0, V - 3, cap)
+    bval = (3 * rng.standard_normal(cap)).astype(np.float32)
+    around = lambda v, g: torch.cat((torch.full((8192,), g, dtype=v.dtype), v, torch.full((8192,), g, dtype=v.dtype))).to(DEV)  # noqa: E731
+    dev = [around(torch.from_numpy(tok.astype(np.int32)), V - 2), around(torch.from_numpy(btok.astype(np.int32)), V - 1),
+           around(torch.from_numpy(bval), 99.0)]
+    at = [dp(d) + 8192 * 4 for d in dev]
+    wild = [0, 20, far, -far - 1, 30, cap + 3, 5, far - 100, far - 4000, cap, -1, far - 4096, cap + 1, far, far, 3, cap]
+    sane = [0, 13, 13, 40, cap]
+    for off, hold in ((wild, cap), (wild, 0), (sane, cap), (sane, far)):
+        B = len(off) - 1
+        x = torch.from_numpy(4 * rng.standard_normal((B, V))).float()
+        xd, out, offd = x.to(DEV), torch.full((B, V), 7.0, device=DEV), i32(off)
+        rep, pres, freq = (torch.full((B,), v, device=DEV) for v in (1.25, 0.5, 0.125))
+        npr = i32([2] * B)
+        d = hip.LogitRules(dtype=0, B=B, V=V, logits=dp(xd), out=dp(out), logits_stride=V, out_stride=V, rep_each=each, hist=at[0], hist_off=dp(offd),
+                           hist_cap=hold, n_prompt=dp(npr), rep=dp(rep), presence=dp(pres), frequency=dp(freq), bias_tok=at[1], bias_val=at[2],
+                           bias_off=dp(offd), bias_cap=hold)
+        print(f"[case] rules V={V} each={each} offsets {off[:4]}.. of {hold}", flush=True)
+        ok(hip.lib().qwen_hip_op_logit_rules(C.byref(d), stream()))
+        got = out.cpu().double()
+        for b in range(B):
+            i0 = min(max(off[b], 0), hold)
+            i1 = min(max(off[b + 1], i0), hold)
+            want, big, n = rules64(x[b], tok[i0:i1].tolist(), 2, 1.25, 0.5, 0.125, dict(zip(btok[i0:i1].tolist(), bval[i0:i1])), None, each)
+            assert bool(((got[b] - want).abs() <= n * 2.0 ** -24 * big).all()), (b, off[b], off[b + 1])
+
+
 def test_rules_then_argmax_is_the_sampler_of_one_stream():
     """rep_each on one f32 row: the token that qwen_hip_op_sample picks greedily with its penalty."""
     rng = np.random.default_rng(4)
