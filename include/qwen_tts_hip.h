@@ -507,7 +507,8 @@ int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *plan, void *stream);
  * cache truncates).  dtype: of q, k, v and q_out; F32 rows go with either cache type, BF16 and F16 rows with their
  * own.  A token whose slot is outside the cache (the plan's -1), or whose pos is outside [0, rope_len) where there
  * are tables, is skipped: nothing of it is written.  Slots of one call have to be distinct.  q may be NULL (k and v
- * only); q_out may be q.  Pointers aligned to 16 bytes, strides (in elements, between tokens) multiples of 16 bytes. */
+ * only); q_out may be q with q's stride, else it shares no memory with q, k or v (rows of one buffer beside theirs, with
+ * their stride, do not).  Pointers aligned to 16 bytes, strides (in elements, between tokens) multiples of 16 bytes. */
 typedef struct {
     const void *q, *k, *v;
     void *q_out;

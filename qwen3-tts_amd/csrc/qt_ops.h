@@ -137,6 +137,18 @@ struct QtOnDevice {
 #define QT_REFUSE(cond, ...) do { if (cond) { qt_seterr(__VA_ARGS__); return -1; } } while (0)
 
 static inline int qt_dt_size(int dt) { return dt == QWEN_HIP_DT_F32 ? 4 : dt == QWEN_HIP_DT_BF16 || dt == QWEN_HIP_DT_F16 ? 2 : 0; }
+// Whether n rows of aw bytes, as apart (at least aw), share memory with n rows of bw bytes, bs apart (0: one row).  Row i of
+// one meets row i + d of the other where a - b + d as lies between -aw and bw: the first d past the lower end decides.  Rows of two
+// strides count as sharing memory where their ranges do.
+static inline bool qt_rows_meet(const void *a, long long as, long long aw, const void *b, long long bs, long long bw, long long n) {
+    const long long D = (long long)((intptr_t)a - (intptr_t)b);
+    if (D >= (n - 1) * bs + bw || -D >= (n - 1) * as + aw) return false;
+    if (n == 1 || (bs != as && bs != 0)) return true;
+    const long long x = -aw - D;                                      // the first d with d as > x
+    long long d = (x >= 0 ? x / as : -((-x + as - 1) / as)) + 1;
+    if (d < (bs ? 1 - n : 0)) d = bs ? 1 - n : 0;
+    return d < n && D + d * as < bw;
+}
 static inline bool qt_off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
 
 // the cache's descriptor; `who` names the call

@@ -326,6 +326,15 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
     QT_REFUSE((p->q && (p->q_stride % A || p->q_stride < 0 || p->q_out_stride % A || p->q_out_stride < qw)) || p->k_stride % A ||
                   p->k_stride < 0 || p->v_stride % A || p->v_stride < 0,
               "page_append: strides have to be multiples of 16 bytes, not negative, q_out's at least a token's %lld elements", qw);
+    // a token's workgroup writes its q after reading its own rows, at no known time before or after the others read theirs
+    const bool in_place = p->q && p->q_out == p->q;
+    QT_REFUSE(in_place && p->T > 1 && p->q_stride != p->q_out_stride, "page_append: q in place with two strides, %lld and %lld", p->q_stride,
+              p->q_out_stride);
+    const long long kw = (long long)kv->n_kv_heads * kv->head_dim * E;
+    QT_REFUSE(p->q && ((!in_place && qt_rows_meet(p->q_out, p->q_out_stride * E, qw * E, p->q, p->q_stride * E, qw * E, p->T)) ||
+                       qt_rows_meet(p->q_out, p->q_out_stride * E, qw * E, p->k, p->k_stride * E, kw, p->T) ||
+                       qt_rows_meet(p->q_out, p->q_out_stride * E, qw * E, p->v, p->v_stride * E, kw, p->T)),
+              "page_append: q_out overlaps rows that are read (it may be q itself)");
     hipStream_t st = (hipStream_t)stream;
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_append: the stream's device: %s", hipGetErrorString(on.err));

@@ -99,6 +99,23 @@ def test_append_refuses(kw, word):
     refused(hip.lib().qwen_hip_op_page_append(C.byref(pages()), C.byref(append(**kw)), None), word)
 
 
+Q = 1 << 20             # bytes from any other operand
+
+
+@pytest.mark.parametrize("kw,word", [
+    # rows of 2048 q, 1024 k and 1024 v, q written densely into the same memory, and by less than a stride apart
+    (dict(q=Q, k=Q + 8192, v=Q + 12288, q_out=Q), "two strides"), (dict(q=Q, k=3 * Q, v=4 * Q, q_out=Q, q_out_stride=4100), "two strides"),
+    (dict(q=Q, k=3 * Q, v=4 * Q, q_out=Q + 16, q_out_stride=4096), "overlaps"), (dict(q=Q, k=3 * Q, v=4 * Q, q_out=Q - 16, q_out_stride=4096), "overlaps"),
+    (dict(q=Q, k=3 * Q, v=4 * Q, q_out=Q + 16384 + 16, q_out_stride=4096), "overlaps"),
+    (dict(q=Q, k=Q + 8192, v=Q + 12288, q_out=Q + 8192, q_out_stride=4096), "overlaps"),
+    (dict(q=Q, k=3 * Q, v=4 * Q, q_out=4 * Q), "overlaps"), (dict(q=Q, k=3 * Q, k_stride=0, v=4 * Q, q_out=3 * Q - 3 * 8192 - 8176), "overlaps"),
+    (dict(q=Q, k=3 * Q, v=4 * Q, q_out=4 * Q + 3 * 16384 + 4080, q_out_stride=2048), "overlaps"),
+    (dict(q=Q, k=3 * Q, v=4 * Q, q_out=Q + 4096, T=1), "overlaps")])
+def test_append_refuses_to_write_q_over_rows_that_are_read(kw, word):
+    refused(hip.lib().qwen_hip_op_page_append(C.byref(pages(k=32 * Q, v=33 * Q)), C.byref(append(**kw)), None), word)
+
+
+
 @pytest.mark.parametrize("kw,word", BAD_PAGES)
 def test_bad_cache_descriptors_are_refused(kw, word):
     L = hip.lib()

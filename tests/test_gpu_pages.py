@@ -317,6 +317,31 @@ def test_append_in_place_and_without_q():
     assert float(((rows[:, :128].double().view(6, 2, 64) - y).abs() / y.abs().clamp(min=1e-30)).max()) < 16 * 2.0 ** -24
 
 
+
+def test_append_writes_q_beside_the_rows_it_reads():
+    """q_out as further columns of the rows' own buffer, and one token in place with a stride of its own."""
+    g = torch.Generator().manual_seed(5)
+    rows = torch.randn(6, 6 * 64 + 16, generator=g).to(DEV)                 # q (2 heads), k, v, q_out (2 heads)
+    before, W = rows.clone(), rows.shape[1]
+    k, v = (pool((4, 1, 4, 64), torch.bfloat16, "head", g) for _ in range(2))
+    slot, gain = i32([3, 5, 7, 9, 11, 0]), torch.full((64,), 2.0, device=DEV)
+    d = hip.PageAppend(dtype=0, n_heads=2, T=6, eps=0.0, q=dp(rows), k=dp(rows) + 128 * 4, v=dp(rows) + 192 * 4, q_out=dp(rows) + 256 * 4, q_stride=W,
+                       k_stride=W, v_stride=W, q_out_stride=W, slot=dp(slot), q_norm=dp(gain))
+    ok(hip.lib().qwen_hip_op_page_append(C.byref(pages_of(k, v, "bf16")), C.byref(d), stream()))
+    torch.cuda.synchronize()
+    keep = [*range(256), *range(384, W)]
+    assert torch.equal(rows[:, keep], before[:, keep])
+    x = before[:, :128].double().view(6, 2, 64)
+    y = 2 * x / x.square().mean(-1, keepdim=True).sqrt()
+    assert float(((rows[:, 256:384].double().view(6, 2, 64) - y).abs() / y.abs().clamp(min=1e-30)).max()) < 16 * 2.0 ** -24
+    for i, s in enumerate(slot.tolist()):
+        assert torch.equal(k[s // 4, 0, s % 4], before[i, 128:192].bfloat16()) and torch.equal(v[s // 4, 0, s % 4], before[i, 192:256].bfloat16())
+    d.T, d.q_out, d.q_out_stride = 1, dp(rows), 128
+    ok(hip.lib().qwen_hip_op_page_append(C.byref(pages_of(k, v, "bf16")), C.byref(d), stream()))
+    torch.cuda.synchronize()
+    assert torch.equal(rows[0, :128], rows[0, 256:384]) and torch.equal(rows[1:, :128], before[1:, :128])
+
+
 def far_pool(n_pages, nkv, page, hd, total):
     """bf16 pages `total` bytes from the first to the end, far apart."""
     far = total // 2 // n_pages // 64 * 64
