@@ -453,9 +453,11 @@ int qwen_hip_op_sd_conv_transpose(float *Y, const float *X, const float *W, cons
  * rules on a batch's logits.  Every pointer in these descriptors is DEVICE memory of the device that `stream`
  * belongs to; the descriptor itself is host memory, read during the call, so one made once can be used for every
  * step.  Calls launch on `stream` (a hipStream_t; NULL = the null stream of the current device) and return
- * without waiting: 0, or -1 with qwen_hip_last_error() set and nothing launched.  They allocate nothing and can
- * be captured into a graph.  Lengths, tables and slots are read on the device: a replayed graph follows what
- * they hold then. */
+ * without waiting: 0, or -1 with qwen_hip_last_error() set and nothing launched.  (HIP's own last error, where an earlier
+ * call left one, is neither reported nor cleared.  Of a call that takes two launches the first may have succeeded: then
+ * attention's rows are unfinished and a plan in place has changed neither lengths nor free count; both can be repeated.)
+ * They allocate nothing and can be captured into a graph.  Lengths, tables and slots are read on the device: a replayed
+ * graph follows what they hold then. */
 enum { QWEN_HIP_DT_F32 = 0, QWEN_HIP_DT_BF16 = 1, QWEN_HIP_DT_F16 = 2 };
 
 /* One layer's cache in pages: position p of a request lies in page table[p / page_size] at place p % page_size

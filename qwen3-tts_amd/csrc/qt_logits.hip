@@ -185,20 +185,16 @@ extern "C" int qwen_hip_op_logit_rules(const qwen_hip_logit_rules_t *p, void *st
     // of 2048: 6.1 us against 6.4).
     const int threads = p->V > 8192 ? 1024 : 256;
     const dim3 grid((p->V + 16 * threads - 1) / (16 * threads), p->B);
-#define RULES3(T, BIAS, EACH) do { \
-        if (threads == 1024) hipLaunchKernelGGL((k_logit_rules<T, BIAS, EACH, 1024>), grid, dim3(1024), 0, st, a); \
-        else hipLaunchKernelGGL((k_logit_rules<T, BIAS, EACH, 256>), grid, dim3(256), 0, st, a); } while (0)
-#define RULES(T) do { \
-        if (p->bias_tok && p->rep_each) RULES3(T, true, true); \
-        else if (p->bias_tok) RULES3(T, true, false); \
-        else if (p->rep_each) RULES3(T, false, true); \
-        else RULES3(T, false, false); } while (0)
-    if (p->dtype == QWEN_HIP_DT_F32) RULES(QtF32);
-    else if (p->dtype == QWEN_HIP_DT_BF16) RULES(QtBf16);
-    else RULES(QtF16);
+#define RULES3(T, BIAS, EACH) (threads == 1024 ? k_logit_rules<T, BIAS, EACH, 1024> : k_logit_rules<T, BIAS, EACH, 256>)
+#define RULES2(T, BIAS) (p->rep_each ? RULES3(T, BIAS, true) : RULES3(T, BIAS, false))
+#define RULES(T) (p->bias_tok ? RULES2(T, true) : RULES2(T, false))
+    void (*const kernel)(RulesArgs) = p->dtype == QWEN_HIP_DT_F32    ? RULES(QtF32)
+                                      : p->dtype == QWEN_HIP_DT_BF16 ? RULES(QtBf16)
+                                                                     : RULES(QtF16);
 #undef RULES
+#undef RULES2
 #undef RULES3
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = qt_launch(kernel, grid, dim3(threads), 0, st, a);
     QT_REFUSE(e != hipSuccess, "logit_rules: launch failed: %s", hipGetErrorString(e));
     return 0;
 }

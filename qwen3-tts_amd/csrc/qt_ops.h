@@ -134,6 +134,16 @@ struct QtOnDevice {
     QtOnDevice &operator=(const QtOnDevice &) = delete;
 };
 
+// Launches a kernel.  The status is this launch's own: the thread's last error may be one that an earlier call left, and
+// stays the caller's to read.
+template <typename Args>
+static inline hipError_t qt_launch(void (*kernel)(Args), dim3 grid, dim3 block, size_t lds, hipStream_t st, Args args) {
+    void *p[] = {&args};
+    const hipError_t e = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, p, lds, st);
+    if (e != hipSuccess) (void)hipGetLastError();
+    return e;
+}
+
 #define QT_REFUSE(cond, ...) do { if (cond) { qt_seterr(__VA_ARGS__); return -1; } } while (0)
 
 static inline int qt_dt_size(int dt) { return dt == QWEN_HIP_DT_F32 ? 4 : dt == QWEN_HIP_DT_BF16 || dt == QWEN_HIP_DT_F16 ? 2 : 0; }

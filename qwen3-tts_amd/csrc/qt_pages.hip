@@ -227,13 +227,11 @@ extern "C" int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *p, void *stream
     const bool in_place = p->kv_len_out == p->kv_len || p->n_free_out == p->n_free;
     a.finish = wgs == 1 || !in_place;
     const size_t lds = (size_t)(4 * p->B + 3) * 4;
-    hipLaunchKernelGGL(k_page_plan, dim3(wgs), dim3(PLAN_T), lds, st, a);
-    hipError_t e = hipGetLastError();
+    hipError_t e = qt_launch(k_page_plan, dim3(wgs), dim3(PLAN_T), lds, st, a);
     if (e == hipSuccess && !a.finish) {
         a.share = 0;
         a.finish = 1;
-        hipLaunchKernelGGL(k_page_plan, dim3(1), dim3(PLAN_T), lds, st, a);
-        e = hipGetLastError();
+        e = qt_launch(k_page_plan, dim3(1), dim3(PLAN_T), lds, st, a);
     }
     QT_REFUSE(e != hipSuccess, "page_plan: launch failed: %s", hipGetErrorString(e));
     return 0;
@@ -343,15 +341,13 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
                           kv->page_stride, kv->head_stride, kv->slot_stride, p->q_norm, p->k_norm, p->rope_cos, p->rope_sin,
                           p->pos, p->slot, p->T, p->n_heads, kv->n_kv_heads, p->rope_len, kv->n_pages * kv->page_size,
                           kv->page_size, p->eps, qt_div_of(kv->page_size)};
-#define APPEND(QT, KT) do { \
-        if (kv->head_dim == 128) hipLaunchKernelGGL((k_page_append<QT, KT, 128>), dim3(p->T), dim3(256), 0, st, a); \
-        else hipLaunchKernelGGL((k_page_append<QT, KT, 64>), dim3(p->T), dim3(256), 0, st, a); } while (0)
-    if (p->dtype == QWEN_HIP_DT_BF16) APPEND(QtBf16, QtBf16);
-    else if (p->dtype == QWEN_HIP_DT_F16) APPEND(QtF16, QtF16);
-    else if (kv->dtype == QWEN_HIP_DT_BF16) APPEND(QtF32, QtBf16);
-    else APPEND(QtF32, QtF16);
+#define APPEND(QT, KT) (kv->head_dim == 128 ? k_page_append<QT, KT, 128> : k_page_append<QT, KT, 64>)
+    void (*const kernel)(AppendArgs) = p->dtype == QWEN_HIP_DT_BF16    ? APPEND(QtBf16, QtBf16)
+                                       : p->dtype == QWEN_HIP_DT_F16   ? APPEND(QtF16, QtF16)
+                                       : kv->dtype == QWEN_HIP_DT_BF16 ? APPEND(QtF32, QtBf16)
+                                                                       : APPEND(QtF32, QtF16);
 #undef APPEND
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = qt_launch(kernel, dim3(p->T), dim3(256), 0, st, a);
     QT_REFUSE(e != hipSuccess, "page_append: launch failed: %s", hipGetErrorString(e));
     return 0;
 }

@@ -1100,15 +1100,14 @@ extern "C" long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_page
 template <typename QT, typename KT, int HD, bool PAGED>
 static hipError_t att_launch(const AttArgs &a, const AttPlan &plan, hipStream_t st) {
     const dim3 grid((unsigned)(plan.slots * a.nkv), a.splits);
-    if (plan.kind == ATT_ONE && PAGED && plan.stream) hipLaunchKernelGGL((k_att_one<QT, KT, HD, PAGED, PAGED>), grid, dim3(64 * ATT_WV), 0, st, a);
-    else if (plan.kind == ATT_ONE) hipLaunchKernelGGL((k_att_one<QT, KT, HD, PAGED, false>), grid, dim3(64 * ATT_WV), 0, st, a);
-    else if constexpr (sizeof(typename QT::elem) == 2) hipLaunchKernelGGL((k_att_tile<QT, HD, PAGED>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((k_att_f32<HD>), grid, dim3(64 * ATT_WV), 0, st, a);
-    hipError_t e = hipGetLastError();
+    hipError_t e;
+    if (plan.kind == ATT_ONE && PAGED && plan.stream) e = qt_launch(k_att_one<QT, KT, HD, PAGED, PAGED>, grid, dim3(64 * ATT_WV), 0, st, a);
+    else if (plan.kind == ATT_ONE) e = qt_launch(k_att_one<QT, KT, HD, PAGED, false>, grid, dim3(64 * ATT_WV), 0, st, a);
+    else if constexpr (sizeof(typename QT::elem) == 2) e = qt_launch(k_att_tile<QT, HD, PAGED>, grid, dim3(256), 0, st, a);
+    else e = qt_launch(k_att_f32<HD>, grid, dim3(64 * ATT_WV), 0, st, a);
     if (e == hipSuccess && a.splits > 1) {
         const long long rows = (long long)a.T * a.nkv * a.G;
-        hipLaunchKernelGGL((k_att_merge<QT, HD>), dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
-        e = hipGetLastError();
+        e = qt_launch(k_att_merge<QT, HD>, dim3((unsigned)((rows + 3) / 4)), dim3(256), 0, st, a);
     }
     return e;
 }

@@ -1163,3 +1163,61 @@ def test_prompts_packed_or_from_the_cache_agree():
     exact, mag = packed_want(rows.cpu(), lens, nh, nkv, hd, 0)
     for x in (got, out):
         close_attention(x.view(T, nh, hd), exact, mag, "bf16", 128, float(rows.abs().max()))
+
+
+@pytest.mark.parametrize("what", ["plan", "plan of two launches", "append", "attention", "attention of two launches", "packed", "rules"])
+def test_an_error_that_was_left_is_not_the_calls(what):
+    """A failed HIP call of the caller's (a device that there is not), whose error nobody has read: the operators launch, say
+    so, and leave it."""
+    L = hip.lib()
+    H = C.CDLL(hip.LIB_PATH)                                    # its own HIP runtime
+    if what.startswith("plan"):
+        rng = np.random.default_rng(1)
+        case = plan_case(rng, 20, 16, 20, 90, 60, 4, cap=9000 if "two" in what else 1000)
+        p, want = Plan(*case, in_place=True), plan_model(*case)
+        call = lambda st: L.qwen_hip_op_page_plan(C.byref(p.d), st)  # noqa: E731
+    elif what == "append":
+        g = torch.Generator().manual_seed(3)
+        rows, slot = torch.randn(2, 192, generator=g).to(DEV), i32([5, 2])
+        k, v = (pool((3, 1, 2, 64), torch.bfloat16, "head", g) for _ in range(2))
+        pages, d = pages_of(k, v, "bf16"), hip.PageAppend(dtype=0, T=2, k=dp(rows), v=dp(rows) + 256, k_stride=192, v_stride=192, slot=dp(slot))
+        call = lambda st: L.qwen_hip_op_page_append(C.byref(pages), C.byref(d), st)  # noqa: E731
+    elif what.startswith("attention"):
+        p = Paged([(900, 1), (40, 1)] if "two" in what else [(40, 1), (3, 1)], 4, 2, 64, "bf16", "bf16", 16, "head", seed=33)
+        n = L.qwen_hip_op_page_attention_workspace(C.byref(p.pages), C.byref(p.d))
+        assert (n > 0) == ("two" in what)
+        ws = torch.zeros(n + 1, dtype=torch.uint8, device=DEV)
+        p.d.workspace, p.d.workspace_bytes = dp(ws), n
+        call = lambda st: L.qwen_hip_op_page_attention(C.byref(p.pages), C.byref(p.d), st)  # noqa: E731
+    elif what == "packed":
+        rows = torch.randn(30, 4 * 64, generator=torch.Generator().manual_seed(4))
+        dev, out, cu = rows.to(DEV), torch.zeros(30, 128, device=DEV), i32([0, 30])
+        d = hip.PackedAttn(dtype=0, n_heads=2, n_kv_heads=1, head_dim=64, B=1, T=30, scale=0.125, q=dp(dev), k=dp(dev) + 512, v=dp(dev) + 768,
+                           out=dp(out), q_stride=256, k_stride=256, v_stride=256, out_stride=128, cu=dp(cu))
+        call = lambda st: L.qwen_hip_op_packed_attention(C.byref(d), st)  # noqa: E731
+    else:
+        x = torch.arange(100, dtype=torch.float32, device=DEV)
+        out = torch.zeros(100, device=DEV)
+        d = hip.LogitRules(dtype=0, B=1, V=100, logits=dp(x), out=dp(out), logits_stride=100, out_stride=100)
+        call = lambda st: L.qwen_hip_op_logit_rules(C.byref(d), st)  # noqa: E731
+    st = stream()
+    torch.cuda.synchronize()
+    assert H.hipGetLastError() == 0
+    left = H.hipSetDevice(1000)
+    rc, stays = call(st), H.hipGetLastError()                   # read before torch's next launch, which would report it
+    assert left != 0
+    assert rc == 0, hip.last_error()
+    assert stays == left and H.hipGetLastError() == 0
+    torch.cuda.synchronize()
+    if what.startswith("plan"):
+        assert p.kv.tolist() == want["kv"] and int(p.nf) == want["n_free"] and p.slot[:p.cap].tolist() == want["slot"]
+    elif what == "append":
+        assert torch.equal(k[2, 0, 1], rows[0, :64].bfloat16()) and torch.equal(v[1, 0, 0], rows[1, 64:128].bfloat16())
+    elif what.startswith("attention"):
+        exact, mag = p.want()
+        close_attention(p.out[:, :256].reshape(2, 4, 64), exact, mag, "bf16", 901, 6.0)
+    elif what == "packed":
+        exact, mag = packed_want(rows, [30], 2, 1, 64, 0)
+        close_attention(out.cpu().view(30, 2, 64), exact, mag, "f32", 30, float(rows.abs().max()))
+    else:
+        assert torch.equal(out, x)
