@@ -25,7 +25,8 @@
 // What a row does not see never reaches it: hidden scores become -infinity before the maximum.  Their probabilities
 // are 0, and 0 times an infinite or NaN v would still be NaN: where a tile ends with anything that is not
 // finite, its rows are done again one by one over what each of them sees (att_serial), which also serves f32 values
-// that have no planes (infinite, NaN, past bf16's range after rounding).
+// that have no planes (infinite, NaN, past bf16's range after rounding).  So are rows whose maximum times c is past
+// f32's range: the 16-bit kernels' s c - m c makes every probability 0 there (a sum of 0 under a maximum shows it) or infinite.
 #include "qt_ops.h"
 #include "qt_planes.h"
 #include <type_traits>
@@ -692,7 +693,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
 #pragma unroll
         for (int u = 0; u < NU; u++) chk = fmaf(v[u], 0.f, chk);
         if (rr < t.rows) {
-            bad = !(chk - chk == 0.f);
+            bad = !(chk - chk == 0.f) || (!QF && L == 0.f && M > -INFINITY);
             const int rt = qt_quot(rr, a.gdiv);
             const size_t tk = t.q0 + rt, hd = head * a.G + rr - rt * a.G;
             if (part) {
@@ -968,7 +969,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                         make_uint2(qt_round2<T>(o[d][4 * i] * inv, o[d][4 * i + 1] * inv), qt_round2<T>(o[d][4 * i + 2] * inv, o[d][4 * i + 3] * inv));
         }
     }
-    if (__ballot(live && !(chk - chk == 0.f))) {
+    if (__ballot(live && (!(chk - chk == 0.f) || (l == 0.f && m > -INFINITY)))) {
         att_stored();
         for (int row = w0; row < min(w0 + 32, t.rows); row++)
             att_serial<T, T, HD, PAGED>(a, t, table, head, row, 64 * kb0, 64 * kb1, part, split);

@@ -630,6 +630,39 @@ def test_large_scores_do_not_overflow():
         assert float((got - exact).norm() / exact.norm()) < 0.02
 
 
+
+@pytest.mark.parametrize("t,kv", KINDS)
+@pytest.mark.parametrize("sign", [1, -1])
+@pytest.mark.parametrize("reqs,packed_too", [([(0, 40), (30, 3)], True), ([(700, 1), (30, 1), (0, 1)], False), ([(0, 900)], True), ([(500, 130), (64, 200)], False)])
+def test_scores_past_f32_once_scaled(t, kv, reqs, packed_too, sign):
+    """Scores that are finite, but not times the scale: still the softmax of their differences.  q and k are whole numbers up
+    to 7 times 2^13 (q negative: scores all below), so every score is a whole number under 64 49 2^26, exact in f32 in any order;
+    scores that differ do so by 2^26 1e30, so a row is the mean of v over its keys of the largest score, to the tolerances above."""
+    nh, nkv, hd = 16, 8, 64
+    p = Paged(reqs, nh, nkv, hd, t, kv, 16, "head", seed=34, scale=1e30)
+    g = torch.Generator().manual_seed(35)
+    p.q[:] = (sign * torch.randint(1, 8, p.q.shape, generator=g) * 2.0 ** 13).to(TYPES[t])
+    p.qd[:, :nh * hd] = p.q.reshape(p.T, -1).to(DEV)
+    for b, (k, _) in enumerate(p.kv):
+        k[:] = (torch.randint(1, 8, k.shape, generator=g) * 2.0 ** 13).to(k.dtype)
+        at = torch.arange(k.shape[0])
+        p.kc[p.table[b].cpu().long()[at // 16].to(DEV), :, (at % 16).to(DEV)] = k.to(DEV)
+    exact, mag = p.want()
+    vmax = float(max(v.abs().max() for _, v in p.kv))
+    close_attention(p.run(), exact, mag, t, 1000, vmax)
+    if not packed_too:
+        return
+    n = reqs[0][1]
+    rows = torch.cat((p.q[:n].reshape(n, -1), p.kv[0][0].reshape(n, -1).to(TYPES[t]), p.kv[0][1].reshape(n, -1).to(TYPES[t])), 1).to(DEV)
+    out, cu, E = torch.full((n, nh * hd), 7.0, dtype=TYPES[t], device=DEV), i32([0, n]), rows.element_size()
+    d = hip.PackedAttn(dtype=hip.DT[t], n_heads=nh, n_kv_heads=nkv, head_dim=hd, B=1, T=n, scale=1e30, q=dp(rows), k=dp(rows) + nh * hd * E,
+                       v=dp(rows) + (nh + nkv) * hd * E, out=dp(out), q_stride=rows.stride(0), k_stride=rows.stride(0), v_stride=rows.stride(0),
+                       out_stride=nh * hd, cu=dp(cu))
+    ok(hip.lib().qwen_hip_op_packed_attention(C.byref(d), stream()))
+    torch.cuda.synchronize()
+    close_attention(out.view(n, nh, hd), exact[:n], mag[:n], t, 1000, vmax)
+
+
 def test_one_key_returns_its_value():
     """With one visible key the output is that key's value to the bit, in every type (f32: its planes sum to it)."""
     for t, kv in KINDS:
