@@ -464,7 +464,9 @@ enum { QWEN_HIP_DT_F32 = 0, QWEN_HIP_DT_BF16 = 1, QWEN_HIP_DT_F16 = 2 };
  * (its slot: page * page_size + place); element (page, head, place, d) of k (of v) is
  * k[page*page_stride + head*head_stride + place*slot_stride + d].  Any order of pages, heads and places is a choice
  * of strides (in elements; [page][head][place][d] and [page][place][head][d] are the usual two).  dtype BF16 or
- * F16; head_dim 64 or 128; k and v aligned to 16 bytes, strides multiples of 8 elements. */
+ * F16; head_dim 64 or 128; k and v aligned to 16 bytes, strides multiples of 8 elements.  To be written, every row
+ * (page, head, place) of k and of v has to be memory of its own, each stride at least the extent of the smaller ones; k and v
+ * may interleave. */
 typedef struct {
     void *k, *v;
     long long page_stride, head_stride, slot_stride;

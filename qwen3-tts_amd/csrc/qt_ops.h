@@ -181,3 +181,33 @@ static inline int qt_check_pages(const char *who, const qwen_hip_kv_pages_t *kv)
               kv->slot_stride, kv->head_dim);
     return 0;
 }
+
+// A cache that is written: every place's row is memory of its own, in k and in v.  The strides nest (each is at least the extent of all
+// smaller ones), as they do in any order of pages, heads and places; so a row of v meets one of k only where their distance
+// is, stride by stride from the largest, the multiple below or above what is left of it, and less than a row at the end.
+struct QtDim { __int128 stride, count; };
+static inline bool qt_dims_meet(const QtDim *d, int n, __int128 left, int row) {
+    if (n == 0) return left < row && -left < row;
+    const __int128 s = d[n - 1].stride, c = left / s - (left % s < 0);
+    return (c < d[n - 1].count && -c < d[n - 1].count && qt_dims_meet(d, n - 1, left - c * s, row)) ||
+           (c + 1 < d[n - 1].count && -(c + 1) < d[n - 1].count && qt_dims_meet(d, n - 1, left - (c + 1) * s, row));
+}
+static inline int qt_check_pages_apart(const char *who, const qwen_hip_kv_pages_t *kv) {
+    QtDim all[3] = {{kv->page_stride, kv->n_pages}, {kv->head_stride, kv->n_kv_heads}, {kv->slot_stride, kv->page_size}}, d[3];
+    int n = 0;
+    __int128 extent = kv->head_dim;
+    for (int i = 0; i < 3; i++) {
+        if (all[i].count == 1) continue;
+        int at = n++;
+        for (; at > 0 && d[at - 1].stride > all[i].stride; at--) d[at] = d[at - 1];
+        d[at] = all[i];
+    }
+    for (int i = 0; i < n; i++) {
+        QT_REFUSE(d[i].stride < extent, "%s: cache strides %lld, %lld, %lld: rows of different places overlap", who, kv->page_stride,
+                  kv->head_stride, kv->slot_stride);
+        extent += (d[i].count - 1) * d[i].stride;
+    }
+    const intptr_t bytes = (intptr_t)kv->v - (intptr_t)kv->k;        // both aligned to 16
+    QT_REFUSE(qt_dims_meet(d, n, bytes / 2, kv->head_dim), "%s: rows of k and v overlap", who);
+    return 0;
+}

@@ -333,6 +333,7 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
                        qt_rows_meet(p->q_out, p->q_out_stride * E, qw * E, p->k, p->k_stride * E, kw, p->T) ||
                        qt_rows_meet(p->q_out, p->q_out_stride * E, qw * E, p->v, p->v_stride * E, kw, p->T)),
               "page_append: q_out overlaps rows that are read (it may be q itself)");
+    if (qt_check_pages_apart("page_append", kv)) return -1;
     hipStream_t st = (hipStream_t)stream;
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_append: the stream's device: %s", hipGetErrorString(on.err));

@@ -116,6 +116,18 @@ def test_append_refuses_to_write_q_over_rows_that_are_read(kw, word):
 
 
 
+@pytest.mark.parametrize("kw,word", [
+    (dict(v=32 * Q), "k and v"), (dict(v=32 * Q + 240), "k and v"), (dict(v=32 * Q - 9 * 32768 - 7 * 4096 - 15 * 256 - 240), "k and v"),
+    # v begins within k's pages, in their gap but for the last 16 bytes
+    (dict(page_stride=4 * 16384, v=32 * Q + 3 * 32768 + 16), "k and v"),
+    (dict(page_stride=2048), "places"), (dict(page_stride=16384 - 8), "places"), (dict(slot_stride=136), "places"),
+    (dict(head_stride=128, slot_stride=1016), "places"), (dict(n_pages=1, page_stride=0, head_stride=128, slot_stride=1016), "places"),
+    (dict(n_pages=(1 << 27) - 1, page_stride=1 << 62, head_stride=1 << 62), "places")])
+def test_append_refuses_a_cache_whose_rows_overlap(kw, word):
+    refused(hip.lib().qwen_hip_op_page_append(C.byref(pages(**{**dict(k=32 * Q, v=40 * Q), **kw})), C.byref(append(q=Q, k=3 * Q, v=4 * Q, q_out=6 * Q)), None), word)
+
+
+
 @pytest.mark.parametrize("kw,word", BAD_PAGES)
 def test_bad_cache_descriptors_are_refused(kw, word):
     L = hip.lib()

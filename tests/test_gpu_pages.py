@@ -342,6 +342,34 @@ def test_append_writes_q_beside_the_rows_it_reads():
     assert torch.equal(rows[0, :128], rows[0, 256:384]) and torch.equal(rows[1:, :128], before[1:, :128])
 
 
+
+@pytest.mark.parametrize("order", ["page k/v head place", "page place head k/v", "head page place k/v", "k/v place head page", "page place, gap"])
+def test_append_into_caches_of_any_order(order):
+    """k and v in one buffer, interleaved at any level: what separate pools hold."""
+    n, nkv, page, hd = 4, 2, 4, 64
+    g = torch.Generator().manual_seed(6)
+    rows = torch.randn(9, 2 * nkv * hd, generator=g).to(torch.bfloat16).to(DEV)
+    slot = i32([3, 5, 7, 9, 11, 0, 15, 8, 1])
+    axes = {"page k/v head place": (1, 0, 2, 3), "page place head k/v": (3, 0, 2, 1), "head page place k/v": (3, 1, 0, 2), "k/v place head page": (0, 3, 2, 1)}
+    if order in axes:                                           # where k/v, page, head and place stand
+        at = axes[order]
+        dims = [0] * 4
+        for i, d in zip(at, (2, n, nkv, page)):
+            dims[i] = d
+        both = torch.zeros(*dims, hd, dtype=torch.bfloat16, device=DEV).permute(*at, 4)
+        k, v = both[0], both[1]
+    else:                                                       # v in the gaps that k's pages leave
+        buf = torch.zeros(n * 2 * page * nkv * hd, dtype=torch.bfloat16, device=DEV)
+        k, v = (buf[o * page * nkv * hd:].as_strided((n, nkv, page, hd), (2 * page * nkv * hd, hd, nkv * hd, 1)) for o in (0, 1))
+    ks, vs = (torch.zeros(n, nkv, page, hd, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    d = hip.PageAppend(dtype=1, T=9, k=dp(rows), v=dp(rows) + nkv * hd * 2, k_stride=2 * nkv * hd, v_stride=2 * nkv * hd, slot=dp(slot))
+    for a, b in ((k, v), (ks, vs)):
+        ok(hip.lib().qwen_hip_op_page_append(C.byref(pages_of(a, b, "bf16")), C.byref(d), stream()))
+    torch.cuda.synchronize()
+    assert torch.equal(k, ks) and torch.equal(v, vs) and bool(ks.any())
+    assert torch.equal(ks[1, :, 1], rows[1, :nkv * hd].view(nkv, hd)) and torch.equal(vs[1, :, 1], rows[1, nkv * hd:].view(nkv, hd))
+
+
 def far_pool(n_pages, nkv, page, hd, total):
     """bf16 pages `total` bytes from the first to the end, far apart."""
     far = total // 2 // n_pages // 64 * 64
