@@ -535,7 +535,7 @@ int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_a
  * F16 rows (over a cache of their own type) the probabilities are rounded to that type for the product with V.
  * max_q and max_kv: the longest request's new tokens and kv_len as far as the host knows; they choose the launch
  * shape and change no result beyond rounding.  scale > 0.  B <= 65535, n_heads / n_kv_heads <= 64, T * n_heads < 2^26.
- * out must not overlap q or the cache.
+ * out must not overlap q (refused) or the cache (not looked at).
  * workspace: qwen_hip_op_page_attention_workspace() bytes (of the same descriptor), aligned to 16; its contents do
  * not matter before or after; calls that may overlap need one each.  Alignment and strides as for append. */
 typedef struct {
@@ -556,7 +556,7 @@ int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_pag
 
 /* The prefill's causal attention for several prompts at once, of different lengths, packed behind each other:
  * sequence b is tokens cu[b] .. cu[b+1] - 1 of q, k, v and out.  q, k, v and out share one dtype (F32: f32 products,
- * as qwen_hip_op_prefill_attention; BF16 / F16 as above); the rest as for the paged form. */
+ * as qwen_hip_op_prefill_attention; BF16 / F16 as above); the rest as for the paged form.  out must not overlap q, k or v. */
 typedef struct {
     const void *q, *k, *v;
     void *out;
@@ -576,7 +576,7 @@ int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *attn, void *strea
  * in f32, rounded once to dtype (of logits and out).  rep, presence, frequency, bias_tok and mask may each be NULL:
  * off.  Tokens outside [0, V) are passed over; offsets are clipped to hist_cap / bias_cap entries, a row's biases to
  * its first 65534, and n_out counts up to 65535.  out may be
- * logits (same stride).  A row whose mask allows nothing is all -infinity.  B <= 65535. */
+ * logits (same stride), and not overlap them otherwise.  A row whose mask allows nothing is all -infinity.  B <= 65535. */
 typedef struct {
     const void *logits;
     void *out;

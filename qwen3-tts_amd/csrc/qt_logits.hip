@@ -174,6 +174,9 @@ extern "C" int qwen_hip_op_logit_rules(const qwen_hip_logit_rules_t *p, void *st
     QT_REFUSE(p->bias_tok && (!p->bias_val || !p->bias_off || p->bias_cap < 0), "logit_rules: biases need values and offsets");
     QT_REFUSE(p->mask && p->mask_stride < (p->V + 31) / 32, "logit_rules: mask_stride %lld under %d words", p->mask_stride, (p->V + 31) / 32);
     QT_REFUSE(((uintptr_t)p->logits | (uintptr_t)p->out) % E, "logit_rules: logits and out have to be aligned to their elements");
+    QT_REFUSE(p->logits != p->out && qt_rows_meet(p->out, p->out_stride * E, (long long)p->V * E, p->logits, p->logits_stride * E,
+                                                  (long long)p->V * E, p->B),
+              "logit_rules: out overlaps logits (it may be them)");
     hipStream_t st = (hipStream_t)stream;
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "logit_rules: the stream's device: %s", hipGetErrorString(on.err));

@@ -1128,6 +1128,8 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     QT_REFUSE(need > 0 && (!p->workspace || p->workspace_bytes < need), "page_attention: a workspace of %lld bytes is needed, %lld given",
               need, p->workspace ? p->workspace_bytes : 0ll);
     QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "page_attention: too many tiles for one launch");
+    const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * kv->head_dim * E;
+    QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T), "page_attention: out overlaps q");
     hipStream_t st = (hipStream_t)stream;
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_attention: the stream's device: %s", hipGetErrorString(on.err));
@@ -1168,6 +1170,11 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
     const AttPlan plan = att_plan(a, p->dtype, false, 0, 0);
     QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "packed_attention: too many tiles for one launch");
+    const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * p->head_dim * E, kw = (long long)p->n_kv_heads * p->head_dim * E;
+    QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T) ||
+                  qt_rows_meet(p->out, p->out_stride * E, row, p->k, p->k_stride * E, kw, p->T) ||
+                  qt_rows_meet(p->out, p->out_stride * E, row, p->v, p->v_stride * E, kw, p->T),
+              "packed_attention: out overlaps q, k or v");
     a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)p->k; a.v = (const uint8_t *)p->v; a.out = (uint8_t *)p->out;
     a.qs = p->q_stride; a.os = p->out_stride; a.ks_slot = p->k_stride; a.vs_slot = p->v_stride;
     a.cu = p->cu;

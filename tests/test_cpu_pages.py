@@ -195,6 +195,26 @@ def test_logit_rules_refuses(kw, word):
     refused(hip.lib().qwen_hip_op_logit_rules(C.byref(hip.LogitRules(**{**d, **kw})), None), word)
 
 
+# rows of 4096 bytes; 4 of them
+@pytest.mark.parametrize("kw", [dict(out=Q + 16), dict(out=Q - 16), dict(out=Q + 4 * 4096 - 16), dict(out=Q - 4 * 4096 + 16), dict(q_stride=0, out=Q - 3 * 4096 - 16),
+                                dict(q_stride=2056, out=Q + 4096), dict(q_stride=6144, out_stride=6144, out=Q + 2 * 4096 + 16)])
+def test_attention_refuses_an_out_that_overlaps(kw):
+    L, d = hip.lib(), {**dict(q=Q, T=4), **kw}
+    refused(L.qwen_hip_op_page_attention(C.byref(pages(k=32 * Q, v=40 * Q)), C.byref(attn(**d)), None), "out overlaps q")
+    for at in ("q", "k", "v"):                                  # k's and v's rows: as wide as q's
+        e = dict(q=8 * Q, k=8 * Q, v=8 * Q, q_stride=2048, k_stride=2048, v_stride=2048, out_stride=2048, cu=P, dtype=1, n_heads=16, n_kv_heads=16,
+                 head_dim=128, B=4, scale=0.1)
+        e.update({at if k == "q" else at + "_stride" if k == "q_stride" else k: v for k, v in d.items()})
+        refused(L.qwen_hip_op_packed_attention(C.byref(hip.PackedAttn(**e)), None), "out overlaps")
+
+
+@pytest.mark.parametrize("kw", [dict(out=Q + 4), dict(out=Q + 396), dict(out=Q - 796 + 4), dict(out=Q + 400, out_stride=101), dict(out=Q + 200, logits_stride=200, out_stride=200)])
+def test_logit_rules_refuse_an_out_that_overlaps(kw):
+    d = dict(logits=Q, out=Q, logits_stride=100, out_stride=100, dtype=0, B=2, V=100)
+    refused(hip.lib().qwen_hip_op_logit_rules(C.byref(hip.LogitRules(**{**d, **kw})), None), "overlaps")
+
+
+
 def test_empty_calls_do_nothing():
     L = hip.lib()
     assert L.qwen_hip_op_page_append(C.byref(pages()), C.byref(append(T=0)), None) == 0

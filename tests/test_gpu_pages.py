@@ -798,6 +798,25 @@ def test_packed_attention(t, nh, nkv, hd, lens, window):
     close_attention(out[:T, :nh * hd].view(T, nh, hd), exact, mag, t, max(lens), float(w.abs().max()))
 
 
+@pytest.mark.parametrize("t", ["f32", "bf16"])
+@pytest.mark.parametrize("n,nh,nkv", [(50, 4, 2), (900, 16, 8)])
+def test_out_beside_the_rows_it_is_made_of(t, n, nh, nkv):
+    """out as further columns of q, k and v's own buffer, and k and v the same rows of it."""
+    hd, g = 64, torch.Generator().manual_seed(24)
+    W = (2 * nh + nkv) * hd
+    rows = torch.randn(n, W, generator=g).to(TYPES[t])
+    dev, cu, E = rows.to(DEV), i32([0, n]), rows.element_size()
+    d = hip.PackedAttn(dtype=hip.DT[t], n_heads=nh, n_kv_heads=nkv, head_dim=hd, B=1, T=n, scale=hd ** -0.5, q=dp(dev), k=dp(dev) + nh * hd * E,
+                       v=dp(dev) + nh * hd * E, out=dp(dev) + (nh + nkv) * hd * E, q_stride=W, k_stride=W, v_stride=W, out_stride=W, cu=dp(cu))
+    ok(hip.lib().qwen_hip_op_packed_attention(C.byref(d), stream()))
+    torch.cuda.synchronize()
+    kv = rows[:, nh * hd:(nh + nkv) * hd]
+    exact, mag = packed_want(torch.cat((rows[:, :nh * hd], kv, kv), 1), [n], nh, nkv, hd, 0)
+    assert torch.equal(dev[:, :(nh + nkv) * hd].cpu(), rows[:, :(nh + nkv) * hd])
+    close_attention(dev[:, (nh + nkv) * hd:].cpu().view(n, nh, hd), exact, mag, t, n, float(rows.abs().max()))
+
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("where", ["v", "k", "q", "all"])
 def test_values_that_are_not_finite(t, where):
