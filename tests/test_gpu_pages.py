@@ -731,6 +731,26 @@ def test_chunk_over_a_cache_past_32_bits(t, kv):
     p.check()
 
 
+@pytest.mark.parametrize("t,kv", KINDS)
+@pytest.mark.parametrize("far", ["page", "place", "head"])
+@pytest.mark.parametrize("reqs", [[(70, 120), (0, 90)], [(150, 1), (31, 1), (0, 1)]])
+def test_a_cache_between_2_and_4_gib(t, kv, far, reqs):
+    """Byte offsets past 2^31 that stay under 2^32, by pages, by places of a page and by heads."""
+    p = Paged(reqs, 8, 2, 128, t, kv, 16, "head", seed=36)
+    n, total = p.pages.n_pages, (1 << 31) - 500000
+    step = {"page": total // n, "place": total // 16, "head": total - (1 << 18)}[far] // 128 * 128
+    assert n <= 64                                              # the rest of a place's offset: under 2^18 elements
+    strides = {"page": (step, 2048, 128), "place": (256, 128, step), "head": (2048, step, 128)}[far]
+    k, v = (torch.zeros(total, dtype=TYPES[kv], device=DEV).as_strided((n, 2, 16, 128), strides + (1,)) for _ in range(2))
+    k.copy_(p.kc)
+    v.copy_(p.vc)
+    last = {"page": int(p.table.max()), "place": 15, "head": 1}[far] * step * 2
+    assert (1 << 31) <= last < 1 << 32
+    p.pages.k, p.pages.v, p.pages.page_stride, p.pages.head_stride, p.pages.slot_stride = dp(k), dp(v), *strides
+    p.check()
+
+
+
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 def test_many_long_requests(t):
     """More requests than the order by length looks at (256), of many rows each."""
