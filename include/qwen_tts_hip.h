@@ -452,7 +452,7 @@ int qwen_hip_op_sd_conv_transpose(float *Y, const float *X, const float *W, cons
  * bookkeeping, the cache's writer, the attention that reads it, whole prompts packed behind each other, and the
  * rules on a batch's logits.  Every pointer in these descriptors is DEVICE memory of the device that `stream`
  * belongs to; the descriptor itself is host memory, read during the call, so one made once can be used for every
- * step.  Calls launch on `stream` (a hipStream_t; NULL = the null stream of the current device) and return
+ * step.  Calls launch on `stream` (a hipStream_t; NULL or hipStreamLegacy = the null stream of the current device) and return
  * without waiting: 0, or -1 with qwen_hip_last_error() set and nothing launched.  (HIP's own last error, where an earlier
  * call left one, is neither reported nor cleared.  Of a call that takes two launches the first may have succeeded: then
  * attention's rows are unfinished and a plan in place has changed neither lengths nor free count; both can be repeated.)

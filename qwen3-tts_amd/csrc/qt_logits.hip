@@ -177,7 +177,7 @@ extern "C" int qwen_hip_op_logit_rules(const qwen_hip_logit_rules_t *p, void *st
     QT_REFUSE(p->logits != p->out && qt_rows_meet(p->out, p->out_stride * E, (long long)p->V * E, p->logits, p->logits_stride * E,
                                                   (long long)p->V * E, p->B),
               "logit_rules: out overlaps logits (it may be them)");
-    hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "logit_rules: the stream's device: %s", hipGetErrorString(on.err));
     const RulesArgs a = {(const uint8_t *)p->logits, (uint8_t *)p->out, p->logits_stride, p->out_stride, p->mask_stride, p->hist,

@@ -116,6 +116,9 @@ __device__ __forceinline__ int wave_max_i(int v) {
 
 // ---- host side ----
 
+// hipStreamLegacy is another name of the null stream, and one that not every runtime's hipStreamGetDevice takes.
+static inline hipStream_t qt_stream(void *stream) { return (hipStream_t)stream == hipStreamLegacy ? nullptr : (hipStream_t)stream; }
+
 // Makes the stream's device the current one while a call launches (kernels are looked up for the
 // current device), and the caller's current again afterwards.
 struct QtOnDevice {

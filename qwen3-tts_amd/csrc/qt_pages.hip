@@ -214,7 +214,7 @@ extern "C" int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *p, void *stream
               "page_plan: table_cols %d (at least 1, 2^30 positions at most)", p->table_cols);
     QT_REFUSE(p->table_stride < p->table_cols, "page_plan: table_stride %lld under table_cols %d", p->table_stride, p->table_cols);
     QT_REFUSE(p->max_tokens < 0 || p->max_tokens > (1 << 28), "page_plan: max_tokens %d out of range (0..2^28)", p->max_tokens);
-    hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_plan: the stream's device: %s", hipGetErrorString(on.err));
     PlanArgs a = {p->new_len, p->kv_len, p->n_free, p->table, p->free_pages, p->kv_len_out, p->n_free_out, p->cu_q, p->pos,
@@ -334,7 +334,7 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
                        qt_rows_meet(p->q_out, p->q_out_stride * E, qw * E, p->v, p->v_stride * E, kw, p->T)),
               "page_append: q_out overlaps rows that are read (it may be q itself)");
     if (qt_check_pages_apart("page_append", kv)) return -1;
-    hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_append: the stream's device: %s", hipGetErrorString(on.err));
     const AppendArgs a = {(const uint8_t *)p->q, (const uint8_t *)p->k, (const uint8_t *)p->v, (uint8_t *)p->q_out,

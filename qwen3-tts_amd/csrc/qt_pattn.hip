@@ -1130,7 +1130,7 @@ extern "C" int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const q
     QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "page_attention: too many tiles for one launch");
     const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * kv->head_dim * E;
     QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T), "page_attention: out overlaps q");
-    hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_attention: the stream's device: %s", hipGetErrorString(on.err));
     a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)kv->k; a.v = (const uint8_t *)kv->v; a.out = (uint8_t *)p->out;
@@ -1180,7 +1180,7 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
     a.cu = p->cu;
     a.window = p->window <= ATT_MAX_KEYS ? p->window : 0;
     a.c = p->scale * QT_LOG2E;
-    hipStream_t st = (hipStream_t)stream;
+    const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "packed_attention: the stream's device: %s", hipGetErrorString(on.err));
     hipError_t e;

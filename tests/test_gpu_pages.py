@@ -1228,6 +1228,30 @@ def test_a_captured_step_is_replayed(t):
         s.check(new, at)
 
 
+@pytest.mark.parametrize("handle", [None, 1, 2], ids=["null", "legacy", "per-thread"])
+def test_the_handles_that_are_no_streams_of_the_callers(handle, monkeypatch):
+    """NULL, hipStreamLegacy and hipStreamPerThread, for a step, a packed call and the rules."""
+    s = Server("bf16", 3, 64)
+    at = s.feed([30, 17, 0])
+    s.out.fill_(7.0)
+    rows = torch.randn(30, 4 * 64, generator=torch.Generator().manual_seed(4))
+    dev, out, x, y = rows.to(DEV), torch.zeros(30, 128, device=DEV), torch.arange(100, dtype=torch.float32, device=DEV), torch.zeros(100, device=DEV)
+    d = hip.LogitRules(dtype=0, B=1, V=100, logits=dp(x), out=dp(y), logits_stride=100, out_stride=100)
+    cu = i32([0, 30])
+    torch.cuda.synchronize()
+    monkeypatch.setitem(globals(), "stream", lambda: handle)
+    s.launch()
+    torch.cuda.synchronize()
+    s.check([30, 17, 0], at)
+    ok(packed(dev, [30], 2, 1, 64, "f32", out, cu=cu))
+    ok(hip.lib().qwen_hip_op_logit_rules(C.byref(d), handle))
+    torch.cuda.synchronize()
+    exact, mag = packed_want(rows, [30], 2, 1, 64, 0)
+    close_attention(out.cpu().view(30, 2, 64), exact, mag, "f32", 30, float(rows.abs().max()))
+    assert torch.equal(x, y)
+
+
+
 def test_a_step_that_cannot_be_planned_leaves_everything():
     s = Server("f32", 3, 64)
     s.feed([30, 17, 0])
