@@ -509,7 +509,7 @@ int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *plan, void *stream);
  * q_norm / k_norm [head_dim] f32; NULL: none), RoPE of both on the halves of a head (tables f32 [rope_len][head_dim/2];
  * NULL: none), q to q_out, k and v to the cache at slot[t], each rounded once to the nearest (the Talker's own
  * cache truncates).  dtype: of q, k, v and q_out; F32 rows go with either cache type, BF16 and F16 rows with their
- * own.  A token whose slot is outside the cache (the plan's -1), or whose pos is outside [0, rope_len) where there
+ * own (attention over an F16 cache takes F16 rows: an F32 q_out is then the caller's to round).  A token whose slot is outside the cache (the plan's -1), or whose pos is outside [0, rope_len) where there
  * are tables, is skipped: nothing of it is written.  Slots of one call have to be distinct.  q may be NULL (k and v
  * only); q_out may be q with q's stride, else it shares no memory with q, k or v (rows of one buffer beside theirs, with
  * their stride, do not).  Pointers aligned to 16 bytes, strides (in elements, between tokens) multiples of 16 bytes. */
@@ -556,7 +556,8 @@ int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_pag
 
 /* The prefill's causal attention for several prompts at once, of different lengths, packed behind each other:
  * sequence b is tokens cu[b] .. cu[b+1] - 1 of q, k, v and out.  q, k, v and out share one dtype (F32: f32 products,
- * as qwen_hip_op_prefill_attention; BF16 / F16 as above); the rest as for the paged form.  out must not overlap q, k or v. */
+ * as qwen_hip_op_prefill_attention, of operands that keep what is above 2^-134 of them: three bf16 planes each; BF16 / F16
+ * as above); the rest as for the paged form.  out must not overlap q, k or v. */
 typedef struct {
     const void *q, *k, *v;
     void *out;

@@ -293,7 +293,7 @@ __device__ __forceinline__ void att_stored() { asm volatile("s_waitcnt vmcnt(0)"
 // A workgroup takes 32 rows; its four waves take the 32-key blocks in turn, each with a softmax of its own, K and V
 // going from memory into operand registers without LDS or barriers and split there; the waves' sums are merged through
 // LDS at the end.  V is loaded when K is used up: both at once spill.  Bound by the splitting (VALU) next to the
-// products: two prompts of 4000 positions 911 us, 144 TFLOP/s of f32 products (a library's f32 matrix product of 8192^3:
+// products: two prompts of 4000 positions 925 us, 142 TFLOP/s of f32 products (a library's f32 matrix product of 8192^3:
 // 153); with V loaded ahead of the scores 1105, in 16-row tiles (k_att_one) 1377.
 template <int HD>
 __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(2))) void k_att_f32(AttArgs a) {
@@ -722,9 +722,9 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
 // A workgroup takes 128 rows, 32 a wave, and goes through its keys 64 at a time: K and V of a block are copied from
 // memory straight into LDS (no registers), two blocks deep, one barrier a block, and every wave reads both
 // operands from there.  16-bit types only.  Block kb + 1's scores do not wait for block kb's softmax: K is a block ahead of
-// V.  Bound by the matrix core's and the vector unit's shares together (53 and 54 % of the cycles of two prompts of 5003 and
-// 8191 f16: 411 to 428 us, 881 TFLOP/s and more at the 1.7 GHz that the load leaves; LDS 27 %, no bank conflicts; 32-row tiles
-// straight from memory 1031 us), by the first loads of each workgroup for short prompts (16 of 40 to 1500 bf16: 84 us, 211).
+// V.  Bound by the matrix core's and the vector unit's shares together (50 and 48 % of the cycles of two prompts of 5003 and
+// 8191 f16: 407 to 428 us, 881 TFLOP/s and more at the 1.7 GHz that the load leaves; LDS 25 %, no bank conflicts; 32-row tiles
+// straight from memory 1031 us), by the first loads of each workgroup for short prompts (16 of 40 to 1500 bf16: 86 us, 211).
 //   K, row k: 16-byte chunk c at place c ^ swk(k): the 16 lanes of a phase of a wave's read (16 rows, one chunk)
 //   fall on 16 different groups of banks.  V: chunk c at place c ^ swv(k): a transposing read takes 4 rows by 64 bytes
 //   a half-wave, which fall on different banks.
@@ -1036,7 +1036,10 @@ static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv
     } else if (rows >= 32ll * a.B && (paged || (rows / 128 + a.B) * a.nkv >= 96)) {
         // 128-row tiles from 32 rows a request on (64 requests of 32 tokens 42 us against 79 in 16-row tiles, 8 of 16 over
         // 3000 keys 27.3 against 27.8, 32 of 4 70 against 60); prompts, whose keys are not split, while there are tiles
-        // enough (8 of 100 to 300 13.1 us against 20.3; one of 512 15.9 against 13.0, three of 21 to 128 9.2 against 8.4)
+        // enough (8 of 100 to 300 13.1 us against 20.3; one of 512 15.9 against 13.0, three of 21 to 128 9.2 against 8.4).
+        // Those are equal requests.  The rule goes by a call's mean, so a step of single tokens and a chunk takes one kernel
+        // for both (bf16, 16 over 8 heads, a chunk over 2000 keys: 64 streams of 1000 to 8000 keys and 512 tokens in 16-row tiles
+        // 259 us, 198 and 33 in a call each; 32 of them and 1024 tokens in 128-row tiles 160, 110 and 49)
         p.kind = ATT_TILE;
     }
     if (p.kind == ATT_ONE) {
