@@ -459,18 +459,28 @@ int qwen_hip_op_sd_conv_transpose(float *Y, const float *X, const float *W, cons
  * They allocate nothing and can be captured into a graph.  Lengths, tables and slots are read on the device: a replayed
  * graph follows what they hold then. */
 enum { QWEN_HIP_DT_F32 = 0, QWEN_HIP_DT_BF16 = 1, QWEN_HIP_DT_F16 = 2 };
+enum { QWEN_HIP_DT_E4M3 = 16 };      /* of caches only */
 
 /* One layer's cache in pages: position p of a request lies in page table[p / page_size] at place p % page_size
  * (its slot: page * page_size + place); element (page, head, place, d) of k (of v) is
  * k[page*page_stride + head*head_stride + place*slot_stride + d].  Any order of pages, heads and places is a choice
- * of strides (in elements; [page][head][place][d] and [page][place][head][d] are the usual two).  dtype BF16 or
- * F16; head_dim 64 or 128; k and v aligned to 16 bytes, strides multiples of 8 elements.  To be written, every row
+ * of strides (in elements; [page][head][place][d] and [page][place][head][d] are the usual two).  dtype BF16,
+ * F16 or E4M3; head_dim 64 or 128; k and v aligned to 16 bytes, strides multiples of 16 bytes.  To be written, every row
  * (page, head, place) of k and of v has to be memory of its own, each stride at least the extent of the smaller ones; k and v
- * may interleave. */
+ * may interleave.
+ * E4M3 is a quantised cache: a row's head_dim codes (8-bit floating point: sign, 4 bits of exponent of bias 7, 3 of mantissa; the largest
+ * 448, 0x7F and 0xFF NaN) and one scale for the row, the byte k_scale[page*scale_page_stride + head*scale_head_stride +
+ * place*scale_slot_stride] (v_scale likewise; strides in bytes): element d is its code times 2^(byte - 127); a byte under 63
+ * counts as 63, one over 246 makes the row NaN.  A row is written with the smallest 2^e, e >= -64, for which its largest magnitude is at most 448 2^e, and each
+ * element divided by it and rounded once to the nearest code, ties to even: off by at most 2^-4 of its value, or 2^-10 2^e where that is
+ * more.  A row with a magnitude of 2^127 or more, infinite or NaN is written as NaN.  The scales' places have to be memory of their
+ * own as the rows have, and pages of scales not lie among the codes of a page.  The scale fields are read for E4M3 only. */
 typedef struct {
     void *k, *v;
     long long page_stride, head_stride, slot_stride;
     int dtype, n_pages, page_size, n_kv_heads, head_dim;
+    uint8_t *k_scale, *v_scale;
+    long long scale_page_stride, scale_head_stride, scale_slot_stride;
 } qwen_hip_kv_pages_t;
 
 /* The bookkeeping of one step.  For every request b < B (B <= 2048): kv_len[b] tokens are cached, in the pages
@@ -508,8 +518,8 @@ int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *plan, void *stream);
 /* New tokens' q, k, v rows into attention's inputs: per-head RMSNorm of q and k (x / sqrt(mean x^2 + eps) times
  * q_norm / k_norm [head_dim] f32; NULL: none), RoPE of both on the halves of a head (tables f32 [rope_len][head_dim/2];
  * NULL: none), q to q_out, k and v to the cache at slot[t], each rounded once to the nearest (the Talker's own
- * cache truncates).  dtype: of q, k, v and q_out; F32 rows go with either cache type, BF16 and F16 rows with their
- * own (attention over an F16 cache takes F16 rows: an F32 q_out is then the caller's to round).  A token whose slot is outside the cache (the plan's -1), or whose pos is outside [0, rope_len) where there
+ * cache truncates).  dtype: of q, k, v and q_out; F32 rows go with any cache type, BF16 and F16 rows with their
+ * own and E4M3 (attention over an F16 cache takes F16 rows: an F32 q_out is then the caller's to round).  A token whose slot is outside the cache (the plan's -1), or whose pos is outside [0, rope_len) where there
  * are tables, is skipped: nothing of it is written.  Slots of one call have to be distinct.  q may be NULL (k and v
  * only); q_out may be q with q's stride, else it shares no memory with q, k or v (rows of one buffer beside theirs, with
  * their stride, do not).  Pointers aligned to 16 bytes, strides (in elements, between tokens) multiples of 16 bytes. */
@@ -531,8 +541,9 @@ int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_a
  * where window > 0; query head h reads kv head h / (n_heads / n_kv_heads).  A row that sees nothing, or
  * only scores of -infinity, is 0; rows before cu_q[0] and behind cu_q[B] stay as they were.  A table entry outside
  * [0, n_pages) holds no keys: its positions are not seen.  What lies in positions that a row does not see never reaches it, infinite or NaN
- * included.  Scores, softmax and sums are f32; with F32 rows (over a BF16 cache) so are the products; with BF16 or
- * F16 rows (over a cache of their own type) the probabilities are rounded to that type for the product with V.
+ * included.  Scores, softmax and sums are f32; with F32 rows (over a BF16 or E4M3 cache) so are the products; with BF16 or
+ * F16 rows (over a cache of their own type or E4M3) the probabilities are rounded to that type for the product with V, which
+ * reads an E4M3 cache's values as they are (F16 rows: what lies under 2^-24 of the largest scale's unit is rounded to that).
  * max_q and max_kv: the longest request's new tokens and kv_len as far as the host knows; they choose the launch
  * shape and change no result beyond rounding.  scale > 0.  B <= 65535, n_heads / n_kv_heads <= 64, T * n_heads < 2^26.
  * out must not overlap q (refused) or the cache (not looked at).
@@ -553,6 +564,95 @@ typedef struct {
 } qwen_hip_page_attn_t;
 long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn);  /* -1: error */
 int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn, void *stream);
+
+/* ---- trees of drafted tokens ----
+ * A step that checks drafts appends, for every request, a tree of tokens: the first of its new tokens is the root (the last token that
+ * was decided, not yet cached), each of the others continues its parent.  page_plan gives them slots one behind the other;
+ * tree_plan gives them positions by depth, and masks of what each sees; page_append and tree_attention do a layer; tree_verify takes
+ * the target's and the draft's probabilities and keeps a path from the root; tree_commit moves the path's rows together in the caches and
+ * gives back the pages that are no longer needed. */
+
+/* parent[t]: token t's parent as an index within its request's new tokens, less than its own index; anything else makes t a
+ * root.  Request b's tokens are cu_q[b] .. cu_q[b+1] - 1, kv_len counts them.  Written for each: pos[t] = kv_len[b] - n + depth (roots: 0), and
+ * mask[t*mask_stride + w], w < mask_words: bit i is set where new token 32 w + i of the request is t or one of its ancestors.
+ * A request of more than 32 * mask_words new tokens is a plain chunk of text: each token at the position behind the one before, its masks
+ * not written, nor read by tree_attention.  Rows before cu_q[0] and behind cu_q[B] stay as they were.  mask_words <= 32. */
+typedef struct {
+    const int *parent;       /* [T] */
+    const int *cu_q;         /* [B + 1] */
+    const int *kv_len;       /* [B] */
+    int *pos;                /* [T] */
+    uint32_t *mask;          /* [T][mask_stride] */
+    long long mask_stride;   /* words, >= mask_words */
+    int B, T, mask_words;
+} qwen_hip_tree_plan_t;
+int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *plan, void *stream);
+
+/* qwen_hip_op_page_attention for steps with trees: a row sees all positions before its request's new tokens, and of those the ones
+ * whose bits are set in its mask; a request of more than 32 * mask_words new tokens is causal as there.  With attn->window > 0
+ * a row sees those positions before the new tokens that are greater than pos[t] - window (pos brought into kv_len - n .. kv_len - 1), and the mask
+ * alone decides on the new ones; pos may be NULL without a window.  Any mask will do: a row without bits sees only what is before.
+ * Everything else, the workspace too (qwen_hip_op_page_attention_workspace), is as there. */
+typedef struct {
+    const uint32_t *mask;    /* [T][mask_stride] */
+    const int *pos;          /* [T] */
+    long long mask_stride;   /* words, >= mask_words */
+    int mask_words;          /* 1 .. 32 */
+} qwen_hip_tree_t;
+int qwen_hip_op_tree_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn, const qwen_hip_tree_t *tree, void *stream);
+
+/* Which drafted tokens are kept, such that every token that comes out is distributed as the target's own.  Rows t of p and q ([T]
+ * rows of V) are the target's and the draft's probabilities of what follows token t, tok[t] is t's token, u[t] and r[b] are
+ * random numbers in [0, 1).  From the request's first new token, the root, the children of the current token are looked at in
+ * the order of their indices: with w = p's row and z = 1 at first, child c of token x is kept, and the current one from then on, where
+ * u[c] * q(x) * z < w(x); else w becomes max(w / z - q, 0) and z its sum (once z is 0, no further child of this token is kept).
+ * When no child is left, the next token is the first v for which w(0) + .. + w(v) > r[b] * sum of w (where w is 0 everywhere:
+ * of p's row; where that is too: -1).  q NULL: drafts that are certain (q(x) = 1): c is kept where u[c] * z < w(x), else w(x) becomes 0 and z
+ * max(z - w(x), 0).  All in 64 bits; probabilities that are not greater than 0 (NaN included) count as 0, rows need not add up to 1 and are not
+ * divided by their sum.  A drafted token outside [0, V) is never kept and changes nothing; one with
+ * u[c] < 0 is kept for certain (text that is given: a chunk of a prompt as a chain).  Written: n_path[b] tokens kept, the root among them (0 for a request without new
+ * tokens), path[cu_q[b] + k] their indices in ascending order, out_tok[cu_q[b] + k] the token that follows path[k]: kept ones,
+ * and at k = n_path[b] - 1 the next token; both -1 from there to the request's last row.  Rows before cu_q[0] and
+ * behind cu_q[B] stay as they were.  dtype of p and q: F32, BF16 or F16; rows aligned to 2 bytes at least (an element).
+ * max_children: the most children that a token has, as far as the host knows (0: unknown); it chooses launches and changes no result. */
+typedef struct {
+    const void *p, *q;
+    long long p_stride, q_stride;   /* elements, >= V */
+    const int *tok, *parent;        /* [T] */
+    const int *cu_q;                /* [B + 1] */
+    const float *u, *r;             /* [T], [B] */
+    int *path, *out_tok;            /* [T] */
+    int *n_path;                    /* [B] */
+    void *workspace;                /* qwen_hip_op_tree_verify_workspace() bytes, aligned to 16; as for attention */
+    long long workspace_bytes;
+    int dtype, B, T, V, max_children;
+} qwen_hip_tree_verify_t;
+long long qwen_hip_op_tree_verify_workspace(const qwen_hip_tree_verify_t *verify);  /* -1: error */
+int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *verify, void *stream);
+
+/* What is left of a step after its verification.  Request b's n = cu_q[b+1] - cu_q[b] new tokens lie at positions kv_len[b] - n on; the
+ * first n_path[b] entries of path (from path[cu_q[b]] on: ascending indices within the request, as tree_verify writes them) say which stay: row
+ * path[k] moves to position kv_len[b] - n + k, codes and scale alike, in the caches of n_layers layers (layer l's k and v are
+ * those of `kv` plus l * layer_stride elements, its scales plus l * scale_layer_stride bytes; the table is the same for all).  An entry of
+ * path that is not in k .. n - 1 moves nothing; n_path is brought into 0 .. n.
+ * Lengths and pages, where kv_len_out is given: kv_len_out[b] = kv_len[b] - n + n_path[b], and the pages of the table that it no
+ * longer reaches go onto the free list's end in the order of requests and positions, as page_plan gives pages back; the table itself is
+ * left as it is.  status 0; QWEN_HIP_PLAN_INVALID where a length is negative, under n or past the table, or more would be free than
+ * there are pages: then lengths and free list are not changed (kv_len_out and n_free_out hold what kv_len and n_free hold).  Without kv_len_out
+ * rows are moved only, for layers that lie apart: a call each, lengths and pages with one of them, the last where kv_len_out is kv_len. */
+typedef struct {
+    const int *path, *n_path;       /* [T], [B] */
+    const int *cu_q, *kv_len;       /* [B + 1], [B]: with the new tokens */
+    const int *table;               /* [B][table_stride] */
+    long long table_stride;
+    int *kv_len_out;                /* [B]; may be kv_len; NULL: rows only */
+    int *free_pages;                /* [n_pages] */
+    const int *n_free;              /* [1] */
+    int *n_free_out, *status;       /* [1]; n_free_out may be n_free */
+    long long layer_stride, scale_layer_stride;
+    int B, T, table_cols, n_layers; /* B <= 2048; n_layers 0: lengths and pages only */
+} qwen_hip_tree_commit_t;
+int qwen_hip_op_tree_commit(const qwen_hip_kv_pages_t *kv, const qwen_hip_tree_commit_t *commit, void *stream);
 
 /* The prefill's causal attention for several prompts at once, of different lengths, packed behind each other:
  * sequence b is tokens cu[b] .. cu[b+1] - 1 of q, k, v and out.  q, k, v and out share one dtype (F32: f32 products,

@@ -14,6 +14,7 @@ extern "C" void qt_seterr(const char *fmt, ...) __attribute__((format(printf, 1,
 struct QtF32 { typedef float elem; };
 struct QtBf16 { typedef uint16_t elem; };
 struct QtF16 { typedef uint16_t elem; };
+struct QtE4m3 { typedef uint8_t elem; };    // codes of a quantised cache, whose rows have a scale beside them
 
 template <typename T> __device__ __forceinline__ uint32_t qt_round2(float a, float b);
 template <> __device__ __forceinline__ uint32_t qt_round2<QtBf16>(float a, float b) {
@@ -54,6 +55,7 @@ template <typename T, int N> __device__ __forceinline__ void qt_widen8(const qt_
     }
 }
 template <typename T, int A = 16> __device__ __forceinline__ void qt_load8(const void *p, float (&v)[8]) {
+    static_assert(sizeof(typename T::elem) >= 2, "codes: qt_widen_e4m3");
     qt_w4 w[sizeof(typename T::elem) / 2];
 #pragma unroll
     for (unsigned e = 0; e < sizeof(typename T::elem) / 2; e++) w[e] = qt_load16<A>((const uint8_t *)p + 16 * e);
@@ -73,8 +75,38 @@ template <typename T, int A = 16> __device__ __forceinline__ void qt_store8(void
         qt_store16<A>(b, x);
     }
 }
+// 8 codes as the numbers they stand for, and 8 numbers of at most 448 as the nearest codes, ties to even
+__device__ __forceinline__ void qt_widen_e4m3(uint32_t lo, uint32_t hi, float (&v)[8]) {
+    typedef float f2 __attribute__((ext_vector_type(2)));
+    const f2 a = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, false), b = __builtin_amdgcn_cvt_pk_f32_fp8((int)lo, true);
+    const f2 c = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, false), d = __builtin_amdgcn_cvt_pk_f32_fp8((int)hi, true);
+    v[0] = a[0]; v[1] = a[1]; v[2] = b[0]; v[3] = b[1]; v[4] = c[0]; v[5] = c[1]; v[6] = d[0]; v[7] = d[1];
+}
+__device__ __forceinline__ uint2 qt_codes_e4m3(const float (&v)[8]) {
+    int lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[0], v[1], 0, false), hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[4], v[5], 0, false);
+    lo = __builtin_amdgcn_cvt_pk_fp8_f32(v[2], v[3], lo, true);
+    hi = __builtin_amdgcn_cvt_pk_fp8_f32(v[6], v[7], hi, true);
+    return make_uint2((unsigned)lo, (unsigned)hi);
+}
+// The byte of a row whose largest magnitude has the bits m: 2^e is enough for 448 2^e = 1.75 2^(e + 8) where e is m's exponent
+// less 8, and one more past a fraction of 1.75, which then carries.  Magnitudes of 2^127 and more, infinities and NaN, whose bits
+// order after them: 255.
+#define QT_SCALE_MIN 63u        // 2^-64
+#define QT_SCALE_MAX 246u       // of 448 2^119, the largest code under 2^127
+__device__ __forceinline__ uint32_t qt_scale_byte(uint32_t m) {
+    if (m >= 0x7F000000u) return 255u;
+    const uint32_t e = (m + 0x1FFFFFu) >> 23;
+    return e < QT_SCALE_MIN + 8u ? QT_SCALE_MIN : e - 8u;
+}
+// a byte as its row is read: 0 past the largest that is written (a NaN row)
+__device__ __forceinline__ uint32_t qt_scale_read(uint32_t byte) { return byte > QT_SCALE_MAX ? 0u : max(byte, QT_SCALE_MIN); }
+__device__ __forceinline__ float qt_scale_of(uint32_t byte) {
+    return byte > QT_SCALE_MAX ? __uint_as_float(0x7FC00000u) : __uint_as_float(max(byte, QT_SCALE_MIN) << 23);
+}
+
 template <typename T> __device__ __forceinline__ float qt_load1(const void *p) {
     if constexpr (sizeof(typename T::elem) == 4) return *reinterpret_cast<const float *>(p);
+    else if constexpr (sizeof(typename T::elem) == 1) return __builtin_amdgcn_cvt_f32_fp8(*reinterpret_cast<const uint8_t *>(p), 0);
     else return qt_lo<T>(*reinterpret_cast<const uint16_t *>(p));
 }
 template <typename T> __device__ __forceinline__ void qt_store1(void *p, float v) {
@@ -164,24 +196,33 @@ static inline bool qt_rows_meet(const void *a, long long as, long long aw, const
 }
 static inline bool qt_off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
 
+// bytes of a cache's element
+static inline int qt_kv_size(int dt) { return dt == QWEN_HIP_DT_E4M3 ? 1 : 2; }
+
 // the cache's descriptor; `who` names the call
 static inline int qt_check_pages(const char *who, const qwen_hip_kv_pages_t *kv) {
     QT_REFUSE(!kv, "%s: null cache descriptor", who);
     QT_REFUSE(!kv->k || !kv->v, "%s: null cache pointer", who);
-    QT_REFUSE(kv->dtype != QWEN_HIP_DT_BF16 && kv->dtype != QWEN_HIP_DT_F16, "%s: cache dtype %d (bf16 or f16)", who, kv->dtype);
+    const bool codes = kv->dtype == QWEN_HIP_DT_E4M3;
+    QT_REFUSE(kv->dtype != QWEN_HIP_DT_BF16 && kv->dtype != QWEN_HIP_DT_F16 && !codes, "%s: cache dtype %d (bf16, f16 or e4m3)", who, kv->dtype);
     QT_REFUSE(kv->head_dim != 64 && kv->head_dim != 128, "%s: head_dim %d (64 or 128)", who, kv->head_dim);
     QT_REFUSE(kv->n_kv_heads < 1 || kv->n_kv_heads > 65535, "%s: n_kv_heads %d out of range (1..65535)", who, kv->n_kv_heads);
     QT_REFUSE(kv->n_pages < 1 || kv->page_size < 1 || (long long)kv->n_pages * kv->page_size > 0x7FFFFFFFll,
               "%s: %d pages of %d (both at least 1, 2^31 - 1 slots at most)", who, kv->n_pages, kv->page_size);
     QT_REFUSE(qt_off16(kv->k) || qt_off16(kv->v), "%s: cache pointers have to be aligned to 16 bytes", who);
-    QT_REFUSE(kv->page_stride % 8 || kv->head_stride % 8 || kv->slot_stride % 8 || kv->page_stride < 0 || kv->head_stride < 0 ||
+    const int A = 16 / qt_kv_size(kv->dtype);
+    QT_REFUSE(kv->page_stride % A || kv->head_stride % A || kv->slot_stride % A || kv->page_stride < 0 || kv->head_stride < 0 ||
                   kv->slot_stride < 0,
-              "%s: cache strides %lld, %lld, %lld (multiples of 8 elements, not negative)", who, kv->page_stride,
-              kv->head_stride, kv->slot_stride);
+              "%s: cache strides %lld, %lld, %lld (multiples of %d elements, not negative)", who, kv->page_stride,
+              kv->head_stride, kv->slot_stride, A);
     QT_REFUSE((kv->n_pages > 1 && kv->page_stride < kv->head_dim) || (kv->n_kv_heads > 1 && kv->head_stride < kv->head_dim) ||
                   (kv->page_size > 1 && kv->slot_stride < kv->head_dim),
               "%s: cache strides %lld, %lld, %lld under head_dim %d: rows would overlap", who, kv->page_stride, kv->head_stride,
               kv->slot_stride, kv->head_dim);
+    if (!codes) return 0;
+    QT_REFUSE(!kv->k_scale || !kv->v_scale, "%s: null scale pointer", who);
+    QT_REFUSE(kv->scale_page_stride < 0 || kv->scale_head_stride < 0 || kv->scale_slot_stride < 0,
+              "%s: scale strides %lld, %lld, %lld are negative", who, kv->scale_page_stride, kv->scale_head_stride, kv->scale_slot_stride);
     return 0;
 }
 
@@ -195,22 +236,47 @@ static inline bool qt_dims_meet(const QtDim *d, int n, __int128 left, int row) {
     return (c < d[n - 1].count && -c < d[n - 1].count && qt_dims_meet(d, n - 1, left - c * s, row)) ||
            (c + 1 < d[n - 1].count && -(c + 1) < d[n - 1].count && qt_dims_meet(d, n - 1, left - (c + 1) * s, row));
 }
-static inline int qt_check_pages_apart(const char *who, const qwen_hip_kv_pages_t *kv) {
-    QtDim all[3] = {{kv->page_stride, kv->n_pages}, {kv->head_stride, kv->n_kv_heads}, {kv->slot_stride, kv->page_size}}, d[3];
+// rows of `row` units (at k, and `between` units further at v); the strides in units
+static inline int qt_check_rows_apart(const char *who, const char *what, const qwen_hip_kv_pages_t *kv, long long page, long long head, long long slot,
+                                      int row, __int128 between, int layers, long long layer) {
+    QtDim all[4] = {{page, kv->n_pages}, {head, kv->n_kv_heads}, {slot, kv->page_size}, {layer, layers}}, d[4];
     int n = 0;
-    __int128 extent = kv->head_dim;
-    for (int i = 0; i < 3; i++) {
+    __int128 extent = row;
+    for (int i = 0; i < 4; i++) {
         if (all[i].count == 1) continue;
         int at = n++;
         for (; at > 0 && d[at - 1].stride > all[i].stride; at--) d[at] = d[at - 1];
         d[at] = all[i];
     }
     for (int i = 0; i < n; i++) {
-        QT_REFUSE(d[i].stride < extent, "%s: cache strides %lld, %lld, %lld: rows of different places overlap", who, kv->page_stride,
-                  kv->head_stride, kv->slot_stride);
+        QT_REFUSE(d[i].stride < extent, "%s: %s strides %lld, %lld, %lld: rows of different places%s overlap", who, what, page, head, slot, layers > 1 ? " or layers" : "");
         extent += (d[i].count - 1) * d[i].stride;
     }
-    const intptr_t bytes = (intptr_t)kv->v - (intptr_t)kv->k;        // both aligned to 16
-    QT_REFUSE(qt_dims_meet(d, n, bytes / 2, kv->head_dim), "%s: rows of k and v overlap", who);
+    QT_REFUSE(qt_dims_meet(d, n, between, row), "%s: %s: rows of k and v overlap", who, what);
+    return 0;
+}
+static inline int qt_check_pages_apart(const char *who, const qwen_hip_kv_pages_t *kv, int layers = 1, long long layer = 0, long long scale_layer = 0) {
+    const int E = qt_kv_size(kv->dtype);
+    if (qt_check_rows_apart(who, "cache", kv, kv->page_stride, kv->head_stride, kv->slot_stride, kv->head_dim,
+                            ((intptr_t)kv->v - (intptr_t)kv->k) / E, layers, layer))     // both aligned to 16
+        return -1;
+    if (kv->dtype != QWEN_HIP_DT_E4M3) return 0;
+    if (qt_check_rows_apart(who, "scale", kv, kv->scale_page_stride, kv->scale_head_stride, kv->scale_slot_stride, 1,
+                            (__int128)((intptr_t)kv->v_scale - (intptr_t)kv->k_scale), layers, scale_layer))
+        return -1;
+    // a page's codes and a page's scales (of one layer), each as one stretch
+    const __int128 cw = (__int128)(kv->n_kv_heads - 1) * kv->head_stride + (__int128)(kv->page_size - 1) * kv->slot_stride + kv->head_dim;
+    const __int128 sw = (__int128)(kv->n_kv_heads - 1) * kv->scale_head_stride + (__int128)(kv->page_size - 1) * kv->scale_slot_stride + 1;
+    const __int128 st = kv->n_pages > 1 ? kv->page_stride : 1, n = kv->n_pages, sp = kv->scale_page_stride;
+    for (const void *c : {kv->k, kv->v})
+        for (const uint8_t *s : {kv->k_scale, kv->v_scale}) {
+            const __int128 D = (intptr_t)s - (intptr_t)c;
+            if (D >= (n - 1) * st + cw || -D >= (n - 1) * sp + sw) continue;
+            // of one stride: the scales of page j meet the codes of page i + j where D - i st lies between -sw and cw: the first
+            // such i past the lower end of codes decides; of two strides: their ranges do
+            __int128 i = (D - cw) / st - ((D - cw) % st < 0) + 1;
+            if (i < 1 - n) i = 1 - n;
+            QT_REFUSE((n > 1 && sp != st) || (i < n && i * st - D < sw), "%s: scales lie among the codes of a page", who);
+        }
     return 0;
 }

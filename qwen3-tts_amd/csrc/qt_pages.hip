@@ -243,10 +243,14 @@ extern "C" int qwen_hip_op_page_plan(const qwen_hip_page_plan_t *p, void *stream
 // other half are lane exchanges.  A workgroup takes one token: its lanes' angles and gains are loaded once
 // and serve every head.  Bound by the rows' bytes for prompts (8190 tokens bf16, 16 query and 8 kv heads of 128: 33 us, 4.2 TB/s,
 // the copy rate being 4.9), by the launch and the latency of slot, angles and rows for a step (32 tokens f32: 6.4 us).
+//
+// Into a quantised cache a row's lanes also exchange its largest magnitude, as bits, whose order is that of the magnitudes with
+// infinities and NaN last; it gives the scale's exponent by one addition (qt_scale_byte), the division by the scale is an exact product, and
+// the conversion rounds once.
 struct AppendArgs {
     const uint8_t *q, *k, *v;
-    uint8_t *qo, *kc, *vc;
-    long long qs, ks, vs, os, ps_page, ps_head, ps_slot;
+    uint8_t *qo, *kc, *vc, *ksc, *vsc;
+    long long qs, ks, vs, os, ps_page, ps_head, ps_slot, ss_page, ss_head, ss_slot;
     const float *qn, *kn, *rc, *rs;
     const int *pos, *slot;
     int T, nh, nkv, rope_len, n_slots, page;
@@ -256,7 +260,7 @@ struct AppendArgs {
 
 template <typename QT, typename KT, int HD>
 __global__ __launch_bounds__(256) void k_page_append(AppendArgs a) {
-    constexpr int E = sizeof(typename QT::elem), L = HD / 8;       // lanes a row
+    constexpr int E = sizeof(typename QT::elem), EK = sizeof(typename KT::elem), L = HD / 8;       // L: lanes a row
     const int t = blockIdx.x, slot = a.slot[t];
     if ((unsigned)slot >= (unsigned)a.n_slots) return;
     const int pos = a.rc ? a.pos[t] : 0;
@@ -272,6 +276,7 @@ __global__ __launch_bounds__(256) void k_page_append(AppendArgs a) {
     if (a.kn) qt_load8<QtF32>(a.kn + 8 * l, gk);
     const int page = qt_quot(slot, a.div);
     const long long dst = page * a.ps_page + (slot - page * a.page) * a.ps_slot + 8 * l;
+    const long long sdst = EK == 1 ? page * a.ss_page + (slot - page * a.page) * a.ss_slot : 0;
     const int nq = a.q ? a.nh : 0;
     for (int r = grp; r < nq + 2 * a.nkv; r += 256 / L) {
         const bool isq = r < nq, isv = r >= nq + a.nkv;
@@ -299,7 +304,20 @@ __global__ __launch_bounds__(256) void k_page_append(AppendArgs a) {
             }
         }
         if (isq) qt_store8<QT>(a.qo + ((size_t)(t * a.os) + (size_t)h * HD + 8 * l) * E, x);
-        else qt_store8<KT>((isv ? a.vc : a.kc) + (dst + h * a.ps_head) * 2, x);
+        else if constexpr (EK == 1) {
+            uint32_t m = 0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) m = max(m, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+#pragma unroll
+            for (int o = 1; o < L; o <<= 1) m = max(m, (uint32_t)__shfl_xor((int)m, o, L));
+            const uint32_t byte = qt_scale_byte(m);
+            const float inv = __uint_as_float((254u - byte) << 23);             // of a NaN row: not used
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] *= inv;
+            const uint2 c = byte == 255u ? make_uint2(0x7F7F7F7Fu, 0x7F7F7F7Fu) : qt_codes_e4m3(x);
+            *reinterpret_cast<uint2 *>((isv ? a.vc : a.kc) + dst + h * a.ps_head) = c;
+            if (l == 0) (isv ? a.vsc : a.ksc)[sdst + h * a.ss_head] = (uint8_t)byte;
+        } else qt_store8<KT>((isv ? a.vc : a.kc) + (dst + h * a.ps_head) * EK, x);
     }
 }
 
@@ -307,7 +325,8 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
     if (qt_check_pages("page_append", kv)) return -1;
     QT_REFUSE(!p, "page_append: null descriptor");
     const int E = qt_dt_size(p->dtype);
-    QT_REFUSE(!E || (p->dtype != QWEN_HIP_DT_F32 && p->dtype != kv->dtype),
+    const bool codes = kv->dtype == QWEN_HIP_DT_E4M3;
+    QT_REFUSE(!E || (p->dtype != QWEN_HIP_DT_F32 && p->dtype != kv->dtype && !codes),
               "page_append: rows of dtype %d into a cache of dtype %d (f32, or the cache's own)", p->dtype, kv->dtype);
     QT_REFUSE(p->T < 0 || p->T >= 1 << 24, "page_append: T %d out of range (0..2^24 - 1)", p->T);
     if (p->T == 0) return 0;
@@ -338,12 +357,16 @@ extern "C" int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "page_append: the stream's device: %s", hipGetErrorString(on.err));
     const AppendArgs a = {(const uint8_t *)p->q, (const uint8_t *)p->k, (const uint8_t *)p->v, (uint8_t *)p->q_out,
-                          (uint8_t *)kv->k, (uint8_t *)kv->v, p->q_stride, p->k_stride, p->v_stride, p->q_out_stride,
-                          kv->page_stride, kv->head_stride, kv->slot_stride, p->q_norm, p->k_norm, p->rope_cos, p->rope_sin,
+                          (uint8_t *)kv->k, (uint8_t *)kv->v, codes ? kv->k_scale : nullptr, codes ? kv->v_scale : nullptr,
+                          p->q_stride, p->k_stride, p->v_stride, p->q_out_stride, kv->page_stride, kv->head_stride, kv->slot_stride,
+                          codes ? kv->scale_page_stride : 0, codes ? kv->scale_head_stride : 0, codes ? kv->scale_slot_stride : 0, p->q_norm, p->k_norm, p->rope_cos, p->rope_sin,
                           p->pos, p->slot, p->T, p->n_heads, kv->n_kv_heads, p->rope_len, kv->n_pages * kv->page_size,
                           kv->page_size, p->eps, qt_div_of(kv->page_size)};
 #define APPEND(QT, KT) (kv->head_dim == 128 ? k_page_append<QT, KT, 128> : k_page_append<QT, KT, 64>)
-    void (*const kernel)(AppendArgs) = p->dtype == QWEN_HIP_DT_BF16    ? APPEND(QtBf16, QtBf16)
+    void (*const kernel)(AppendArgs) = codes && p->dtype == QWEN_HIP_DT_F32    ? APPEND(QtF32, QtE4m3)
+                                       : codes && p->dtype == QWEN_HIP_DT_BF16 ? APPEND(QtBf16, QtE4m3)
+                                       : codes                                 ? APPEND(QtF16, QtE4m3)
+                                       : p->dtype == QWEN_HIP_DT_BF16    ? APPEND(QtBf16, QtBf16)
                                        : p->dtype == QWEN_HIP_DT_F16   ? APPEND(QtF16, QtF16)
                                        : kv->dtype == QWEN_HIP_DT_BF16 ? APPEND(QtF32, QtBf16)
                                                                        : APPEND(QtF32, QtF16);

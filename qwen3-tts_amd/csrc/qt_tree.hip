@@ -1,0 +1,640 @@
+// qt_tree.hip — trees of drafted tokens: a step's positions and masks (qwen_hip_op_tree_plan), verification against the
+// target's probabilities (qwen_hip_op_tree_verify), and what is kept of the step (qwen_hip_op_tree_commit).
+#include "qt_ops.h"
+
+#define TREE_MAX_LEN (1 << 30)
+
+// A request's tokens: offsets are the caller's, one out of range is brought into it.
+struct TreeReq { int q0, n; };
+__device__ __forceinline__ TreeReq tree_req(const int *cu, int b, int T) {
+    const int q0 = min(max(cu[b], 0), T);
+    return {q0, max(min(max(cu[b + 1], 0), T) - q0, 0)};
+}
+
+// ---- positions and masks ---------------------------------------------------------------------------
+// A workgroup a request.  A token walks up through its parents, held in LDS: they have smaller indices, so the words of its mask
+// come from the highest down and each is stored once.  Bound by the launch: 8 requests of up to 16 tokens, 512 of up to 61.
+struct TreePlanArgs {
+    const int *parent, *cu, *kv;
+    int *pos;
+    uint32_t *mask;
+    long long ms;
+    int T, words;
+};
+
+__global__ __launch_bounds__(256) void k_tree_plan(TreePlanArgs a) {
+    __shared__ int up[1024];
+    const int b = blockIdx.x, nt = blockDim.x;
+    const TreeReq r = tree_req(a.cu, b, a.T);
+    const int first = min(max(a.kv[b], 0), TREE_MAX_LEN) - r.n;
+    if (r.n > 32 * a.words) {
+        for (int i = threadIdx.x; i < r.n; i += nt) a.pos[r.q0 + i] = first + i;
+        return;
+    }
+    for (int i = threadIdx.x; i < r.n; i += nt) {
+        const int p = a.parent[r.q0 + i];
+        up[i] = p >= 0 && p < i ? p : -1;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < r.n; i += nt) {
+        uint32_t *m = a.mask + (r.q0 + i) * a.ms;
+        int w = i >> 5, depth = 0;
+        for (int z = a.words - 1; z > w; z--) m[z] = 0u;
+        uint32_t bits = 1u << (i & 31);
+        for (int j = up[i]; j >= 0; j = up[j]) {
+            depth++;
+            for (; w > j >> 5; w--) { m[w] = bits; bits = 0u; }
+            bits |= 1u << (j & 31);
+        }
+        for (; w >= 0; w--) { m[w] = bits; bits = 0u; }
+        a.pos[r.q0 + i] = first + depth;
+    }
+}
+
+extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream) {
+    QT_REFUSE(!p, "tree_plan: null descriptor");
+    QT_REFUSE(p->B < 0 || p->B > 65535, "tree_plan: B %d out of range (0..65535)", p->B);
+    QT_REFUSE(p->T < 0 || p->T > 1 << 26, "tree_plan: T %d out of range (0..2^26)", p->T);
+    QT_REFUSE(p->mask_words < 1 || p->mask_words > 32 || p->mask_stride < p->mask_words,
+              "tree_plan: mask_words %d of stride %lld (1..32, the stride at least as many)", p->mask_words, p->mask_stride);
+    if (p->B == 0 || p->T == 0) return 0;
+    QT_REFUSE(!p->parent || !p->cu_q || !p->kv_len || !p->pos || !p->mask, "tree_plan: null pointer");
+    const hipStream_t st = qt_stream(stream);
+    QtOnDevice on(st);
+    QT_REFUSE(on.err != hipSuccess, "tree_plan: the stream's device: %s", hipGetErrorString(on.err));
+    const TreePlanArgs a = {p->parent, p->cu_q, p->kv_len, p->pos, p->mask, p->mask_stride, p->T, p->mask_words};
+    const hipError_t e = qt_launch(k_tree_plan, dim3(p->B), dim3(p->mask_words > 4 ? 256 : p->mask_words > 2 ? 128 : 64), 0, st, a);
+    QT_REFUSE(e != hipSuccess, "tree_plan: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+// ---- verification ----------------------------------------------------------------------------------
+// From the current token, w = p's row and z = 1; child c of token x is kept where u q(x) z < w(x), else w <- max(w / z - q, 0),
+// z <- sum w.  After rejections w is max(A p - B q, 0) with two numbers: A, B -> A / z, B / z + 1 (a token whose w
+// has become 0 stays at 0).  So the walk needs each token's p and q at its parent's row, gathered once for 64 tokens, and a pass over the
+// vocabulary only where a sum is asked for: by a further child after a rejection, and by the next token at the end.
+// The pass sums tiles of 4096 entries; the next token's tile is found in the tiles' sums, the token by a scan of its tile.
+// All in f64: an f32 sum over a vocabulary would move the border between two tokens by more than some tokens have.
+//
+// Large vocabularies: a first launch walks to the first sum (every workgroup for itself: a few dependent loads) and sums a tile a
+// workgroup, a second one, a workgroup a request, goes on from there; sums that it finds it needs beyond the first it makes itself.
+#define VF_T 256
+#define VF_TILE 4096
+#define VF_ONE 1                    // vocabularies of so many tiles take one launch
+
+struct VerifyState { double A, B, z; int cur, last, kept, ask; };      // ask: z is the sum that is to be made
+struct VerifyArgs {
+    const uint8_t *p, *q;
+    long long ps, qs;
+    const int *tok, *parent, *cu;
+    const float *u, *r;
+    int *path, *out, *n_path;
+    VerifyState *state;             // [B]
+    double *sums;                   // [B][tiles]
+    int T, V, tiles, second;
+};
+
+template <typename TY> __device__ __forceinline__ double vf_at(const uint8_t *row, long long i) {
+    const float x = qt_load1<TY>(row + i * (long long)sizeof(typename TY::elem));
+    return x > 0.f ? (double)x : 0.0;
+}
+
+// A wave: goes on from s to the next sum that is asked for (s.ask = 1) or to the last kept token (0).  `put`: writes what is kept.
+template <typename TY, bool DRAFT>
+__device__ __forceinline__ void vf_walk(const VerifyArgs &a, TreeReq r, VerifyState &s, bool put) {
+    constexpr int E = sizeof(typename TY::elem);
+    const int lane = threadIdx.x & 63;
+    for (int base = (s.last + 1) & ~63; base < r.n; base += 64) {
+        const int i = base + lane;
+        const bool real = i < r.n && i > s.last;
+        int up = -2, x = -1;
+        float u = 0.f;
+        double px = 0.0, qx = 1.0;
+        if (real) {
+            up = a.parent[r.q0 + i];
+            x = a.tok[r.q0 + i];
+            u = a.u[r.q0 + i];
+            if (up < 0 || up >= i || x < 0 || x >= a.V) up = -2;       // no one's child
+            else {
+                px = vf_at<TY>(a.p + (r.q0 + up) * a.ps * E, x);
+                if (DRAFT) qx = vf_at<TY>(a.q + (r.q0 + up) * a.qs * E, x);
+            }
+        }
+        for (;;) {
+            const unsigned long long kids = __ballot(up == s.cur && i > s.last);
+            if (!kids) break;
+            const int c = __ffsll(kids) - 1, id = base + c, cx = __builtin_amdgcn_readlane(x, c);
+            if (s.ask) return;                                          // (after a rejection, and only if another child comes)
+            const double cp = __shfl(px, c), cq = __shfl(qx, c);
+            const float cu = lane_bcast(u, c);
+            double w;
+            if (DRAFT) {
+                w = fmax(s.A * cp - s.B * cq, 0.0);
+            } else {                                                    // 0 where a sibling before it had the same token
+                w = cp;
+                bool again = __ballot(up == s.cur && i < id && x == cx) != 0;
+                for (int j = s.cur + 1 + lane; j < base; j += 64)
+                    again |= __ballot(a.parent[r.q0 + j] == s.cur && a.tok[r.q0 + j] == cx) != 0;
+                if (__ballot(again)) w = 0.0;
+            }
+            if (cu < 0.f || (double)cu * cq * s.z < w) {
+                if (put && lane == 0) {
+                    a.out[r.q0 + s.kept - 1] = cx;
+                    a.path[r.q0 + s.kept] = id;
+                }
+                s.kept++;
+                s.cur = id;
+                s.A = 1.0; s.B = 0.0; s.z = 1.0;
+            } else if (!DRAFT) {
+                s.z = fmax(s.z - w, 0.0);
+                s.B = 1.0;                                              // some siblings' tokens are out
+            } else if (s.z > 0.0) {
+                s.A /= s.z;
+                s.B = s.B / s.z + 1.0;
+                s.ask = 1;
+            }
+            s.last = id;
+        }
+        if (base + 63 > s.last) s.last = min(base + 63, r.n - 1);
+    }
+    s.ask = 0;
+}
+
+// w of 8 entries from v on: max(A p - B q, 0), or p where no rejected sibling has that token (`out`: bits of a tile's tokens)
+template <typename TY, bool DRAFT>
+__device__ __forceinline__ void vf_eight(const VerifyArgs &a, const uint8_t *p, const uint8_t *q, const VerifyState &s, const uint32_t *out, int at, int v,
+                                         double (&w)[8]) {
+    constexpr int E = sizeof(typename TY::elem);
+    float x[8], y[8];
+    const bool whole = v + 8 <= a.V;
+    if (whole) {
+        qt_load8<TY, E>(p + (long long)v * E, x);
+        if (DRAFT) qt_load8<TY, E>(q + (long long)v * E, y);
+    } else {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            x[e] = v + e < a.V ? qt_load1<TY>(p + (long long)(v + e) * E) : 0.f;
+            if (DRAFT) y[e] = v + e < a.V ? qt_load1<TY>(q + (long long)(v + e) * E) : 0.f;
+        }
+    }
+    uint32_t gone = 0;
+    if (!DRAFT && out) gone = out[at >> 5] >> (at & 31) & 0xFFu;       // at: a multiple of 8
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const double px = x[e] > 0.f ? (double)x[e] : 0.0;
+        if (DRAFT) w[e] = fmax(s.A * px - s.B * (y[e] > 0.f ? (double)y[e] : 0.0), 0.0);
+        else w[e] = gone >> e & 1u ? 0.0 : px;
+    }
+}
+
+__device__ __forceinline__ double vf_wave_sum(double v) {
+#pragma unroll
+    for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
+    return v;
+}
+__device__ __forceinline__ double vf_wave_scan(double v) {
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double y = __shfl_up(v, o, 64);
+        if (lane >= o) v += y;
+    }
+    return v;
+}
+
+// The workgroup: marks a tile's tokens that rejected siblings have (certain drafts only).
+template <bool DRAFT>
+__device__ __forceinline__ const uint32_t *vf_marks(const VerifyArgs &a, TreeReq r, const VerifyState &s, int tile, uint32_t *bits) {
+    if (DRAFT || s.B == 0.0) return nullptr;
+    __syncthreads();
+    for (int i = threadIdx.x; i < VF_TILE / 32; i += VF_T) bits[i] = 0u;
+    __syncthreads();
+    for (int i = s.cur + 1 + threadIdx.x; i < r.n; i += VF_T)
+        if (a.parent[r.q0 + i] == s.cur) {
+            const int t = a.tok[r.q0 + i] - tile * VF_TILE;
+            if (a.tok[r.q0 + i] >= 0 && t >= 0 && t < VF_TILE) atomicOr(&bits[t >> 5], 1u << (t & 31));
+        }
+    __syncthreads();
+    return bits;
+}
+
+// The workgroup: a tile's sum, in every thread.
+template <typename TY, bool DRAFT>
+__device__ __forceinline__ double vf_tile(const VerifyArgs &a, TreeReq r, const VerifyState &s, int tile, uint32_t *bits, double *part) {
+    constexpr int E = sizeof(typename TY::elem);
+    const uint8_t *p = a.p + (r.q0 + s.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + s.cur) * a.qs * E : nullptr;
+    const uint32_t *out = vf_marks<DRAFT>(a, r, s, tile, bits);
+    double sum = 0.0;
+#pragma unroll
+    for (int k = 0; k < VF_TILE / (8 * VF_T); k++) {
+        const int at = 8 * (k * VF_T + (int)threadIdx.x);
+        double w[8];
+        if (tile * VF_TILE + at < a.V) {
+            vf_eight<TY, DRAFT>(a, p, q, s, out, at, tile * VF_TILE + at, w);
+            sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        }
+    }
+    sum = vf_wave_sum(sum);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
+    __syncthreads();
+    sum = 0.0;
+#pragma unroll
+    for (int w = 0; w < VF_T / 64; w++) sum += part[w];
+    return sum;
+}
+
+template <typename TY, bool DRAFT>
+__global__ __launch_bounds__(VF_T) void k_tree_sums(VerifyArgs a) {
+    __shared__ VerifyState s;
+    __shared__ uint32_t bits[VF_TILE / 32];
+    __shared__ double part[VF_T / 64];
+    const int b = blockIdx.y, tile = blockIdx.x;
+    const TreeReq r = tree_req(a.cu, b, a.T);
+    if (r.n == 0) return;
+    if (threadIdx.x < 64) {
+        VerifyState w = {1.0, 0.0, 1.0, 0, 0, 1, 0};
+        vf_walk<TY, DRAFT>(a, r, w, tile == 0);
+        if (threadIdx.x == 0) {
+            s = w;
+            if (tile == 0) a.state[b] = w;
+        }
+    }
+    __syncthreads();
+    const double sum = vf_tile<TY, DRAFT>(a, r, s, tile, bits, part);
+    if (threadIdx.x == 0) a.sums[(long long)b * a.tiles + tile] = sum;
+}
+
+template <typename TY, bool DRAFT>
+__global__ __launch_bounds__(VF_T) void k_tree_pick(VerifyArgs a) {
+    constexpr int E = sizeof(typename TY::elem);
+    __shared__ VerifyState s;
+    __shared__ uint32_t bits[VF_TILE / 32];
+    __shared__ double part[VF_T / 64], total_s, before_s;
+    __shared__ int tile_s, token_s;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const TreeReq r = tree_req(a.cu, b, a.T);
+    if (r.n == 0) {
+        if (threadIdx.x == 0) a.n_path[b] = 0;
+        return;
+    }
+    double *sums = a.sums + (long long)b * a.tiles;
+    bool made = a.second != 0;                          // the tiles' sums are those of s
+    if (threadIdx.x < 64) {
+        VerifyState w = {1.0, 0.0, 1.0, 0, 0, 1, 0};
+        if (made) w = a.state[b];
+        else vf_walk<TY, DRAFT>(a, r, w, true);
+        if (threadIdx.x == 0) s = w;
+    }
+    __syncthreads();
+    const auto total = [&] {                            // the tiles' sum, in their order within a lane's share
+        if (threadIdx.x < 64) {
+            const int per = (a.tiles + 63) / 64, t1 = min((lane + 1) * per, a.tiles);
+            double x = 0.0;
+            for (int t = lane * per; t < t1; t++) x += sums[t];
+            x = vf_wave_sum(x);
+            if (lane == 0) total_s = x;
+        }
+        __syncthreads();
+    };
+    const auto make = [&] {
+        for (int t = 0; t < a.tiles; t++) {
+            const double x = vf_tile<TY, DRAFT>(a, r, s, t, bits, part);
+            if (threadIdx.x == 0) sums[t] = x;
+        }
+        __syncthreads();
+    };
+    for (;;) {                                          // at most one round for each of the request's tokens
+        if (!made) make();
+        total();
+        if (!s.ask) break;
+        __syncthreads();
+        if (threadIdx.x < 64) {
+            VerifyState w = s;
+            w.z = total_s;
+            w.ask = 0;
+            vf_walk<TY, DRAFT>(a, r, w, true);
+            if (threadIdx.x == 0) {
+                part[0] = w.A != s.A || w.B != s.B || w.cur != s.cur ? 1.0 : 0.0;
+                s = w;
+            }
+        }
+        __syncthreads();
+        made = part[0] == 0.0;
+        __syncthreads();
+    }
+    if (!(total_s > 0.0)) {                             // nothing is left: p's row as it is
+        __syncthreads();
+        if (threadIdx.x == 0) { s.A = 1.0; s.B = 0.0; }
+        __syncthreads();
+        make();
+        total();
+    }
+    const double goal = (double)a.r[b] * total_s;
+    if (threadIdx.x == 0) {
+        double x = 0.0;
+        int t = 0, last = -1;
+        double last_before = 0.0;
+        for (; t < a.tiles; t++) {
+            const double y = sums[t];
+            if (y > 0.0) { last = t; last_before = x; }
+            if (x + y > goal) break;
+            x += y;
+        }
+        tile_s = t < a.tiles ? t : last;                // (sums that rounding leaves just under the goal)
+        before_s = t < a.tiles ? x : last_before;
+        token_s = -1;
+    }
+    __syncthreads();
+    if (tile_s >= 0) {
+        const int tile = tile_s;
+        const uint8_t *p = a.p + (r.q0 + s.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + s.cur) * a.qs * E : nullptr;
+        const uint32_t *out = vf_marks<DRAFT>(a, r, s, tile, bits);
+        double before = before_s;
+        int found = 0x7FFFFFFF, any = -1;               // the first entry past the goal, and the last one that is not 0
+        for (int k = 0; k < VF_TILE / (8 * VF_T); k++) {
+            const int at = 8 * (k * VF_T + (int)threadIdx.x), v = tile * VF_TILE + at;
+            double w[8], mine = 0.0;
+            if (v < a.V) {
+                vf_eight<TY, DRAFT>(a, p, q, s, out, at, v, w);
+#pragma unroll
+                for (int e = 0; e < 8; e++) mine += w[e];
+            }
+            const double upto = vf_wave_scan(mine);
+            __syncthreads();
+            if (lane == 63) part[wave] = upto;
+            __syncthreads();
+            double x = before;
+#pragma unroll
+            for (int o = 0; o < VF_T / 64; o++) {
+                if (o < wave) x += part[o];
+                before += part[o];
+            }
+            const double lower = __shfl_up(upto, 1, 64);
+            if (lane > 0) x += lower;
+            if (v < a.V)
+#pragma unroll
+                for (int e = 0; e < 8; e++) {
+                    x += w[e];
+                    if (w[e] > 0.0) any = v + e;
+                    if (w[e] > 0.0 && x > goal) found = min(found, v + e);
+                }
+        }
+        // over the workgroup: the least `found`, else the greatest `any`
+#pragma unroll
+        for (int o = 32; o; o >>= 1) { found = min(found, __shfl_xor(found, o, 64)); any = max(any, __shfl_xor(any, o, 64)); }
+        __shared__ int ends[2][VF_T / 64];
+        if (lane == 0) { ends[0][wave] = found; ends[1][wave] = any; }
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            for (int o = 1; o < VF_T / 64; o++) { found = min(found, ends[0][o]); any = max(any, ends[1][o]); }
+            token_s = found != 0x7FFFFFFF ? found : any;
+        }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        a.path[r.q0] = 0;
+        a.out[r.q0 + s.kept - 1] = token_s;
+        a.n_path[b] = s.kept;
+    }
+    for (int k = s.kept + threadIdx.x; k < r.n; k += VF_T) a.path[r.q0 + k] = a.out[r.q0 + k] = -1;
+}
+
+static int verify_args(const qwen_hip_tree_verify_t *p, VerifyArgs &a) {
+    QT_REFUSE(!p, "tree_verify: null descriptor");
+    QT_REFUSE(!qt_dt_size(p->dtype), "tree_verify: dtype %d (f32, bf16 or f16)", p->dtype);
+    QT_REFUSE(p->B < 0 || p->B > 65535, "tree_verify: B %d out of range (0..65535)", p->B);
+    QT_REFUSE(p->T < 0 || p->T > 1 << 26, "tree_verify: T %d out of range (0..2^26)", p->T);
+    QT_REFUSE(p->V < 1 || p->V > 1 << 24, "tree_verify: V %d out of range (1..2^24)", p->V);
+    QT_REFUSE(p->max_children < 0, "tree_verify: max_children %d is negative", p->max_children);
+    a = VerifyArgs{};
+    a.T = p->T; a.V = p->V;
+    a.tiles = (p->V + VF_TILE - 1) / VF_TILE;
+    return 0;
+}
+static long long verify_bytes(const VerifyArgs &a, int B) { return (long long)B * (sizeof(VerifyState) + 8ll * a.tiles); }
+
+extern "C" long long qwen_hip_op_tree_verify_workspace(const qwen_hip_tree_verify_t *p) {
+    VerifyArgs a;
+    if (verify_args(p, a)) return -1;
+    return verify_bytes(a, p->B);
+}
+
+template <typename TY, bool DRAFT> static hipError_t verify_launch(VerifyArgs a, int B, hipStream_t st) {
+    hipError_t e = hipSuccess;
+    if (a.tiles > VF_ONE) {
+        e = qt_launch(k_tree_sums<TY, DRAFT>, dim3(a.tiles, B), dim3(VF_T), 0, st, a);
+        a.second = 1;
+    }
+    if (e == hipSuccess) e = qt_launch(k_tree_pick<TY, DRAFT>, dim3(B), dim3(VF_T), 0, st, a);
+    return e;
+}
+
+extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *stream) {
+    VerifyArgs a;
+    if (verify_args(p, a)) return -1;
+    if (p->B == 0) return 0;
+    QT_REFUSE(!p->cu_q || !p->n_path || !p->r || (p->T > 0 && (!p->p || !p->tok || !p->parent || !p->u || !p->path || !p->out_tok)),
+              "tree_verify: null pointer");
+    const int E = qt_dt_size(p->dtype);
+    QT_REFUSE((uintptr_t)p->p % E || (uintptr_t)p->q % E, "tree_verify: p and q have to be aligned to their elements");
+    QT_REFUSE(p->p_stride < p->V || (p->q && p->q_stride < p->V), "tree_verify: strides %lld, %lld under %d entries", p->p_stride, p->q_stride, p->V);
+    const long long need = verify_bytes(a, p->B);
+    QT_REFUSE(!p->workspace || p->workspace_bytes < need, "tree_verify: a workspace of %lld bytes is needed, %lld given", need,
+              p->workspace ? p->workspace_bytes : 0ll);
+    QT_REFUSE(qt_off16(p->workspace), "tree_verify: the workspace has to be aligned to 16 bytes");
+    const hipStream_t st = qt_stream(stream);
+    QtOnDevice on(st);
+    QT_REFUSE(on.err != hipSuccess, "tree_verify: the stream's device: %s", hipGetErrorString(on.err));
+    a.p = (const uint8_t *)p->p; a.q = (const uint8_t *)p->q;
+    a.ps = p->p_stride; a.qs = p->q_stride;
+    a.tok = p->tok; a.parent = p->parent; a.cu = p->cu_q; a.u = p->u; a.r = p->r;
+    a.path = p->path; a.out = p->out_tok; a.n_path = p->n_path;
+    a.state = (VerifyState *)p->workspace;
+    a.sums = (double *)(a.state + p->B);
+#define VERIFY(TY) (p->q ? verify_launch<TY, true>(a, p->B, st) : verify_launch<TY, false>(a, p->B, st))
+    const hipError_t e = p->dtype == QWEN_HIP_DT_F32 ? VERIFY(QtF32) : p->dtype == QWEN_HIP_DT_BF16 ? VERIFY(QtBf16) : VERIFY(QtF16);
+#undef VERIFY
+    QT_REFUSE(e != hipSuccess, "tree_verify: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}
+
+// ---- what is kept ----------------------------------------------------------------------------------
+// Row path[k] goes to place k.  Since path[k] >= k, a place that has been written is no later row's source: a thread that takes 16
+// bytes of a head's rows through all moves in the order of k, four loads before their stores, reads every source before it
+// is overwritten, and no two threads share bytes.  A workgroup takes a request's rows in one layer.  Lengths and pages: one workgroup more,
+// or a launch of its own where it replaces lengths that the moves read.
+// Bound by the latency of path, table, rows for few, by the rows' bytes for many layers.
+#define CM_T 256
+#define CM_MAX_B 2048
+struct CommitArgs {
+    const int *path, *n_path, *cu, *kv, *table, *n_free;
+    long long ts;
+    int *kv_out, *free_pages, *n_free_out, *status;
+    uint8_t *k, *v, *ks, *vs;                           // codes and strides in bytes
+    long long layer, page, head, slot, s_layer, s_page, s_head, s_slot;
+    int B, T, cols, ps, n_pages, layers, nkv, row;      // row: bytes of a head's row
+    int moves, lengths;                                 // this launch moves rows; makes lengths and pages
+    QtDiv div;
+};
+
+__device__ __forceinline__ int commit_kept(const CommitArgs &a, int b, int n) { return min(max(a.n_path[b], 0), n); }
+// whether a request's lengths are ones that a table can hold
+__device__ __forceinline__ bool commit_fits(const CommitArgs &a, int kv, int n) { return kv >= n && (long long)kv <= (long long)a.cols * a.ps; }
+__device__ __forceinline__ int commit_pages(const CommitArgs &a, int len) { return qt_quot(len, a.div) + (len % a.ps != 0); }
+
+__device__ __forceinline__ void commit_move(const CommitArgs &a, int b, int layer) {
+    __shared__ int from[CM_T], to[CM_T], moves_s[CM_T / 64];
+    const TreeReq r = tree_req(a.cu, b, a.T);
+    const int kv = a.kv[b], keep = commit_kept(a, b, r.n), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (!commit_fits(a, kv, r.n)) return;
+    const int *table = a.table + b * a.ts;
+    for (int k0 = 0; k0 < keep; k0 += CM_T) {
+        const int k = k0 + threadIdx.x;
+        int f = -1, t = -1;
+        if (k < keep) {
+            const int src = a.path[r.q0 + k];
+            if (src > k && src < r.n) {
+                const int ps = kv - r.n + src, pd = kv - r.n + k, cs = qt_quot(ps, a.div), cd = qt_quot(pd, a.div);
+                const int pgs = table[cs], pgd = table[cd];
+                if ((unsigned)pgs < (unsigned)a.n_pages && (unsigned)pgd < (unsigned)a.n_pages) {
+                    f = pgs * a.ps + ps - cs * a.ps;
+                    t = pgd * a.ps + pd - cd * a.ps;
+                }
+            }
+        }
+        const unsigned long long some = __ballot(f >= 0);
+        __syncthreads();                                // the last round's list is read
+        if (lane == 0) moves_s[wave] = __popcll(some);
+        __syncthreads();
+        int at = __popcll(some & ((1ull << lane) - 1)), n = 0;
+#pragma unroll
+        for (int w = 0; w < CM_T / 64; w++) {
+            if (w < wave) at += moves_s[w];
+            n += moves_s[w];
+        }
+        if (f >= 0) { from[at] = f; to[at] = t; }
+        __syncthreads();
+        const int chunks = a.row / 16, items = 2 * a.nkv * chunks;
+        const auto offset = [&](int slot, long long page, long long place) {
+            const int p = qt_quot(slot, a.div);
+            return p * page + (slot - p * a.ps) * place;
+        };
+        for (int i = threadIdx.x; i < items; i += CM_T) {
+            const int c = i % chunks, h = i / chunks % a.nkv;
+            uint8_t *base = (i >= items / 2 ? a.v : a.k) + layer * a.layer + h * a.head + 16 * c;
+            for (int j = 0; j < n; j += 4) {
+                qt_w4 x[4];
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (j + e < n) x[e] = qt_load16<16>(base + offset(from[j + e], a.page, a.slot));
+#pragma unroll
+                for (int e = 0; e < 4; e++)
+                    if (j + e < n) qt_store16<16>(base + offset(to[j + e], a.page, a.slot), x[e]);
+            }
+        }
+        if (a.ks)
+            for (int i = threadIdx.x; i < 2 * a.nkv; i += CM_T) {
+                uint8_t *base = (i >= a.nkv ? a.vs : a.ks) + layer * a.s_layer + (i % a.nkv) * a.s_head;
+                for (int j = 0; j < n; j++) base[offset(to[j], a.s_page, a.s_slot)] = base[offset(from[j], a.s_page, a.s_slot)];
+            }
+    }
+}
+
+__device__ __forceinline__ void commit_lengths(const CommitArgs &a) {
+    __shared__ unsigned long long wsum[CM_T / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, n_free = a.n_free[0];
+    const int per = (a.B + CM_T - 1) / CM_T, b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
+    unsigned long long mine = 0;
+    bool bad = n_free < 0 || n_free > a.n_pages;
+    for (int b = b0; b < b1; b++) {
+        const int n = tree_req(a.cu, b, a.T).n, kv = a.kv[b];
+        if (!commit_fits(a, kv, n)) bad = true;
+        else mine += commit_pages(a, kv) - commit_pages(a, kv - n + commit_kept(a, b, n));
+    }
+    bad |= mine > (unsigned long long)a.n_pages;
+    unsigned long long upto = mine;                     // 2048 requests of 2^30 pages at most
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const unsigned long long y = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += y;
+    }
+    if (lane == 63) wsum[wave] = upto;
+    bad = __syncthreads_or(bad);
+    unsigned long long before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < CM_T / 64; w++) {
+        if (w < wave) before += wsum[w];
+        all += wsum[w];
+    }
+    bad |= (unsigned long long)max(n_free, 0) + all > (unsigned long long)a.n_pages;
+    if (!bad) {
+        int at = n_free + (int)(before + upto - mine);
+        for (int b = b0; b < b1; b++) {
+            const int n = tree_req(a.cu, b, a.T).n, kv = a.kv[b], len = kv - n + commit_kept(a, b, n);
+            for (int c = commit_pages(a, len); c < commit_pages(a, kv); c++) a.free_pages[at++] = a.table[b * a.ts + c];
+            a.kv_out[b] = len;
+        }
+    } else if (a.kv_out != a.kv) {
+        for (int b = b0; b < b1; b++) a.kv_out[b] = a.kv[b];
+    }
+    if (threadIdx.x == 0) {
+        a.n_free_out[0] = bad ? n_free : n_free + (int)all;
+        a.status[0] = bad ? QWEN_HIP_PLAN_INVALID : 0;
+    }
+}
+
+__global__ __launch_bounds__(CM_T) void k_tree_commit(CommitArgs a) {
+    if (a.moves) {
+        const int b = blockIdx.x % a.B, layer = blockIdx.x / a.B;
+        if (layer < a.layers) { commit_move(a, b, layer); return; }
+    }
+    commit_lengths(a);
+}
+
+extern "C" int qwen_hip_op_tree_commit(const qwen_hip_kv_pages_t *kv, const qwen_hip_tree_commit_t *p, void *stream) {
+    if (qt_check_pages("tree_commit", kv)) return -1;
+    QT_REFUSE(!p, "tree_commit: null descriptor");
+    QT_REFUSE(p->B < 0 || p->B > CM_MAX_B, "tree_commit: B %d out of range (0..%d)", p->B, CM_MAX_B);
+    QT_REFUSE(p->T < 0 || p->T > 1 << 26, "tree_commit: T %d out of range (0..2^26)", p->T);
+    QT_REFUSE(p->n_layers < 0 || (long long)p->n_layers * p->B > 0xFFFFFFll, "tree_commit: %d layers of %d requests (2^24 - 1 at most)", p->n_layers, p->B);
+    QT_REFUSE(p->table_cols < 1 || (long long)p->table_cols * kv->page_size > TREE_MAX_LEN || p->table_stride < p->table_cols,
+              "tree_commit: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
+    if (p->B == 0) return 0;
+    QT_REFUSE(!p->n_path || !p->cu_q || !p->kv_len || !p->table || (p->T > 0 && !p->path), "tree_commit: null pointer");
+    QT_REFUSE(p->kv_len_out && (!p->free_pages || !p->n_free || !p->n_free_out || !p->status), "tree_commit: null pointer (lengths need the free list and status)");
+    const bool codes = kv->dtype == QWEN_HIP_DT_E4M3;
+    const int E = qt_kv_size(kv->dtype);
+    if (p->n_layers > 0 && qt_check_pages_apart("tree_commit", kv, p->n_layers, p->layer_stride, p->scale_layer_stride)) return -1;
+    QT_REFUSE(p->n_layers > 1 && p->layer_stride % (16 / E), "tree_commit: layer_stride %lld (a multiple of 16 bytes)", p->layer_stride);
+    const hipStream_t st = qt_stream(stream);
+    QtOnDevice on(st);
+    QT_REFUSE(on.err != hipSuccess, "tree_commit: the stream's device: %s", hipGetErrorString(on.err));
+    CommitArgs a = {};
+    a.path = p->path; a.n_path = p->n_path; a.cu = p->cu_q; a.kv = p->kv_len; a.table = p->table; a.n_free = p->n_free;
+    a.ts = p->table_stride;
+    a.kv_out = p->kv_len_out; a.free_pages = p->free_pages; a.n_free_out = p->n_free_out; a.status = p->status;
+    a.k = (uint8_t *)kv->k; a.v = (uint8_t *)kv->v;
+    a.layer = p->layer_stride * E; a.page = kv->page_stride * E; a.head = kv->head_stride * E; a.slot = kv->slot_stride * E;
+    if (codes) {
+        a.ks = kv->k_scale; a.vs = kv->v_scale;
+        a.s_layer = p->scale_layer_stride; a.s_page = kv->scale_page_stride; a.s_head = kv->scale_head_stride; a.s_slot = kv->scale_slot_stride;
+    }
+    a.B = p->B; a.T = p->T; a.cols = p->table_cols; a.ps = kv->page_size; a.n_pages = kv->n_pages; a.layers = p->n_layers;
+    a.nkv = kv->n_kv_heads; a.row = kv->head_dim * E;
+    a.div = qt_div_of(kv->page_size);
+    const bool in_place = p->kv_len_out == p->kv_len;
+    const bool apart = p->kv_len_out && in_place && p->n_layers > 0 && p->T > 0;         // lengths in a launch of their own
+    a.moves = p->n_layers > 0 && p->T > 0;
+    a.lengths = p->kv_len_out && !apart;
+    const unsigned wgs = (unsigned)(a.moves ? p->n_layers * p->B : 0);
+    hipError_t e = hipSuccess;
+    if (wgs || a.lengths) e = qt_launch(k_tree_commit, dim3(wgs + (a.lengths ? 1 : 0)), dim3(CM_T), 0, st, a);
+    if (e == hipSuccess && apart) {
+        a.moves = 0;
+        a.lengths = 1;
+        e = qt_launch(k_tree_commit, dim3(1), dim3(CM_T), 0, st, a);
+    }
+    QT_REFUSE(e != hipSuccess, "tree_commit: launch failed: %s", hipGetErrorString(e));
+    return 0;
+}

@@ -17,6 +17,7 @@ BF16, INT8, Q4_0 = 0, 1, 2
 PREC = {"bf16": BF16, "int8": INT8, "int4": Q4_0, "q4_0": Q4_0}
 # element types of the paged, batched operators (QWEN_HIP_DT_*)
 DT = {"f32": 0, "bf16": 1, "f16": 2}
+E4M3 = 16               # of caches
 PLAN_NO_PAGES, PLAN_TABLE_FULL, PLAN_TOO_MANY, PLAN_INVALID = 1, 2, 4, 8
 
 # every symbol the header declares (checked by the CPU test suite)
@@ -47,6 +48,8 @@ EXPORTS = [
     "qwen_hip_sd_stream_reset", "qwen_hip_sd_stream_free",
     "qwen_hip_op_page_plan", "qwen_hip_op_page_append", "qwen_hip_op_page_attention_workspace",
     "qwen_hip_op_page_attention", "qwen_hip_op_packed_attention", "qwen_hip_op_logit_rules",
+    "qwen_hip_op_tree_plan", "qwen_hip_op_tree_attention", "qwen_hip_op_tree_verify_workspace", "qwen_hip_op_tree_verify",
+    "qwen_hip_op_tree_commit",
 ]
 
 SD_GET_FN = C.CFUNCTYPE(C.c_void_p, C.c_void_p, C.c_char_p, C.c_longlong)
@@ -88,7 +91,8 @@ class SampleParams(C.Structure):
 class KvPages(C.Structure):
     _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_longlong), ("head_stride", C.c_longlong),
                 ("slot_stride", C.c_longlong), ("dtype", C.c_int), ("n_pages", C.c_int), ("page_size", C.c_int),
-                ("n_kv_heads", C.c_int), ("head_dim", C.c_int)]
+                ("n_kv_heads", C.c_int), ("head_dim", C.c_int), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("scale_page_stride", C.c_longlong), ("scale_head_stride", C.c_longlong), ("scale_slot_stride", C.c_longlong)]
 
 
 class PagePlan(C.Structure):
@@ -125,6 +129,28 @@ class LogitRules(C.Structure):
                [(n, C.c_void_p) for n in ("hist", "hist_off", "n_prompt", "rep", "presence", "frequency", "bias_tok", "bias_val",
                                           "bias_off", "mask")] + \
                [("mask_stride", C.c_longlong)] + [(n, C.c_int) for n in ("dtype", "B", "V", "hist_cap", "bias_cap", "rep_each")]
+
+
+class TreePlan(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("parent", "cu_q", "kv_len", "pos", "mask")] + [("mask_stride", C.c_longlong)] + \
+               [(n, C.c_int) for n in ("B", "T", "mask_words")]
+
+
+class Tree(C.Structure):
+    _fields_ = [("mask", C.c_void_p), ("pos", C.c_void_p), ("mask_stride", C.c_longlong), ("mask_words", C.c_int)]
+
+
+class TreeVerify(C.Structure):
+    _fields_ = [("p", C.c_void_p), ("q", C.c_void_p), ("p_stride", C.c_longlong), ("q_stride", C.c_longlong)] + \
+               [(n, C.c_void_p) for n in ("tok", "parent", "cu_q", "u", "r", "path", "out_tok", "n_path", "workspace")] + \
+               [("workspace_bytes", C.c_longlong)] + [(n, C.c_int) for n in ("dtype", "B", "T", "V", "max_children")]
+
+
+class TreeCommit(C.Structure):
+    _fields_ = [(n, C.c_void_p) for n in ("path", "n_path", "cu_q", "kv_len", "table")] + [("table_stride", C.c_longlong)] + \
+               [(n, C.c_void_p) for n in ("kv_len_out", "free_pages", "n_free", "n_free_out", "status")] + \
+               [("layer_stride", C.c_longlong), ("scale_layer_stride", C.c_longlong)] + \
+               [(n, C.c_int) for n in ("B", "T", "table_cols", "n_layers")]
 
 
 def _p(a):
@@ -246,6 +272,14 @@ def lib():
         L.qwen_hip_op_page_attention.restype = i
         L.qwen_hip_op_packed_attention.argtypes = [C.POINTER(PackedAttn), vp]
         L.qwen_hip_op_packed_attention.restype = i
+        L.qwen_hip_op_tree_plan.argtypes = [C.POINTER(TreePlan), vp]; L.qwen_hip_op_tree_plan.restype = i
+        L.qwen_hip_op_tree_attention.argtypes = [C.POINTER(KvPages), C.POINTER(PageAttn), C.POINTER(Tree), vp]
+        L.qwen_hip_op_tree_attention.restype = i
+        L.qwen_hip_op_tree_verify_workspace.argtypes = [C.POINTER(TreeVerify)]
+        L.qwen_hip_op_tree_verify_workspace.restype = C.c_longlong
+        L.qwen_hip_op_tree_verify.argtypes = [C.POINTER(TreeVerify), vp]; L.qwen_hip_op_tree_verify.restype = i
+        L.qwen_hip_op_tree_commit.argtypes = [C.POINTER(KvPages), C.POINTER(TreeCommit), vp]
+        L.qwen_hip_op_tree_commit.restype = i
         L.qwen_hip_op_logit_rules.argtypes = [C.POINTER(LogitRules), vp]; L.qwen_hip_op_logit_rules.restype = i
         _lib = L
     return _lib
