@@ -162,28 +162,29 @@ __device__ __forceinline__ AttTile att_tile(const AttArgs &a, AttReq q, int tile
 __device__ __forceinline__ int att_first(const AttTile &t, int first) { return t.chain ? t.shift + first : t.shift - 1; }
 __device__ __forceinline__ int att_last(const AttTile &t, int last) { return t.shift + (t.chain ? last : t.n - 1); }
 
-// Steps with trees: which of the 32 keys from k0 on token `tok` of the request sees, if they exist.  A tree's word is 32 bits of what
-// comes before the new tokens (all seen), of the token's mask, and of what comes behind it (none).
-__device__ __forceinline__ uint32_t att_sees(const AttArgs &a, const AttTile &t, int tok, int k0) {
-    const int c0 = k0 - t.shift;                        // the first key among the new tokens
-    uint32_t see;
+// Steps with trees.  The last position before token `tok`'s window, -1 without one; a tree's position is the caller's, brought into the range of
+// its depths.
+__device__ __forceinline__ int att_past(const AttArgs &a, const AttTile &t, int tok) {
+    if (a.window <= 0) return -1;
+    const int pos = t.chain ? t.shift + tok : min(max(a.pos[t.q0 + tok], t.shift), t.shift + t.n - 1);
+    return max(pos - a.window, -1);
+}
+// Which of the 32 keys from k0 on the token sees, if they exist.  A tree's word is 32 bits of what comes before the new tokens (all
+// seen, after the window's start), of the token's mask, and of what comes behind it (none).
+__device__ __forceinline__ uint32_t att_sees(const AttArgs &a, const AttTile &t, int tok, int past, int k0) {
+    const int c0 = k0 - t.shift, y = past - k0;         // the first key among the new tokens; keys past y are in the window
+    const uint32_t in = y < 0 ? ~0u : y >= 31 ? 0u : ~((2u << y) - 1u);
     if (t.chain) {
         const int d = tok - c0;
-        see = d < 0 ? 0u : d >= 31 ? ~0u : (2u << d) - 1u;
-    } else {
-        const uint32_t *m = a.mask + (t.q0 + tok) * a.mstride;
-        const int w = c0 >> 5;
-        const uint32_t lo = w < 0 ? ~0u : w < a.mwords ? m[w] : 0u, hi = w + 1 < 0 ? ~0u : w + 1 < a.mwords ? m[w + 1] : 0u;
-        see = (uint32_t)(((unsigned long long)hi << 32 | lo) >> (c0 & 31));
+        return (d < 0 ? 0u : d >= 31 ? ~0u : (2u << d) - 1u) & in;
     }
-    if (a.window > 0) {
-        const int pos = t.chain ? t.shift + tok : min(max(a.pos[t.q0 + tok], t.shift), t.shift + t.n - 1);
-        const long long y = (long long)pos - a.window - k0;        // keys past y
-        uint32_t in = y < 0 ? ~0u : y >= 31 ? 0u : ~((2u << y) - 1u);
-        if (!t.chain) in |= c0 >= 0 ? ~0u : c0 <= -32 ? 0u : ~0u << -c0;
-        see &= in;
-    }
-    return see;
+    const uint32_t *m = a.mask + (t.q0 + tok) * a.mstride;
+    const int w = c0 >> 5, top = a.mwords - 1;
+    uint32_t lo = m[min(max(w, 0), top)], hi = m[min(max(w + 1, 0), top)];
+    lo = w < 0 ? ~0u : w > top ? 0u : lo;
+    hi = w < -1 ? ~0u : w >= top ? 0u : hi;
+    const uint32_t fresh = c0 >= 0 ? ~0u : c0 <= -32 ? 0u : ~0u << (-c0 & 31);
+    return (uint32_t)(((unsigned long long)hi << 32 | lo) >> (c0 & 31)) & (in | fresh);
 }
 
 // The tile of 128 rows that comes at `slot` when the requests are in the order of their keys, longest first (in 64s), and
@@ -289,13 +290,14 @@ __device__ __forceinline__ void att_serial(const AttArgs &a, AttTile t, const in
 #pragma unroll
     for (int e = 0; e < D; e++) o[e] = 0.f;
     constexpr bool K8 = EK == 1;
+    const int past = TREE ? att_past(a, t, tok) : -1;
     if (!TREE) k0 = max(k0, a.window > 0 ? pos - a.window + 1 : 0);
     k0 = max(k0, 0);
     k1 = min(k1, TREE ? t.kmax : min(t.kmax, pos + 1));
     for (int j0 = k0; j0 < k1 && l == l; j0 += 64) {
         const int j = j0 + lane;
         bool see = j < k1;
-        if (TREE && see) see = att_sees(a, t, tok, j) & 1u;
+        if (TREE && see) see = att_sees(a, t, tok, past, j) & 1u;
         long long ko = 0, vo = 0;
         float ks = 1.f, vs = 0.f;
         if (PAGED) {
@@ -588,6 +590,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     if (tile < 0 || t.r0 >= t.rows) return;               // (offsets that fall give tiles before the first)
     const int r = min(t.r0 + li, t.rows - 1), tok = qt_quot(r, a.gdiv), qh = head * a.G + r - tok * a.G, pos = t.shift + tok;
     const int first = att_first(t, qt_quot(t.r0, a.gdiv)), last = att_last(t, qt_quot(min(t.r0 + 15, t.rows - 1), a.gdiv));
+    const int past = TREE ? att_past(a, t, tok) : -1;
     // the range's 32-key blocks
     const int blk0 = t.lo / 32, blk1 = t.hi > t.lo ? (t.hi + 31) / 32 : blk0;
     const int n = att_ranges(a, blk1 - blk0, a.chunk), size = (blk1 - blk0 + n - 1) / n;
@@ -719,7 +722,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         }
         if (!(ok == 0xFFFFFFFFu && 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window))) {
             const int d = pos - 32 * kb - 4 * g, w = a.window > 0 ? d - a.window : -1000;
-            const uint32_t mine = (TREE ? ok & att_sees(a, t, tok, 32 * kb) : ok) >> (4 * g);
+            const uint32_t mine = (TREE ? ok & att_sees(a, t, tok, past, 32 * kb) : ok) >> (4 * g);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll
@@ -886,15 +889,15 @@ __device__ __forceinline__ void att_copy16(const uint8_t *base, unsigned off, un
 __device__ __forceinline__ void att_wait() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 //
-// Over e4m3 codes a block goes through registers: loaded two blocks ahead, a quarter of a row a thread, it is widened to T and stored at the
-// same places of LDS when the step before it needs no more of the vector unit.  bf16 takes a row's value as it is, its scale in the
-// conversion.  f16, whose range is small, takes K relative to the block's largest scale (ek), which the scores are multiplied by, and V
-// relative to the largest so far (ev), which the sums carry.
+// Over e4m3 codes a block's bytes are copied into LDS as they are, and a step later each thread widens what its own wave copied, a quarter of
+// a row, to T in its place: K two blocks ahead, V one, after the products, when the scores' registers are free.  bf16 takes a row's
+// value as it is, its scale in the conversion.  f16, whose range is small, takes K relative to the block's largest scale (ek), which the
+// scores are multiplied by, and V relative to the largest so far (ev), which the sums carry.
 template <typename T, int HD, bool PAGED, typename KT = T, bool TREE = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_att_tile(AttArgs a) {
     constexpr int NT = HD / 32, NS = HD / 16, RB = 2 * HD, CPR = RB / 16, RPC = 64 / CPR, NC = 64 / RPC / 4;
     constexpr bool K8 = sizeof(typename KT::elem) == 1, E16 = K8 && std::is_same<T, QtF16>::value;
-    __shared__ __align__(16) uint8_t sk[2 * 64 * RB], sv[3 * 64 * RB];
+    __shared__ __align__(16) uint8_t sk[2 * 64 * RB], sv[3 * 64 * RB];      // K8: of sv the last third is codes, 64 rows of K, 64 of V
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
     int b, tile;
@@ -910,7 +913,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     tile = __builtin_amdgcn_readfirstlane(tile);
     req = {__builtin_amdgcn_readfirstlane(req.q0), __builtin_amdgcn_readfirstlane(req.n), __builtin_amdgcn_readfirstlane(req.kv)};
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
-    // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4
+    // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4.  The places of the other steps differ from the
+    // first's in bits of their own: TIGHT kernels, which have no registers for them over the loop, make them from it.
+    constexpr bool TIGHT = K8 || TREE;
     int ka[NS], va[NT];
 #pragma unroll
     for (int s = 0; s < NS; s++) ka[s] = lr * RB + 16 * ((2 * s + h) ^ att_swk<HD>(lr));
@@ -933,6 +938,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
         for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + 32 * s);
     }
+    const int past = TREE ? att_past(a, t, tok) : -1;
     // the range's 64-key blocks; chunk is in blocks of 32, even
     const int blk0 = t.lo / 64, blk1 = t.hi > t.lo ? (t.hi + 63) / 64 : blk0;
     const int n = att_ranges(a, blk1 - blk0, a.chunk / 2), size = (blk1 - blk0 + n - 1) / n;
@@ -950,52 +956,54 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + (PAGED ? 0 : t.q0 * a.vs_slot)) * EK;
     int page = -1;                                                       // PAGED: of key 64 kb + lane, block kb the next to copy
     unsigned long long okv = ~0ull, okk = ~0ull, okn = ~0ull;            // keys that exist: of the block of V, of K, of the next K
-    // e4m3: block kb into registers, row tid / 4 and chunks tid % 4 + 4 e of 16 codes, and the scales of key 64 kb + lane; from there to a K
-    // and a V buffer; E16: exponents of the block of V, of K, of the next K, and that which o carries
-    qt_u32x4 gk[HD / 64], gv[HD / 64];
-    uint32_t gks = 0, gvs = 0, ekv = 0, ekk = 0, ekn = 0, evv = 0, evk = 0, evn = QT_SCALE_MIN, evo = QT_SCALE_MIN;
-    const auto fetch = [&](int kb) {
-        const bool has = att_has(a, page);
+    // e4m3.  copy_codes: rows of block kb (whose pages are `pg`) to `to`, row 16 wave + lane / 4, chunks lane % 4 + 4 e of 16 codes, and the
+    // scale of key 64 kb + lane.  widen: from there into a buffer, relative to 2^(rel - 127).
+    const unsigned lk = att_lds(sk), lv = att_lds(sv);
+    uint8_t *const rawk = sv + 2 * 64 * RB, *const rawv = rawk + 64 * HD;
+    int page_v = -1;                                                     // of the block whose V is the next to copy
+    uint32_t gks = 0, gvs = 0, ekv = 0, ekk = 0, ekn = 0, evn = QT_SCALE_MIN, evo = QT_SCALE_MIN;   // E16: of K of this block, the next ones; of V, of o
+    const auto copy_codes = [&](int kb, int pg, const uint8_t *base, const uint8_t *scales, unsigned to, uint32_t &sc) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));                                     // addresses are formed here: held over the loop they spill
+        const bool has = att_has(a, pg);
         okn = __ballot(has);
-        const int key = 64 * kb + lane, row = 16 * wave + (lane >> 2);
-        const long long off = att_instead(att_slot(a, page, key), has, okn);
-        const long long so = att_instead(att_scale_slot(a, page, key), has, okn) + head * a.ss_head;
-        const long long at = (((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row)) + 16 * (lane & 3);
-        gks = a.ksc[so];
-        gvs = a.vsc[so];
+        const int key = 64 * kb + ln, row = 16 * wave + (ln >> 2);
+        const long long off = att_instead(att_slot(a, pg, key), has, okn);
+        sc = scales[att_instead(att_scale_slot(a, pg, key), has, okn) + head * a.ss_head];
+        const long long at = (((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row)) + 16 * (ln & 3);
+#pragma unroll
+        for (int e = 0; e < HD / 64; e++) att_copy16(base + at + 64 * e, to + 1024 * (wave * (HD / 64) + e));
+    };
+    const auto widen = [&](const uint8_t *from, uint32_t sc, auto swizzle, uint8_t *buf, uint32_t rel) {
+        int ln = lane;
+        asm volatile("" : "+v"(ln));
+        const int row = 16 * wave + (ln >> 2);
+        float f = qt_scale_of((uint32_t)__shfl((int)sc, row));
+        if constexpr (E16) f *= __uint_as_float((254u - rel) << 23);
 #pragma unroll
         for (int e = 0; e < HD / 64; e++) {
-            gk[e] = *reinterpret_cast<const qt_u32x4 *>(kbase + at + 64 * e);
-            gv[e] = *reinterpret_cast<const qt_u32x4 *>(vbase + at + 64 * e);
-        }
-        page = kb + 1 < kb1 ? att_page(a, table, t, 64 * (kb + 1) + lane) : -1;
-    };
-    const auto put = [&](uint8_t *kbuf, uint8_t *vbuf) {
-        const int row = 16 * wave + (lane >> 2);
-        float fk = qt_scale_of((uint32_t)__shfl((int)gks, row)), fv = qt_scale_of((uint32_t)__shfl((int)gvs, row));
-        if constexpr (E16) {
-            ekn = (uint32_t)max(wave_max_i((int)qt_scale_read(gks)), (int)QT_SCALE_MIN);
-            evn = max(evn, (uint32_t)wave_max_i((int)qt_scale_read(gvs)));
-            fk *= __uint_as_float((254u - ekn) << 23);
-            fv *= __uint_as_float((254u - evn) << 23);
-        }
-#pragma unroll
-        for (int e = 0; e < HD / 64; e++)
+            const qt_u32x4 c = qt_lds16(from + 1024 * (wave * (HD / 64) + e) + 16 * ln);
 #pragma unroll
             for (int x = 0; x < 2; x++) {
-                const int c = 2 * ((lane & 3) + 4 * e) + x;
-                qt_u32x4 wk, wv;
+                qt_u32x4 w;
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    wk[i] = att_code2<T>(gk[e][2 * x + (i >> 1)], i & 1, fk);
-                    wv[i] = att_code2<T>(gv[e][2 * x + (i >> 1)], i & 1, fv);
-                }
-                *reinterpret_cast<qt_u32x4 *>(kbuf + row * RB + 16 * (c ^ att_swk<HD>(row))) = wk;
-                *reinterpret_cast<qt_u32x4 *>(vbuf + row * RB + 16 * (c ^ att_swv<HD>(row))) = wv;
+                for (int i = 0; i < 4; i++) w[i] = att_code2<T>(c[2 * x + (i >> 1)], i & 1, f);
+                *reinterpret_cast<qt_u32x4 *>(buf + row * RB + 16 * ((2 * ((ln & 3) + 4 * e) + x) ^ swizzle(row))) = w;
             }
+        }
     };
+    const auto swk = [](int row) { return att_swk<HD>(row); };
+    const auto swv = [](int row) { return att_swv<HD>(row); };
+    const auto widen_k = [&](const uint8_t *from, uint32_t sc, uint8_t *buf) {
+        if constexpr (E16) ekn = (uint32_t)max(wave_max_i((int)qt_scale_read(sc)), (int)QT_SCALE_MIN);
+        widen(from, sc, swk, buf, ekn);
+    };
+    const auto widen_v = [&](const uint8_t *from, uint32_t sc, uint8_t *buf) {
+        if constexpr (E16) evn = max(evn, (uint32_t)wave_max_i((int)qt_scale_read(sc)));
+        widen(from, sc, swv, buf, evn);
+    };
+    const auto page_of = [&](int kb) { return kb < kb1 ? att_page(a, table, t, 64 * kb + lane) : -1; };
     // block kb to a K and a V buffer
-    const unsigned lk = att_lds(sk), lv = att_lds(sv);
     const auto copy = [&](int kb, unsigned kdst, unsigned vdst) {
         if constexpr (PAGED) {
             const bool has = att_has(a, page);
@@ -1037,14 +1045,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         }
     };
     const auto scores = [&](qt_f32x16 (&sc)[2], const uint8_t *kbuf) {
+        int k0 = ka[0];
+        if constexpr (TIGHT) asm volatile("" : "+v"(k0));
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
 #pragma unroll
-        for (int s = 0; s < NS; s++)
+        for (int s = 0; s < NS; s++) {
+            const int at = TIGHT ? k0 ^ (32 * s) : ka[s];
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) sc[kt] = att_mma<T>(qt_lds16(kbuf + 32 * kt * RB + ka[s]), qf[s], sc[kt]);
+            for (int kt = 0; kt < 2; kt++) sc[kt] = att_mma<T>(qt_lds16(kbuf + 32 * kt * RB + at), qf[s], sc[kt]);
+        }
     };
     // block kb: its scores are in sc, K of block kb + 1 is in the other K buffer than kb's was, V in buffer vb
     int vb = 0;
@@ -1059,20 +1071,20 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         float pk = 1.f;                                                  // E16: of this block's scores
         if constexpr (E16) {
             ekv = ekk; ekk = ekn;
-            evv = evk; evk = evn;
             pk = __uint_as_float(ekv << 23);
         }
-        const uint8_t *vbuf = sv + vb * 64 * RB;
-        vb = vb == 2 ? 0 : vb + 1;
-        if (kb + 2 < kb1) {
-            if constexpr (K8) fetch(kb + 2);
-            else copy(kb + 2, lk + BUF * 64 * RB, lv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
+        const uint8_t *vbuf = sv + (K8 ? BUF : vb) * 64 * RB;
+        if constexpr (!K8) {
+            vb = vb == 2 ? 0 : vb + 1;
+            if (kb + 2 < kb1) copy(kb + 2, lk + BUF * 64 * RB, lv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
         }
         if (64 * kb + 63 > first || (a.window > 0 && 64 * kb <= last - a.window)) {
             const int d = pos - 64 * kb - 4 * h, w = a.window > 0 ? d - a.window : -1000;
+            int row = tok;
+            if constexpr (TREE) asm volatile("" : "+v"(row));            // its mask's place is formed here: held over the loop it spills
 #pragma unroll
             for (int kt = 0; kt < 2; kt++) {
-                const uint32_t mine = TREE ? att_sees(a, t, tok, 64 * kb + 32 * kt) >> (4 * h) : 0u;
+                const uint32_t mine = TREE ? att_sees(a, t, row, past, 64 * kb + 32 * kt) >> (4 * h) : 0u;
 #pragma unroll
                 for (int i = 0; i < 16; i++) {
                     const int j = 32 * kt + 8 * (i >> 2) + (i & 3);
@@ -1096,12 +1108,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         bm = fmaxf(bm, att_other_half(bm));
         if constexpr (E16) bm *= pk;
         // probabilities up to 2^8 are as good as up to 1: the sums shrink only when a row's maximum has risen by more
-        if (__ballot((bm - m) * a.c > 8.0f || (m == -INFINITY && bm > m)) || (E16 && evv != evo)) {
+        if (__ballot((bm - m) * a.c > 8.0f || (m == -INFINITY && bm > m)) || (E16 && evn != evo)) {
             const float mn = fmaxf(m, bm), f = mn == -INFINITY ? 0.f : qt_exp2((m - mn) * a.c);
             float fo = f;
             if constexpr (E16) {
-                fo *= __uint_as_float((127u + evo < evv ? 0u : 127u + evo - evv) << 23);
-                evo = evv;
+                fo *= __uint_as_float((127u + evo < evn ? 0u : 127u + evo - evn) << 23);
+                evo = evn;
             }
             m = mn;
             l *= f;
@@ -1120,6 +1132,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int s = 0; s < 4; s++) {
             qt_u32x4 pb;
             float sum = 0.f;
+            int v0 = va[0];
+            if constexpr (TIGHT) asm volatile("" : "+v"(v0));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
@@ -1128,25 +1142,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             l += sum;
 #pragma unroll
             for (int d = 0; d < NT; d++) {
-                const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + va[d]);
+                const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + (TIGHT ? v0 ^ (64 * d) : va[d]));
                 o[d] = att_mma<T>(qt_lds_tr8x2(vp, vp + 8 * HD), pb, o[d]);
             }
         }
-        if constexpr (K8)
-            if (kb + 2 < kb1) put(sk + BUF * 64 * RB, sv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
+        if constexpr (K8) {
+            __builtin_amdgcn_sched_barrier(0);
+            att_wait();                                                  // the codes of K of block kb + 2 and V of kb + 1, and their scales
+            if (kb + 2 < kb1) widen_k(rawk, gks, sk + BUF * 64 * RB);
+            if (kb + 1 < kb1) widen_v(rawv, gvs, sv + (BUF ^ 1) * 64 * RB);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // they are read before others take their place
+            if (kb + 3 < kb1) copy_codes(kb + 3, page, kbase, a.ksc, lv + 2 * 64 * RB, gks);
+            if (kb + 2 < kb1) copy_codes(kb + 2, page_v, vbase, a.vsc, lv + 2 * 64 * RB + 64 * HD, gvs);
+            page_v = page;
+            page = page_of(kb + 4);
+        }
     };
     if (kb0 < kb1) {
         if (PAGED) page = att_page(a, table, t, 64 * kb0 + lane);
         if constexpr (K8) {
-            fetch(kb0);
-            put(sk, sv);
+            // K of two blocks and V of the first, which comes in where V of the second will stand
+            const int page1 = page_of(kb0 + 1), page2 = page_of(kb0 + 2);
+            uint32_t gk1 = 0;
+            if (kb0 + 1 < kb1) copy_codes(kb0 + 1, page1, kbase, a.ksc, lv + 2 * 64 * RB + 64 * HD, gk1);
+            copy_codes(kb0, page, kbase, a.ksc, lv + 2 * 64 * RB, gks);
+            copy_codes(kb0, page, vbase, a.vsc, lv + 64 * RB, gvs);
             okk = okn;
+            att_wait();
+            widen_k(rawk, gks, sk);
             ekk = ekn;
-            evk = evn;
-            if (kb0 + 1 < kb1) {
-                fetch(kb0 + 1);
-                put(sk + 64 * RB, sv + 64 * RB);
-            }
+            widen_v(sv + 64 * RB, gvs, sv);
+            if (kb0 + 1 < kb1) widen_k(rawv, gk1, sk + 64 * RB);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+            if (kb0 + 2 < kb1) copy_codes(kb0 + 2, page2, kbase, a.ksc, lv + 2 * 64 * RB, gks);
+            if (kb0 + 1 < kb1) copy_codes(kb0 + 1, page1, vbase, a.vsc, lv + 2 * 64 * RB + 64 * HD, gvs);
+            page_v = page2;
+            page = page_of(kb0 + 3);
         } else {
             copy(kb0, lk, lv);
             okk = okn;
