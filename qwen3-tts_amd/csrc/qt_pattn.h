@@ -913,9 +913,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     tile = __builtin_amdgcn_readfirstlane(tile);
     req = {__builtin_amdgcn_readfirstlane(req.q0), __builtin_amdgcn_readfirstlane(req.n), __builtin_amdgcn_readfirstlane(req.kv)};
     const int *table = PAGED ? a.table + b * a.ts : nullptr;
-    // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4.  The places of the other steps differ from the
-    // first's in bits of their own: TIGHT kernels, which have no registers for them over the loop, make them from it.
-    constexpr bool TIGHT = K8 || TREE;
+    // where this lane reads a block's operands: K row lr, V rows 4 h + (lane % 16) / 4.
     int ka[NS], va[NT];
 #pragma unroll
     for (int s = 0; s < NS; s++) ka[s] = lr * RB + 16 * ((2 * s + h) ^ att_swk<HD>(lr));
@@ -956,24 +954,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + (PAGED ? 0 : t.q0 * a.vs_slot)) * EK;
     int page = -1;                                                       // PAGED: of key 64 kb + lane, block kb the next to copy
     unsigned long long okv = ~0ull, okk = ~0ull, okn = ~0ull;            // keys that exist: of the block of V, of K, of the next K
-    // e4m3.  copy_codes: rows of block kb (whose pages are `pg`) to `to`, row 16 wave + lane / 4, chunks lane % 4 + 4 e of 16 codes, and the
-    // scale of key 64 kb + lane.  widen: from there into a buffer, relative to 2^(rel - 127).
+    // e4m3.  locate: where a block's codes and scales lie, of row 16 wave + lane / 4 from chunk lane % 4 on, and of key 64 kb + lane.
+    // copy_codes: from there to `to`, chunks lane % 4 + 4 e of 16 codes, and the scale.  widen: codes into a buffer, relative to 2^(rel - 127).
     const unsigned lk = att_lds(sk), lv = att_lds(sv);
     uint8_t *const rawk = sv + 2 * 64 * RB, *const rawv = rawk + 64 * HD;
-    int page_v = -1;                                                     // of the block whose V is the next to copy
+    struct Where { long long codes, scale; };
+    Where next_v = {0, 0};                                               // of the block whose V is the next to copy
+    unsigned long long ok_v = 0;
     uint32_t gks = 0, gvs = 0, ekv = 0, ekk = 0, ekn = 0, evn = QT_SCALE_MIN, evo = QT_SCALE_MIN;   // E16: of K of this block, the next ones; of V, of o
-    const auto copy_codes = [&](int kb, int pg, const uint8_t *base, const uint8_t *scales, unsigned to, uint32_t &sc) {
+    const auto locate = [&](int kb, int pg) {
         int ln = lane;
         asm volatile("" : "+v"(ln));                                     // addresses are formed here: held over the loop they spill
         const bool has = att_has(a, pg);
-        okn = __ballot(has);
+        ok_v = __ballot(has);
         const int key = 64 * kb + ln, row = 16 * wave + (ln >> 2);
-        const long long off = att_instead(att_slot(a, pg, key), has, okn);
-        sc = scales[att_instead(att_scale_slot(a, pg, key), has, okn) + head * a.ss_head];
-        const long long at = (((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row)) + 16 * (ln & 3);
-#pragma unroll
-        for (int e = 0; e < HD / 64; e++) att_copy16(base + at + 64 * e, to + 1024 * (wave * (HD / 64) + e));
+        Where w;
+        if (a.near) {
+            const int c = qt_quot(key, a.div), from = ok_v ? __ffsll(ok_v) - 1 : 0;
+            unsigned off = (unsigned)pg * (unsigned)a.ks_page + (unsigned)(key - c * a.ps) * (unsigned)a.ks_slot;
+            unsigned so = (unsigned)pg * (unsigned)a.ss_page + (unsigned)(key - c * a.ps) * (unsigned)a.ss_slot;
+            const unsigned other = ok_v ? (unsigned)__builtin_amdgcn_readlane((int)off, from) : 0u, so_other = ok_v ? (unsigned)__builtin_amdgcn_readlane((int)so, from) : 0u;
+            off = has ? off : other;
+            w.scale = has ? so : so_other;
+            w.codes = (unsigned)__shfl((int)off, row) + 16u * (ln & 3);
+        } else {
+            const long long off = att_instead(att_slot(a, pg, key), has, ok_v);
+            w.scale = att_instead(att_scale_slot(a, pg, key), has, ok_v);
+            w.codes = (((long long)__shfl((int)(off >> 32), row) << 32) | (unsigned)__shfl((int)off, row)) + 16 * (ln & 3);
+        }
+        return w;
     };
+    const auto copy_codes = [&](Where w, const uint8_t *base, const uint8_t *scales, unsigned to, uint32_t &sc) {
+        sc = scales[w.scale];
+#pragma unroll
+        for (int e = 0; e < HD / 64; e++) att_copy16(base + w.codes + 64 * e, to + 1024 * (wave * (HD / 64) + e));
+    };
+    const uint8_t *const kscale = a.ksc + head * a.ss_head, *const vscale = a.vsc + head * a.ss_head;
     const auto widen = [&](const uint8_t *from, uint32_t sc, auto swizzle, uint8_t *buf, uint32_t rel) {
         int ln = lane;
         asm volatile("" : "+v"(ln));
@@ -1045,18 +1061,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         }
     };
     const auto scores = [&](qt_f32x16 (&sc)[2], const uint8_t *kbuf) {
-        int k0 = ka[0];
-        if constexpr (TIGHT) asm volatile("" : "+v"(k0));
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
             for (int i = 0; i < 16; i++) sc[kt][i] = 0.f;
 #pragma unroll
-        for (int s = 0; s < NS; s++) {
-            const int at = TIGHT ? k0 ^ (32 * s) : ka[s];
+        for (int s = 0; s < NS; s++)
 #pragma unroll
-            for (int kt = 0; kt < 2; kt++) sc[kt] = att_mma<T>(qt_lds16(kbuf + 32 * kt * RB + at), qf[s], sc[kt]);
-        }
+            for (int kt = 0; kt < 2; kt++) sc[kt] = att_mma<T>(qt_lds16(kbuf + 32 * kt * RB + ka[s]), qf[s], sc[kt]);
     };
     // block kb: its scores are in sc, K of block kb + 1 is in the other K buffer than kb's was, V in buffer vb
     int vb = 0;
@@ -1132,8 +1144,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         for (int s = 0; s < 4; s++) {
             qt_u32x4 pb;
             float sum = 0.f;
-            int v0 = va[0];
-            if constexpr (TIGHT) asm volatile("" : "+v"(v0));
 #pragma unroll
             for (int j = 0; j < 4; j++) {
                 pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
@@ -1142,7 +1152,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             l += sum;
 #pragma unroll
             for (int d = 0; d < NT; d++) {
-                const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + (TIGHT ? v0 ^ (64 * d) : va[d]));
+                const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + va[d]);
                 o[d] = att_mma<T>(qt_lds_tr8x2(vp, vp + 8 * HD), pb, o[d]);
             }
         }
@@ -1152,9 +1162,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             if (kb + 2 < kb1) widen_k(rawk, gks, sk + BUF * 64 * RB);
             if (kb + 1 < kb1) widen_v(rawv, gvs, sv + (BUF ^ 1) * 64 * RB);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // they are read before others take their place
-            if (kb + 3 < kb1) copy_codes(kb + 3, page, kbase, a.ksc, lv + 2 * 64 * RB, gks);
-            if (kb + 2 < kb1) copy_codes(kb + 2, page_v, vbase, a.vsc, lv + 2 * 64 * RB + 64 * HD, gvs);
-            page_v = page;
+            if (kb + 2 < kb1) {
+                okn = ok_v;
+                copy_codes(next_v, vbase, vscale, lv + 2 * 64 * RB + 64 * HD, gvs);
+            }
+            if (kb + 3 < kb1) {
+                next_v = locate(kb + 3, page);
+                copy_codes(next_v, kbase, kscale, lv + 2 * 64 * RB, gks);
+            }
             page = page_of(kb + 4);
         }
     };
@@ -1164,19 +1179,26 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             // K of two blocks and V of the first, which comes in where V of the second will stand
             const int page1 = page_of(kb0 + 1), page2 = page_of(kb0 + 2);
             uint32_t gk1 = 0;
-            if (kb0 + 1 < kb1) copy_codes(kb0 + 1, page1, kbase, a.ksc, lv + 2 * 64 * RB + 64 * HD, gk1);
-            copy_codes(kb0, page, kbase, a.ksc, lv + 2 * 64 * RB, gks);
-            copy_codes(kb0, page, vbase, a.vsc, lv + 64 * RB, gvs);
-            okk = okn;
+            Where w = locate(kb0, page);
+            okk = ok_v;
+            copy_codes(w, kbase, kscale, lv + 2 * 64 * RB, gks);
+            copy_codes(w, vbase, vscale, lv + 64 * RB, gvs);
+            if (kb0 + 1 < kb1) {
+                w = locate(kb0 + 1, page1);
+                okn = ok_v;
+                copy_codes(w, kbase, kscale, lv + 2 * 64 * RB + 64 * HD, gk1);
+            }
             att_wait();
             widen_k(rawk, gks, sk);
             ekk = ekn;
             widen_v(sv + 64 * RB, gvs, sv);
             if (kb0 + 1 < kb1) widen_k(rawv, gk1, sk + 64 * RB);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-            if (kb0 + 2 < kb1) copy_codes(kb0 + 2, page2, kbase, a.ksc, lv + 2 * 64 * RB, gks);
-            if (kb0 + 1 < kb1) copy_codes(kb0 + 1, page1, vbase, a.vsc, lv + 2 * 64 * RB + 64 * HD, gvs);
-            page_v = page2;
+            if (kb0 + 1 < kb1) copy_codes(w, vbase, vscale, lv + 2 * 64 * RB + 64 * HD, gvs);
+            if (kb0 + 2 < kb1) {
+                next_v = locate(kb0 + 2, page2);
+                copy_codes(next_v, kbase, kscale, lv + 2 * 64 * RB, gks);
+            }
             page = page_of(kb0 + 3);
         } else {
             copy(kb0, lk, lv);

@@ -1,6 +1,7 @@
 // qt_pattn.hip — the host side of attention over paged caches and packed prompts, and the kernels over 16-bit and f32
 // operands.
 #include "qt_pattn.h"
+#include <stdlib.h>
 
 // ---- host side -------------------------------------------------------------------------------------
 
@@ -35,7 +36,7 @@ static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv
     // only reads; a tile's sums are large, and two workgroups a CU are enough (chunks over up to 7000 keys: 2 ranges
     // 171 us, 1 226, 3 190, 4 205).
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
-    long long n = wgs > 0 && paged ? ((p.kind == ATT_TILE ? 512 : 4096) + wgs - 1) / wgs : 1;
+    long long n = wgs > 0 && paged ? ((p.kind == ATT_TILE ? (getenv("QTW") ? atoi(getenv("QTW")) : 512) : 4096) + wgs - 1) / wgs : 1;
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
     if (n < 1) n = 1;
@@ -144,6 +145,7 @@ static int paged_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_at
     if (codes) {
         a.ksc = kv->k_scale; a.vsc = kv->v_scale;
         a.ss_page = kv->scale_page_stride; a.ss_head = kv->scale_head_stride; a.ss_slot = kv->scale_slot_stride;
+        a.near = a.near && (kv->n_pages - 1.0) * kv->scale_page_stride + (kv->page_size - 1.0) * kv->scale_slot_stride < 2147000000.0;
     }
     if (tree) { a.mask = tree->mask; a.pos = tree->pos; a.mstride = tree->mask_stride; a.mwords = tree->mask_words; }
     hipError_t e = codes  ? att_launch_codes(a, plan, p->dtype, kv->head_dim, tree != nullptr, st)
