@@ -1072,8 +1072,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     };
     // block kb: its scores are in sc, K of block kb + 1 is in the other K buffer than kb's was, V in buffer vb
     int vb = 0;
-    const auto step = [&](int kb, qt_f32x16 (&sc)[2], qt_f32x16 (&sn)[2], auto bufc) {
+    const auto step = [&](int kb, qt_f32x16 (&sc)[2], qt_f32x16 (&sn)[2], auto bufc, auto maskc) {
         constexpr int BUF = decltype(bufc)::value;
+        constexpr bool MASK = decltype(maskc)::value;                    // the block may hold keys that some row does not see
         // K of the next block is in, V of this one since the last step (the wave's own copies by the wait, the others' by
         // the barrier, which they pass after theirs), and every wave has left the buffers that block kb + 2 takes
         if constexpr (!K8) att_wait();
@@ -1090,7 +1091,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             vb = vb == 2 ? 0 : vb + 1;
             if (kb + 2 < kb1) copy(kb + 2, lk + BUF * 64 * RB, lv + (vb == 2 ? 0 : vb + 1) * 64 * RB);
         }
-        if (64 * kb + 63 > first || (a.window > 0 && 64 * kb <= last - a.window)) {
+        if (MASK && (64 * kb + 63 > first || (a.window > 0 && 64 * kb <= last - a.window))) {
             const int d = pos - 64 * kb - 4 * h, w = a.window > 0 ? d - a.window : -1000;
             int row = tok;
             if constexpr (TREE) asm volatile("" : "+v"(row));            // its mask's place is formed here: held over the loop it spills
@@ -1136,6 +1137,21 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         }
         const float mc = m == -INFINITY ? 0.f : m * a.c;
         if (kb + 1 < kb1) scores(sn, sk + (BUF ^ 1) * 64 * RB);
+        if constexpr (K8) {
+            att_wait();                                                  // the codes of K of block kb + 2 and V of kb + 1, and their scales
+            if (kb + 2 < kb1) widen_k(rawk, gks, sk + BUF * 64 * RB);
+            if (kb + 1 < kb1) widen_v(rawv, gvs, sv + (BUF ^ 1) * 64 * RB);
+            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // they are read before others take their place
+            if (kb + 2 < kb1) {
+                okn = ok_v;
+                copy_codes(next_v, vbase, vscale, lv + 2 * 64 * RB + 64 * HD, gvs);
+            }
+            if (kb + 3 < kb1) {
+                next_v = locate(kb + 3, page);
+                copy_codes(next_v, kbase, kscale, lv + 2 * 64 * RB, gks);
+            }
+            page = page_of(kb + 4);
+        }
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
@@ -1155,22 +1171,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
                 const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + va[d]);
                 o[d] = att_mma<T>(qt_lds_tr8x2(vp, vp + 8 * HD), pb, o[d]);
             }
-        }
-        if constexpr (K8) {
-            __builtin_amdgcn_sched_barrier(0);
-            att_wait();                                                  // the codes of K of block kb + 2 and V of kb + 1, and their scales
-            if (kb + 2 < kb1) widen_k(rawk, gks, sk + BUF * 64 * RB);
-            if (kb + 1 < kb1) widen_v(rawv, gvs, sv + (BUF ^ 1) * 64 * RB);
-            asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");           // they are read before others take their place
-            if (kb + 2 < kb1) {
-                okn = ok_v;
-                copy_codes(next_v, vbase, vscale, lv + 2 * 64 * RB + 64 * HD, gvs);
-            }
-            if (kb + 3 < kb1) {
-                next_v = locate(kb + 3, page);
-                copy_codes(next_v, kbase, kscale, lv + 2 * 64 * RB, gks);
-            }
-            page = page_of(kb + 4);
         }
     };
     if (kb0 < kb1) {
@@ -1209,9 +1209,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         __syncthreads();
         qt_f32x16 s0[2], s1[2];
         scores(s0, sk);
-        for (int kb = kb0; kb < kb1; kb += 2) {
-            step(kb, s0, s1, std::integral_constant<int, 0>{});
-            if (kb + 1 < kb1) step(kb + 1, s1, s0, std::integral_constant<int, 1>{});
+        int kb = kb0;
+        // blocks that every row sees whole, in a loop of their own where the masks would take its registers
+        if constexpr (K8 || TREE) {
+            const int clear = a.window > 0 ? kb0 : min(kb1, (att_first(t, qt_quot(t.r0, a.gdiv)) + 1) / 64);
+            for (; kb + 1 < clear; kb += 2) {
+                step(kb, s0, s1, std::integral_constant<int, 0>{}, std::false_type{});
+                step(kb + 1, s1, s0, std::integral_constant<int, 1>{}, std::false_type{});
+            }
+        }
+        for (; kb < kb1; kb += 2) {
+            step(kb, s0, s1, std::integral_constant<int, 0>{}, std::true_type{});
+            if (kb + 1 < kb1) step(kb + 1, s1, s0, std::integral_constant<int, 1>{}, std::true_type{});
         }
     }
     // the rows' results; o[d][i] is dim 32 d + 8 (i / 4) + 4 h + i % 4

@@ -1,13 +1,12 @@
 // qt_pattn.hip — the host side of attention over paged caches and packed prompts, and the kernels over 16-bit and f32
 // operands.
 #include "qt_pattn.h"
-#include <stdlib.h>
 
 // ---- host side -------------------------------------------------------------------------------------
 
 // The kernel, its launch slots and key ranges.  Launch slots: by request (max_q as far as known) or by rows, whichever is
 // fewer.  Key ranges: enough workgroups to fill the CUs, 256 keys each at least.
-static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv) {
+static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv, bool more) {
     AttPlan p = {ATT_ONE, 0, false};
     a.gdiv = qt_div_of(a.G);
     a.tps = 0;
@@ -34,9 +33,12 @@ static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv
     }
     // Single tokens want many ranges (64 streams of up to 8000 keys: 2 of them 217 us, 8 199, 16 200), since a workgroup
     // only reads; a tile's sums are large, and two workgroups a CU are enough (chunks over up to 7000 keys: 2 ranges
-    // 171 us, 1 226, 3 190, 4 205).
+    // 171 us, 1 226, 3 190, 4 205).  Over codes, and for trees, requests of one tile each take up to four a CU, since their lengths
+    // differ by more than a tile's (32 trees of 33 to 64 tokens over 500 to 6000 keys of codes: 2 ranges 138 us, 3 128, 4 139, 5 129; chunks
+    // of several tiles 168, 171, 182, 180).
+    const bool one_tile = more && max_q > 0 && (long long)max_q * a.G <= 128;
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
-    long long n = wgs > 0 && paged ? ((p.kind == ATT_TILE ? (getenv("QTW") ? atoi(getenv("QTW")) : 512) : 4096) + wgs - 1) / wgs : 1;
+    long long n = wgs > 0 && paged ? ((p.kind == ATT_TILE ? (one_tile ? 1024 : 512) : 4096) + wgs - 1) / wgs : 1;
     if (n > (blocks + 7) / 8) n = (blocks + 7) / 8;
     if (n > 64) n = 64;
     if (n < 1) n = 1;
@@ -61,7 +63,7 @@ static int check_rows(const char *who, int dtype, int n_heads, int nkv, int hd, 
     return 0;
 }
 
-static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, AttArgs &a, AttPlan &plan) {
+static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, bool tree, AttArgs &a, AttPlan &plan) {
     if (qt_check_pages("page_attention", kv)) return -1;
     QT_REFUSE(!p, "page_attention: null descriptor");
     if (check_rows("page_attention", p->dtype, p->n_heads, kv->n_kv_heads, kv->head_dim, p->B, p->T, p->window, p->scale)) return -1;
@@ -72,16 +74,17 @@ static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t 
               "page_attention: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
     a = AttArgs{};
     a.B = p->B; a.T = p->T; a.nkv = kv->n_kv_heads; a.G = p->n_heads / kv->n_kv_heads;
-    plan = att_plan(a, p->dtype, true, p->max_q < p->T ? p->max_q : p->T, p->max_kv);
+    plan = att_plan(a, p->dtype, true, p->max_q < p->T ? p->max_q : p->T, p->max_kv, tree || kv->dtype == QWEN_HIP_DT_E4M3);
     plan.stream = plan.stream && 2ll * qt_kv_size(kv->dtype) * p->B * p->max_kv * kv->n_kv_heads * kv->head_dim > 256ll << 20;
     return 0;
 }
 
 extern "C" long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p) {
-    AttArgs a;
+    AttArgs a, t;                                     // with and without trees
     AttPlan plan;
-    if (paged_args(kv, p, a, plan)) return -1;
-    return a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
+    if (paged_args(kv, p, false, a, plan) || paged_args(kv, p, true, t, plan)) return -1;
+    const long long n = a.splits > t.splits ? a.splits : t.splits;
+    return n > 1 ? n * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
 }
 
 template <typename QT, int HD, bool PAGED>
@@ -109,7 +112,7 @@ static hipError_t att_merge(const AttArgs &a, int dtype, int hd, hipStream_t st)
 static int paged_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, const qwen_hip_tree_t *tree, void *stream) {
     AttArgs a;
     AttPlan plan;
-    if (paged_args(kv, p, a, plan)) return -1;
+    if (paged_args(kv, p, tree != nullptr, a, plan)) return -1;
     if (p->B == 0 || p->T == 0) return 0;
     if (tree) {
         QT_REFUSE(tree->mask_words < 1 || tree->mask_words > 32 || tree->mask_stride < tree->mask_words,
@@ -179,7 +182,7 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
               p->k_stride, p->v_stride, p->out_stride);
     AttArgs a = {};
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
-    const AttPlan plan = att_plan(a, p->dtype, false, 0, 0);
+    const AttPlan plan = att_plan(a, p->dtype, false, 0, 0, false);
     QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "packed_attention: too many tiles for one launch");
     const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * p->head_dim * E, kw = (long long)p->n_kv_heads * p->head_dim * E;
     QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T) ||
