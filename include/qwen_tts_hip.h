@@ -613,7 +613,7 @@ int qwen_hip_op_tree_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_pag
  * u[c] < 0 is kept for certain (text that is given: a chunk of a prompt as a chain).  Written: n_path[b] tokens kept, the root among them (0 for a request without new
  * tokens), path[cu_q[b] + k] their indices in ascending order, out_tok[cu_q[b] + k] the token that follows path[k]: kept ones,
  * and at k = n_path[b] - 1 the next token; both -1 from there to the request's last row.  Rows before cu_q[0] and
- * behind cu_q[B] stay as they were.  dtype of p and q: F32, BF16 or F16; rows aligned to 2 bytes at least (an element).
+ * behind cu_q[B] stay as they were.  dtype of p and q: F32, BF16 or F16, aligned to an element.  V <= 2^20.
  * max_children: the most children that a token has, as far as the host knows (0: unknown); it chooses launches and changes no result. */
 typedef struct {
     const void *p, *q;

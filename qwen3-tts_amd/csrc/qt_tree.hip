@@ -73,25 +73,28 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
 // z <- sum w.  After rejections w is max(A p - B q, 0) with two numbers: A, B -> A / z, B / z + 1 (a token whose w
 // has become 0 stays at 0).  So the walk needs each token's p and q at its parent's row, gathered once for 64 tokens, and a pass over the
 // vocabulary only where a sum is asked for: by a further child after a rejection, and by the next token at the end.
-// The pass sums tiles of 4096 entries; the next token's tile is found in the tiles' sums, the token by a scan of its tile.
+// The pass sums tiles of 1024 entries, four a wave; the next token's tile is found in the tiles' sums, the token by a scan of its tile.
 // All in f64: an f32 sum over a vocabulary would move the border between two tokens by more than some tokens have.
 //
-// Large vocabularies: a first launch walks to the first sum (every workgroup for itself: a few dependent loads) and sums a tile a
-// workgroup, a second one, a workgroup a request, goes on from there; sums that it finds it needs beyond the first it makes itself.
-#define VF_T 256
-#define VF_TILE 4096
-#define VF_ONE 1                    // vocabularies of so many tiles take one launch
+// Large vocabularies: launches of a wave for four tiles, the first of which walks to the first sum (every workgroup for itself: a few
+// dependent loads), the others from the sum before to the next where there is one; then a launch of a workgroup a request, which goes on
+// from there, makes further sums itself, and picks.
+#define VF_TILE 1024
+#define VF_MAX_V (1 << 20)
+#define VF_MANY 4                   // tiles of a wave at a time, their loads in flight together
+#define VF_WAVES 16                 // of the workgroup that picks
+#define VF_SUM_WAVES 4
 
-struct VerifyState { double A, B, z; int cur, last, kept, ask; };      // ask: z is the sum that is to be made
+struct VerifyState { double A, B, z; int cur, last, kept, ask, buf, pad; };   // ask: z is the sum that is to be made; buf: which sums are w's
 struct VerifyArgs {
     const uint8_t *p, *q;
     long long ps, qs;
     const int *tok, *parent, *cu;
     const float *u, *r;
     int *path, *out, *n_path;
-    VerifyState *state;             // [B]
-    double *sums;                   // [B][tiles]
-    int T, V, tiles, second;
+    VerifyState *state;             // [2][B]
+    double *sums;                   // [2][B][tiles]
+    int B, T, V, tiles, round;      // round: launches of sums before this one
 };
 
 template <typename TY> __device__ __forceinline__ double vf_at(const uint8_t *row, long long i) {
@@ -160,14 +163,28 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs &a, TreeReq r, VerifySt
     s.ask = 0;
 }
 
-// w of 8 entries from v on: max(A p - B q, 0), or p where no rejected sibling has that token (`out`: bits of a tile's tokens)
+// w of 8 entries of p and q: max(A p - B q, 0), or p where no rejected sibling has that token (`gone`: a bit for each)
+template <bool DRAFT>
+__device__ __forceinline__ void vf_weigh(const VerifyState &s, const float (&x)[8], const float (&y)[8], uint32_t gone, double (&w)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+        const double px = x[e] > 0.f ? (double)x[e] : 0.0;
+        if (DRAFT) w[e] = fmax(s.A * px - s.B * (y[e] > 0.f ? (double)y[e] : 0.0), 0.0);
+        else w[e] = gone >> e & 1u ? 0.0 : px;
+    }
+}
+__device__ __forceinline__ double vf_add(const double (&w)[8]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); }
+// which of 8 tokens from `at` on (a multiple of 8) of a tile rejected siblings have
+template <bool DRAFT> __device__ __forceinline__ uint32_t vf_gone(const VerifyState &s, const uint32_t *bits, int at) {
+    return !DRAFT && s.B != 0.0 ? bits[at >> 5] >> (at & 31) & 0xFFu : 0u;
+}
+// 8 entries from v on, those past the row's end 0
 template <typename TY, bool DRAFT>
-__device__ __forceinline__ void vf_eight(const VerifyArgs &a, const uint8_t *p, const uint8_t *q, const VerifyState &s, const uint32_t *out, int at, int v,
+__device__ __forceinline__ void vf_eight(const VerifyArgs &a, const uint8_t *p, const uint8_t *q, const VerifyState &s, const uint32_t *bits, int at, int v,
                                          double (&w)[8]) {
     constexpr int E = sizeof(typename TY::elem);
-    float x[8], y[8];
-    const bool whole = v + 8 <= a.V;
-    if (whole) {
+    float x[8], y[8] = {};
+    if (v + 8 <= a.V) {
         qt_load8<TY, E>(p + (long long)v * E, x);
         if (DRAFT) qt_load8<TY, E>(q + (long long)v * E, y);
     } else {
@@ -177,14 +194,7 @@ __device__ __forceinline__ void vf_eight(const VerifyArgs &a, const uint8_t *p, 
             if (DRAFT) y[e] = v + e < a.V ? qt_load1<TY>(q + (long long)(v + e) * E) : 0.f;
         }
     }
-    uint32_t gone = 0;
-    if (!DRAFT && out) gone = out[at >> 5] >> (at & 31) & 0xFFu;       // at: a multiple of 8
-#pragma unroll
-    for (int e = 0; e < 8; e++) {
-        const double px = x[e] > 0.f ? (double)x[e] : 0.0;
-        if (DRAFT) w[e] = fmax(s.A * px - s.B * (y[e] > 0.f ? (double)y[e] : 0.0), 0.0);
-        else w[e] = gone >> e & 1u ? 0.0 : px;
-    }
+    vf_weigh<DRAFT>(s, x, y, vf_gone<DRAFT>(s, bits, at), w);
 }
 
 __device__ __forceinline__ double vf_wave_sum(double v) {
@@ -192,6 +202,7 @@ __device__ __forceinline__ double vf_wave_sum(double v) {
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
+__device__ __forceinline__ double lane_bcast_d(double v, int lane) { return __shfl(v, lane, 64); }
 __device__ __forceinline__ double vf_wave_scan(double v) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -202,202 +213,251 @@ __device__ __forceinline__ double vf_wave_scan(double v) {
     return v;
 }
 
-// The workgroup: marks a tile's tokens that rejected siblings have (certain drafts only).
+// A wave: marks a tile's tokens that rejected siblings have (certain drafts only).
 template <bool DRAFT>
-__device__ __forceinline__ const uint32_t *vf_marks(const VerifyArgs &a, TreeReq r, const VerifyState &s, int tile, uint32_t *bits) {
-    if (DRAFT || s.B == 0.0) return nullptr;
-    __syncthreads();
-    for (int i = threadIdx.x; i < VF_TILE / 32; i += VF_T) bits[i] = 0u;
-    __syncthreads();
-    for (int i = s.cur + 1 + threadIdx.x; i < r.n; i += VF_T)
+__device__ __forceinline__ void vf_marks(const VerifyArgs &a, TreeReq r, const VerifyState &s, int tile, uint32_t *bits) {
+    if (DRAFT || s.B == 0.0) return;
+    const int lane = threadIdx.x & 63;
+    __threadfence_block();                              // the words are the wave's own: its stores and atomics in their order
+    for (int i = lane; i < VF_TILE / 32; i += 64) bits[i] = 0u;
+    __threadfence_block();
+    for (int i = s.cur + 1 + lane; i < r.n; i += 64)
         if (a.parent[r.q0 + i] == s.cur) {
-            const int t = a.tok[r.q0 + i] - tile * VF_TILE;
-            if (a.tok[r.q0 + i] >= 0 && t >= 0 && t < VF_TILE) atomicOr(&bits[t >> 5], 1u << (t & 31));
+            const int x = a.tok[r.q0 + i], t = x - tile * VF_TILE;
+            if (x >= 0 && t >= 0 && t < VF_TILE) atomicOr(&bits[t >> 5], 1u << (t & 31));
         }
-    __syncthreads();
-    return bits;
+    __threadfence_block();
 }
 
-// The workgroup: a tile's sum, in every thread.
+// A wave: the sums of VF_MANY tiles from the first on, in every lane; a lane takes 8 entries of every 512.  Where all of them are in the row
+// their loads are in flight together.
+#define VF_PARTS (VF_TILE / 512)
 template <typename TY, bool DRAFT>
-__device__ __forceinline__ double vf_tile(const VerifyArgs &a, TreeReq r, const VerifyState &s, int tile, uint32_t *bits, double *part) {
-    constexpr int E = sizeof(typename TY::elem);
+__device__ __forceinline__ void vf_tiles(const VerifyArgs &a, TreeReq r, const VerifyState &s, int first, uint32_t *bits, double (&sum)[VF_MANY]) {
+    constexpr int E = sizeof(typename TY::elem), NW = E / 2, N = VF_MANY * VF_PARTS;
+    const int lane = threadIdx.x & 63, v0 = first * VF_TILE + 8 * lane;
     const uint8_t *p = a.p + (r.q0 + s.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + s.cur) * a.qs * E : nullptr;
-    const uint32_t *out = vf_marks<DRAFT>(a, r, s, tile, bits);
-    double sum = 0.0;
+    double part[N];
+    if ((first + VF_MANY) * VF_TILE <= a.V) {
+        qt_w4 x[N][NW], y[DRAFT ? N : 1][NW];
 #pragma unroll
-    for (int k = 0; k < VF_TILE / (8 * VF_T); k++) {
-        const int at = 8 * (k * VF_T + (int)threadIdx.x);
-        double w[8];
-        if (tile * VF_TILE + at < a.V) {
-            vf_eight<TY, DRAFT>(a, p, q, s, out, at, tile * VF_TILE + at, w);
-            sum += ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7]));
+        for (int k = 0; k < N; k++)
+#pragma unroll
+            for (int i = 0; i < NW; i++) {
+                x[k][i] = qt_load16<E>(p + (long long)(v0 + 512 * k) * E + 16 * i);
+                if (DRAFT) y[k][i] = qt_load16<E>(q + (long long)(v0 + 512 * k) * E + 16 * i);
+            }
+#pragma unroll
+        for (int t = 0; t < VF_MANY; t++) {
+            vf_marks<DRAFT>(a, r, s, first + t, bits);
+#pragma unroll
+            for (int k = VF_PARTS * t; k < VF_PARTS * (t + 1); k++) {
+                float fx[8], fy[8] = {};
+                double w[8];
+                qt_widen8<TY>(x[k], fx);
+                if constexpr (DRAFT) qt_widen8<TY>(y[k], fy);
+                vf_weigh<DRAFT>(s, fx, fy, vf_gone<DRAFT>(s, bits, 8 * lane + 512 * (k - VF_PARTS * t)), w);
+                part[k] = vf_add(w);
+            }
+        }
+    } else {
+        for (int t = 0; t < VF_MANY; t++) {
+            vf_marks<DRAFT>(a, r, s, first + t, bits);
+#pragma unroll
+            for (int k = 0; k < VF_PARTS; k++) {
+                const int at = 8 * lane + 512 * k, v = (first + t) * VF_TILE + at;
+                double w[8], x = 0.0;
+                if (v < a.V) {
+                    vf_eight<TY, DRAFT>(a, p, q, s, bits, at, v, w);
+                    x = vf_add(w);
+                }
+#pragma unroll
+                for (int u = 0; u < VF_MANY; u++)
+                    if (u == t) part[VF_PARTS * u + k] = x;
+            }
         }
     }
-    sum = vf_wave_sum(sum);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = sum;
-    __syncthreads();
-    sum = 0.0;
 #pragma unroll
-    for (int w = 0; w < VF_T / 64; w++) sum += part[w];
-    return sum;
+    for (int t = 0; t < VF_MANY; t++) {
+        double x = 0.0;
+#pragma unroll
+        for (int k = 0; k < VF_PARTS; k++) x += part[VF_PARTS * t + k];
+        sum[t] = vf_wave_sum(x);
+    }
 }
+// A wave: the sum of the tiles' sums.
+template <typename P> __device__ __forceinline__ double vf_total(P sums, int tiles) {
+    const int lane = threadIdx.x & 63, per = (tiles + 63) / 64, t1 = min((lane + 1) * per, tiles);
+    double x = 0.0;
+    for (int t = lane * per; t < t1; t++) x += sums[t];
+    return vf_wave_sum(x);
+}
+__device__ __forceinline__ bool vf_same(const VerifyState &x, const VerifyState &y) { return x.A == y.A && x.B == y.B && x.cur == y.cur; }
 
 template <typename TY, bool DRAFT>
-__global__ __launch_bounds__(VF_T) void k_tree_sums(VerifyArgs a) {
+__global__ __launch_bounds__(64 * VF_SUM_WAVES) void k_tree_sums(VerifyArgs a) {
     __shared__ VerifyState s;
-    __shared__ uint32_t bits[VF_TILE / 32];
-    __shared__ double part[VF_T / 64];
-    const int b = blockIdx.y, tile = blockIdx.x;
+    __shared__ uint32_t bits[VF_SUM_WAVES][VF_TILE / 32];
+    __shared__ int more;
+    const int b = blockIdx.y, wave = threadIdx.x >> 6, tile = (blockIdx.x * VF_SUM_WAVES + wave) * VF_MANY, now = a.round & 1;
+    const bool first = blockIdx.x == 0;                 // writes what the request's workgroups all find
     const TreeReq r = tree_req(a.cu, b, a.T);
     if (r.n == 0) return;
-    if (threadIdx.x < 64) {
-        VerifyState w = {1.0, 0.0, 1.0, 0, 0, 1, 0};
-        vf_walk<TY, DRAFT>(a, r, w, tile == 0);
+    if (wave == 0) {
+        VerifyState w = {1.0, 0.0, 1.0, 0, 0, 1, 0, 0, 0};
+        bool make = true;
+        if (a.round > 0) {
+            w = a.state[(size_t)(now ^ 1) * a.B + b];
+            make = w.ask;
+            if (make) {
+                const VerifyState before = w;
+                w.z = vf_total(a.sums + ((size_t)w.buf * a.B + b) * a.tiles, a.tiles);
+                w.ask = 0;
+                vf_walk<TY, DRAFT>(a, r, w, first);
+                make = !vf_same(w, before);
+            }
+        } else {
+            vf_walk<TY, DRAFT>(a, r, w, first);
+        }
+        if (make) w.buf = now;
         if (threadIdx.x == 0) {
             s = w;
-            if (tile == 0) a.state[b] = w;
+            more = make;
+            if (first) a.state[(size_t)now * a.B + b] = w;
         }
     }
     __syncthreads();
-    const double sum = vf_tile<TY, DRAFT>(a, r, s, tile, bits, part);
-    if (threadIdx.x == 0) a.sums[(long long)b * a.tiles + tile] = sum;
+    if (!more || tile >= a.tiles) return;
+    const VerifyState mine = s;
+    double sum[VF_MANY];
+    vf_tiles<TY, DRAFT>(a, r, mine, tile, bits[wave], sum);
+#pragma unroll
+    for (int t = 0; t < VF_MANY; t++)
+        if (tile + t < a.tiles && (threadIdx.x & 63) == t) a.sums[((size_t)now * a.B + b) * a.tiles + tile + t] = sum[t];
 }
 
 template <typename TY, bool DRAFT>
-__global__ __launch_bounds__(VF_T) void k_tree_pick(VerifyArgs a) {
-    constexpr int E = sizeof(typename TY::elem);
+__global__ __launch_bounds__(64 * VF_WAVES) void k_tree_pick(VerifyArgs a) {
     __shared__ VerifyState s;
-    __shared__ uint32_t bits[VF_TILE / 32];
-    __shared__ double part[VF_T / 64], total_s, before_s;
-    __shared__ int tile_s, token_s;
-    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    __shared__ uint32_t bits[VF_WAVES][VF_TILE / 32];
+    __shared__ double sums[VF_MAX_V / VF_TILE];
+    __shared__ int state_s;                             // 0: the sums are to be made, 1: they are, 2: and no more are asked for
+    __shared__ double total_s;
+    const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const TreeReq r = tree_req(a.cu, b, a.T);
     if (r.n == 0) {
         if (threadIdx.x == 0) a.n_path[b] = 0;
         return;
     }
-    double *sums = a.sums + (long long)b * a.tiles;
-    bool made = a.second != 0;                          // the tiles' sums are those of s
-    if (threadIdx.x < 64) {
-        VerifyState w = {1.0, 0.0, 1.0, 0, 0, 1, 0};
-        if (made) w = a.state[b];
+    if (wave == 0) {
+        VerifyState w = {1.0, 0.0, 1.0, 0, 0, 1, 0, 0, 0};
+        if (a.round > 0) w = a.state[(size_t)((a.round - 1) & 1) * a.B + b];
         else vf_walk<TY, DRAFT>(a, r, w, true);
-        if (threadIdx.x == 0) s = w;
+        if (lane == 0) { s = w; state_s = a.round > 0; }
     }
     __syncthreads();
-    const auto total = [&] {                            // the tiles' sum, in their order within a lane's share
-        if (threadIdx.x < 64) {
-            const int per = (a.tiles + 63) / 64, t1 = min((lane + 1) * per, a.tiles);
-            double x = 0.0;
-            for (int t = lane * per; t < t1; t++) x += sums[t];
-            x = vf_wave_sum(x);
-            if (lane == 0) total_s = x;
-        }
+    if (a.round > 0) {
+        const double *from = a.sums + ((size_t)s.buf * a.B + b) * a.tiles;
+        for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) sums[t] = from[t];
+    }
+    for (bool again = false;;) {                        // a sum for each rejected child at most, and one more
+        const bool make = state_s == 0;
         __syncthreads();
-    };
-    const auto make = [&] {
-        for (int t = 0; t < a.tiles; t++) {
-            const double x = vf_tile<TY, DRAFT>(a, r, s, t, bits, part);
-            if (threadIdx.x == 0) sums[t] = x;
-        }
-        __syncthreads();
-    };
-    for (;;) {                                          // at most one round for each of the request's tokens
-        if (!made) make();
-        total();
-        if (!s.ask) break;
-        __syncthreads();
-        if (threadIdx.x < 64) {
-            VerifyState w = s;
-            w.z = total_s;
-            w.ask = 0;
-            vf_walk<TY, DRAFT>(a, r, w, true);
-            if (threadIdx.x == 0) {
-                part[0] = w.A != s.A || w.B != s.B || w.cur != s.cur ? 1.0 : 0.0;
-                s = w;
+        if (make) {
+            const VerifyState mine = s;
+            for (int t = wave * VF_MANY; t < a.tiles; t += waves * VF_MANY) {
+                double sum[VF_MANY];
+                vf_tiles<TY, DRAFT>(a, r, mine, t, bits[wave], sum);
+#pragma unroll
+                for (int u = 0; u < VF_MANY; u++)
+                    if (t + u < a.tiles && lane == u) sums[t + u] = sum[u];
             }
+            __syncthreads();
+        }
+        if (wave == 0) {
+            VerifyState w = s;
+            const double z = vf_total(sums, a.tiles);
+            int next = 2;
+            if (s.ask) {
+                w.z = z;
+                w.ask = 0;
+                vf_walk<TY, DRAFT>(a, r, w, true);
+                next = !vf_same(w, s) ? 0 : w.ask ? 1 : 2;
+            }
+            if (next == 2 && !(z > 0.0) && !again) {    // nothing is left: p's row as it is
+                again = true;
+                w.A = 1.0; w.B = 0.0;
+                next = 0;
+            }
+            if (lane == 0) { s = w; state_s = next; total_s = z; }
         }
         __syncthreads();
-        made = part[0] == 0.0;
-        __syncthreads();
+        if (state_s == 2) break;
     }
-    if (!(total_s > 0.0)) {                             // nothing is left: p's row as it is
-        __syncthreads();
-        if (threadIdx.x == 0) { s.A = 1.0; s.B = 0.0; }
-        __syncthreads();
-        make();
-        total();
-    }
-    const double goal = (double)a.r[b] * total_s;
-    if (threadIdx.x == 0) {
-        double x = 0.0;
-        int t = 0, last = -1;
-        double last_before = 0.0;
-        for (; t < a.tiles; t++) {
+    if (wave == 0) {
+        // the first tile whose sum takes the running sum past the goal, or else the last one that is not 0 (sums that rounding
+        // leaves just under it); then the first of its entries in the same way
+        const double goal = (double)a.r[b] * total_s;
+        const int per = (a.tiles + 63) / 64, t0 = min(lane * per, a.tiles), t1 = min(t0 + per, a.tiles);
+        double mine = 0.0;
+        for (int t = t0; t < t1; t++) mine += sums[t];
+        const double upto = vf_wave_scan(mine), lower = __shfl_up(upto, 1, 64);
+        double x = lane ? lower : 0.0;
+        int tile = -1, some = -1;
+        double x_tile = 0.0, x_some = 0.0;
+        for (int t = t0; t < t1; t++) {
             const double y = sums[t];
-            if (y > 0.0) { last = t; last_before = x; }
-            if (x + y > goal) break;
+            if (y > 0.0) { some = t; x_some = x; }
+            if (tile < 0 && y > 0.0 && x + y > goal) { tile = t; x_tile = x; }
             x += y;
         }
-        tile_s = t < a.tiles ? t : last;                // (sums that rounding leaves just under the goal)
-        before_s = t < a.tiles ? x : last_before;
-        token_s = -1;
-    }
-    __syncthreads();
-    if (tile_s >= 0) {
-        const int tile = tile_s;
-        const uint8_t *p = a.p + (r.q0 + s.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + s.cur) * a.qs * E : nullptr;
-        const uint32_t *out = vf_marks<DRAFT>(a, r, s, tile, bits);
-        double before = before_s;
-        int found = 0x7FFFFFFF, any = -1;               // the first entry past the goal, and the last one that is not 0
-        for (int k = 0; k < VF_TILE / (8 * VF_T); k++) {
-            const int at = 8 * (k * VF_T + (int)threadIdx.x), v = tile * VF_TILE + at;
-            double w[8], mine = 0.0;
-            if (v < a.V) {
-                vf_eight<TY, DRAFT>(a, p, q, s, out, at, v, w);
+        int token = -1;
+        unsigned long long who = __ballot(tile >= 0);
+        int from = who ? __ffsll(who) - 1 : -1;
+        if (!who && (who = __ballot(some >= 0))) { from = 63 - __clzll((long long)who); tile = some; x_tile = x_some; }
+        if (from >= 0) {
+            tile = __builtin_amdgcn_readlane(tile, from);
+            double before = __shfl(x_tile, from);
+            constexpr int E = sizeof(typename TY::elem);
+            const VerifyState w = s;
+            const uint8_t *p = a.p + (r.q0 + w.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + w.cur) * a.qs * E : nullptr;
+            vf_marks<DRAFT>(a, r, w, tile, bits[0]);
+            double e8[VF_PARTS][8];
 #pragma unroll
-                for (int e = 0; e < 8; e++) mine += w[e];
-            }
-            const double upto = vf_wave_scan(mine);
-            __syncthreads();
-            if (lane == 63) part[wave] = upto;
-            __syncthreads();
-            double x = before;
+            for (int k = 0; k < VF_PARTS; k++) {
+                const int in = 8 * lane + 512 * k, v = tile * VF_TILE + in;
 #pragma unroll
-            for (int o = 0; o < VF_T / 64; o++) {
-                if (o < wave) x += part[o];
-                before += part[o];
+                for (int e = 0; e < 8; e++) e8[k][e] = 0.0;
+                if (v < a.V) vf_eight<TY, DRAFT>(a, p, q, w, bits[0], in, v, e8[k]);
             }
-            const double lower = __shfl_up(upto, 1, 64);
-            if (lane > 0) x += lower;
-            if (v < a.V)
+            int found = -1, any = -1;                   // the wave's
+#pragma unroll
+            for (int k = 0; k < VF_PARTS; k++) {
+                const double scan = vf_wave_scan(vf_add(e8[k])), below = __shfl_up(scan, 1, 64);
+                double y = before + (lane ? below : 0.0);
+                int f = -1, last = -1;
 #pragma unroll
                 for (int e = 0; e < 8; e++) {
-                    x += w[e];
-                    if (w[e] > 0.0) any = v + e;
-                    if (w[e] > 0.0 && x > goal) found = min(found, v + e);
+                    y += e8[k][e];
+                    if (e8[k][e] > 0.0) {
+                        last = tile * VF_TILE + 8 * lane + 512 * k + e;
+                        if (f < 0 && y > goal) f = last;
+                    }
                 }
+                const unsigned long long fs = __ballot(f >= 0), ls = __ballot(last >= 0);
+                if (found < 0 && fs) found = __builtin_amdgcn_readlane(f, __ffsll(fs) - 1);
+                if (ls) any = __builtin_amdgcn_readlane(last, 63 - __clzll((long long)ls));
+                before += lane_bcast_d(scan, 63);
+            }
+            token = found >= 0 ? found : any;
         }
-        // over the workgroup: the least `found`, else the greatest `any`
-#pragma unroll
-        for (int o = 32; o; o >>= 1) { found = min(found, __shfl_xor(found, o, 64)); any = max(any, __shfl_xor(any, o, 64)); }
-        __shared__ int ends[2][VF_T / 64];
-        if (lane == 0) { ends[0][wave] = found; ends[1][wave] = any; }
-        __syncthreads();
-        if (threadIdx.x == 0) {
-            for (int o = 1; o < VF_T / 64; o++) { found = min(found, ends[0][o]); any = max(any, ends[1][o]); }
-            token_s = found != 0x7FFFFFFF ? found : any;
+        if (lane == 0) {
+            a.path[r.q0] = 0;
+            a.out[r.q0 + s.kept - 1] = token;
+            a.n_path[b] = s.kept;
         }
     }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-        a.path[r.q0] = 0;
-        a.out[r.q0 + s.kept - 1] = token_s;
-        a.n_path[b] = s.kept;
-    }
-    for (int k = s.kept + threadIdx.x; k < r.n; k += VF_T) a.path[r.q0 + k] = a.out[r.q0 + k] = -1;
+    for (int k = s.kept + threadIdx.x; k < r.n; k += blockDim.x) a.path[r.q0 + k] = a.out[r.q0 + k] = -1;
 }
 
 static int verify_args(const qwen_hip_tree_verify_t *p, VerifyArgs &a) {
@@ -405,28 +465,32 @@ static int verify_args(const qwen_hip_tree_verify_t *p, VerifyArgs &a) {
     QT_REFUSE(!qt_dt_size(p->dtype), "tree_verify: dtype %d (f32, bf16 or f16)", p->dtype);
     QT_REFUSE(p->B < 0 || p->B > 65535, "tree_verify: B %d out of range (0..65535)", p->B);
     QT_REFUSE(p->T < 0 || p->T > 1 << 26, "tree_verify: T %d out of range (0..2^26)", p->T);
-    QT_REFUSE(p->V < 1 || p->V > 1 << 24, "tree_verify: V %d out of range (1..2^24)", p->V);
+    QT_REFUSE(p->V < 1 || p->V > VF_MAX_V, "tree_verify: V %d out of range (1..2^20)", p->V);
     QT_REFUSE(p->max_children < 0, "tree_verify: max_children %d is negative", p->max_children);
     a = VerifyArgs{};
-    a.T = p->T; a.V = p->V;
+    a.B = p->B; a.T = p->T; a.V = p->V;
     a.tiles = (p->V + VF_TILE - 1) / VF_TILE;
     return 0;
 }
-static long long verify_bytes(const VerifyArgs &a, int B) { return (long long)B * (sizeof(VerifyState) + 8ll * a.tiles); }
+static long long verify_bytes(const VerifyArgs &a) { return 2ll * a.B * (sizeof(VerifyState) + 8ll * a.tiles); }
 
 extern "C" long long qwen_hip_op_tree_verify_workspace(const qwen_hip_tree_verify_t *p) {
     VerifyArgs a;
     if (verify_args(p, a)) return -1;
-    return verify_bytes(a, p->B);
+    return verify_bytes(a);
 }
 
-template <typename TY, bool DRAFT> static hipError_t verify_launch(VerifyArgs a, int B, hipStream_t st) {
+// Launches of sums before the one that picks.
+static int verify_rounds(const VerifyArgs &a, bool draft, int max_children) {
+    if (a.tiles <= VF_WAVES * VF_MANY) return 0;
+    return draft && max_children != 1 ? 3 : 1;
+}
+static int vf_waves(int tiles) { return tiles < VF_WAVES * VF_MANY ? (tiles + VF_MANY - 1) / VF_MANY : VF_WAVES; }
+template <typename TY, bool DRAFT> static hipError_t verify_launch(VerifyArgs a, int rounds, hipStream_t st) {
     hipError_t e = hipSuccess;
-    if (a.tiles > VF_ONE) {
-        e = qt_launch(k_tree_sums<TY, DRAFT>, dim3(a.tiles, B), dim3(VF_T), 0, st, a);
-        a.second = 1;
-    }
-    if (e == hipSuccess) e = qt_launch(k_tree_pick<TY, DRAFT>, dim3(B), dim3(VF_T), 0, st, a);
+    for (; a.round < rounds && e == hipSuccess; a.round++)
+        e = qt_launch(k_tree_sums<TY, DRAFT>, dim3((a.tiles + VF_SUM_WAVES * VF_MANY - 1) / (VF_SUM_WAVES * VF_MANY), a.B), dim3(64 * VF_SUM_WAVES), 0, st, a);
+    if (e == hipSuccess) e = qt_launch(k_tree_pick<TY, DRAFT>, dim3(a.B), dim3(64 * vf_waves(a.tiles)), 0, st, a);
     return e;
 }
 
@@ -439,7 +503,7 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
     const int E = qt_dt_size(p->dtype);
     QT_REFUSE((uintptr_t)p->p % E || (uintptr_t)p->q % E, "tree_verify: p and q have to be aligned to their elements");
     QT_REFUSE(p->p_stride < p->V || (p->q && p->q_stride < p->V), "tree_verify: strides %lld, %lld under %d entries", p->p_stride, p->q_stride, p->V);
-    const long long need = verify_bytes(a, p->B);
+    const long long need = verify_bytes(a);
     QT_REFUSE(!p->workspace || p->workspace_bytes < need, "tree_verify: a workspace of %lld bytes is needed, %lld given", need,
               p->workspace ? p->workspace_bytes : 0ll);
     QT_REFUSE(qt_off16(p->workspace), "tree_verify: the workspace has to be aligned to 16 bytes");
@@ -451,8 +515,9 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
     a.tok = p->tok; a.parent = p->parent; a.cu = p->cu_q; a.u = p->u; a.r = p->r;
     a.path = p->path; a.out = p->out_tok; a.n_path = p->n_path;
     a.state = (VerifyState *)p->workspace;
-    a.sums = (double *)(a.state + p->B);
-#define VERIFY(TY) (p->q ? verify_launch<TY, true>(a, p->B, st) : verify_launch<TY, false>(a, p->B, st))
+    a.sums = (double *)(a.state + 2ll * p->B);
+    const int rounds = verify_rounds(a, p->q != nullptr, p->max_children);
+#define VERIFY(TY) (p->q ? verify_launch<TY, true>(a, rounds, st) : verify_launch<TY, false>(a, rounds, st))
     const hipError_t e = p->dtype == QWEN_HIP_DT_F32 ? VERIFY(QtF32) : p->dtype == QWEN_HIP_DT_BF16 ? VERIFY(QtBf16) : VERIFY(QtF16);
 #undef VERIFY
     QT_REFUSE(e != hipSuccess, "tree_verify: launch failed: %s", hipGetErrorString(e));

@@ -109,7 +109,7 @@ def verify(**kw):
 @pytest.mark.parametrize("kw,word", [
     *[(({n: None}), "null") for n in ("p", "tok", "parent", "cu_q", "u", "r", "path", "out_tok", "n_path")],
     (dict(dtype=3), "dtype"), (dict(dtype=hip.E4M3), "dtype"), (dict(B=-1), "B -1"), (dict(B=65536), "B 65536"), (dict(T=-1), "T -1"), (dict(V=0), "V 0"),
-    (dict(V=(1 << 24) + 1), "V 16777217"), (dict(p=P + 1), "aligned"), (dict(q=P + 1), "aligned"), (dict(p_stride=999), "strides"), (dict(q_stride=999), "strides"),
+    (dict(V=(1 << 20) + 1, p_stride=1 << 21, q_stride=1 << 21), "V 1048577"), (dict(p=P + 1), "aligned"), (dict(q=P + 1), "aligned"), (dict(p_stride=999), "strides"), (dict(q_stride=999), "strides"),
     (dict(workspace=None), "workspace"), (dict(workspace_bytes=8), "workspace"), (dict(workspace=P + 8), "aligned"), (dict(max_children=-1), "max_children")])
 def test_tree_verify_refuses(kw, word):
     refused(hip.lib().qwen_hip_op_tree_verify(C.byref(verify(**kw)), None), word)
