@@ -1,6 +1,7 @@
 // qt_tree.hip — trees of drafted tokens: a step's positions and masks (qwen_hip_op_tree_plan), verification against the
 // target's probabilities (qwen_hip_op_tree_verify), and what is kept of the step (qwen_hip_op_tree_commit).
 #include "qt_ops.h"
+#include <type_traits>
 
 #define TREE_MAX_LEN (1 << 30)
 
@@ -73,15 +74,15 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
 // z <- sum w.  After rejections w is max(A p - B q, 0) with two numbers: A, B -> A / z, B / z + 1 (a token whose w
 // has become 0 stays at 0).  So the walk needs each token's p and q at its parent's row, gathered once for 64 tokens, and a pass over the
 // vocabulary only where a sum is asked for: by a further child after a rejection, and by the next token at the end.
-// The pass sums tiles of 1024 entries, four a wave; the next token's tile is found in the tiles' sums, the token by a scan of its tile.
+// The pass sums tiles of 1024 entries, two a wave; the next token's tile is found in the tiles' sums, the token by a scan of its tile.
 // All in f64: an f32 sum over a vocabulary would move the border between two tokens by more than some tokens have.
 //
-// Large vocabularies: launches of a wave for four tiles, the first of which walks to the first sum (every workgroup for itself: a few
+// Large vocabularies: launches of a wave for two tiles, the first of which walks to the first sum (every workgroup for itself: a few
 // dependent loads), the others from the sum before to the next where there is one; then a launch of a workgroup a request, which goes on
 // from there, makes further sums itself, and picks.
 #define VF_TILE 1024
 #define VF_MAX_V (1 << 20)
-#define VF_MANY 4                   // tiles of a wave at a time, their loads in flight together
+#define VF_MANY 2                   // tiles of a wave at a time, their loads in flight together
 #define VF_WAVES 16                 // of the workgroup that picks
 #define VF_SUM_WAVES 4
 
@@ -100,6 +101,13 @@ struct VerifyArgs {
 template <typename TY> __device__ __forceinline__ double vf_at(const uint8_t *row, long long i) {
     const float x = qt_load1<TY>(row + i * (long long)sizeof(typename TY::elem));
     return x > 0.f ? (double)x : 0.0;
+}
+
+// lane `l`'s value (l uniform)
+__device__ __forceinline__ double vf_lane(double v, int l) {
+    const long long u = __builtin_bit_cast(long long, v);
+    const unsigned lo = __builtin_amdgcn_readlane((int)u, l), hi = __builtin_amdgcn_readlane((int)(u >> 32), l);
+    return __builtin_bit_cast(double, (long long)((unsigned long long)hi << 32 | lo));
 }
 
 // A wave: goes on from s to the next sum that is asked for (s.ask = 1) or to the last kept token (0).  `put`: writes what is kept.
@@ -128,7 +136,7 @@ __device__ __forceinline__ void vf_walk(const VerifyArgs &a, TreeReq r, VerifySt
             if (!kids) break;
             const int c = __ffsll(kids) - 1, id = base + c, cx = __builtin_amdgcn_readlane(x, c);
             if (s.ask) return;                                          // (after a rejection, and only if another child comes)
-            const double cp = __shfl(px, c), cq = __shfl(qx, c);
+            const double cp = vf_lane(px, c), cq = vf_lane(qx, c);
             const float cu = lane_bcast(u, c);
             double w;
             if (DRAFT) {
@@ -174,35 +182,67 @@ __device__ __forceinline__ void vf_weigh(const VerifyState &s, const float (&x)[
     }
 }
 __device__ __forceinline__ double vf_add(const double (&w)[8]) { return ((w[0] + w[1]) + (w[2] + w[3])) + ((w[4] + w[5]) + (w[6] + w[7])); }
-// which of 8 tokens from `at` on (a multiple of 8) of a tile rejected siblings have
-template <bool DRAFT> __device__ __forceinline__ uint32_t vf_gone(const VerifyState &s, const uint32_t *bits, int at) {
-    return !DRAFT && s.B != 0.0 ? bits[at >> 5] >> (at & 31) & 0xFFu : 0u;
-}
-// 8 entries from v on, those past the row's end 0
-template <typename TY, bool DRAFT>
-__device__ __forceinline__ void vf_eight(const VerifyArgs &a, const uint8_t *p, const uint8_t *q, const VerifyState &s, const uint32_t *bits, int at, int v,
-                                         double (&w)[8]) {
-    constexpr int E = sizeof(typename TY::elem);
-    float x[8], y[8] = {};
-    if (v + 8 <= a.V) {
-        qt_load8<TY, E>(p + (long long)v * E, x);
-        if (DRAFT) qt_load8<TY, E>(q + (long long)v * E, y);
-    } else {
+// Entries v .. v + 7 of a row.  A lane whose eight pass the row's end loads the row's last eight instead, `skip` of which come before v: those
+// are 0, and so is everything past the end.
+template <typename TY, bool DRAFT> struct VfEight {
+    static constexpr int E = sizeof(typename TY::elem), NW = E / 2;
+    qt_w4 x[NW], y[DRAFT ? NW : 1];
+    __device__ __forceinline__ static int base(const VerifyArgs &a, int v) { return min(v, max(a.V - 8, 0)); }
+    __device__ __forceinline__ void load(const VerifyArgs &a, const uint8_t *p, const uint8_t *q, int v) {
+        const long long at = (long long)base(a, v) * E;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            x[e] = v + e < a.V ? qt_load1<TY>(p + (long long)(v + e) * E) : 0.f;
-            if (DRAFT) y[e] = v + e < a.V ? qt_load1<TY>(q + (long long)(v + e) * E) : 0.f;
+        for (int i = 0; i < NW; i++) {
+            x[i] = qt_load16<E>(p + at + 16 * i);
+            if (DRAFT) y[i] = qt_load16<E>(q + at + 16 * i);
         }
     }
-    vf_weigh<DRAFT>(s, x, y, vf_gone<DRAFT>(s, bits, at), w);
-}
+    // of a row that has no eight
+    __device__ __forceinline__ void load_few(const VerifyArgs &a, const uint8_t *p, const uint8_t *q) {
+        typename TY::elem ex[8] = {}, ey[8] = {};
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            if (e < a.V) ex[e] = reinterpret_cast<const typename TY::elem *>(p)[e];
+            if (DRAFT && e < a.V) ey[e] = reinterpret_cast<const typename TY::elem *>(q)[e];
+        }
+        __builtin_memcpy(x, ex, sizeof ex);
+        if (DRAFT) __builtin_memcpy(y, ey, sizeof ey);
+    }
+    template <int N> __device__ __forceinline__ static void load_all(VfEight (&x)[N], const VerifyArgs &a, const uint8_t *p, const uint8_t *q, int v0) {
+        if (a.V < 8) {
+#pragma unroll
+            for (int k = 0; k < N; k++) x[k].load_few(a, p, q);
+        } else {
+#pragma unroll
+            for (int k = 0; k < N; k++) x[k].load(a, p, q, v0 + 512 * k);
+        }
+    }
+    // their w; bits: those of the tile's tokens that rejected siblings have, the tile beginning at v0
+    __device__ __forceinline__ void weigh(const VerifyArgs &a, const VerifyState &s, const uint32_t *bits, int v0, int v, double (&w)[8]) const {
+        float fx[8], fy[8] = {};
+        qt_widen8<TY>(x, fx);
+        if constexpr (DRAFT) qt_widen8<TY>(y, fy);
+        const int skip = v - base(a, v), at = v - v0;
+        uint32_t gone = 0;
+        if (!DRAFT && s.B != 0.0) {
+            gone = bits[at >> 5] >> (at & 31) & 0xFFu;                 // at: a multiple of 8
+            gone = skip < 8 ? gone << skip : 0u;
+        }
+        if (skip > 0) {
+#pragma unroll
+            for (int e = 0; e < 8; e++)
+                if (e < skip) fx[e] = 0.f;
+        }
+        vf_weigh<DRAFT>(s, fx, fy, gone, w);
+    }
+    // the entry that w[e] is of
+    __device__ __forceinline__ static int entry(const VerifyArgs &a, int v, int e) { return base(a, v) + e; }
+};
 
 __device__ __forceinline__ double vf_wave_sum(double v) {
 #pragma unroll
     for (int o = 32; o; o >>= 1) v += __shfl_xor(v, o, 64);
     return v;
 }
-__device__ __forceinline__ double lane_bcast_d(double v, int lane) { return __shfl(v, lane, 64); }
 __device__ __forceinline__ double vf_wave_scan(double v) {
     const int lane = threadIdx.x & 63;
 #pragma unroll
@@ -229,60 +269,27 @@ __device__ __forceinline__ void vf_marks(const VerifyArgs &a, TreeReq r, const V
     __threadfence_block();
 }
 
-// A wave: the sums of VF_MANY tiles from the first on, in every lane; a lane takes 8 entries of every 512.  Where all of them are in the row
-// their loads are in flight together.
+// A wave: the sums of N tiles from the first on, in every lane; a lane takes 8 entries of every 512, all loads in flight together.
 #define VF_PARTS (VF_TILE / 512)
-template <typename TY, bool DRAFT>
-__device__ __forceinline__ void vf_tiles(const VerifyArgs &a, TreeReq r, const VerifyState &s, int first, uint32_t *bits, double (&sum)[VF_MANY]) {
-    constexpr int E = sizeof(typename TY::elem), NW = E / 2, N = VF_MANY * VF_PARTS;
-    const int lane = threadIdx.x & 63, v0 = first * VF_TILE + 8 * lane;
+template <typename TY, bool DRAFT, int N>
+__device__ __forceinline__ void vf_tiles(const VerifyArgs &a, TreeReq r, const VerifyState &s, int first, uint32_t *bits, double (&sum)[N]) {
+    constexpr int E = sizeof(typename TY::elem);
+    const int lane = threadIdx.x & 63;
     const uint8_t *p = a.p + (r.q0 + s.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + s.cur) * a.qs * E : nullptr;
-    double part[N];
-    if ((first + VF_MANY) * VF_TILE <= a.V) {
-        qt_w4 x[N][NW], y[DRAFT ? N : 1][NW];
+    VfEight<TY, DRAFT> x[N * VF_PARTS];
+    const int v0 = first * VF_TILE + 8 * lane;
+    VfEight<TY, DRAFT>::load_all(x, a, p, q, v0);
 #pragma unroll
-        for (int k = 0; k < N; k++)
+    for (int t = 0; t < N; t++) {
+        vf_marks<DRAFT>(a, r, s, first + t, bits);
+        double y = 0.0;
 #pragma unroll
-            for (int i = 0; i < NW; i++) {
-                x[k][i] = qt_load16<E>(p + (long long)(v0 + 512 * k) * E + 16 * i);
-                if (DRAFT) y[k][i] = qt_load16<E>(q + (long long)(v0 + 512 * k) * E + 16 * i);
-            }
-#pragma unroll
-        for (int t = 0; t < VF_MANY; t++) {
-            vf_marks<DRAFT>(a, r, s, first + t, bits);
-#pragma unroll
-            for (int k = VF_PARTS * t; k < VF_PARTS * (t + 1); k++) {
-                float fx[8], fy[8] = {};
-                double w[8];
-                qt_widen8<TY>(x[k], fx);
-                if constexpr (DRAFT) qt_widen8<TY>(y[k], fy);
-                vf_weigh<DRAFT>(s, fx, fy, vf_gone<DRAFT>(s, bits, 8 * lane + 512 * (k - VF_PARTS * t)), w);
-                part[k] = vf_add(w);
-            }
+        for (int k = 0; k < VF_PARTS; k++) {
+            double w[8];
+            x[VF_PARTS * t + k].weigh(a, s, bits, (first + t) * VF_TILE, v0 + 512 * (VF_PARTS * t + k), w);
+            y += vf_add(w);
         }
-    } else {
-        for (int t = 0; t < VF_MANY; t++) {
-            vf_marks<DRAFT>(a, r, s, first + t, bits);
-#pragma unroll
-            for (int k = 0; k < VF_PARTS; k++) {
-                const int at = 8 * lane + 512 * k, v = (first + t) * VF_TILE + at;
-                double w[8], x = 0.0;
-                if (v < a.V) {
-                    vf_eight<TY, DRAFT>(a, p, q, s, bits, at, v, w);
-                    x = vf_add(w);
-                }
-#pragma unroll
-                for (int u = 0; u < VF_MANY; u++)
-                    if (u == t) part[VF_PARTS * u + k] = x;
-            }
-        }
-    }
-#pragma unroll
-    for (int t = 0; t < VF_MANY; t++) {
-        double x = 0.0;
-#pragma unroll
-        for (int k = 0; k < VF_PARTS; k++) x += part[VF_PARTS * t + k];
-        sum[t] = vf_wave_sum(x);
+        sum[t] = vf_wave_sum(y);
     }
 }
 // A wave: the sum of the tiles' sums.
@@ -330,7 +337,7 @@ __global__ __launch_bounds__(64 * VF_SUM_WAVES) void k_tree_sums(VerifyArgs a) {
     if (!more || tile >= a.tiles) return;
     const VerifyState mine = s;
     double sum[VF_MANY];
-    vf_tiles<TY, DRAFT>(a, r, mine, tile, bits[wave], sum);
+    vf_tiles<TY, DRAFT, VF_MANY>(a, r, mine, tile, bits[wave], sum);
 #pragma unroll
     for (int t = 0; t < VF_MANY; t++)
         if (tile + t < a.tiles && (threadIdx.x & 63) == t) a.sums[((size_t)now * a.B + b) * a.tiles + tile + t] = sum[t];
@@ -343,6 +350,7 @@ __global__ __launch_bounds__(64 * VF_WAVES) void k_tree_pick(VerifyArgs a) {
     __shared__ double sums[VF_MAX_V / VF_TILE];
     __shared__ int state_s;                             // 0: the sums are to be made, 1: they are, 2: and no more are asked for
     __shared__ double total_s;
+    constexpr int E = sizeof(typename TY::elem);
     const int b = blockIdx.x, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, waves = blockDim.x >> 6;
     const TreeReq r = tree_req(a.cu, b, a.T);
     if (r.n == 0) {
@@ -361,17 +369,22 @@ __global__ __launch_bounds__(64 * VF_WAVES) void k_tree_pick(VerifyArgs a) {
         for (int t = threadIdx.x; t < a.tiles; t += blockDim.x) sums[t] = from[t];
     }
     for (bool again = false;;) {                        // a sum for each rejected child at most, and one more
-        const bool make = state_s == 0;
+        const bool none = state_s == 0;
         __syncthreads();
-        if (make) {
+        if (none) {
             const VerifyState mine = s;
-            for (int t = wave * VF_MANY; t < a.tiles; t += waves * VF_MANY) {
-                double sum[VF_MANY];
-                vf_tiles<TY, DRAFT>(a, r, mine, t, bits[wave], sum);
+            const auto make = [&](auto n) {             // n tiles at a time
+                constexpr int N = decltype(n)::value;
+                for (int t = wave * N; t < a.tiles; t += waves * N) {
+                    double sum[N];
+                    vf_tiles<TY, DRAFT, N>(a, r, mine, t, bits[wave], sum);
 #pragma unroll
-                for (int u = 0; u < VF_MANY; u++)
-                    if (t + u < a.tiles && lane == u) sums[t + u] = sum[u];
-            }
+                    for (int u = 0; u < N; u++)
+                        if (t + u < a.tiles && lane == u) sums[t + u] = sum[u];
+                }
+            };
+            if (a.tiles <= waves) make(std::integral_constant<int, 1>{});
+            else make(std::integral_constant<int, VF_MANY>{});
             __syncthreads();
         }
         if (wave == 0) {
@@ -417,19 +430,16 @@ __global__ __launch_bounds__(64 * VF_WAVES) void k_tree_pick(VerifyArgs a) {
         if (!who && (who = __ballot(some >= 0))) { from = 63 - __clzll((long long)who); tile = some; x_tile = x_some; }
         if (from >= 0) {
             tile = __builtin_amdgcn_readlane(tile, from);
-            double before = __shfl(x_tile, from);
-            constexpr int E = sizeof(typename TY::elem);
+            double before = vf_lane(x_tile, from);
             const VerifyState w = s;
             const uint8_t *p = a.p + (r.q0 + w.cur) * a.ps * E, *q = DRAFT ? a.q + (r.q0 + w.cur) * a.qs * E : nullptr;
             vf_marks<DRAFT>(a, r, w, tile, bits[0]);
             double e8[VF_PARTS][8];
+            VfEight<TY, DRAFT> x8[VF_PARTS];
+            const int v0 = tile * VF_TILE + 8 * lane;
+            VfEight<TY, DRAFT>::load_all(x8, a, p, q, v0);
 #pragma unroll
-            for (int k = 0; k < VF_PARTS; k++) {
-                const int in = 8 * lane + 512 * k, v = tile * VF_TILE + in;
-#pragma unroll
-                for (int e = 0; e < 8; e++) e8[k][e] = 0.0;
-                if (v < a.V) vf_eight<TY, DRAFT>(a, p, q, w, bits[0], in, v, e8[k]);
-            }
+            for (int k = 0; k < VF_PARTS; k++) x8[k].weigh(a, w, bits[0], tile * VF_TILE, v0 + 512 * k, e8[k]);
             int found = -1, any = -1;                   // the wave's
 #pragma unroll
             for (int k = 0; k < VF_PARTS; k++) {
@@ -440,14 +450,14 @@ __global__ __launch_bounds__(64 * VF_WAVES) void k_tree_pick(VerifyArgs a) {
                 for (int e = 0; e < 8; e++) {
                     y += e8[k][e];
                     if (e8[k][e] > 0.0) {
-                        last = tile * VF_TILE + 8 * lane + 512 * k + e;
+                        last = x8[k].entry(a, v0 + 512 * k, e);
                         if (f < 0 && y > goal) f = last;
                     }
                 }
                 const unsigned long long fs = __ballot(f >= 0), ls = __ballot(last >= 0);
                 if (found < 0 && fs) found = __builtin_amdgcn_readlane(f, __ffsll(fs) - 1);
                 if (ls) any = __builtin_amdgcn_readlane(last, 63 - __clzll((long long)ls));
-                before += lane_bcast_d(scan, 63);
+                before += vf_lane(scan, 63);
             }
             token = found >= 0 ? found : any;
         }
@@ -485,7 +495,7 @@ static int verify_rounds(const VerifyArgs &a, bool draft, int max_children) {
     if (a.tiles <= VF_WAVES * VF_MANY) return 0;
     return draft && max_children != 1 ? 3 : 1;
 }
-static int vf_waves(int tiles) { return tiles < VF_WAVES * VF_MANY ? (tiles + VF_MANY - 1) / VF_MANY : VF_WAVES; }
+static int vf_waves(int tiles) { return tiles < VF_WAVES ? tiles : VF_WAVES; }
 template <typename TY, bool DRAFT> static hipError_t verify_launch(VerifyArgs a, int rounds, hipStream_t st) {
     hipError_t e = hipSuccess;
     for (; a.round < rounds && e == hipSuccess; a.round++)
