@@ -170,21 +170,28 @@ __device__ __forceinline__ int att_past(const AttArgs &a, const AttTile &t, int 
     return max(pos - a.window, -1);
 }
 // Which of the 32 keys from k0 on the token sees, if they exist.  A tree's word is 32 bits of what comes before the new tokens (all
-// seen, after the window's start), of the token's mask, and of what comes behind it (none).
-__device__ __forceinline__ uint32_t att_sees(const AttArgs &a, const AttTile &t, int tok, int past, int k0) {
+// seen, after the window's start), of the token's mask, and of what comes behind it (none): of two words of the mask, which att_words loads.
+struct AttWords { uint32_t lo, hi; };
+__device__ __forceinline__ AttWords att_words(const AttArgs &a, const AttTile &t, int tok, int k0) {
+    if (t.chain) return {0u, 0u};
+    const uint32_t *m = a.mask + (t.q0 + tok) * a.mstride;
+    const int w = (k0 - t.shift) >> 5, top = a.mwords - 1;
+    return {m[min(max(w, 0), top)], m[min(max(w + 1, 0), top)]};
+}
+__device__ __forceinline__ uint32_t att_sees(const AttArgs &a, const AttTile &t, AttWords m, int tok, int past, int k0) {
     const int c0 = k0 - t.shift, y = past - k0;         // the first key among the new tokens; keys past y are in the window
     const uint32_t in = y < 0 ? ~0u : y >= 31 ? 0u : ~((2u << y) - 1u);
     if (t.chain) {
         const int d = tok - c0;
         return (d < 0 ? 0u : d >= 31 ? ~0u : (2u << d) - 1u) & in;
     }
-    const uint32_t *m = a.mask + (t.q0 + tok) * a.mstride;
     const int w = c0 >> 5, top = a.mwords - 1;
-    uint32_t lo = m[min(max(w, 0), top)], hi = m[min(max(w + 1, 0), top)];
-    lo = w < 0 ? ~0u : w > top ? 0u : lo;
-    hi = w < -1 ? ~0u : w >= top ? 0u : hi;
+    const uint32_t lo = w < 0 ? ~0u : w > top ? 0u : m.lo, hi = w < -1 ? ~0u : w >= top ? 0u : m.hi;
     const uint32_t fresh = c0 >= 0 ? ~0u : c0 <= -32 ? 0u : ~0u << (-c0 & 31);
     return (uint32_t)(((unsigned long long)hi << 32 | lo) >> (c0 & 31)) & (in | fresh);
+}
+__device__ __forceinline__ uint32_t att_sees(const AttArgs &a, const AttTile &t, int tok, int past, int k0) {
+    return att_sees(a, t, att_words(a, t, tok, k0), tok, past, k0);
 }
 
 // The tile of 128 rows that comes at `slot` when the requests are in the order of their keys, longest first (in 64s), and
@@ -561,7 +568,7 @@ template <typename V, bool STREAM> __device__ __forceinline__ V att_ld(const uin
     else return *reinterpret_cast<const V *>(p);
 }
 
-// Over e4m3 codes a lane takes HD / 4 neighbouring dims of a key's row (16 bytes a load) and 4 or 8 of a value's, as bf16 or, for f16
+// Over e4m3 codes a lane takes 16 neighbouring dims of a key's row at a time (the four groups 64 bytes) and 4 or 8 of a value's, as bf16 or, for f16
 // rows, f16: codes are exact in both.  A key's scale multiplies its score.  A value's multiplies the probability: exactly in bf16, so that a
 // row's sum is the rounded products' times the scales' reciprocals; in f16, whose range is small, by the part of the scale that lies under the
 // largest one so far (ev), and the sums carry that one as they carry the maximum.
@@ -572,7 +579,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     constexpr int NU = HD / 16, NS = HD / 32, NQ = QF ? 3 : 1, NK = KF ? 3 : 1;
     constexpr bool K8 = EK == 1, E16 = K8 && std::is_same<QT, QtF16>::value;
     typedef typename std::conditional<!K8, KT, typename std::conditional<QF, QtBf16, QT>::type>::type MT;     // what the products take
-    constexpr int NL = K8 ? HD / 64 : NS, GD = K8 ? HD / 4 : 8;         // loads of a key's row; dims to the next group's
+    constexpr int NL = K8 ? HD / 64 : NS, GD = K8 ? 16 : 8;             // loads of a key's row; dims of one, to the next group's
     constexpr int OB = 16 * HD * 4;                     // one wave's sums
     __shared__ __align__(16) uint8_t sm[OB * ATT_WV];   // QF: first the queries' planes [plane][16][HD] bf16
     __shared__ float sst[2][ATT_WV][16];
@@ -616,7 +623,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     } else {
         const uint8_t *qp = a.q + ((size_t)((t.q0 + tok) * a.qs) + (size_t)qh * HD + GD * g) * EQ;
 #pragma unroll
-        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + (K8 ? 8 : 32) * s * EQ);
+        for (int s = 0; s < NS; s++) qf[s] = *reinterpret_cast<const qt_u32x4 *>(qp + (K8 ? 64 * (s >> 1) + 8 * (s & 1) : 32 * s) * EQ);
     }
     float m = -INFINITY, l = 0.f;                       // l: of this group's keys
     const qt_f32x4 zero = {0.f, 0.f, 0.f, 0.f};
@@ -633,6 +640,9 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         uint32_t vr[8][NU * EK / 4];
         uint32_t ok;                                    // keys of the block that exist
         long long koff[2];
+        const bool whole = 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window);       // seen by every row
+        AttWords mw = {0u, 0u};
+        if (TREE && !whole) mw = att_words(a, t, tok, 32 * kb);                                         // (ahead of the longer loads)
         if constexpr (PAGED) {
             const bool has = att_has(a, page);
             ok = (uint32_t)__ballot(has);
@@ -655,7 +665,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
             for (int s = 0; s < NL; s++)
 #pragma unroll
                 for (int e = 0; e < (KF ? 2 : 1); e++)
-                    kr[u][s][e] = att_ld<qt_u32x4, STREAM>(kbase + (koff[u] + (K8 ? 16 : 32) * s) * EK + 16 * e);
+                    kr[u][s][e] = att_ld<qt_u32x4, STREAM>(kbase + (koff[u] + (K8 ? 64 : 32) * s) * EK + 16 * e);
         const auto values = [&] {
 #pragma unroll
             for (int j = 0; j < 8; j++) {
@@ -710,7 +720,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
                 }
 #pragma unroll
                 for (int p = 0; p < NQ; p++)
-                    if constexpr (QF) qa[p] = qt_lds16(sm + (p * 16 + li) * HD * 2 + 16 * ((K8 ? NS * g + s : 4 * s + g) ^ (li & (HD / 8 - 1))));
+                    if constexpr (QF) qa[p] = qt_lds16(sm + (p * 16 + li) * HD * 2 + 16 * ((K8 ? 8 * (s >> 1) + 2 * g + (s & 1) : 4 * s + g) ^ (li & (HD / 8 - 1))));
                     else qa[p] = qf[s];
                 sc[u] = att_planes16<MT, NK, NQ>(ka, qa, sc[u]);
             }
@@ -720,9 +730,9 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
             __builtin_amdgcn_sched_barrier(0);
             values();
         }
-        if (!(ok == 0xFFFFFFFFu && 32 * kb + 31 <= first && (a.window <= 0 || 32 * kb > last - a.window))) {
+        if (!(ok == 0xFFFFFFFFu && whole)) {
             const int d = pos - 32 * kb - 4 * g, w = a.window > 0 ? d - a.window : -1000;
-            const uint32_t mine = (TREE ? ok & att_sees(a, t, tok, past, 32 * kb) : ok) >> (4 * g);
+            const uint32_t mine = (TREE ? ok & (whole ? ~0u : att_sees(a, t, mw, tok, past, 32 * kb)) : ok) >> (4 * g);
 #pragma unroll
             for (int u = 0; u < 2; u++)
 #pragma unroll

@@ -492,7 +492,7 @@ extern "C" long long qwen_hip_op_tree_verify_workspace(const qwen_hip_tree_verif
 
 // Launches of sums before the one that picks.
 static int verify_rounds(const VerifyArgs &a, bool draft, int max_children) {
-    if (a.tiles <= VF_WAVES * VF_MANY) return 0;
+    if (a.tiles <= 48) return 0;
     return draft && max_children != 1 ? 3 : 1;
 }
 static int vf_waves(int tiles) { return tiles < VF_WAVES ? tiles : VF_WAVES; }
