@@ -194,6 +194,21 @@ static inline bool qt_rows_meet(const void *a, long long as, long long aw, const
     if (d < (bs ? 1 - n : 0)) d = bs ? 1 - n : 0;
     return d < n && D + d * as < bw;
 }
+// Whether one of the outputs shares memory with another one or with an input.  `same`: an output that may be that input itself.
+struct QtMem { const void *p; long long bytes; const char *name; const void *same; };
+static inline const QtMem *qt_meets(const QtMem *out, int n_out, const QtMem *in, int n_in) {
+    const auto meet = [](const QtMem &a, const QtMem &b) {
+        const intptr_t x = (intptr_t)a.p, y = (intptr_t)b.p;
+        return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+    };
+    for (int i = 0; i < n_out; i++) {
+        for (int j = i + 1; j < n_out; j++)
+            if (meet(out[i], out[j])) return &out[i];
+        for (int j = 0; j < n_in; j++)
+            if (meet(out[i], in[j]) && !(out[i].p == in[j].p && out[i].same == in[j].p)) return &out[i];
+    }
+    return nullptr;
+}
 static inline bool qt_off16(const void *p) { return ((uintptr_t)p & 15) != 0; }
 
 // bytes of a cache's element

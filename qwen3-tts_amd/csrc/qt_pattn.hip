@@ -64,14 +64,15 @@ static int check_rows(const char *who, int dtype, int n_heads, int nkv, int hd, 
 }
 
 static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, bool tree, AttArgs &a, AttPlan &plan) {
-    if (qt_check_pages("page_attention", kv)) return -1;
-    QT_REFUSE(!p, "page_attention: null descriptor");
-    if (check_rows("page_attention", p->dtype, p->n_heads, kv->n_kv_heads, kv->head_dim, p->B, p->T, p->window, p->scale)) return -1;
+    const char *const who = tree ? "tree_attention" : "page_attention";
+    if (qt_check_pages(who, kv)) return -1;
+    QT_REFUSE(!p, "%s: null descriptor", who);
+    if (check_rows(who, p->dtype, p->n_heads, kv->n_kv_heads, kv->head_dim, p->B, p->T, p->window, p->scale)) return -1;
     QT_REFUSE(kv->dtype != QWEN_HIP_DT_E4M3 && (p->dtype == QWEN_HIP_DT_F32 ? kv->dtype != QWEN_HIP_DT_BF16 : p->dtype != kv->dtype),
-              "page_attention: rows of dtype %d over a cache of dtype %d (f32 over bf16, else the cache's own; any over e4m3)", p->dtype, kv->dtype);
-    QT_REFUSE(p->max_q < 0 || p->max_kv < 0, "page_attention: max_q %d, max_kv %d", p->max_q, p->max_kv);
+              "%s: rows of dtype %d over a cache of dtype %d (f32 over bf16, else the cache's own; any over e4m3)", who, p->dtype, kv->dtype);
+    QT_REFUSE(p->max_q < 0 || p->max_kv < 0, "%s: max_q %d, max_kv %d", who, p->max_q, p->max_kv);
     QT_REFUSE(p->table_cols < 1 || (long long)p->table_cols * kv->page_size > ATT_MAX_KEYS || p->table_stride < p->table_cols,
-              "page_attention: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
+              "%s: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", who, p->table_cols, p->table_stride);
     a = AttArgs{};
     a.B = p->B; a.T = p->T; a.nkv = kv->n_kv_heads; a.G = p->n_heads / kv->n_kv_heads;
     plan = att_plan(a, p->dtype, true, p->max_q < p->T ? p->max_q : p->T, p->max_kv, tree || kv->dtype == QWEN_HIP_DT_E4M3);
@@ -110,6 +111,7 @@ static hipError_t att_merge(const AttArgs &a, int dtype, int hd, hipStream_t st)
 }
 
 static int paged_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *p, const qwen_hip_tree_t *tree, void *stream) {
+    const char *const who = tree ? "tree_attention" : "page_attention";
     AttArgs a;
     AttPlan plan;
     if (paged_args(kv, p, tree != nullptr, a, plan)) return -1;
@@ -119,21 +121,21 @@ static int paged_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_at
                   "tree_attention: mask_words %d of stride %lld (1..32, the stride at least as many)", tree->mask_words, tree->mask_stride);
         QT_REFUSE(!tree->mask || (p->window > 0 && !tree->pos), "tree_attention: null pointer (a window needs pos)");
     }
-    QT_REFUSE(!p->q || !p->out || !p->cu_q || !p->kv_len || !p->table, "page_attention: null pointer");
-    QT_REFUSE(p->out == p->q, "page_attention: out must not be q");
+    QT_REFUSE(!p->q || !p->out || !p->cu_q || !p->kv_len || !p->table, "%s: null pointer", who);
+    QT_REFUSE(p->out == p->q, "%s: out must not be q", who);
     const int A = 16 / qt_dt_size(p->dtype);
-    QT_REFUSE(qt_off16(p->q) || qt_off16(p->out) || qt_off16(p->workspace), "page_attention: pointers have to be aligned to 16 bytes");
+    QT_REFUSE(qt_off16(p->q) || qt_off16(p->out) || qt_off16(p->workspace), "%s: pointers have to be aligned to 16 bytes", who);
     QT_REFUSE(p->q_stride % A || p->q_stride < 0 || p->out_stride % A || p->out_stride < (long long)p->n_heads * kv->head_dim,
-              "page_attention: strides %lld, %lld (multiples of 16 bytes, out's at least a token's)", p->q_stride, p->out_stride);
+              "%s: strides %lld, %lld (multiples of 16 bytes, out's at least a token's)", who, p->q_stride, p->out_stride);
     const long long need = a.splits > 1 ? (long long)a.splits * a.T * p->n_heads * (kv->head_dim + 2) * 4 : 0;
-    QT_REFUSE(need > 0 && (!p->workspace || p->workspace_bytes < need), "page_attention: a workspace of %lld bytes is needed, %lld given",
+    QT_REFUSE(need > 0 && (!p->workspace || p->workspace_bytes < need), "%s: a workspace of %lld bytes is needed, %lld given", who,
               need, p->workspace ? p->workspace_bytes : 0ll);
-    QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "page_attention: too many tiles for one launch");
+    QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "%s: too many tiles for one launch", who);
     const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * kv->head_dim * E;
-    QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T), "page_attention: out overlaps q");
+    QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T), "%s: out overlaps q", who);
     const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
-    QT_REFUSE(on.err != hipSuccess, "page_attention: the stream's device: %s", hipGetErrorString(on.err));
+    QT_REFUSE(on.err != hipSuccess, "%s: the stream's device: %s", who, hipGetErrorString(on.err));
     a.q = (const uint8_t *)p->q; a.k = (const uint8_t *)kv->k; a.v = (const uint8_t *)kv->v; a.out = (uint8_t *)p->out;
     a.qs = p->q_stride; a.os = p->out_stride;
     a.ks_page = kv->page_stride; a.ks_head = kv->head_stride; a.ks_slot = a.vs_slot = kv->slot_stride;
@@ -155,7 +157,7 @@ static int paged_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_at
                    : tree ? att_launch_tree(a, plan, p->dtype, kv->head_dim, st)
                           : att_launch_rows<true>(a, plan, p->dtype, kv->head_dim, st);
     if (e == hipSuccess && a.splits > 1) e = att_merge(a, p->dtype, kv->head_dim, st);
-    QT_REFUSE(e != hipSuccess, "page_attention: launch failed: %s", hipGetErrorString(e));
+    QT_REFUSE(e != hipSuccess, "%s: launch failed: %s", who, hipGetErrorString(e));
     return 0;
 }
 

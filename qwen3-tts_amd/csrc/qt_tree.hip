@@ -60,6 +60,11 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
               "tree_plan: mask_words %d of stride %lld (1..32, the stride at least as many)", p->mask_words, p->mask_stride);
     if (p->B == 0 || p->T == 0) return 0;
     QT_REFUSE(!p->parent || !p->cu_q || !p->kv_len || !p->pos || !p->mask, "tree_plan: null pointer");
+    const long long T = p->T, B = p->B;
+    const QtMem out[] = {{p->pos, 4 * T, "pos", nullptr}, {p->mask, 4 * ((T - 1) * p->mask_stride + p->mask_words), "mask", nullptr}};
+    const QtMem in[] = {{p->parent, 4 * T, 0, 0}, {p->cu_q, 4 * (B + 1), 0, 0}, {p->kv_len, 4 * B, 0, 0}};
+    const QtMem *const bad = qt_meets(out, 2, in, 3);
+    QT_REFUSE(bad, "tree_plan: %s overlaps what is read or written beside it", bad->name);
     const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "tree_plan: the stream's device: %s", hipGetErrorString(on.err));
@@ -517,6 +522,13 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
     QT_REFUSE(!p->workspace || p->workspace_bytes < need, "tree_verify: a workspace of %lld bytes is needed, %lld given", need,
               p->workspace ? p->workspace_bytes : 0ll);
     QT_REFUSE(qt_off16(p->workspace), "tree_verify: the workspace has to be aligned to 16 bytes");
+    const long long T = p->T, B = p->B;
+    const QtMem out[] = {{p->path, 4 * T, "path", nullptr}, {p->out_tok, 4 * T, "out_tok", nullptr}, {p->n_path, 4 * B, "n_path", nullptr},
+                         {p->workspace, need, "workspace", nullptr}};
+    const QtMem in[] = {{p->tok, 4 * T, 0, 0}, {p->parent, 4 * T, 0, 0}, {p->u, 4 * T, 0, 0}, {p->cu_q, 4 * (B + 1), 0, 0}, {p->r, 4 * B, 0, 0},
+                        {p->p, E * ((T - 1) * p->p_stride + p->V), 0, 0}, {p->q, E * ((T - 1) * p->q_stride + p->V), 0, 0}};
+    const QtMem *const bad = qt_meets(out, 4, in, 7);
+    QT_REFUSE(bad, "tree_verify: %s overlaps what is read or written beside it", bad->name);
     const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "tree_verify: the stream's device: %s", hipGetErrorString(on.err));
@@ -682,6 +694,15 @@ extern "C" int qwen_hip_op_tree_commit(const qwen_hip_kv_pages_t *kv, const qwen
     const int E = qt_kv_size(kv->dtype);
     if (p->n_layers > 0 && qt_check_pages_apart("tree_commit", kv, p->n_layers, p->layer_stride, p->scale_layer_stride)) return -1;
     QT_REFUSE(p->n_layers > 1 && p->layer_stride % (16 / E), "tree_commit: layer_stride %lld (a multiple of 16 bytes)", p->layer_stride);
+    if (p->kv_len_out) {
+        const long long T = p->T, B = p->B;
+        const QtMem out[] = {{p->kv_len_out, 4 * B, "kv_len_out", p->kv_len}, {p->n_free_out, 4, "n_free_out", p->n_free}, {p->status, 4, "status", nullptr},
+                             {p->free_pages, 4ll * kv->n_pages, "free_pages", nullptr}};
+        const QtMem in[] = {{p->path, 4 * T, 0, 0}, {p->n_path, 4 * B, 0, 0}, {p->cu_q, 4 * (B + 1), 0, 0}, {p->kv_len, 4 * B, 0, 0}, {p->n_free, 4, 0, 0},
+                            {p->table, 4 * ((B - 1) * p->table_stride + p->table_cols), 0, 0}};
+        const QtMem *const bad = qt_meets(out, 4, in, 6);
+        QT_REFUSE(bad, "tree_commit: %s overlaps what is read or written beside it", bad->name);
+    }
     const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "tree_commit: the stream's device: %s", hipGetErrorString(on.err));

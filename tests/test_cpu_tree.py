@@ -160,3 +160,39 @@ def test_empty_calls_do_nothing():
     assert L.qwen_hip_op_tree_verify(C.byref(verify(B=0)), None) == 0
     assert L.qwen_hip_op_tree_commit(C.byref(codes()), C.byref(commit(B=0)), None) == 0
     assert L.qwen_hip_op_tree_commit(C.byref(codes()), C.byref(commit(n_layers=0, kv_len_out=None)), None) == 0
+
+
+def apart(**kw):
+    """A descriptor's buffers far from each other."""
+    return {n: (i + 8) * 64 * Q for i, n in enumerate(kw["names"])}
+
+
+@pytest.mark.parametrize("a,b", [("pos", "parent"), ("pos", "cu_q"), ("mask", "kv_len"), ("mask", "pos")])
+def test_tree_plan_refuses_outputs_that_overlap(a, b):
+    d = apart(names=("parent", "cu_q", "kv_len", "pos", "mask"))
+    d[a] = d[b]
+    refused(hip.lib().qwen_hip_op_tree_plan(C.byref(tree_plan(**d)), None), "overlaps")
+
+
+@pytest.mark.parametrize("a,b,off", [("out_tok", "tok", 0), ("path", "parent", 32), ("path", "out_tok", -32), ("n_path", "r", 8), ("n_path", "cu_q", 12), ("out_tok", "u", 0),
+                                     ("path", "p", 2000 * 9 - 8), ("path", "q", 0), ("workspace", "p", 0), ("n_path", "workspace", 0)])
+def test_tree_verify_refuses_outputs_that_overlap(a, b, off):
+    d = apart(names=("p", "q", "tok", "parent", "cu_q", "u", "r", "path", "out_tok", "n_path", "workspace"))
+    d[a] = d[b] + off
+    refused(hip.lib().qwen_hip_op_tree_verify(C.byref(verify(**d)), None), "overlaps")
+
+
+@pytest.mark.parametrize("a,b,off", [("kv_len_out", "kv_len", 4), ("kv_len_out", "path", 0), ("kv_len_out", "n_path", 0), ("n_free_out", "kv_len", 0), ("n_free_out", "status", 0),
+                                     ("free_pages", "table", 0), ("free_pages", "n_free", -8), ("status", "cu_q", 0), ("n_free_out", "free_pages", 36)])
+def test_tree_commit_refuses_outputs_that_overlap(a, b, off):
+    d = apart(names=("path", "n_path", "cu_q", "kv_len", "table", "kv_len_out", "free_pages", "n_free", "n_free_out", "status"))
+    d[a] = d[b] + off
+    refused(hip.lib().qwen_hip_op_tree_commit(C.byref(codes()), C.byref(commit(**d)), None), "overlaps")
+
+
+def test_errors_name_the_call():
+    L = hip.lib()
+    for f, who in ((lambda a: L.qwen_hip_op_page_attention(C.byref(pages()), C.byref(a), None), "page_attention"),
+                   (lambda a: L.qwen_hip_op_tree_attention(C.byref(pages()), C.byref(a), C.byref(tree()), None), "tree_attention")):
+        for kw in (dict(scale=0.0), dict(q=None), dict(out_stride=1024), dict(max_kv=1 << 16, workspace=None)):
+            refused(f(attn(**kw)), who + ":")

@@ -935,3 +935,189 @@ def test_commit_of_paths_that_are_none():
     for x, y in zip(c.pools, before):
         y[:, c.table[0][1], :, 0] = y[:, c.table[0][4], :, 0]
         assert torch.equal(x, y)
+
+
+# ---- a run of them together ------------------------------------------------------------------------
+
+
+class Decoder:
+    """One attention layer as a language model: a token's q | k | v rows are looked up, its logits a product of what attention
+    gives. Tokens come one at a time, or several a step from a tree of drafts. Everything stays on the device."""
+
+    NH, NKV, HD, V, PAGE, COLS = 4, 2, 64, 50, 4, 30
+
+    def __init__(self, B, cache, t="f32", max_tokens=64, words=2, seed=0):
+        g = torch.Generator().manual_seed(seed)
+        self.B, self.t, self.T, self.words, self.cache = B, t, max_tokens, words, cache
+        nh, nkv, hd = self.NH, self.NKV, self.HD
+        self.table_e = torch.randn(self.V, (nh + 2 * nkv) * hd, generator=g).to(TYPES[t]).to(DEV)
+        self.w = torch.randn(nh * hd, self.V, generator=g).to(DEV)
+        self.n_pages = B * self.COLS
+        ang = torch.arange(self.PAGE * self.COLS, dtype=torch.float64)[:, None] * 1e4 ** (-torch.arange(0, hd, 2, dtype=torch.float64) / hd)
+        z = lambda *s: torch.zeros(*s, dtype=torch.int32, device=DEV)  # noqa: E731
+        self.cos, self.sin, self.norm = ang.cos().float().to(DEV), ang.sin().float().to(DEV), torch.ones(hd, device=DEV)
+        shape = (self.n_pages, nkv, self.PAGE, hd)
+        if cache == "e4m3":
+            self.pools = [torch.zeros(s, dtype=torch.uint8, device=DEV) for s in (shape, shape[:3], shape, shape[:3])]
+            self.pages = pages8(*self.pools)
+        else:
+            self.pools = [torch.zeros(shape, dtype=TYPES[cache], device=DEV) for _ in range(2)]
+            self.pages = pages_of(*self.pools, cache)
+        self.new, self.kv, self.table, self.free, self.n_free = z(B), z(B), z(B, self.COLS) - 1, i32(list(range(self.n_pages))), i32([self.n_pages])
+        self.cu, self.pos, self.slot, self.status, self.status2 = z(B + 1), z(self.T), z(self.T), z(1), z(1)
+        self.parent, self.tok, self.mask, self.tpos = z(self.T), z(self.T), z(self.T, words), z(self.T) - 1
+        self.u, self.r = torch.zeros(self.T, device=DEV), torch.zeros(B, device=DEV)
+        self.q = torch.zeros(self.T, nh * hd, dtype=TYPES[t], device=DEV)
+        self.out, self.rows = torch.zeros_like(self.q), torch.zeros(self.T, (nh + 2 * nkv) * hd, dtype=TYPES[t], device=DEV)
+        self.p = torch.zeros(self.T, self.V, device=DEV)
+        self.path, self.out_tok, self.n_path = z(self.T), z(self.T), z(B)
+        E, W = self.rows.element_size(), self.rows.stride(0)
+        self.plan = hip.PagePlan(new_len=dp(self.new), kv_len=dp(self.kv), n_free=dp(self.n_free), table=dp(self.table), free_pages=dp(self.free),
+                                 kv_len_out=dp(self.kv), n_free_out=dp(self.n_free), cu_q=dp(self.cu), pos=dp(self.pos), slot=dp(self.slot), status=dp(self.status),
+                                 table_stride=self.COLS, B=B, page_size=self.PAGE, n_pages=self.n_pages, table_cols=self.COLS, max_tokens=self.T)
+        self.tplan = hip.TreePlan(parent=dp(self.parent), cu_q=dp(self.cu), kv_len=dp(self.kv), pos=dp(self.tpos), mask=dp(self.mask), mask_stride=words, B=B, T=self.T,
+                                  mask_words=words)
+        self.app = hip.PageAppend(dtype=hip.DT[t], n_heads=nh, T=self.T, rope_len=self.cos.shape[0], eps=1e-6, q=dp(self.rows), k=dp(self.rows) + nh * hd * E,
+                                  v=dp(self.rows) + (nh + nkv) * hd * E, q_stride=W, k_stride=W, v_stride=W, q_out=dp(self.q), q_out_stride=nh * hd, q_norm=dp(self.norm),
+                                  k_norm=dp(self.norm), rope_cos=dp(self.cos), rope_sin=dp(self.sin), pos=dp(self.tpos), slot=dp(self.slot))
+        self.att = hip.PageAttn(dtype=hip.DT[t], n_heads=nh, B=B, T=self.T, table_cols=self.COLS, max_q=0, max_kv=self.PAGE * self.COLS, scale=hd ** -0.5, q=dp(self.q),
+                                out=dp(self.out), q_stride=nh * hd, out_stride=nh * hd, cu_q=dp(self.cu), kv_len=dp(self.kv), table=dp(self.table), table_stride=self.COLS)
+        n = hip.lib().qwen_hip_op_page_attention_workspace(C.byref(self.pages), C.byref(self.att))
+        self.ws = torch.zeros(max(n, 16), dtype=torch.uint8, device=DEV)
+        self.att.workspace, self.att.workspace_bytes = dp(self.ws), n
+        self.tree = hip.Tree(mask=dp(self.mask), pos=dp(self.tpos), mask_stride=words, mask_words=words)
+        self.ver = hip.TreeVerify(dtype=0, B=B, T=self.T, V=self.V, p=dp(self.p), p_stride=self.V, tok=dp(self.tok), parent=dp(self.parent), cu_q=dp(self.cu), u=dp(self.u),
+                                  r=dp(self.r), path=dp(self.path), out_tok=dp(self.out_tok), n_path=dp(self.n_path))
+        n = hip.lib().qwen_hip_op_tree_verify_workspace(C.byref(self.ver))
+        self.ws2 = torch.zeros(n, dtype=torch.uint8, device=DEV)
+        self.ver.workspace, self.ver.workspace_bytes = dp(self.ws2), n
+        self.com = hip.TreeCommit(path=dp(self.path), n_path=dp(self.n_path), cu_q=dp(self.cu), kv_len=dp(self.kv), table=dp(self.table), table_stride=self.COLS,
+                                  kv_len_out=dp(self.kv), free_pages=dp(self.free), n_free=dp(self.n_free), n_free_out=dp(self.n_free), status=dp(self.status2), B=B,
+                                  T=self.T, table_cols=self.COLS, n_layers=1)
+
+    def step(self):
+        """A step on the tokens that `put` has left; the model's own arithmetic is torch's."""
+        L, s, kv = hip.lib(), stream(), C.byref(self.pages)
+        ok(L.qwen_hip_op_page_plan(C.byref(self.plan), s))
+        ok(L.qwen_hip_op_tree_plan(C.byref(self.tplan), s))
+        self.rows.copy_(self.table_e[self.tok.long()])
+        ok(L.qwen_hip_op_page_append(kv, C.byref(self.app), s))
+        ok(L.qwen_hip_op_tree_attention(kv, C.byref(self.att), C.byref(self.tree), s))
+        logits = self.out.float() @ self.w
+        self.p.copy_((logits == logits.amax(-1, keepdim=True)).float())           # greedy
+        ok(L.qwen_hip_op_tree_verify(C.byref(self.ver), s))
+        ok(L.qwen_hip_op_tree_commit(kv, C.byref(self.com), s))
+
+    def put(self, trees):
+        """(parents, tokens) for each request."""
+        pad = self.T - sum(len(u) for u, _ in trees)
+        self.new.copy_(i32([len(u) for u, _ in trees]))
+        self.parent.copy_(i32(sum([u for u, _ in trees], []) + [-1] * pad))
+        self.tok.copy_(i32(sum([x for _, x in trees], []) + [0] * pad))
+
+    def took(self, trees):
+        """Each request's tokens of the step."""
+        torch.cuda.synchronize()
+        assert int(self.status) == 0 and int(self.status2) == 0
+        out, n, at, got = self.out_tok.tolist(), self.n_path.tolist(), 0, []
+        for b, (u, _) in enumerate(trees):
+            got.append(out[at:at + n[b]])
+            at += len(u)
+        used = sum(-(-k // self.PAGE) for k in self.kv.tolist())
+        assert used + int(self.n_free) == self.n_pages
+        live = [p for b, k in enumerate(self.kv.tolist()) for p in self.table[b, :-(-k // self.PAGE)].tolist()]
+        assert sorted(live + self.free[:int(self.n_free)].tolist()) == list(range(self.n_pages))
+        return got
+
+
+def draft_tree(truth, g, V):
+    """A tree behind the last token: the true continuation now and then, other tokens beside it; each with siblings."""
+    up, tok, at = [-1], [truth[0]], 0
+    for t in truth[1:]:
+        right = float(torch.rand((), generator=g)) < 0.8
+        kids = int(torch.randint(1, 4, (), generator=g))
+        which = int(torch.randint(0, kids, (), generator=g))
+        first = len(up)
+        for i in range(kids):
+            up.append(at)
+            tok.append(t if right and i == which else int(torch.randint(0, V, (), generator=g)))
+        at = first + which
+    return up, tok
+
+
+@pytest.mark.parametrize("t,cache", [("f32", "bf16"), ("f32", "e4m3"), ("bf16", "bf16")])
+@pytest.mark.parametrize("replayed", [False, True])
+def test_drafted_steps_give_the_tokens_of_single_ones(t, cache, replayed):
+    """Greedy tokens of three requests one at a time, and the same tokens in fewer steps from drafts, eager and from a graph: lengths, pages and
+    what each step keeps follow."""
+    print(f"[case] drafted steps {t} {cache} replayed={replayed}", flush=True)
+    B, n = 3, 40
+    one = Decoder(B, cache, t, max_tokens=3, words=1)
+    seqs = [[7], [11], [49]]
+    for _ in range(n):
+        trees = [([-1], [s[-1]]) for s in seqs]
+        one.put(trees)
+        one.step()
+        for s, x in zip(seqs, one.took(trees)):
+            s += x
+    assert all(len(s) == n + 1 for s in seqs)
+    many = Decoder(B, cache, t)
+    g = torch.Generator().manual_seed(4)
+    if replayed:
+        trees = [([-1], [0])] * B
+        many.put(trees)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            many.step()                                 # (the library's products set themselves up)
+            side.synchronize()
+            many.kv.zero_()
+            many.n_free.fill_(many.n_pages)
+            many.free.copy_(i32(list(range(many.n_pages))))
+            many.table.fill_(-1)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            many.step()
+    at, steps, most = [0] * B, 0, 0
+    while min(at) < n - 6:
+        trees = [draft_tree(s[a:a + 1 + (steps + b) % 5], g, Decoder.V) for b, (s, a) in enumerate(zip(seqs, at))]
+        many.put(trees)
+        graph.replay() if replayed else many.step()
+        for b, x in enumerate(many.took(trees)):
+            assert x == seqs[b][at[b] + 1:at[b] + 1 + len(x)][:len(x)] or at[b] + len(x) > n, (b, at[b], x)
+            at[b] = min(at[b] + len(x), n - 1)
+            most = max(most, len(x))
+        assert many.kv.tolist() == at or max(at) >= n - 1
+        if max(at) >= n - 6:
+            break
+        steps += 1
+    assert most >= 3 and steps < 30
+
+
+@pytest.mark.parametrize("what", ["attention", "verify"])
+def test_two_calls_at_once_have_their_own_workspaces(what):
+    """Two calls on two streams, each with its workspace, twenty times over."""
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    if what == "attention":
+        reqs = [(700, 9), (300, 13), (90, 5)]
+        x = [Steps(reqs, 8, 4, 128, "bf16", "e4m3", 16, "head", seed=s, words=1) for s in (1, 2)]
+        want = [s.run().clone() for s in x]
+        for s in x:
+            s.out.fill_(7.0)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for s, st in zip(x, (a, b)):
+                with torch.cuda.stream(st):
+                    s.call()
+        torch.cuda.synchronize()
+        assert all(torch.equal(s.out[:, :1024].view(-1, 8, 128), w) for s, w in zip(x, want))
+        return
+    x = [Verify([5, 9, 13], 60_000, "bf16", 1, seed=s) for s in (1, 2)]
+    want = [v.want() for v in x]
+    got = []
+    for _ in range(5):
+        for v, st in zip(x, (a, b)):
+            with torch.cuda.stream(st):
+                got.append(v.run())
+    assert all(g == want[i % 2] for i, g in enumerate(got))
