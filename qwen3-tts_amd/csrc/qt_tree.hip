@@ -689,7 +689,7 @@ extern "C" int qwen_hip_op_tree_commit(const qwen_hip_kv_pages_t *kv, const qwen
     QT_REFUSE(!p, "tree_commit: null descriptor");
     QT_REFUSE(p->B < 0 || p->B > CM_MAX_B, "tree_commit: B %d out of range (0..%d)", p->B, CM_MAX_B);
     QT_REFUSE(p->T < 0 || p->T > 1 << 26, "tree_commit: T %d out of range (0..2^26)", p->T);
-    QT_REFUSE(p->n_layers < 0 || (long long)p->n_layers * p->B > 0xFFFFFFll, "tree_commit: %d layers of %d requests (2^24 - 1 at most)", p->n_layers, p->B);
+    QT_REFUSE(p->n_layers < 0 || (long long)p->n_layers * p->B > 0xFFFFFEll, "tree_commit: %d layers of %d requests (2^24 - 2 at most)", p->n_layers, p->B);
     QT_REFUSE(p->table_cols < 1 || (long long)p->table_cols * kv->page_size > TREE_MAX_LEN || p->table_stride < p->table_cols,
               "tree_commit: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", p->table_cols, p->table_stride);
     if (p->B == 0) return 0;

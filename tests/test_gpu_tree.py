@@ -798,6 +798,24 @@ def test_verify_offsets_out_of_range_stay_inside():
     assert (path, out, n_path) == v.want()
 
 
+def test_steps_without_new_tokens():
+    """All requests idle, and buffers for no tokens at all."""
+    for T in (0, 5):
+        n_path, cu, r, kv = i32([7, 7, 7]), i32([0] * 4), torch.zeros(3, device=DEV), i32([0, 4, 9])
+        buf = [torch.full((max(T, 1),), 7, dtype=torch.int32, device=DEV) for _ in range(6)]
+        p = torch.zeros(max(T, 1), 9, device=DEV)
+        d = hip.TreeVerify(dtype=0, B=3, T=T, V=9, p=dp(p), p_stride=9, tok=dp(buf[0]), parent=dp(buf[1]), cu_q=dp(cu), u=dp(buf[2]), r=dp(r), path=dp(buf[3]),
+                           out_tok=dp(buf[4]), n_path=dp(n_path))
+        ws = torch.zeros(hip.lib().qwen_hip_op_tree_verify_workspace(C.byref(d)), dtype=torch.uint8, device=DEV)
+        d.workspace, d.workspace_bytes = dp(ws), ws.numel()
+        ok(hip.lib().qwen_hip_op_tree_verify(C.byref(d), stream()))
+        plan = hip.TreePlan(parent=dp(buf[1]), cu_q=dp(cu), kv_len=dp(kv), pos=dp(buf[5]), mask=dp(buf[0]), mask_stride=1, B=3, T=T, mask_words=1)
+        ok(hip.lib().qwen_hip_op_tree_plan(C.byref(plan), stream()))
+        torch.cuda.synchronize()
+        assert n_path.tolist() == [0, 0, 0] and all(bool((b == 7).all()) for b in buf)
+    Commit([(5, 0, 0), (0, 0, 0), (17, 0, 3)], "e4m3", 2, 2, 64, 4, "head", seed=1).check()
+
+
 # ---- commit ----------------------------------------------------------------------------------------
 
 
