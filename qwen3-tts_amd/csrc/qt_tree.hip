@@ -552,7 +552,7 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
 
 // ---- what is kept ----------------------------------------------------------------------------------
 // Row path[k] goes to place k.  Since path[k] >= k, a place that has been written is no later row's source: a thread that takes 16
-// bytes of a head's rows through all moves in the order of k, four loads before their stores, reads every source before it
+// bytes of a head's rows, or a head's scales, through all moves in the order of k, eight loads before their stores, reads every source before it
 // is overwritten, and no two threads share bytes.  A workgroup takes a request's rows in one layer.  Lengths and pages: one workgroup more,
 // or a launch of its own where it replaces lengths that the moves read.
 // Bound by the latency of path, table, rows for few (8 requests, one layer of bf16: 6.3 us a pass, the kernel 3.7), by the rows' bytes for many
@@ -575,28 +575,42 @@ __device__ __forceinline__ int commit_kept(const CommitArgs &a, int b, int n) { 
 __device__ __forceinline__ bool commit_fits(const CommitArgs &a, int kv, int n) { return kv >= n && (long long)kv <= (long long)a.cols * a.ps; }
 __device__ __forceinline__ int commit_pages(const CommitArgs &a, int len) { return qt_quot(len, a.div) + (len % a.ps != 0); }
 
+// A piece of every row through n moves.
+template <typename V> __device__ __forceinline__ void commit_piece(uint8_t *base, int n, const long long *from, const long long *to) {
+    for (int j = 0; j < n; j += 8) {
+        V x[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (j + e < n) x[e] = *reinterpret_cast<const V *>(base + from[j + e]);
+#pragma unroll
+        for (int e = 0; e < 8; e++)
+            if (j + e < n) *reinterpret_cast<V *>(base + to[j + e]) = x[e];
+    }
+}
+
 __device__ __forceinline__ void commit_move(const CommitArgs &a, int b, int layer) {
-    __shared__ int from[CM_T], to[CM_T], moves_s[CM_T / 64];
+    __shared__ long long from[2][CM_T], to[2][CM_T];    // of codes, of scales
+    __shared__ int moves_s[CM_T / 64];
     const TreeReq r = tree_req(a.cu, b, a.T);
     const int kv = a.kv[b], keep = commit_kept(a, b, r.n), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     if (!commit_fits(a, kv, r.n)) return;
     const int *table = a.table + b * a.ts;
     for (int k0 = 0; k0 < keep; k0 += CM_T) {
         const int k = k0 + threadIdx.x;
-        int f = -1, t = -1;
+        int pgs = -1, pgd = -1, os = 0, od = 0;
         if (k < keep) {
             const int src = a.path[r.q0 + k];
             if (src > k && src < r.n) {
                 const int ps = kv - r.n + src, pd = kv - r.n + k, cs = qt_quot(ps, a.div), cd = qt_quot(pd, a.div);
-                const int pgs = table[cs], pgd = table[cd];
-                if ((unsigned)pgs < (unsigned)a.n_pages && (unsigned)pgd < (unsigned)a.n_pages) {
-                    f = pgs * a.ps + ps - cs * a.ps;
-                    t = pgd * a.ps + pd - cd * a.ps;
-                }
+                pgs = table[cs];
+                pgd = table[cd];
+                os = ps - cs * a.ps;
+                od = pd - cd * a.ps;
             }
         }
-        const unsigned long long some = __ballot(f >= 0);
-        __syncthreads();                                // the last round's list is read
+        const bool moves = (unsigned)pgs < (unsigned)a.n_pages && (unsigned)pgd < (unsigned)a.n_pages;
+        const unsigned long long some = __ballot(moves);
+        __syncthreads();                                // the last rounds' list is read
         if (lane == 0) moves_s[wave] = __popcll(some);
         __syncthreads();
         int at = __popcll(some & ((1ull << lane) - 1)), n = 0;
@@ -605,31 +619,23 @@ __device__ __forceinline__ void commit_move(const CommitArgs &a, int b, int laye
             if (w < wave) at += moves_s[w];
             n += moves_s[w];
         }
-        if (f >= 0) { from[at] = f; to[at] = t; }
+        if (moves) {
+            from[0][at] = pgs * a.page + os * a.slot;
+            to[0][at] = pgd * a.page + od * a.slot;
+            from[1][at] = pgs * a.s_page + os * a.s_slot;
+            to[1][at] = pgd * a.s_page + od * a.s_slot;
+        }
         __syncthreads();
-        const int chunks = a.row / 16, items = 2 * a.nkv * chunks;
-        const auto offset = [&](int slot, long long page, long long place) {
-            const int p = qt_quot(slot, a.div);
-            return p * page + (slot - p * a.ps) * place;
-        };
-        for (int i = threadIdx.x; i < items; i += CM_T) {
-            const int c = i % chunks, h = i / chunks % a.nkv;
-            uint8_t *base = (i >= items / 2 ? a.v : a.k) + layer * a.layer + h * a.head + 16 * c;
-            for (int j = 0; j < n; j += 4) {
-                qt_w4 x[4];
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (j + e < n) x[e] = qt_load16<16>(base + offset(from[j + e], a.page, a.slot));
-#pragma unroll
-                for (int e = 0; e < 4; e++)
-                    if (j + e < n) qt_store16<16>(base + offset(to[j + e], a.page, a.slot), x[e]);
+        const int chunks = a.row / 16, rows = a.nkv * chunks, pieces = 2 * rows + (a.ks ? 2 * a.nkv : 0);
+        for (int i = threadIdx.x; i < pieces; i += CM_T) {
+            if (i < 2 * rows) {
+                const int j = i >= rows ? i - rows : i;
+                commit_piece<qt_w4>((i >= rows ? a.v : a.k) + layer * a.layer + j / chunks * a.head + 16 * (j % chunks), n, from[0], to[0]);
+            } else {
+                const int j = i - 2 * rows;
+                commit_piece<uint8_t>((j >= a.nkv ? a.vs + (j - a.nkv) * a.s_head : a.ks + j * a.s_head) + layer * a.s_layer, n, from[1], to[1]);
             }
         }
-        if (a.ks)
-            for (int i = threadIdx.x; i < 2 * a.nkv; i += CM_T) {
-                uint8_t *base = (i >= a.nkv ? a.vs : a.ks) + layer * a.s_layer + (i % a.nkv) * a.s_head;
-                for (int j = 0; j < n; j++) base[offset(to[j], a.s_page, a.s_slot)] = base[offset(from[j], a.s_page, a.s_slot)];
-            }
     }
 }
 
