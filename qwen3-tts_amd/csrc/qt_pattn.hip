@@ -6,22 +6,27 @@
 
 // The kernel, its launch slots and key ranges.  Launch slots: by request (max_q as far as known) or by rows, whichever is
 // fewer.  Key ranges: enough workgroups to fill the CUs, 256 keys each at least.
-static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv, bool more) {
+static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv, bool tree, bool codes) {
     AttPlan p = {ATT_ONE, 0, false};
     a.gdiv = qt_div_of(a.G);
     a.tps = 0;
     const long long rows = (long long)a.T * a.G;
+    const bool more = tree || codes, little = more && max_kv > 0 && rows * a.nkv * max_kv < 4ll << 20;
     if (dtype == QWEN_HIP_DT_F32) {
         // 32-row tiles for prompts while they give every CU work (one of 512 positions 23.7 us against 25.4 in 16-row tiles,
         // 16 of 64 16.6 against 20.4; three of 21 to 128 11.9 against 8.9)
         if (!paged && (rows / 32 + a.B) * a.nkv >= 256) p.kind = ATT_F32;
-    } else if (rows >= 32ll * a.B && (paged || (rows / 128 + a.B) * a.nkv >= 96)) {
+    } else if (rows >= (codes ? 56ll : 32ll) * a.B && !little && (paged || (rows / 128 + a.B) * a.nkv >= 96)) {
         // 128-row tiles from 32 rows a request on (64 requests of 32 tokens 42 us against 79 in 16-row tiles, 8 of 16 over
         // 3000 keys 27.3 against 27.8, 32 of 4 70 against 60); prompts, whose keys are not split, while there are tiles
         // enough (8 of 100 to 300 13.1 us against 20.3; one of 512 15.9 against 13.0, three of 21 to 128 9.2 against 8.4).
         // Those are equal requests.  The rule goes by a call's mean, so a step of single tokens and a chunk takes one kernel
         // for both (bf16, 16 over 8 heads, a chunk over 2000 keys: 64 streams of 1000 to 8000 keys and 512 tokens in 16-row tiles
         // 259 us, 198 and 33 in a call each; 32 of them and 1024 tokens in 128-row tiles 160, 110 and 49)
+        // Over codes, which 16-row tiles read half as fast again, from 56 rows on (32 trees over 3000 keys, 48 rows: 128-row tiles 99.5 us, 16-row
+        // 91.7; 64 rows 102 and 111; over bf16 48 rows 112 and 139, 32 rows 107 and 111); codes and trees, while there is work for two
+        // launches (64 rows each over 1000 keys, 16 heads on 8: 4 requests 18.9 to 19.7 and 15.7 to 16.9, 8 requests 24.7 to 25.7 and 24.2 to 25.5; one of
+        // 128 rows over 1000 keys 19.7 and 14, over 6000 28 and 30).
         p.kind = ATT_TILE;
     }
     if (p.kind == ATT_ONE) {
@@ -75,7 +80,7 @@ static int paged_args(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t 
               "%s: table_cols %d of stride %lld (at least 1, 2^30 positions at most)", who, p->table_cols, p->table_stride);
     a = AttArgs{};
     a.B = p->B; a.T = p->T; a.nkv = kv->n_kv_heads; a.G = p->n_heads / kv->n_kv_heads;
-    plan = att_plan(a, p->dtype, true, p->max_q < p->T ? p->max_q : p->T, p->max_kv, tree || kv->dtype == QWEN_HIP_DT_E4M3);
+    plan = att_plan(a, p->dtype, true, p->max_q < p->T ? p->max_q : p->T, p->max_kv, tree, kv->dtype == QWEN_HIP_DT_E4M3);
     plan.stream = plan.stream && 2ll * qt_kv_size(kv->dtype) * p->B * p->max_kv * kv->n_kv_heads * kv->head_dim > 256ll << 20;
     return 0;
 }
@@ -184,7 +189,7 @@ extern "C" int qwen_hip_op_packed_attention(const qwen_hip_packed_attn_t *p, voi
               p->k_stride, p->v_stride, p->out_stride);
     AttArgs a = {};
     a.B = p->B; a.T = p->T; a.nkv = p->n_kv_heads; a.G = p->n_heads / p->n_kv_heads;
-    const AttPlan plan = att_plan(a, p->dtype, false, 0, 0, false);
+    const AttPlan plan = att_plan(a, p->dtype, false, 0, 0, false, false);
     QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "packed_attention: too many tiles for one launch");
     const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * p->head_dim * E, kw = (long long)p->n_kv_heads * p->head_dim * E;
     QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T) ||

@@ -362,6 +362,8 @@ class Steps:
         close(got, exact, mag, self.t, max(a + n for a, n in self.reqs), float(max(v.abs().max() for _, v in self.kv if v.numel())))
 
 
+# No bound on the keys lets requests of several rows take the kernel for many rows however little there is to do.
+HINTS = pytest.mark.parametrize("max_kv", [None, 0])
 HEADS = [(16, 8, 128), (16, 16, 64), (12, 2, 64), (32, 4, 128), (7, 1, 128), (128, 2, 64)]
 ROWS = ["f32", "bf16", "f16"]
 CACHES = KINDS + [(t, "e4m3") for t in ROWS]
@@ -394,25 +396,28 @@ def test_codes_long_chunks(t, nh, nkv, hd, page, layout, window):
     reqs = [(0, 300), (513, 257), (64, 128), (1, 191)]
     Steps(reqs, nh, nkv, hd, t, "e4m3", page, layout, seed=4, window=window, T=900).check()
     Steps(reqs, nh, nkv, hd, t, "e4m3", page, layout, seed=5, window=window, max_kv=6000).check()
+    Steps(reqs, nh, nkv, hd, t, "e4m3", page, layout, seed=6, window=window, max_kv=0).check()
 
 
 @pytest.mark.parametrize("t", ROWS)
 @pytest.mark.parametrize("reqs", [[(700, 1), (30, 1), (0, 1)], [(0, 300), (400, 140)]])
 @pytest.mark.parametrize("ke,ve", [((-1, 1), (-60, -55)), ((-1, 1), (55, 60)), ((-20, 1), (-20, 12)), ((-62, 0), (-62, -30))])
-def test_scales_of_any_size(t, reqs, ke, ve):
+@HINTS
+def test_scales_of_any_size(t, reqs, ke, ve, max_kv):
     """Values under f16's range, past it, and of scales that differ by more than it holds."""
     if t == "f16" and ve[1] > 20:
         pytest.skip("f16 rows hold no such values")
-    s = Steps(reqs, 16, 8, 128, t, "e4m3", 16, "head", seed=8, ke=ke, ve=ve)
+    s = Steps(reqs, 16, 8, 128, t, "e4m3", 16, "head", seed=8, ke=ke, ve=ve, max_kv=max_kv)
     s.check()
 
 
 @pytest.mark.parametrize("t", ROWS)
 @pytest.mark.parametrize("reqs", [[(40, 1), (100, 1)], [(0, 40), (90, 45)], [(200, 150)]])
 @pytest.mark.parametrize("what", ["code", "scale"])
-def test_codes_that_are_nan_reach_those_who_see_them(t, reqs, what):
+@HINTS
+def test_codes_that_are_nan_reach_those_who_see_them(t, reqs, what, max_kv):
     """A key's scale byte over 246, or a code that is NaN: NaN for the rows that see it, the others exact."""
-    s = Steps(reqs, 4, 2, 64, t, "e4m3", 16, "head", seed=9)
+    s = Steps(reqs, 4, 2, 64, t, "e4m3", 16, "head", seed=9, max_kv=max_kv)
     clean = s.run().clone()
     b = len(reqs) - 1
     L = sum(reqs[b])
@@ -440,9 +445,10 @@ def test_codes_that_are_nan_reach_those_who_see_them(t, reqs, what):
             x.copy_(y)
 
 
-def test_codes_in_bad_pages_hold_no_keys():
+@HINTS
+def test_codes_in_bad_pages_hold_no_keys(max_kv):
     for t, n in (("f32", 1), ("bf16", 1), ("bf16", 60), ("f16", 60)):
-        s = Steps([(96, n)], 4, 2, 64, t, "e4m3", 16, "head", seed=10)
+        s = Steps([(96, n)], 4, 2, 64, t, "e4m3", 16, "head", seed=10, max_kv=max_kv)
         s.table[0, 2], s.table[0, 4] = 10 ** 6, -1
         got = s.run()
         see = see_of(n, 96 + n, 0)
@@ -453,9 +459,10 @@ def test_codes_in_bad_pages_hold_no_keys():
 
 @pytest.mark.parametrize("t", ["f32", "bf16"])
 @pytest.mark.parametrize("n", [1, 70])
-def test_a_quantised_cache_past_32_bits(t, n):
+@HINTS
+def test_a_quantised_cache_past_32_bits(t, n, max_kv):
     """Codes and scales whose offsets pass 2^32."""
-    s = Steps([(50, n)], 2, 1, 64, t, "e4m3", 16, "head", seed=11)
+    s = Steps([(50, n)], 2, 1, 64, t, "e4m3", 16, "head", seed=11, max_kv=max_kv)
     n_pages = s.pools[0].shape[0]
     far = (5 << 30) // (n_pages - 1) // 64 * 64
     big = []
@@ -527,11 +534,13 @@ def test_large_trees_and_chunks(t, cache, nh, nkv, hd, page, window):
     reqs = [(300, 64), (0, 61), (129, 33), (63, 64), (64, 50), (500, 130), (0, 70)]
     Steps(reqs, nh, nkv, hd, t, cache, page, "head", seed=3, words=2, window=window).check()
     Steps(reqs, nh, nkv, hd, t, cache, page, "slot", seed=4, words=5, window=window, max_kv=5000).check()
+    Steps(reqs, nh, nkv, hd, t, cache, page, "slot", seed=5, words=3, window=window, max_kv=0).check()
 
 
 @pytest.mark.parametrize("t,cache", CACHES)
 @pytest.mark.parametrize("reqs", [[(0, 9), (40, 12), (3, 5)], [(0, 60), (100, 64), (5, 40)]])
-def test_any_mask(t, cache, reqs):
+@HINTS
+def test_any_mask(t, cache, reqs, max_kv):
     """Masks that are no trees: bits after a token, none at all, all; rows that see nothing are 0."""
     g = torch.Generator().manual_seed(2)
     masks = []
@@ -541,7 +550,7 @@ def test_any_mask(t, cache, reqs):
         m[n // 2] = True
         m[-1] = False
         masks.append((m, torch.zeros(n, dtype=torch.long)))
-    s = Steps(reqs, 4, 2, 64, t, cache, 16, "head", seed=5, words=2, masks=masks)
+    s = Steps(reqs, 4, 2, 64, t, cache, 16, "head", seed=5, words=2, masks=masks, max_kv=max_kv)
     s.check()
     assert bool((s.run()[0] == 0).all()) and bool((s.run()[reqs[0][1] - 1] == 0).all())
 
@@ -549,13 +558,14 @@ def test_any_mask(t, cache, reqs):
 @pytest.mark.parametrize("t,cache", CACHES)
 @pytest.mark.parametrize("value", [math.nan, math.inf])
 @pytest.mark.parametrize("reqs", [[(20, 9)], [(70, 64)]])
-def test_what_a_mask_hides_never_reaches_a_row(t, cache, value, reqs):
+@HINTS
+def test_what_a_mask_hides_never_reaches_a_row(t, cache, value, reqs, max_kv):
     """Token 4 is no number in k, then in v: only its descendants and itself are touched."""
     n = reqs[0][1]
     g = torch.Generator().manual_seed(3)
     up = random_tree(n, 3, g)
     see, depth = closure(up)
-    s = Steps(reqs, 4, 2, 64, t, cache, 16, "head", seed=6, words=2, masks=[(see, depth)])
+    s = Steps(reqs, 4, 2, 64, t, cache, 16, "head", seed=6, words=2, masks=[(see, depth)], max_kv=max_kv)
     clean = s.run().clone()
     p, o = s.rows[0][0][reqs[0][0] + 4], s.rows[0][1][reqs[0][0] + 4]
     hidden = ~see[:, 4]
@@ -578,25 +588,27 @@ def test_what_a_mask_hides_never_reaches_a_row(t, cache, value, reqs):
 
 
 @pytest.mark.parametrize("t,cache", CACHES)
-def test_chains_are_what_causal_attention_gives(t, cache):
+@HINTS
+def test_chains_are_what_causal_attention_gives(t, cache, max_kv):
     """A chain's masks, and a mask too short for its requests: the same rows as without trees."""
     for reqs in ([(40, 9), (200, 13), (0, 30)], [(100, 64), (0, 50), (300, 40)]):
         chain = [(torch.ones(n, n).tril().bool(), torch.arange(n)) for _, n in reqs]
         for window in (0, 25):
-            a = Steps(reqs, 8, 4, 128, t, cache, 16, "head", seed=7, window=window)
+            a = Steps(reqs, 8, 4, 128, t, cache, 16, "head", seed=7, window=window, max_kv=max_kv)
             got = a.run().clone()
-            b = Steps(reqs, 8, 4, 128, t, cache, 16, "head", seed=7, words=2, masks=chain)
-            c = Steps([(x, n + 33) for x, n in reqs], 8, 4, 128, t, cache, 16, "head", seed=7, words=1, window=window)
+            b = Steps(reqs, 8, 4, 128, t, cache, 16, "head", seed=7, words=2, masks=chain, max_kv=max_kv)
+            c = Steps([(x, n + 33) for x, n in reqs], 8, 4, 128, t, cache, 16, "head", seed=7, words=1, window=window, max_kv=max_kv)
             c.masks = [None] * 3
             c.check()
             if not window:                              # (a window's end moves over new tokens too; a mask's does not)
                 assert float((b.run().double() - got.double()).abs().max()) <= 2 * torch.finfo(TYPES[t]).eps * float(got.abs().max())
 
 
-def test_trees_with_lengths_that_do_not_hold_their_tokens():
+@HINTS
+def test_trees_with_lengths_that_do_not_hold_their_tokens(max_kv):
     """kv_len under the number of new tokens: the last tokens' keys are what there is."""
     for t, n in (("f32", 9), ("bf16", 60)):
-        s = Steps([(0, n), (20, n)], 4, 2, 64, t, "bf16", 16, "head", seed=12, words=2)
+        s = Steps([(0, n), (20, n)], 4, 2, 64, t, "bf16", 16, "head", seed=12, words=2, max_kv=max_kv)
         s.kvl.copy_(i32([n - 4, 20 + n]))
         got = s.run()
         see = see_of(n, n - 4, 0, s.masks[0])
