@@ -85,7 +85,7 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
 //
 // Large vocabularies: launches of a wave for two tiles, the first of which walks to the first sum (every workgroup for itself: a few
 // dependent loads), the others from the sum before to the next where there is one; then a launch of a workgroup a request, which goes on
-// from there, makes further sums itself, and picks.  64 trees of 5 to 13 tokens over 128 003 bf16: 29 us, of which the rows' bytes are 6.7 (all sums but
+// from there, makes further sums itself, and picks.  64 trees of 5 to 13 tokens over 128 003 bf16: 27 to 29 us, of which the rows' bytes are 6.7 (all sums but
 // the first in the launch that picks 44, but the first two 36; one workgroup a request for everything past the first sum, without tiles a wave, 96);
 // bound by sums that wait for each other.  6 chains over 2048 f32, one launch: 6.9, a chain of five dependent loads.
 #define VF_TILE 1024
@@ -555,8 +555,8 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
 // bytes of a head's rows, or a head's scales, through all moves in the order of k, eight loads before their stores, reads every source before it
 // is overwritten, and no two threads share bytes.  A workgroup takes a request's rows in one layer.  Lengths and pages: one workgroup more,
 // or a launch of its own where it replaces lengths that the moves read.
-// Bound by the latency of path, table, rows for few (8 requests, one layer of bf16: 6.3 us a pass, the kernel 3.7), by the rows' bytes for many
-// layers (64 requests, 28 layers of codes: 18.0).
+// Bound by the latency of path, table, rows for few (8 requests, one layer of bf16: 6.4 us a pass, the kernel 3.5), by the rows' bytes for many
+// layers (64 requests, 28 layers of codes: 16.0, the kernel 14.4; with four loads before their stores and scales after the codes 18.0 and 17.4).
 #define CM_T 256
 #define CM_MAX_B 2048
 struct CommitArgs {
