@@ -542,8 +542,8 @@ int qwen_hip_op_page_append(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_a
  * only scores of -infinity, is 0; rows before cu_q[0] and behind cu_q[B] stay as they were.  A table entry outside
  * [0, n_pages) holds no keys: its positions are not seen.  What lies in positions that a row does not see never reaches it, infinite or NaN
  * included.  Scores, softmax and sums are f32; with F32 rows (over a BF16 or E4M3 cache) so are the products; with BF16 or
- * F16 rows (over a cache of their own type or E4M3) the probabilities are rounded to that type for the product with V, which
- * reads an E4M3 cache's values as they are (F16 rows: what lies under 2^-24 of the largest scale's unit is rounded to that).
+ * F16 rows (over a cache of their own type or E4M3) the probabilities are rounded to that type for the product with V (F16 rows over
+ * E4M3: to two bf16 numbers, within 2^-17 of each), which reads an E4M3 cache's values as they are.
  * max_q and max_kv: the longest request's new tokens and kv_len as far as the host knows; they choose the launch
  * shape and change no result beyond rounding.  scale > 0.  B <= 65535, n_heads / n_kv_heads <= 64, T * n_heads < 2^26.
  * out must not overlap q (refused) or the cache (not looked at).

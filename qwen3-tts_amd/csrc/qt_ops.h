@@ -98,8 +98,7 @@ __device__ __forceinline__ uint32_t qt_scale_byte(uint32_t m) {
     const uint32_t e = (m + 0x1FFFFFu) >> 23;
     return e < QT_SCALE_MIN + 8u ? QT_SCALE_MIN : e - 8u;
 }
-// a byte as its row is read: 0 past the largest that is written (a NaN row)
-__device__ __forceinline__ uint32_t qt_scale_read(uint32_t byte) { return byte > QT_SCALE_MAX ? 0u : max(byte, QT_SCALE_MIN); }
+// a byte as its row is read: NaN past the largest that is written
 __device__ __forceinline__ float qt_scale_of(uint32_t byte) {
     return byte > QT_SCALE_MAX ? __uint_as_float(0x7FC00000u) : __uint_as_float(max(byte, QT_SCALE_MIN) << 23);
 }

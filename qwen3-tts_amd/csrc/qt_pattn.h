@@ -31,6 +31,7 @@
 #include "qt_ops.h"
 #include "qt_planes.h"
 #include <type_traits>
+#include <utility>
 
 typedef float qt_f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 qt_f16x8 __attribute__((ext_vector_type(8)));
@@ -90,6 +91,15 @@ template <typename T> __device__ __forceinline__ uint32_t att_code2(uint32_t cod
         return __builtin_bit_cast(uint32_t, upper ? __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, true)
                                                   : __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(codes, scale, false));
 }
+// 8 values as two bf16 planes: their sum is within 2^-17 of each
+__device__ __forceinline__ void att_planes2(const float (&v)[8], qt_u32x4 (&p)[2]) {
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t h = qt_bf16x2(v[2 * i], v[2 * i + 1]);
+        p[0][i] = h;
+        p[1][i] = qt_bf16x2(v[2 * i] - qt_bf_lo(h), v[2 * i + 1] - qt_bf_hi(h));
+    }
+}
 // sum over planes, the smallest products first
 template <typename T, int NA, int NB>
 __device__ __forceinline__ qt_f32x16 att_planes(const qt_u32x4 (&a)[NA], const qt_u32x4 (&b)[NB], qt_f32x16 c) {
@@ -99,6 +109,11 @@ __device__ __forceinline__ qt_f32x16 att_planes(const qt_u32x4 (&a)[NA], const q
         for (int i = 0; i < NA; i++)
             if (s - i >= 0 && s - i < NB && s <= 2) c = att_mma<T>(a[i], b[s - i], c);
     return c;
+}
+
+// register i times lane i's factor of the lane's row of 16
+template <int... I> __device__ __forceinline__ void att_keys(qt_f32x16 &x, float f, std::integer_sequence<int, I...>) {
+    ((x[I] *= __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp(0, (int)__float_as_uint(f), 0x150 + I, 0xf, 0xf, true))), ...);
 }
 
 __device__ __forceinline__ float att_other_half(float v) {
@@ -569,9 +584,9 @@ template <typename V, bool STREAM> __device__ __forceinline__ V att_ld(const uin
 }
 
 // Over e4m3 codes a lane takes 16 neighbouring dims of a key's row at a time (the four groups 64 bytes) and 4 or 8 of a value's, as bf16 or, for f16
-// rows, f16: codes are exact in both.  A key's scale multiplies its score.  A value's multiplies the probability: exactly in bf16, so that a
-// row's sum is the rounded products' times the scales' reciprocals; in f16, whose range is small, by the part of the scale that lies under the
-// largest one so far (ev), and the sums carry that one as they carry the maximum.  64 streams of 1000 to 8000 keys bf16: 111 us with the merge, 5.4 TB/s
+// rows, f16: codes are exact in both.  A key's scale multiplies its score.  A value's multiplies the probability, exactly in bf16, so that a
+// row's sum is the rounded products' times the scales' reciprocals.  f16's range is too small for that: f16 rows' probabilities times
+// scales are two bf16 planes (within 2^-17 of them), over values as bf16, and no key's scale touches another's product.  64 streams of 1000 to 8000 keys bf16: 111 us with the merge, 5.4 TB/s
 // (over bf16 196); the next block's K in registers ahead of this one's sums 126.
 template <typename QT, typename KT, int HD, bool PAGED, bool STREAM, bool TREE = false>
 __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(sizeof(typename KT::elem) == 4 ? 2 : 3))) void k_att_one(AttArgs a) {
@@ -580,6 +595,8 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     constexpr int NU = HD / 16, NS = HD / 32, NQ = QF ? 3 : 1, NK = KF ? 3 : 1;
     constexpr bool K8 = EK == 1, E16 = K8 && std::is_same<QT, QtF16>::value;
     typedef typename std::conditional<!K8, KT, typename std::conditional<QF, QtBf16, QT>::type>::type MT;     // what the products take
+    typedef typename std::conditional<E16, QtBf16, MT>::type VT;        // and V's
+    constexpr int NP = E16 ? 2 : NQ;                                    // planes of the probabilities
     constexpr int NL = K8 ? HD / 64 : NS, GD = K8 ? 16 : 8;             // loads of a key's row; dims of one, to the next group's
     constexpr int OB = 16 * HD * 4;                     // one wave's sums
     __shared__ __align__(16) uint8_t sm[OB * ATT_WV];   // QF: first the queries' planes [plane][16][HD] bf16
@@ -631,7 +648,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
     qt_f32x4 o[NU];
 #pragma unroll
     for (int u = 0; u < NU; u++) o[u] = zero;
-    uint32_t ev = QT_SCALE_MIN;                         // E16: the exponent that o carries
     const uint8_t *kbase = a.k + (head * (PAGED ? a.ks_head : (long long)HD) + GD * g) * EK;
     const uint8_t *vbase = a.v + (head * (PAGED ? a.ks_head : (long long)HD) + NU * li) * EK;
     for (int kb = kb0 + wave; kb < kb1; kb += ATT_WV) {
@@ -682,7 +698,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         };
         if constexpr (!KF) values();
         qt_f32x4 sc[2], ksl[2], vsl[2];
-        float fe = 1.f;
         if constexpr (K8) {
             scl[wave][lane] = qt_scale_of(sb);
             __builtin_amdgcn_wave_barrier();
@@ -690,16 +705,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
             for (int u = 0; u < 2; u++) {
                 ksl[u] = *reinterpret_cast<const qt_f32x4 *>(&scl[wave][16 * u + 4 * g]);
                 vsl[u] = *reinterpret_cast<const qt_f32x4 *>(&scl[wave][32 + 16 * u + 4 * g]);
-            }
-            if constexpr (E16) {
-                const uint32_t most = max(ev, (uint32_t)wave_max_i(lane < 32 ? 0 : (int)qt_scale_read(sb)));
-                fe = __uint_as_float((127u + ev < most ? 0u : 127u + ev - most) << 23);
-                ev = most;
-                const float un = __uint_as_float((254u - ev) << 23);
-#pragma unroll
-                for (int u = 0; u < 2; u++)
-#pragma unroll
-                    for (int i = 0; i < 4; i++) vsl[u][i] *= un;
             }
         }
 #pragma unroll
@@ -751,23 +756,15 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         for (int j = 0; j < 8; j++) {
             // f32: the difference first, since the rounding of a large m c would not cancel between blocks
             p[j] = QF ? qt_exp2((sc[j >> 2][j & 3] - mr) * a.c) : qt_exp2(fmaf(sc[j >> 2][j & 3], a.c, -mc));
-            if (QF) sum += p[j];
+            if (QF || E16) sum += p[j];
         }
-        qt_u32x4 pb[NQ];
-        if constexpr (QF) {
+        qt_u32x4 pb[NP];
+        if constexpr (QF || E16) {
             if constexpr (K8)
 #pragma unroll
                 for (int j = 0; j < 8; j++) p[j] *= vsl[j >> 2][j & 3];
-            qt_planes8(p, pb);
-        } else if constexpr (E16) {
-            typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const uint32_t r = qt_round2<QT>(p[2 * j], p[2 * j + 1]);
-                sum = att_add2<QT>(r, sum);
-                const h2 f = {(_Float16)vsl[j >> 1][2 * (j & 1)], (_Float16)vsl[j >> 1][2 * (j & 1) + 1]};
-                pb[0][j] = __builtin_bit_cast(uint32_t, __builtin_bit_cast(h2, r) * f);
-            }
+            if constexpr (E16) att_planes2(p, pb);
+            else qt_planes8(p, pb);
         } else if constexpr (K8) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
@@ -784,7 +781,6 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
             }
         }
         l = l * f + sum;
-        const float fo = E16 ? f * fe : f;
         if constexpr (K8) {
 #pragma unroll
             for (int u = 0; u < NU; u += 2) {           // two dims of eight keys: the keys' bytes in pairs
@@ -792,11 +788,11 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
                     const uint32_t x = __builtin_amdgcn_perm(vr[2 * j + 1][u >> 2], vr[2 * j][u >> 2], u & 2 ? 0x07030602u : 0x05010400u);
-                    va[0][0][j] = att_code2<MT>(x, 0);
-                    va[1][0][j] = att_code2<MT>(x, 1);
+                    va[0][0][j] = att_code2<VT>(x, 0);
+                    va[1][0][j] = att_code2<VT>(x, 1);
                 }
-                o[u] = att_planes16<MT, 1, NQ>(va[0], pb, o[u] * fo);
-                o[u + 1] = att_planes16<MT, 1, NQ>(va[1], pb, o[u + 1] * fo);
+                o[u] = att_planes16<VT, 1, NP>(va[0], pb, o[u] * f);
+                o[u + 1] = att_planes16<VT, 1, NP>(va[1], pb, o[u + 1] * f);
             }
         } else
 #pragma unroll
@@ -812,7 +808,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
                 for (int j = 0; j < 4; j++)
                     va[0][j] = __builtin_amdgcn_perm(vr[2 * j + 1][u >> 1], vr[2 * j][u >> 1], u & 1 ? 0x07060302u : 0x05040100u);
             }
-            o[u] = att_planes16<MT, NK, NQ>(va, pb, o[u] * fo);
+            o[u] = att_planes16<MT, NK, NQ>(va, pb, o[u] * f);
         }
     }
     l = att_sum4(l);
@@ -822,7 +818,7 @@ __global__ __launch_bounds__(64 * ATT_WV) __attribute__((amdgpu_waves_per_eu(siz
         float M = -INFINITY;
 #pragma unroll
         for (int w = 0; w < ATT_WV; w++) M = fmaxf(M, sst[0][w][li]);
-        const float f = (M == -INFINITY ? 0.f : qt_exp2((m - M) * a.c)) * (E16 ? __uint_as_float(ev << 23) : 1.f);
+        const float f = M == -INFINITY ? 0.f : qt_exp2((m - M) * a.c);
         float *os = reinterpret_cast<float *>(sm + wave * OB) + li * HD;
 #pragma unroll
         for (int i = 0; i < 4; i++)
@@ -901,15 +897,17 @@ __device__ __forceinline__ void att_wait() { asm volatile("s_waitcnt vmcnt(0)" :
 
 //
 // Over e4m3 codes a block's bytes are copied into LDS as they are, and a step later each thread widens what its own wave copied, a quarter of
-// a row, to T in its place: K two blocks ahead, V one, after the products, when the scores' registers are free.  bf16 takes a row's
-// value as it is, its scale in the conversion.  f16, whose range is small, takes K relative to the block's largest scale (ek), which the
-// scores are multiplied by, and V relative to the largest so far (ev), which the sums carry.  6 chunks of 100 to 1024 over up to 6000 keys
+// a row, in its place: K two blocks ahead, V one, after the products, when the scores' registers are free.  bf16 takes a row's
+// value as it is, its scale in the conversion.  f16's range is too small for that: f16 rows take K's codes alone as f16, each score times
+// its key's scale, and V as bf16, values as they are, with the probabilities in two bf16 planes (within 2^-17 of them): no key's scale
+// touches what another one gives (chunks 213 us, trees 145, on a card where bf16 rows take 164 and 115).  6 chunks of 100 to 1024 over up to 6000 keys
 // bf16: 167 us with the merge (over bf16 157; with the codes in registers for a step, which spills, 352).  Trees: 32 of 33 to 64 tokens over 500
 // to 6000 keys of codes 127; bound by the vector unit's work on tiles of uneven length.
 template <typename T, int HD, bool PAGED, typename KT = T, bool TREE = false>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k_att_tile(AttArgs a) {
     constexpr int NT = HD / 32, NS = HD / 16, RB = 2 * HD, CPR = RB / 16, RPC = 64 / CPR, NC = 64 / RPC / 4;
     constexpr bool K8 = sizeof(typename KT::elem) == 1, E16 = K8 && std::is_same<T, QtF16>::value;
+    typedef typename std::conditional<E16, QtBf16, T>::type VT;             // of V's product
     __shared__ __align__(16) uint8_t sk[2 * 64 * RB], sv[3 * 64 * RB];      // K8: of sv the last third is codes, 64 rows of K, 64 of V
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63, lr = lane & 31, h = lane >> 5;
     const int head = blockIdx.x % a.nkv, slot = blockIdx.x / a.nkv, split = blockIdx.y;
@@ -968,13 +966,14 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     int page = -1;                                                       // PAGED: of key 64 kb + lane, block kb the next to copy
     unsigned long long okv = ~0ull, okk = ~0ull, okn = ~0ull;            // keys that exist: of the block of V, of K, of the next K
     // e4m3.  locate: where a block's codes and scales lie, of row 16 wave + lane / 4 from chunk lane % 4 on, and of key 64 kb + lane.
-    // copy_codes: from there to `to`, chunks lane % 4 + 4 e of 16 codes, and the scale.  widen: codes into a buffer, relative to 2^(rel - 127).
+    // copy_codes: from there to `to`, chunks lane % 4 + 4 e of 16 codes, and the scale.  widen: codes into a buffer.
     const unsigned lk = att_lds(sk), lv = att_lds(sv);
     uint8_t *const rawk = sv + 2 * 64 * RB, *const rawv = rawk + 64 * HD;
     struct Where { long long codes, scale; };
     Where next_v = {0, 0};                                               // of the block whose V is the next to copy
     unsigned long long ok_v = 0;
-    uint32_t gks = 0, gvs = 0, ekv = 0, ekk = 0, ekn = 0, evn = QT_SCALE_MIN, evo = QT_SCALE_MIN;   // E16: of K of this block, the next ones; of V, of o
+    uint32_t gks = 0, gvs = 0;
+    float ksv = 1.f, ksk = 1.f, ksn = 1.f;                               // E16: the scale of key `lane` of this block, of the next ones
     const auto locate = [&](int kb, int pg) {
         int ln = lane;
         asm volatile("" : "+v"(ln));                                     // addresses are formed here: held over the loop they spill
@@ -1005,9 +1004,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     const uint8_t *const kscale = a.ksc + head * a.ss_head, *const vscale = a.vsc + head * a.ss_head;
     const int wrow = 16 * wave + (lane >> 2);
     // (a lane's chunks 2 (lane % 4) + 8 e + x: bits of their own)
-    const auto widen = [&](const uint8_t *from, uint32_t sc, int swizzle, uint8_t *buf, uint32_t rel) {
-        float f = qt_scale_of((uint32_t)__shfl((int)sc, wrow));
-        if constexpr (E16) f *= __uint_as_float((254u - rel) << 23);
+    const auto widen = [&](const uint8_t *from, float f, int swizzle, uint8_t *buf, auto type) {
         const int at = wrow * RB + 16 * ((2 * (lane & 3)) ^ swizzle);
 #pragma unroll
         for (int e = 0; e < HD / 64; e++) {
@@ -1016,18 +1013,17 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             for (int x = 0; x < 2; x++) {
                 qt_u32x4 w;
 #pragma unroll
-                for (int i = 0; i < 4; i++) w[i] = att_code2<T>(c[2 * x + (i >> 1)], i & 1, f);
+                for (int i = 0; i < 4; i++) w[i] = att_code2<decltype(type)>(c[2 * x + (i >> 1)], i & 1, f);
                 *reinterpret_cast<qt_u32x4 *>(buf + (at ^ 16 * (8 * e + x))) = w;
             }
         }
     };
     const auto widen_k = [&](const uint8_t *from, uint32_t sc, uint8_t *buf) {
-        if constexpr (E16) ekn = (uint32_t)max(wave_max_i((int)qt_scale_read(sc)), (int)QT_SCALE_MIN);
-        widen(from, sc, att_swk<HD>(wrow), buf, ekn);
+        if constexpr (E16) ksn = qt_scale_of(sc);
+        widen(from, E16 ? 1.f : qt_scale_of((uint32_t)__shfl((int)sc, wrow)), att_swk<HD>(wrow), buf, T());
     };
     const auto widen_v = [&](const uint8_t *from, uint32_t sc, uint8_t *buf) {
-        if constexpr (E16) evn = max(evn, (uint32_t)wave_max_i((int)qt_scale_read(sc)));
-        widen(from, sc, att_swv<HD>(wrow), buf, evn);
+        widen(from, qt_scale_of((uint32_t)__shfl((int)sc, wrow)), att_swv<HD>(wrow), buf, VT());
     };
     const auto page_of = [&](int kb) { return kb < kb1 ? att_page(a, table, t, 64 * kb + lane) : -1; };
     // block kb to a K and a V buffer
@@ -1092,10 +1088,12 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
         __syncthreads();
         okv = okk;
         okk = okn;
-        float pk = 1.f;                                                  // E16: of this block's scores
         if constexpr (E16) {
-            ekv = ekk; ekk = ekn;
-            pk = __uint_as_float(ekv << 23);
+            ksv = ksk; ksk = ksn;
+            // lane i of each row of 16 gets the scale of the key that register i holds there
+            const int from = 8 * ((lane & 15) >> 2) + 4 * h + (lane & 3);
+#pragma unroll
+            for (int kt = 0; kt < 2; kt++) att_keys(sc[kt], __shfl(ksv, 32 * kt + from), std::make_integer_sequence<int, 16>{});
         }
         const uint8_t *vbuf = sv + (K8 ? BUF : vb) * 64 * RB;
         if constexpr (!K8) {
@@ -1130,21 +1128,15 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
             for (int i = 0; i < 16; i++) bm = fmaxf(bm, sc[kt][i]);
         bm = fmaxf(bm, att_other_half(bm));
-        if constexpr (E16) bm *= pk;
         // probabilities up to 2^8 are as good as up to 1: the sums shrink only when a row's maximum has risen by more
-        if (__ballot((bm - m) * a.c > 8.0f || (m == -INFINITY && bm > m)) || (E16 && evn != evo)) {
+        if (__ballot((bm - m) * a.c > 8.0f || (m == -INFINITY && bm > m))) {
             const float mn = fmaxf(m, bm), f = mn == -INFINITY ? 0.f : qt_exp2((m - mn) * a.c);
-            float fo = f;
-            if constexpr (E16) {
-                fo *= __uint_as_float((127u + evo < evn ? 0u : 127u + evo - evn) << 23);
-                evo = evn;
-            }
             m = mn;
             l *= f;
 #pragma unroll
             for (int d = 0; d < NT; d++)
 #pragma unroll
-                for (int i = 0; i < 16; i++) o[d][i] *= fo;
+                for (int i = 0; i < 16; i++) o[d][i] *= f;
         }
         const float mc = m == -INFINITY ? 0.f : m * a.c;
         if (kb + 1 < kb1) scores(sn, sk + (BUF ^ 1) * 64 * RB);
@@ -1166,21 +1158,32 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
 #pragma unroll
         for (int kt = 0; kt < 2; kt++)
 #pragma unroll
-            for (int i = 0; i < 16; i++) sc[kt][i] = qt_exp2(fmaf(sc[kt][i], E16 ? a.c * pk : a.c, -mc));
+            for (int i = 0; i < 16; i++) sc[kt][i] = qt_exp2(fmaf(sc[kt][i], a.c, -mc));
 #pragma unroll
         for (int s = 0; s < 4; s++) {
-            qt_u32x4 pb;
+            qt_u32x4 pb[E16 ? 2 : 1];
             float sum = 0.f;
+            if constexpr (E16) {
+                float p[8];
 #pragma unroll
-            for (int j = 0; j < 4; j++) {
-                pb[j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
-                sum = att_add2<T>(pb[j], sum);
+                for (int j = 0; j < 8; j++) {
+                    p[j] = sc[s >> 1][8 * (s & 1) + j];
+                    sum += p[j];
+                }
+                att_planes2(p, pb);
+            } else {
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    pb[0][j] = qt_round2<T>(sc[s >> 1][8 * (s & 1) + 2 * j], sc[s >> 1][8 * (s & 1) + 2 * j + 1]);
+                    sum = att_add2<T>(pb[0][j], sum);
+                }
             }
             l += sum;
 #pragma unroll
             for (int d = 0; d < NT; d++) {
                 const uint16_t *vp = reinterpret_cast<const uint16_t *>(vbuf + 16 * s * RB + va[d]);
-                o[d] = att_mma<T>(qt_lds_tr8x2(vp, vp + 8 * HD), pb, o[d]);
+                const qt_u32x4 v[1] = {qt_lds_tr8x2(vp, vp + 8 * HD)};
+                o[d] = att_planes<VT>(v, pb, o[d]);
             }
         }
     };
@@ -1201,7 +1204,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
             }
             att_wait();
             widen_k(rawk, gks, sk);
-            ekk = ekn;
+            ksk = ksn;
             widen_v(sv + 64 * RB, gvs, sv);
             if (kb0 + 1 < kb1) widen_k(rawv, gk1, sk + 64 * RB);
             asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
@@ -1236,13 +1239,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2))) void k
     }
     // the rows' results; o[d][i] is dim 32 d + 8 (i / 4) + 4 h + i % 4
     l += att_other_half(l);
-    if constexpr (E16) {
-        const float f = __uint_as_float(evo << 23);
-#pragma unroll
-        for (int d = 0; d < NT; d++)
-#pragma unroll
-            for (int i = 0; i < 16; i++) o[d][i] *= f;
-    }
     float chk = l;
 #pragma unroll
     for (int d = 0; d < NT; d++)

@@ -1151,3 +1151,71 @@ def test_two_calls_at_once_have_their_own_workspaces(what):
             with torch.cuda.stream(st):
                 got.append(v.run())
     assert all(g == want[i % 2] for i, g in enumerate(got))
+
+
+# ---- what a row does not see, in finite numbers ------------------------------------------------------
+
+
+def rows_close(got, s, rows):
+    """The rows of truth values `rows` against 64 bits."""
+    exact, mag = s.want()
+    close(got.cpu()[rows], exact[rows], mag[rows], s.t, max(a + n for a, n in s.reqs), float(max(v.abs().max() for _, v in s.kv)))
+
+
+@pytest.mark.parametrize("t", ROWS)
+@pytest.mark.parametrize("n", [9, 64])
+@pytest.mark.parametrize("what", ["later", "sibling", "window", "bad page"])
+@HINTS
+def test_codes_of_large_scales_that_a_row_does_not_see(t, n, what, max_kv):
+    """A key with the largest scale there is, finite, that rows do not see, or at the place that stands in for keys in bad pages: in
+    k, then in v, those rows stay as they are."""
+    print(f"[case] hidden scales {t} n={n} {what} max_kv={max_kv}", flush=True)
+    rows = torch.ones(n, dtype=torch.bool)
+    if what == "sibling":
+        g = torch.Generator().manual_seed(3)
+        see, depth = closure(random_tree(n, 3, g))
+        s = Steps([(70, n)], 4, 2, 64, t, "e4m3", 16, "head", seed=6, words=2, masks=[(see, depth)], max_kv=max_kv)
+        p, o, rows = s.rows[0][0][74], s.rows[0][1][74], ~see[:, 4]
+    elif what == "bad page":
+        s = Steps([(200, n)], 4, 2, 64, t, "e4m3", 16, "head", seed=0, max_kv=max_kv)
+        p, o = 0, 0
+        assert not bool((s.rows[0][0] == 0).any())                           # page 0 is no request's
+        for x, y in zip(s.pools, (0x30, 127, 0x30, 127)):
+            x[0, :, 0] = y
+        s.table[0, 4:8] = -1
+        see = see_of(n, 200 + n, 0)
+        see[:, 64:128] = False
+        s.want = lambda: attend_see(s.q, *s.kv[0], see, s.scale)
+    else:
+        s = Steps([(90, n)], 4, 2, 64, t, "e4m3", 16, "head", seed=7, max_kv=max_kv, window=80 if what == "window" else 0)
+        at = 5 if what == "window" else 89 + n
+        p, o = s.rows[0][0][at], s.rows[0][1][at]
+        if what == "later":
+            rows[-1] = False
+    assert bool(rows.any())
+    for which in (1, 3):                                                      # of k, of v
+        before = s.pools[which].clone()
+        s.pools[which][p, :, o] = 246
+        rows_close(s.run(), s, rows)
+        s.pools[which].copy_(before)
+
+
+@pytest.mark.parametrize("t", ROWS)
+@pytest.mark.parametrize("reqs", [[(700, 1), (30, 1)], [(200, 9), (64, 64)], [(0, 300)]])
+@HINTS
+def test_keys_of_large_scales_that_weigh_nothing(t, reqs, max_kv):
+    """A key whose score is far under the others' and whose scales are 2^40 and 2^60 times theirs: the others keep their scores and values."""
+    s = Steps(reqs, 4, 2, 64, t, "e4m3", 16, "head", seed=12, max_kv=max_kv)
+    s.q = s.q.abs()
+    s.qd[:, :4 * 64] = s.q.reshape(s.T, -1).to(DEV)
+    for b in range(len(reqs)):
+        (p, o), (k, v) = s.rows[b], s.kv[b]
+        for at in (1, min(70, sum(reqs[b]) - 2)):
+            s.pools[0][p[at], :, o[at]], s.pools[1][p[at], :, o[at]] = 0xB8, 167   # -1 times 2^40
+            s.pools[2][p[at], :, o[at]], s.pools[3][p[at], :, o[at]] = 0x38, 187   # 1 times 2^60
+            k[at], v[at] = -2.0 ** 40, 2.0 ** 60
+    got = s.run()
+    exact, mag = s.want()
+    rows = torch.cat([torch.arange(n) + a > 1 for a, n in reqs])               # (the first two rows of a request see little else)
+    vmax = max(float(v[v.abs() < 2.0 ** 59].abs().max()) for _, v in s.kv)
+    close(got.cpu()[rows], exact[rows], mag[rows], t, max(a + n for a, n in reqs), vmax)
