@@ -638,8 +638,10 @@ int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *verify, void *stream);
  * Lengths and pages, where kv_len_out is given: kv_len_out[b] = kv_len[b] - n + n_path[b], and the pages of the table that it no
  * longer reaches go onto the free list's end in the order of requests and positions, as page_plan gives pages back; the table itself is
  * left as it is.  status 0; QWEN_HIP_PLAN_INVALID where a length is negative, under n or past the table, or more would be free than
- * there are pages: then lengths and free list are not changed (kv_len_out and n_free_out hold what kv_len and n_free hold).  Without kv_len_out
- * rows are moved only, for layers that lie apart: a call each, lengths and pages with one of them, the last where kv_len_out is kv_len. */
+ * there are pages: then lengths and free list are not changed (kv_len_out and n_free_out hold what kv_len and n_free hold), and no request's rows
+ * are moved.  Without kv_len_out rows are moved only, for layers that lie apart: a call each, lengths and pages with one of them, the last where
+ * kv_len_out is kv_len.  Such a call moves nothing where a request's length cannot be, and does not look at the free list.  Rows are moved once a step: the same moves
+ * over again are others. */
 typedef struct {
     const int *path, *n_path;       /* [T], [B] */
     const int *cu_q, *kv_len;       /* [B + 1], [B]: with the new tokens */

@@ -553,12 +553,16 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
 // ---- what is kept ----------------------------------------------------------------------------------
 // Row path[k] goes to place k.  Since path[k] >= k, a place that has been written is no later row's source: a thread that takes 16
 // bytes of a head's rows, or a head's scales, through all moves in the order of k, eight loads before their stores, reads every source before it
-// is overwritten, and no two threads share bytes.  A workgroup takes a request's rows in one layer.  Lengths and pages: one workgroup more,
-// or a launch of its own where it replaces lengths that the moves read.
-// Bound by the latency of path, table, rows for few (8 requests, one layer of bf16: 6.4 us a pass, the kernel 3.5), by the rows' bytes for many
-// layers (64 requests, 28 layers of codes: 16.0, the kernel 14.4; with four loads before their stores and scales after the codes 18.0 and 17.4).
+// is overwritten, and no two threads share bytes.  A workgroup takes a request's rows in one layer.  Lengths and pages: one workgroup.
+// Moves done twice are not moves done once, so a commit that cannot be moves nothing.  While that is CM_LOOK looks in all, each workgroup looks at all requests
+// first (commit_stands), and the lengths' workgroup is one more of the launch; past it, and where lengths or the count are replaced in place, the lengths'
+// launch is before the moves', which go by its status (bf16, 2 heads of 64, one launch and two: 300 requests of 8 layers 8.0 and 9.6 us, 1024 of one 7.5
+// and 9.8, 512 of 8 11.8 and 11.1, 300 of 28 18.5 and 14.5; without looking 512 of 8 7.2).
+// Bound by the latency of lengths, path, table, rows for few (8 requests, one layer of bf16: 6.7 us a pass), by the rows' bytes for many
+// layers (64 requests, 28 layers of codes: 15.2; without the look at all requests 13.9).
 #define CM_T 256
 #define CM_MAX_B 2048
+#define CM_LOOK (1 << 20)
 struct CommitArgs {
     const int *path, *n_path, *cu, *kv, *table, *n_free;
     long long ts;
@@ -567,6 +571,8 @@ struct CommitArgs {
     long long layer, page, head, slot, s_layer, s_page, s_head, s_slot;
     int B, T, cols, ps, n_pages, layers, nkv, row;      // row: bytes of a head's row
     int moves, lengths;                                 // this launch moves rows; makes lengths and pages
+    int made;                                           // lengths and status are there: kv_out is of after the moves
+    int count;                                          // the call makes them: its moves look at the free list's count, too
     QtDiv div;
 };
 
@@ -574,6 +580,35 @@ __device__ __forceinline__ int commit_kept(const CommitArgs &a, int b, int n) { 
 // whether a request's lengths are ones that a table can hold
 __device__ __forceinline__ bool commit_fits(const CommitArgs &a, int kv, int n) { return kv >= n && (long long)kv <= (long long)a.cols * a.ps; }
 __device__ __forceinline__ int commit_pages(const CommitArgs &a, int len) { return qt_quot(len, a.div) + (len % a.ps != 0); }
+
+// The pages that a request gives back; `bad` where its lengths cannot be.
+__device__ __forceinline__ unsigned commit_back(const CommitArgs &a, int b, bool &bad) {
+    const int n = tree_req(a.cu, b, a.T).n, kv = a.kv[b], kept = commit_kept(a, b, n);
+    if (commit_fits(a, kv, n)) return commit_pages(a, kv) - commit_pages(a, kv - n + kept);
+    bad = true;
+    return 0;
+}
+// A workgroup: whether the call is one that can be, by what commit_lengths refuses.
+__device__ __forceinline__ bool commit_stands(const CommitArgs &a) {
+    __shared__ unsigned long long wsum[CM_T / 64];
+    bool bad = false;
+    if (!a.count) {                                     // rows only: lengths alone
+        for (int b = threadIdx.x; b < a.B; b += CM_T) bad |= !commit_fits(a, a.kv[b], tree_req(a.cu, b, a.T).n);
+        return !__syncthreads_or(bad);
+    }
+    const int n_free = a.n_free[0];
+    unsigned long long mine = 0;                        // 2048 requests of 2^30 pages at most
+    bad = n_free < 0 || n_free > a.n_pages;
+    for (int b = threadIdx.x; b < a.B; b += CM_T) mine += commit_back(a, b, bad);
+#pragma unroll
+    for (int o = 32; o; o >>= 1) mine += __shfl_xor(mine, o, 64);
+    if ((threadIdx.x & 63) == 0) wsum[threadIdx.x >> 6] = mine;
+    bad = __syncthreads_or(bad);
+    unsigned long long all = max(n_free, 0);
+#pragma unroll
+    for (int w = 0; w < CM_T / 64; w++) all += wsum[w];
+    return !bad && all <= (unsigned long long)a.n_pages;
+}
 
 // A piece of every row through n moves.
 template <typename V> __device__ __forceinline__ void commit_piece(uint8_t *base, int n, const long long *from, const long long *to) {
@@ -592,8 +627,8 @@ __device__ __forceinline__ void commit_move(const CommitArgs &a, int b, int laye
     __shared__ long long from[2][CM_T], to[2][CM_T];    // of codes, of scales
     __shared__ int moves_s[CM_T / 64];
     const TreeReq r = tree_req(a.cu, b, a.T);
-    const int kv = a.kv[b], keep = commit_kept(a, b, r.n), lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (!commit_fits(a, kv, r.n)) return;
+    const int keep = commit_kept(a, b, r.n), kv = a.made ? a.kv_out[b] + r.n - keep : a.kv[b], lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (a.made ? a.status[0] != 0 : !commit_stands(a)) return;
     const int *table = a.table + b * a.ts;
     for (int k0 = 0; k0 < keep; k0 += CM_T) {
         const int k = k0 + threadIdx.x;
@@ -645,12 +680,7 @@ __device__ __forceinline__ void commit_lengths(const CommitArgs &a) {
     const int per = (a.B + CM_T - 1) / CM_T, b0 = min((int)threadIdx.x * per, a.B), b1 = min(b0 + per, a.B);
     unsigned long long mine = 0;
     bool bad = n_free < 0 || n_free > a.n_pages;
-    for (int b = b0; b < b1; b++) {
-        const int n = tree_req(a.cu, b, a.T).n, kv = a.kv[b];
-        if (!commit_fits(a, kv, n)) bad = true;
-        else mine += commit_pages(a, kv) - commit_pages(a, kv - n + commit_kept(a, b, n));
-    }
-    bad |= mine > (unsigned long long)a.n_pages;
+    for (int b = b0; b < b1; b++) mine += commit_back(a, b, bad);
     unsigned long long upto = mine;                     // 2048 requests of 2^30 pages at most
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
@@ -730,17 +760,17 @@ extern "C" int qwen_hip_op_tree_commit(const qwen_hip_kv_pages_t *kv, const qwen
     a.B = p->B; a.T = p->T; a.cols = p->table_cols; a.ps = kv->page_size; a.n_pages = kv->n_pages; a.layers = p->n_layers;
     a.nkv = kv->n_kv_heads; a.row = kv->head_dim * E;
     a.div = qt_div_of(kv->page_size);
-    const bool in_place = p->kv_len_out == p->kv_len;
-    const bool apart = p->kv_len_out && in_place && p->n_layers > 0 && p->T > 0;         // lengths in a launch of their own
-    a.moves = p->n_layers > 0 && p->T > 0;
-    a.lengths = p->kv_len_out && !apart;
-    const unsigned wgs = (unsigned)(a.moves ? p->n_layers * p->B : 0);
+    const bool in_place = p->kv_len_out == p->kv_len || p->n_free_out == p->n_free;
+    const bool moves = p->n_layers > 0 && p->T > 0, first = p->kv_len_out && moves && (in_place || (long long)p->n_layers * p->B * p->B > CM_LOOK);     // lengths in a launch before the moves'
+    a.moves = moves && !first;
+    a.lengths = a.count = p->kv_len_out != nullptr;
+    const unsigned wgs = (unsigned)(moves ? p->n_layers * p->B : 0);
     hipError_t e = hipSuccess;
-    if (wgs || a.lengths) e = qt_launch(k_tree_commit, dim3(wgs + (a.lengths ? 1 : 0)), dim3(CM_T), 0, st, a);
-    if (e == hipSuccess && apart) {
-        a.moves = 0;
-        a.lengths = 1;
-        e = qt_launch(k_tree_commit, dim3(1), dim3(CM_T), 0, st, a);
+    if (a.moves || a.lengths) e = qt_launch(k_tree_commit, dim3((a.moves ? wgs : 0) + (a.lengths ? 1 : 0)), dim3(CM_T), 0, st, a);
+    if (e == hipSuccess && first) {
+        a.moves = a.made = 1;
+        a.lengths = 0;
+        e = qt_launch(k_tree_commit, dim3(wgs), dim3(CM_T), 0, st, a);
     }
     QT_REFUSE(e != hipSuccess, "tree_commit: launch failed: %s", hipGetErrorString(e));
     return 0;

@@ -1219,3 +1219,73 @@ def test_keys_of_large_scales_that_weigh_nothing(t, reqs, max_kv):
     rows = torch.cat([torch.arange(n) + a > 1 for a, n in reqs])               # (the first two rows of a request see little else)
     vmax = max(float(v[v.abs() < 2.0 ** 59].abs().max()) for _, v in s.kv)
     close(got.cpu()[rows], exact[rows], mag[rows], t, max(a + n for a, n in reqs), vmax)
+
+
+# ---- a commit is whole or not at all -----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("what,how", [(w, h) for h in ("apart", "in place", "count in place") for w in ("n_free", "full", "negative", "short", "long")] +
+                         [(w, "rows only") for w in ("negative", "short", "long")])
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_a_commit_that_cannot_be_moves_nothing(cache, what, how):
+    c = Commit([(5, 9, 4), (20, 12, 2), (0, 3, 3)] + [(9, 5, 2)] * 300, cache, 2, 2, 64, 4, "head", seed=7)
+    if what == "n_free":
+        c.n_free = c.n_pages + 1
+    elif what == "full":
+        c.n_free = c.n_pages
+    else:
+        c.kvl[290] = {"negative": -3, "short": 4, "long": c.cols * 4 + 1}[what]
+    before = [x.clone() for x in c.pools]
+    if how == "count in place":                         # the free count is replaced, the lengths are not
+        keep = hip.TreeCommit
+
+        def one(**kw):
+            kw["n_free_out"] = kw["n_free"]
+            return keep(**kw)
+        try:
+            hip.TreeCommit = one
+            got = c.run()
+        finally:
+            hip.TreeCommit = keep
+        assert got["kv"] == c.kvl and got["status"] == hip.PLAN_INVALID
+    else:
+        got = c.run(in_place=how == "in place", lengths=how != "rows only")
+        if how != "rows only":
+            assert got == dict(kv=c.kvl, n_free=c.n_free, free=c.free, status=hip.PLAN_INVALID, table=c.table)
+    assert all(torch.equal(x, y) for x, y in zip(c.pools, before))
+
+
+@pytest.mark.parametrize("cache", ["bf16", "e4m3"])
+def test_a_commit_whose_free_count_is_replaced(cache):
+    """The count in place, lengths apart: rows, lengths and pages as ever, many requests and layers."""
+    for seed in range(4):
+        c = Commit([(20 + b % 50, 1 + b % 17, (1 + b % 17) // 3) for b in range(150)], cache, 4, 2, 64, 4, "head", seed=seed)
+        pools, want = c.want()
+        keep = hip.TreeCommit
+        out = {}
+
+        def one(**kw):
+            kw["n_free_out"] = kw["n_free"]
+            out["d"] = kw["n_free"]
+            return keep(**kw)
+        try:
+            hip.TreeCommit = one
+            got = c.run()
+        finally:
+            hip.TreeCommit = keep
+        assert {k: v for k, v in got.items() if k != "n_free"} == {k: v for k, v in want.items() if k != "n_free"}
+        for x, y in zip(c.pools, pools):
+            assert torch.equal(x.cpu(), y)
+
+@pytest.mark.parametrize("layers", [1, 3])
+@pytest.mark.parametrize("in_place", [False, True])
+def test_commits_of_many_requests(layers, in_place):
+    """Enough of them that lengths are made before the rows are moved: whole, and one that cannot be."""
+    reqs = [(b % 40, 1 + b % 7, (1 + b % 7) // 2) for b in range(1500)]
+    Commit(reqs, "e4m3", layers, 1, 64, 4, "head", seed=6).check(in_place=in_place)
+    c = Commit(reqs, "e4m3", layers, 1, 64, 4, "head", seed=6)
+    c.kvl[1400] = -1
+    before = [x.clone() for x in c.pools]
+    got = c.run(in_place=in_place)
+    assert got == dict(kv=c.kvl, n_free=c.n_free, free=c.free, status=hip.PLAN_INVALID, table=c.table)
+    assert all(torch.equal(x, y) for x, y in zip(c.pools, before))
