@@ -574,7 +574,8 @@ int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_pag
 
 /* parent[t]: token t's parent as an index within its request's new tokens, less than its own index; anything else makes t a
  * root.  Request b's tokens are cu_q[b] .. cu_q[b+1] - 1, kv_len counts them.  Written for each: pos[t] = kv_len[b] - n + depth (roots: 0), and
- * mask[t*mask_stride + w], w < mask_words: bit i is set where new token 32 w + i of the request is t or one of its ancestors.
+ * mask[t*mask_stride + w], w < mask_words: bit i is set where new token 32 w + i of the request is t or one of its ancestors (window > 0: fewer
+ * than window steps up, as the window of attention has it).
  * A request of more than 32 * mask_words new tokens is a plain chunk of text: each token at the position behind the one before, its masks
  * not written, nor read by tree_attention.  Rows before cu_q[0] and behind cu_q[B] stay as they were.  mask_words <= 32. */
 typedef struct {
@@ -585,13 +586,14 @@ typedef struct {
     uint32_t *mask;          /* [T][mask_stride] */
     long long mask_stride;   /* words, >= mask_words */
     int B, T, mask_words;
+    int window;              /* 0: none */
 } qwen_hip_tree_plan_t;
 int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *plan, void *stream);
 
 /* qwen_hip_op_page_attention for steps with trees: a row sees all positions before its request's new tokens, and of those the ones
  * whose bits are set in its mask; a request of more than 32 * mask_words new tokens is causal as there.  With attn->window > 0
  * a row sees those positions before the new tokens that are greater than pos[t] - window (pos brought into kv_len - n .. kv_len - 1), and the mask
- * alone decides on the new ones; pos may be NULL without a window.  Any mask will do: a row without bits sees only what is before.
+ * alone decides on the new ones: tree_plan with the same window leaves out what lies before it; pos may be NULL without a window.  Any mask will do: a row without bits sees only what is before.
  * Everything else, the workspace too (qwen_hip_op_page_attention_workspace), is as there. */
 typedef struct {
     const uint32_t *mask;    /* [T][mask_stride] */

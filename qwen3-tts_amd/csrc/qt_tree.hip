@@ -14,14 +14,14 @@ __device__ __forceinline__ TreeReq tree_req(const int *cu, int b, int T) {
 
 // ---- positions and masks ---------------------------------------------------------------------------
 // A workgroup a request.  A token walks up through its parents, held in LDS: they have smaller indices, so the words of its mask
-// come from the highest down and each is stored once.  Bound by the launch (8 requests of 5 to 16 tokens and 512 of 1 to 61 both 6.1 us a pass, the
+// come from the highest down and each is stored once; `window` steps up and further its ancestors are counted only.  Bound by the launch (8 requests of 5 to 16 tokens and 512 of 1 to 61 both 6.1 us a pass, the
 // kernel 2.7 and 4.4).
 struct TreePlanArgs {
     const int *parent, *cu, *kv;
     int *pos;
     uint32_t *mask;
     long long ms;
-    int T, words;
+    int T, words, window;
 };
 
 __global__ __launch_bounds__(256) void k_tree_plan(TreePlanArgs a) {
@@ -46,7 +46,7 @@ __global__ __launch_bounds__(256) void k_tree_plan(TreePlanArgs a) {
         for (int j = up[i]; j >= 0; j = up[j]) {
             depth++;
             for (; w > j >> 5; w--) { m[w] = bits; bits = 0u; }
-            bits |= 1u << (j & 31);
+            if (depth < a.window) bits |= 1u << (j & 31);
         }
         for (; w >= 0; w--) { m[w] = bits; bits = 0u; }
         a.pos[r.q0 + i] = first + depth;
@@ -59,6 +59,7 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
     QT_REFUSE(p->T < 0 || p->T > 1 << 26, "tree_plan: T %d out of range (0..2^26)", p->T);
     QT_REFUSE(p->mask_words < 1 || p->mask_words > 32 || p->mask_stride < p->mask_words,
               "tree_plan: mask_words %d of stride %lld (1..32, the stride at least as many)", p->mask_words, p->mask_stride);
+    QT_REFUSE(p->window < 0, "tree_plan: window %d is negative", p->window);
     if (p->B == 0 || p->T == 0) return 0;
     QT_REFUSE(!p->parent || !p->cu_q || !p->kv_len || !p->pos || !p->mask, "tree_plan: null pointer");
     const long long T = p->T, B = p->B;
@@ -69,7 +70,7 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
     const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "tree_plan: the stream's device: %s", hipGetErrorString(on.err));
-    const TreePlanArgs a = {p->parent, p->cu_q, p->kv_len, p->pos, p->mask, p->mask_stride, p->T, p->mask_words};
+    const TreePlanArgs a = {p->parent, p->cu_q, p->kv_len, p->pos, p->mask, p->mask_stride, p->T, p->mask_words, p->window > 0 ? p->window : 1024};      // (no token has as many above it)
     const hipError_t e = qt_launch(k_tree_plan, dim3(p->B), dim3(p->mask_words > 4 ? 256 : p->mask_words > 2 ? 128 : 64), 0, st, a);
     QT_REFUSE(e != hipSuccess, "tree_plan: launch failed: %s", hipGetErrorString(e));
     return 0;

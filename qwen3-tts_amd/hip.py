@@ -133,7 +133,7 @@ class LogitRules(C.Structure):
 
 class TreePlan(C.Structure):
     _fields_ = [(n, C.c_void_p) for n in ("parent", "cu_q", "kv_len", "pos", "mask")] + [("mask_stride", C.c_longlong)] + \
-               [(n, C.c_int) for n in ("B", "T", "mask_words")]
+               [(n, C.c_int) for n in ("B", "T", "mask_words", "window")]
 
 
 class Tree(C.Structure):

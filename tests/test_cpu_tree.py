@@ -196,3 +196,7 @@ def test_errors_name_the_call():
                    (lambda a: L.qwen_hip_op_tree_attention(C.byref(pages()), C.byref(a), C.byref(tree()), None), "tree_attention")):
         for kw in (dict(scale=0.0), dict(q=None), dict(out_stride=1024), dict(max_kv=1 << 16, workspace=None)):
             refused(f(attn(**kw)), who + ":")
+
+
+def test_tree_plan_refuses_a_window_under_none():
+    refused(hip.lib().qwen_hip_op_tree_plan(C.byref(tree_plan(window=-1)), None), "window")

@@ -1221,6 +1221,48 @@ def test_keys_of_large_scales_that_weigh_nothing(t, reqs, max_kv):
     close(got.cpu()[rows], exact[rows], mag[rows], t, max(a + n for a, n in reqs), vmax)
 
 
+# ---- windows and trees -------------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("lens,words,window", [([7, 1, 30], 1, 1), ([64, 33, 5], 2, 4), ([64, 40], 2, 31), ([300], 10, 33), ([40], 2, 1000), ([33], 1, 2)])
+def test_tree_plan_with_a_window(lens, words, window):
+    """Masks leave out ancestors `window` tokens back and further; positions and chunks are as without."""
+    g = torch.Generator().manual_seed(sum(lens))
+    ups = [random_tree(n, 2, g) for n in lens]
+    kv, cu, T = [n + 7 for n in lens], cu_of(lens), sum(lens)
+    plain, keep = tree_plan(sum(ups, []), cu, kv, T, words, words), hip.TreePlan
+    try:
+        hip.TreePlan = lambda **kw: keep(window=window, **kw)
+        pos, mask = tree_plan(sum(ups, []), cu, kv, T, words, words)
+    finally:
+        hip.TreePlan = keep
+    assert torch.equal(pos, plain[0])
+    for b, up in enumerate(ups):
+        if lens[b] > 32 * words:
+            assert bool((mask[cu[b]:cu[b + 1]] == 7).all())
+            continue
+        see, depth = closure(up)
+        see &= depth[:, None] - depth[None] < window
+        assert torch.equal(mask[cu[b]:cu[b + 1]], words_of(see, words))
+
+
+@pytest.mark.parametrize("t,cache", CACHES)
+@pytest.mark.parametrize("window", [1, 5, 25])
+@HINTS
+def test_windows_over_planned_chains_are_those_of_causal_attention(t, cache, window, max_kv):
+    """Chains longer than the window: the plan's masks and positions give what attention without trees gives."""
+    for reqs in ([(40, 9), (200, 30), (0, 30)], [(100, 64), (0, 50), (300, 40)]):
+        got = Steps(reqs, 8, 4, 128, t, cache, 16, "head", seed=7, window=window, max_kv=max_kv).run().clone()
+        chain = [(torch.ones(n, n).tril().bool(), torch.arange(n)) for _, n in reqs]
+        s = Steps(reqs, 8, 4, 128, t, cache, 16, "head", seed=7, window=window, max_kv=max_kv, words=2, masks=chain)
+        up = i32(sum([list(range(-1, n - 1)) for _, n in reqs], []))
+        s.m.fill_(-1)
+        s.pos.fill_(-1)
+        d = hip.TreePlan(parent=dp(up), cu_q=dp(s.cud), kv_len=dp(s.kvl), pos=dp(s.pos), mask=dp(s.m), mask_stride=3, B=len(reqs), T=s.T, mask_words=2, window=window)
+        ok(hip.lib().qwen_hip_op_tree_plan(C.byref(d), stream()))
+        assert float((s.run().double() - got.double()).abs().max()) <= 2 * torch.finfo(TYPES[t]).eps * float(got.abs().max())
+
+
 # ---- a commit is whole or not at all -----------------------------------------------------------------
 
 
