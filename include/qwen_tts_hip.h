@@ -474,7 +474,7 @@ enum { QWEN_HIP_DT_E4M3 = 16 };      /* of caches only */
  * counts as 63, one over 246 makes the row NaN.  A row is written with the smallest 2^e, e >= -64, for which its largest magnitude is at most 448 2^e, and each
  * element divided by it and rounded once to the nearest code, ties to even: off by at most 2^-4 of its value, or 2^-10 2^e where that is
  * more.  A row with a magnitude of 2^127 or more, infinite or NaN is written as NaN.  The scales' places have to be memory of their
- * own as the rows have, and pages of scales not lie among the codes of a page.  The scale fields are read for E4M3 only. */
+ * own as the rows have, and pages of scales not lie among the codes of a page (of any layer, where a call writes several).  The scale fields are read for E4M3 only. */
 typedef struct {
     void *k, *v;
     long long page_stride, head_stride, slot_stride;

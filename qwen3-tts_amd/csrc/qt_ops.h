@@ -250,6 +250,23 @@ static inline bool qt_dims_meet(const QtDim *d, int n, __int128 left, int row) {
     return (c < d[n - 1].count && -c < d[n - 1].count && qt_dims_meet(d, n - 1, left - c * s, row)) ||
            (c + 1 < d[n - 1].count && -(c + 1) < d[n - 1].count && qt_dims_meet(d, n - 1, left - (c + 1) * s, row));
 }
+// Whether one of the stretches `bw` wide meets one of those `aw` wide, the first of which is `left` before theirs: two of them are left + sum t_i stride_i
+// apart, lo_i <= t_i <= hi_i, the largest stride last.  Those that reach over many strides count as meeting.
+struct QtRange { __int128 stride, lo, hi; };
+static inline bool qt_stretches_meet(const QtRange *d, int n, __int128 left, __int128 aw, __int128 bw) {
+    if (n == 0) return left < aw && -left < bw;
+    const __int128 s = d[n - 1].stride;
+    __int128 least = 0, most = 0;                                     // what the smaller strides add
+    for (int i = 0; i < n - 1; i++) { least += d[i].lo * d[i].stride; most += d[i].hi * d[i].stride; }
+    const auto down = [s](__int128 x) { return x / s - (x % s < 0); };
+    __int128 t = down(-bw - left - most) + 1, end = -down(-(aw - left - least)) - 1;
+    if (t < d[n - 1].lo) t = d[n - 1].lo;
+    if (end > d[n - 1].hi) end = d[n - 1].hi;
+    if (end - t > 8) return true;
+    for (; t <= end; t++)
+        if (qt_stretches_meet(d, n - 1, left + t * s, aw, bw)) return true;
+    return false;
+}
 // rows of `row` units (at k, and `between` units further at v); the strides in units
 static inline int qt_check_rows_apart(const char *who, const char *what, const qwen_hip_kv_pages_t *kv, long long page, long long head, long long slot,
                                       int row, __int128 between, int layers, long long layer) {
@@ -278,19 +295,28 @@ static inline int qt_check_pages_apart(const char *who, const qwen_hip_kv_pages_
     if (qt_check_rows_apart(who, "scale", kv, kv->scale_page_stride, kv->scale_head_stride, kv->scale_slot_stride, 1,
                             (__int128)((intptr_t)kv->v_scale - (intptr_t)kv->k_scale), layers, scale_layer))
         return -1;
-    // a page's codes and a page's scales (of one layer), each as one stretch
-    const __int128 cw = (__int128)(kv->n_kv_heads - 1) * kv->head_stride + (__int128)(kv->page_size - 1) * kv->slot_stride + kv->head_dim;
-    const __int128 sw = (__int128)(kv->n_kv_heads - 1) * kv->scale_head_stride + (__int128)(kv->page_size - 1) * kv->scale_slot_stride + 1;
-    const __int128 st = kv->n_pages > 1 ? kv->page_stride : 1, n = kv->n_pages, sp = kv->scale_page_stride;
+    // A page's codes and a page's scales, each as one stretch, and all pages' as one more where they are of two strides
+    __int128 cw = (__int128)(kv->n_kv_heads - 1) * kv->head_stride + (__int128)(kv->page_size - 1) * kv->slot_stride + kv->head_dim;
+    __int128 sw = (__int128)(kv->n_kv_heads - 1) * kv->scale_head_stride + (__int128)(kv->page_size - 1) * kv->scale_slot_stride + 1;
+    const __int128 pages = kv->n_pages - 1, more = layers - 1;
+    QtRange d[3];
+    int n = 0;
+    if (pages && kv->page_stride == kv->scale_page_stride) {
+        d[n++] = {kv->page_stride, -pages, pages};
+    } else {
+        cw += pages * kv->page_stride;
+        sw += pages * kv->scale_page_stride;
+    }
+    if (more && layer == scale_layer) {
+        d[n++] = {layer, -more, more};
+    } else if (more) {
+        d[n++] = {layer, -more, 0};
+        d[n++] = {scale_layer, 0, more};
+    }
+    for (int i = 1; i < n; i++)
+        for (int k = i; k > 0 && d[k - 1].stride > d[k].stride; k--) { const QtRange x = d[k]; d[k] = d[k - 1]; d[k - 1] = x; }
     for (const void *c : {kv->k, kv->v})
-        for (const uint8_t *s : {kv->k_scale, kv->v_scale}) {
-            const __int128 D = (intptr_t)s - (intptr_t)c;
-            if (D >= (n - 1) * st + cw || -D >= (n - 1) * sp + sw) continue;
-            // of one stride: the scales of page j meet the codes of page i + j where D - i st lies between -sw and cw: the first
-            // such i past the lower end of codes decides; of two strides: their ranges do
-            __int128 i = (D - cw) / st - ((D - cw) % st < 0) + 1;
-            if (i < 1 - n) i = 1 - n;
-            QT_REFUSE((n > 1 && sp != st) || (i < n && i * st - D < sw), "%s: scales lie among the codes of a page", who);
-        }
+        for (const uint8_t *s : {kv->k_scale, kv->v_scale})
+            QT_REFUSE(qt_stretches_meet(d, n, (intptr_t)s - (intptr_t)c, cw, sw), "%s: scales lie among the codes of a page", who);
     return 0;
 }

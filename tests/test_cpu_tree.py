@@ -200,3 +200,15 @@ def test_errors_name_the_call():
 
 def test_tree_plan_refuses_a_window_under_none():
     refused(hip.lib().qwen_hip_op_tree_plan(C.byref(tree_plan(window=-1)), None), "window")
+
+
+@pytest.mark.parametrize("kw,layer,scale_layer", [
+    (dict(k_scale=32 * Q + 10 * 16384), 10 * 16384, 2 * Q),                                     # layer 1's codes begin where layer 0's scales do
+    (dict(v_scale=32 * Q + 2 * 10 * 16384 + 77), 10 * 16384, 10 * 16384),                       # layer 0's scales, layer 2's codes
+    (dict(k_scale=32 * Q - 1280 - 10), 10 * 16384, 1290),                                       # layer 1's scales, layer 0's codes
+    # [page][layer][codes | scales]: the scales 16 bytes too early
+    (dict(page_stride=3 * 17000 // 16 * 16, scale_page_stride=3 * 17000 // 16 * 16, k_scale=32 * Q + 16384 - 16, v=64 * Q, v_scale=66 * Q), 16992, 16992),
+    # the same, the scales of the page before over the next page's layer 0
+    (dict(page_stride=3 * 16384, scale_page_stride=3 * 16384, k_scale=32 * Q + 3 * 16384 - 100, v=64 * Q, v_scale=66 * Q), 16384, 16384)])
+def test_commit_refuses_scales_among_another_layers_codes(kw, layer, scale_layer):
+    refused(hip.lib().qwen_hip_op_tree_commit(C.byref(codes(**kw)), C.byref(commit(n_layers=3, layer_stride=layer, scale_layer_stride=scale_layer)), None), "among")

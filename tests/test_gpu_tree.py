@@ -1331,3 +1331,37 @@ def test_commits_of_many_requests(layers, in_place):
     got = c.run(in_place=in_place)
     assert got == dict(kv=c.kvl, n_free=c.n_free, free=c.free, status=hip.PLAN_INVALID, table=c.table)
     assert all(torch.equal(x, y) for x, y in zip(c.pools, before))
+
+
+# ---- layers' codes and scales in one buffer ----------------------------------------------------------
+
+
+@pytest.mark.parametrize("order", ["layers", "pages", "apart", "between"])
+def test_commits_over_layers_in_one_buffer(order):
+    """Codes and scales of several layers beside each other: what separate pools give."""
+    L, nkv, page, hd = 3, 2, 4, 64
+    reqs = [(5, 9, 4), (20, 12, 2), (0, 3, 3), (9, 30, 17)]
+    c = Commit(reqs, "e4m3", L, nkv, hd, page, "head", seed=5)
+    n, code, scale = c.n_pages, nkv * page * hd, nkv * page
+    pools, want = c.want()
+    buf = torch.zeros(16 * L * n * (code + scale), dtype=torch.uint8, device=DEV)
+    one = 2 * code + 2 * scale                          # a page: codes of k and v, scales of k and v
+    if order == "layers":                               # [layer][k codes | v codes | k scales | v scales], pages within each
+        at = [(0, (n * one, code)), (2 * n * code, (n * one, scale)), (n * code, (n * one, code)), (2 * n * code + n * scale, (n * one, scale))]
+    elif order == "pages":                              # [page][layer][the same]
+        at = [(o, (one, L * one)) for o in (0, 2 * code, code, 2 * code + scale)]
+    elif order == "apart":
+        at = [(0, (n * code, code)), (2 * L * n * code, (n * scale, scale)), (L * n * code, (n * code, code)), (2 * L * n * code + L * n * scale, (n * scale, scale))]
+    else:                                               # all scales between the first two layers' codes
+        far = 4 * n * code
+        at = [(0, (far, code)), (2 * n * code, (n * scale, scale)), (n * code, (far, code)), (3 * n * code, (n * scale, scale))]
+    new = []
+    for x, (o, (layer, pg)) in zip(c.pools, at):
+        inner = (page * hd, hd, 1) if x.dim() == 5 else (page, 1)
+        y = buf[o:].as_strided(x.shape, (layer, pg, *inner))
+        y.copy_(x)
+        new.append(y)
+    c.pools, c.kv = new, pages8(*(x[0] for x in new))
+    assert c.run() == want
+    for x, y in zip(c.pools, pools):
+        assert torch.equal(x.cpu(), y)
