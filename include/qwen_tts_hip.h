@@ -594,6 +594,7 @@ int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *plan, void *stream);
  * whose bits are set in its mask; a request of more than 32 * mask_words new tokens is causal as there.  With attn->window > 0
  * a row sees those positions before the new tokens that are greater than pos[t] - window (pos brought into kv_len - n .. kv_len - 1), and the mask
  * alone decides on the new ones: tree_plan with the same window leaves out what lies before it; pos may be NULL without a window.  Any mask will do: a row without bits sees only what is before.
+ * out and the workspace must not overlap mask or pos (refused).
  * Everything else, the workspace too (qwen_hip_op_page_attention_workspace), is as there. */
 typedef struct {
     const uint32_t *mask;    /* [T][mask_stride] */

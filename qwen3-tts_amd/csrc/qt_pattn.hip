@@ -138,6 +138,15 @@ static int paged_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_at
     QT_REFUSE(plan.slots * a.nkv > 0xFFFFFFll, "%s: too many tiles for one launch", who);
     const long long E = qt_dt_size(p->dtype), row = (long long)p->n_heads * kv->head_dim * E;
     QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, p->q, p->q_stride * E, row, p->T), "%s: out overlaps q", who);
+    if (tree) {
+        const int *const pos = p->window > 0 ? tree->pos : nullptr;
+        QT_REFUSE(qt_rows_meet(p->out, p->out_stride * E, row, tree->mask, tree->mask_stride * 4, 4ll * tree->mask_words, p->T) ||
+                      (pos && qt_rows_meet(p->out, p->out_stride * E, row, pos, 4, 4, p->T)),
+                  "tree_attention: out overlaps mask or pos");
+        const QtMem ws[] = {{p->workspace, need, "workspace", nullptr}};
+        const QtMem in[] = {{tree->mask, 4 * ((p->T - 1) * tree->mask_stride + tree->mask_words), 0, 0}, {pos, 4ll * p->T, 0, 0}};
+        QT_REFUSE(need > 0 && qt_meets(ws, 1, in, 2), "tree_attention: the workspace overlaps mask or pos");
+    }
     const hipStream_t st = qt_stream(stream);
     QtOnDevice on(st);
     QT_REFUSE(on.err != hipSuccess, "%s: the stream's device: %s", who, hipGetErrorString(on.err));

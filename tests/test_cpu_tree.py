@@ -212,3 +212,16 @@ def test_tree_plan_refuses_a_window_under_none():
     (dict(page_stride=3 * 16384, scale_page_stride=3 * 16384, k_scale=32 * Q + 3 * 16384 - 100, v=64 * Q, v_scale=66 * Q), 16384, 16384)])
 def test_commit_refuses_scales_among_another_layers_codes(kw, layer, scale_layer):
     refused(hip.lib().qwen_hip_op_tree_commit(C.byref(codes(**kw)), C.byref(commit(n_layers=3, layer_stride=layer, scale_layer_stride=scale_layer)), None), "among")
+
+
+@pytest.mark.parametrize("t", [0, 1])
+@pytest.mark.parametrize("what,at,window", [("out", "mask", 0), ("out", "mask", 5), ("out", "pos", 5), ("workspace", "mask", 0), ("workspace", "pos", 5)])
+def test_tree_attention_refuses_outputs_that_overlap(t, what, at, window):
+    """The last bytes of one, the first of the other."""
+    L, heads = hip.lib(), dict(dtype=t, B=1, T=9, n_heads=16, q=96 * Q, out=98 * Q, workspace=128 * Q, workspace_bytes=64 * Q, max_kv=1 << 16, window=window,
+                               q_stride=2048, out_stride=2048)
+    kv, a, tr = pages(k=8 * Q, v=16 * Q), attn(**heads), tree(mask=100 * Q, pos=101 * Q)
+    end = {"mask": 100 * Q + 4 * (8 * 2 + 2), "pos": 101 * Q + 4 * 9}[at]
+    setattr(a, what, (end - 1) // 16 * 16)
+    refused(L.qwen_hip_op_tree_attention(C.byref(kv), C.byref(a), C.byref(tr), None), what)
+    assert "overlap" in hip.last_error()
