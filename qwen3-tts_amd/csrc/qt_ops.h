@@ -198,7 +198,7 @@ struct QtMem { const void *p; long long bytes; const char *name; const void *sam
 static inline const QtMem *qt_meets(const QtMem *out, int n_out, const QtMem *in, int n_in) {
     const auto meet = [](const QtMem &a, const QtMem &b) {
         const intptr_t x = (intptr_t)a.p, y = (intptr_t)b.p;
-        return a.p && b.p && x < y + b.bytes && y < x + a.bytes;
+        return a.p && b.p && a.bytes > 0 && b.bytes > 0 && x < y + b.bytes && y < x + a.bytes;
     };
     for (int i = 0; i < n_out; i++) {
         for (int j = i + 1; j < n_out; j++)

@@ -1365,3 +1365,16 @@ def test_commits_over_layers_in_one_buffer(order):
     assert c.run() == want
     for x, y in zip(c.pools, pools):
         assert torch.equal(x.cpu(), y)
+
+
+def test_buffers_of_no_tokens_overlap_nothing():
+    """No tokens at all: buffers of no length inside others are no overlap."""
+    n_path, cu, r, kv = i32([7, 7, 7, 7]), i32([0] * 4), torch.zeros(3, device=DEV), i32([0, 4, 9])
+    p = torch.zeros(16, device=DEV)
+    d = hip.TreeVerify(dtype=0, B=3, T=0, V=9, p=dp(p), p_stride=9, tok=dp(n_path) + 4, parent=dp(n_path) + 4, cu_q=dp(cu), u=dp(n_path) + 4, r=dp(r), path=dp(n_path) + 4,
+                       out_tok=dp(n_path) + 8, n_path=dp(n_path))
+    ws = torch.zeros(hip.lib().qwen_hip_op_tree_verify_workspace(C.byref(d)), dtype=torch.uint8, device=DEV)
+    d.workspace, d.workspace_bytes = dp(ws), ws.numel()
+    ok(hip.lib().qwen_hip_op_tree_verify(C.byref(d), stream()))
+    torch.cuda.synchronize()
+    assert n_path.tolist() == [0, 0, 0, 7]
