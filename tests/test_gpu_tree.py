@@ -1378,3 +1378,77 @@ def test_buffers_of_no_tokens_overlap_nothing():
     ok(hip.lib().qwen_hip_op_tree_verify(C.byref(d), stream()))
     torch.cuda.synchronize()
     assert n_path.tolist() == [0, 0, 0, 7]
+
+
+# ---- verification in several launches ----------------------------------------------------------------
+
+
+@pytest.mark.parametrize("draft", [0, 1])
+def test_verify_edges_of_large_vocabularies(draft):
+    test_verify_edges(draft, 50_001)
+
+
+@pytest.mark.parametrize("draft", [0, 1])
+@pytest.mark.parametrize("children", [0, 1])
+def test_verify_many_children_of_large_vocabularies(draft, children):
+    """More rejections than launches, requests of more than 64 tokens, and a bound on the children that does not hold."""
+    for seed in range(4):
+        v = Verify([90, 6, 130], 50_001, "f32", draft, seed=seed, width=2, noise=3.0, children=children)
+        for b in (0, 2):
+            for i in range(1, v.lens[b]):
+                v.up[v.cu[b] + i] = 0 if i < 66 + seed else v.up[v.cu[b] + i]
+        v.u = 0.9 + 0.1 * v.u if seed % 2 else v.u
+        if seed == 3:
+            v.u[v.cu[0] + 70] = v.u[v.cu[2] + 100] = -1.0                    # kept for certain, if it is looked at
+        v.check()
+
+
+class VerifyCall(Verify):
+    """The same call on buffers that stay, so that several are under way at once."""
+
+    def build(self):
+        dev = lambda x: None if x is None else x.to(DEV)  # noqa: E731
+        n, T = len(self.lens), self.T
+        self.buf = [dev(self.p), dev(self.q), i32(self.tok), i32(self.up), i32(self.cu), dev(self.u), dev(self.r)]
+        self.res = [torch.full((m,), 77, dtype=torch.int32, device=DEV) for m in (T, T, n)]
+        p, q, tok, up, cu, u, r = (dp(x) if x is not None else None for x in self.buf)
+        self.d = hip.TreeVerify(dtype=hip.DT[self.t], B=n, T=T, V=self.V, p=p, p_stride=self.V, q=q, q_stride=self.V, tok=tok, parent=up, cu_q=cu, u=u, r=r,
+                                path=dp(self.res[0]), out_tok=dp(self.res[1]), n_path=dp(self.res[2]), max_children=self.children)
+        self.ws = torch.full((hip.lib().qwen_hip_op_tree_verify_workspace(C.byref(self.d)),), 255, dtype=torch.uint8, device=DEV)
+        self.d.workspace, self.d.workspace_bytes = dp(self.ws), self.ws.numel()
+        return self
+
+    def call(self):
+        ok(hip.lib().qwen_hip_op_tree_verify(C.byref(self.d), stream()))
+
+
+@pytest.mark.parametrize("V", [3000, 60_000])
+def test_verifications_under_way_at_once(V):
+    """Two verifications on two streams, issued in turn without a wait, each with its workspace."""
+    st = [torch.cuda.Stream(), torch.cuda.Stream()]
+    x = [VerifyCall([5, 9, 13], V, "bf16", 1, seed=s).build() for s in (1, 2)]
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for v, s in zip(x, st):
+            with torch.cuda.stream(s):
+                v.call()
+    torch.cuda.synchronize()
+    for v in x:
+        assert tuple(r.tolist() for r in v.res) == v.want()
+
+
+@pytest.mark.parametrize("V", [3000, 60_000])
+def test_verifications_replayed(V):
+    """A captured verification follows what its buffers hold at each replay."""
+    v = VerifyCall([5, 9, 13, 0, 70], V, "bf16", 1, seed=3).build()
+    v.call()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        v.call()
+    for seed in range(3):
+        w = Verify([13, 5, 0, 70, 9], V, "bf16", 1, seed=10 + seed)
+        for a, b in zip(v.buf, (w.p, w.q, torch.tensor(w.tok), torch.tensor(w.up), torch.tensor(w.cu), w.u, w.r)):
+            a.copy_(b)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert tuple(r.tolist() for r in v.res) == w.want()
