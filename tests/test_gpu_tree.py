@@ -1452,3 +1452,29 @@ def test_verifications_replayed(V):
         graph.replay()
         torch.cuda.synchronize()
         assert tuple(r.tolist() for r in v.res) == w.want()
+
+
+# ---- the largest there are ---------------------------------------------------------------------------
+
+
+@pytest.mark.parametrize("t,cache", [("f32", "bf16"), ("bf16", "bf16"), ("f32", "e4m3"), ("bf16", "e4m3"), ("f16", "e4m3")])
+@pytest.mark.parametrize("window", [0, 100])
+def test_trees_of_as_many_tokens_as_masks_hold(t, cache, window):
+    s = Steps([(70, 1024), (5, 1000), (40, 1025), (300, 7)], 4, 2, 64, t, cache, 16, "head", seed=31, words=32, window=window)
+    s.check()
+
+
+@pytest.mark.parametrize("draft", [0, 1])
+def test_verify_the_largest_vocabulary(draft):
+    Verify([3, 1, 4], 1 << 20, "bf16", draft, seed=9, width=3).check()
+
+
+@pytest.mark.parametrize("draft", [0, 1])
+@pytest.mark.parametrize("V", [300, 50_001])
+def test_verify_a_chunk_of_text(draft, V):
+    """A long chain that is given, kept for certain up to its drafts at the end, beside a tree."""
+    v = Verify([400, 9], V, "bf16", draft, seed=4, width=3)
+    v.up[:400] = list(range(-1, 399))
+    v.u[:395] = -1.0
+    v.check()
+    assert v.run()[2][0] >= 395
