@@ -39,8 +39,10 @@ static AttPlan att_plan(AttArgs &a, int dtype, bool paged, int max_q, int max_kv
     // Single tokens want many ranges (64 streams of up to 8000 keys: 2 of them 217 us, 8 199, 16 200), since a workgroup
     // only reads; a tile's sums are large, and two workgroups a CU are enough (chunks over up to 7000 keys: 2 ranges
     // 171 us, 1 226, 3 190, 4 205).  Over codes, and for trees, requests of one tile each take up to four a CU, since their lengths
-    // differ by more than a tile's (32 trees of 33 to 64 tokens over 500 to 6000 keys of codes: 2 ranges 138 us, 3 128, 4 139, 5 129; chunks
-    // of several tiles 168, 171, 182, 180).
+    // differ by more than a tile's.  Two, three, four, five and six a CU over codes: 32 trees of 33 to 64 tokens over 500 to 6000 keys 124, 125, 115,
+    // 115, 129 us; 32 of 64 over 3000 each 105, 86, 85, 103, 103; 16 of 40 to 64 over 1000 to 8000 116, 91, 79, 105, 100; 24 of 33 to 60 over 100
+    // to 2500 61, 50, 50, 50, 57; 48 of 30 to 64 over 200 to 4000 137, 102, 102, 102, 121; 20 chunks of 40 to 64 over 500 to 7000 136, 96, 82, 93,
+    // 92.  Chunks of several tiles, ranges 2 to 5: 168, 171, 182, 180.
     const bool one_tile = more && max_q > 0 && (long long)max_q * a.G <= 128;
     const long long wgs = p.slots * a.nkv, blocks = ((long long)max_kv + 31) / 32;
     long long n = wgs > 0 && paged ? ((p.kind == ATT_TILE ? (one_tile ? 1024 : 512) : 4096) + wgs - 1) / wgs : 1;

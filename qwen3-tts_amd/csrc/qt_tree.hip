@@ -14,8 +14,8 @@ __device__ __forceinline__ TreeReq tree_req(const int *cu, int b, int T) {
 
 // ---- positions and masks ---------------------------------------------------------------------------
 // A workgroup a request.  A token walks up through its parents, held in LDS: they have smaller indices, so the words of its mask
-// come from the highest down and each is stored once; `window` steps up and further its ancestors are counted only.  Bound by the launch (8 requests of 5 to 16 tokens and 512 of 1 to 61 both 6.1 us a pass, the
-// kernel 2.7 and 4.4).
+// come from the highest down and each is stored once; `window` steps up and further its ancestors are counted only.  Bound by the launch (8 requests of 5 to 16 tokens and 512 of 1 to 61 both about 6 us a pass, the
+// kernel 2.8 and 4.5).
 struct TreePlanArgs {
     const int *parent, *cu, *kv;
     int *pos;
@@ -86,7 +86,7 @@ extern "C" int qwen_hip_op_tree_plan(const qwen_hip_tree_plan_t *p, void *stream
 //
 // Large vocabularies: launches of a wave for two tiles, the first of which walks to the first sum (every workgroup for itself: a few
 // dependent loads), the others from the sum before to the next where there is one; then a launch of a workgroup a request, which goes on
-// from there, makes further sums itself, and picks.  64 trees of 5 to 13 tokens over 128 003 bf16: 27 to 29 us, of which the rows' bytes are 6.7 (all sums but
+// from there, makes further sums itself, and picks.  64 trees of 5 to 13 tokens over 128 003 bf16: 25 to 29 us, of which the rows' bytes are 6.7 (all sums but
 // the first in the launch that picks 44, but the first two 36; one workgroup a request for everything past the first sum, without tiles a wave, 96);
 // bound by sums that wait for each other.  6 chains over 2048 f32, one launch: 6.9, a chain of five dependent loads.
 #define VF_TILE 1024
@@ -559,8 +559,8 @@ extern "C" int qwen_hip_op_tree_verify(const qwen_hip_tree_verify_t *p, void *st
 // first (commit_stands), and the lengths' workgroup is one more of the launch; past it, and where lengths or the count are replaced in place, the lengths'
 // launch is before the moves', which go by its status (bf16, 2 heads of 64, one launch and two: 300 requests of 8 layers 8.0 and 9.6 us, 1024 of one 7.5
 // and 9.8, 512 of 8 11.8 and 11.1, 300 of 28 18.5 and 14.5; without looking 512 of 8 7.2).
-// Bound by the latency of lengths, path, table, rows for few (8 requests, one layer of bf16: 6.7 us a pass), by the rows' bytes for many
-// layers (64 requests, 28 layers of codes: 15.2; without the look at all requests 13.9).
+// Bound by a chain of dependent loads (lengths, path, table, rows): 8 requests, one layer of bf16 6.7 us a pass, the kernel 4.6; 64 requests,
+// 28 layers of codes 15.2 (without the look at all requests 13.9), the rows' 42 to 49 MB being 10.
 #define CM_T 256
 #define CM_MAX_B 2048
 #define CM_LOOK (1 << 20)
