@@ -562,7 +562,7 @@ typedef struct {
     int dtype, n_heads, B, T, table_cols, max_q, max_kv, window;
     float scale;
 } qwen_hip_page_attn_t;
-long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn);  /* -1: error */
+long long qwen_hip_op_page_attention_workspace(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn);  /* of tree_attention on these descriptors too; -1: error */
 int qwen_hip_op_page_attention(const qwen_hip_kv_pages_t *kv, const qwen_hip_page_attn_t *attn, void *stream);
 
 /* ---- trees of drafted tokens ----
